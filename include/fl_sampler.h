@@ -40,7 +40,7 @@
 extern "C" {
 #endif
 
-#define FL_ABI_VERSION 6
+#define FL_ABI_VERSION 7
 
 enum fl_dtype { FL_DTYPE_F32 = 0, FL_DTYPE_BF16 = 1, FL_DTYPE_F16 = 2 };
 
@@ -370,6 +370,141 @@ int fl_lm_head_sample(const fl_lm_head_args* args, void* stream);
 /* Bytes of workspace fl_lm_head_sample needs for `batch` rows of `vocab`
  * values (no counterpart in the reference). */
 int fl_lm_head_workspace_bytes(int64_t batch, int64_t vocab, size_t* out_bytes);
+
+/*
+ * Scores of given tokens from logits rows (any of the outputs; NULL: not asked
+ * for).  With p = softmax(x_r) over the row's vocabulary, in float32 or more:
+ *   out_lse[r]      = log(sum(exp(x_r)))
+ *   out_logprob[r]  = x_r[t] - lse, t = tokens[r]; -0.0 where t == ignore_index
+ *                     (as fl_row_stats), NaN where t is outside [0, vocab)
+ *   out_entropy[r]  = -sum(p log p), a masked value (-inf) adding nothing
+ *   out_rank[r]     = the number of values greater than x_r[t]; -1 where
+ *                     tokens[r] is ignored or outside [0, vocab)
+ *   out_top_ids / out_top_logprobs [rows, top_k]: the top_k largest values,
+ *                     descending, equal ones by ascending index
+ * A row without a distribution (a NaN or +inf logit, or -inf alone) has NaN in
+ * every float output (lse: -inf for -inf alone), rank -1 and top_ids -1.
+ * out_saved (float [rows, 4]) is what fl_score_tokens_grad reads: lse in two
+ * floats, and the entropy if out_entropy is asked for.  top_k: 0 (none) to
+ * min(vocab, FL_SCORE_MAX_TOPK); vocab up to FL_MAX_VOCAB_F32.  workspace
+ * (fl_score_workspace_bytes, 8-byte aligned; 0 bytes for vocab <= 16384): calls
+ * that overlap in time must not share one.  A row's results are a function of
+ * the row alone.
+ */
+#define FL_SCORE_MAX_TOPK 64
+typedef struct fl_score_args {
+  uint32_t struct_size;
+  int32_t dtype;
+  const void* logits;          /* [rows, vocab], row stride ld */
+  int64_t rows;
+  int64_t vocab;
+  int64_t ld;
+  const int64_t* tokens;       /* [rows] or NULL */
+  int64_t ignore_index;
+  int64_t top_k;
+  float* out_logprob;          /* [rows] */
+  float* out_entropy;          /* [rows] */
+  float* out_lse;              /* [rows] */
+  int32_t* out_rank;           /* [rows] */
+  int64_t* out_top_ids;        /* [rows, top_k] */
+  float* out_top_logprobs;     /* [rows, top_k] */
+  float* out_saved;            /* [rows, 4] */
+  void* workspace;
+  int64_t workspace_bytes;
+} fl_score_args;
+
+int fl_score_tokens(const fl_score_args* args, void* stream);
+int fl_score_workspace_bytes(int64_t rows, int64_t vocab, int64_t top_k, size_t* out_bytes);
+
+/*
+ * The logits' gradient of fl_score_tokens for upstream gradients a, b, c of
+ * logprob, entropy and lse ([rows] each, NULL: 0):
+ *   out_grad[r, i] = a (1[i == t] - p_i) - b p_i (log p_i + entropy) + c p_i
+ * rounded once to the logits' dtype.  a counts as 0 where the token is ignored.
+ * A masked value's gradient is 0, and so is a row's whose a, b and c are 0; else
+ * a row without a distribution has NaN.  saved and the logits are the forward
+ * call's (its out_entropy asked for if grad_entropy is given).
+ */
+typedef struct fl_score_grad_args {
+  uint32_t struct_size;
+  int32_t dtype;
+  const void* logits;
+  int64_t rows;
+  int64_t vocab;
+  int64_t ld;
+  const int64_t* tokens;       /* [rows] or NULL (then grad_logprob is NULL) */
+  int64_t ignore_index;
+  const float* saved;          /* [rows, 4] */
+  const float* grad_logprob;
+  const float* grad_entropy;
+  const float* grad_lse;
+  void* out_grad;              /* [rows, vocab], row stride out_ld */
+  int64_t out_ld;
+} fl_score_grad_args;
+
+int fl_score_tokens_grad(const fl_score_grad_args* args, void* stream);
+
+/*
+ * Layer norm over the last dimension of rows [rows, dim] (dim up to
+ * FL_NORM_MAX_DIM), statistics in float32:
+ *   out[r] = (x_r - mean_r) rstd_r weight + bias
+ *   rstd_r = 1 / sqrt(mean((x_r - mean_r)^2) + eps)
+ * x and out have dtype; weight and bias (contiguous [dim], NULL: 1 and 0) have
+ * wdtype, which is dtype or FL_DTYPE_F32.  out_mean and out_rstd ([rows], may
+ * be NULL) are what fl_layer_norm_grad reads.  out may be x.
+ */
+#define FL_NORM_MAX_DIM 16384
+typedef struct fl_norm_args {
+  uint32_t struct_size;
+  int32_t dtype;
+  int32_t wdtype;
+  float eps;                   /* >= 0, finite */
+  const void* x;               /* row stride ld */
+  int64_t rows;
+  int64_t dim;
+  int64_t ld;
+  const void* weight;
+  const void* bias;
+  void* out;                   /* row stride out_ld */
+  int64_t out_ld;
+  float* out_mean;
+  float* out_rstd;
+} fl_norm_args;
+
+int fl_layer_norm(const fl_norm_args* args, void* stream);
+
+/*
+ * The gradients of fl_layer_norm for the upstream gradient grad ([rows, dim],
+ * dtype, row stride grad_ld), each NULL if not asked for: out_dx (dtype, row
+ * stride out_ld), out_dweight and out_dbias ([dim], wdtype; sums over the rows in
+ * a fixed order).  mean and rstd are the forward call's.  workspace
+ * (fl_layer_norm_grad_workspace_bytes, 16-byte aligned): calls that overlap in
+ * time must not share one; not needed without out_dweight and out_dbias.
+ */
+typedef struct fl_norm_grad_args {
+  uint32_t struct_size;
+  int32_t dtype;
+  int32_t wdtype;
+  int32_t reserved;            /* 0 */
+  const void* x;
+  int64_t rows;
+  int64_t dim;
+  int64_t ld;
+  const void* weight;
+  const void* grad;
+  int64_t grad_ld;
+  const float* mean;
+  const float* rstd;
+  void* out_dx;
+  int64_t out_ld;
+  void* out_dweight;
+  void* out_dbias;
+  void* workspace;
+  int64_t workspace_bytes;
+} fl_norm_grad_args;
+
+int fl_layer_norm_grad(const fl_norm_grad_args* args, void* stream);
+int fl_layer_norm_grad_workspace_bytes(int64_t rows, int64_t dim, int32_t dtype, size_t* out_bytes);
 
 /* Thread-local description of the last error returned on this thread. */
 const char* fl_last_error(void);

@@ -18,6 +18,11 @@ lm_head_sample, LmHeadPlan
 token_logprobs_from_logits, entropy_from_logits, kl_full_distribution, row_stats
     Full-distribution log-prob / entropy / KL in one pass (models/policy.py,
     training/common/logprobs.py).
+score_tokens, score_tokens_backward
+    Log-probabilities of given tokens with entropy, rank and top alternatives, and
+    the logits' gradient (models/policy.py, training/common/logprobs.py).
+layer_norm, layer_norm_backward
+    The norm in front of the head, with its gradients.
 SamplingParams
     Per-request parameters with the reference's validation (inference/requests.py).
 """
@@ -28,6 +33,8 @@ from .sampling import (SampleOutput, SamplerPlan, SamplingError, apply_sampling_
 from .speculative import MTPSpeculativeGenerator, SpeculativeGenerator, SpecOutput, SpecPlan, speculative_verify
 from .engine import BatchedSampler
 from .logprobs import RowStats, entropy_from_logits, kl_full_distribution, row_stats, token_logprobs_from_logits
+from .norm import NormStats, layer_norm, layer_norm_backward
+from .scores import TokenScores, score_tokens, score_tokens_backward
 from .lmhead import LmHeadOutput, LmHeadPlan, lm_head_sample
 
 __all__ = [
@@ -36,5 +43,6 @@ __all__ = [
     "speculative_verify", "SpeculativeGenerator", "MTPSpeculativeGenerator", "SpecOutput", "SpecPlan",
     "BatchedSampler", "row_stats", "RowStats", "token_logprobs_from_logits", "entropy_from_logits", "kl_full_distribution",
     "SamplingParams", "GenerationSettings", "SamplingParamsError",
+    "score_tokens", "score_tokens_backward", "TokenScores", "layer_norm", "layer_norm_backward", "NormStats",
     "lm_head_sample", "LmHeadPlan", "LmHeadOutput",
 ]

@@ -18,7 +18,7 @@ import torch  # noqa: F401  (loads the HIP runtime the library binds to)
 LIB_PATH = os.environ.get("FL_SAMPLER_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib",
                                                             "libflsampler.so")
 
-FL_ABI_VERSION = 6
+FL_ABI_VERSION = 7
 FL_DTYPE_F32, FL_DTYPE_BF16, FL_DTYPE_F16 = 0, 1, 2
 FL_OK, FL_EIO, FL_EINVAL, FL_ENOTSUP = 0, -5, -22, -95
 FL_ROW_OK, FL_ROW_NAN, FL_ROW_INF, FL_ROW_BAD_HISTORY, FL_ROW_LIMIT, FL_ROW_ALL_MASKED = 0, 1, 2, 4, 8, 16
@@ -97,6 +97,47 @@ class LmHeadArgs(ctypes.Structure):
     ]
 
 
+class ScoreArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32),
+        ("logits", _p), ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("ld", ctypes.c_int64),
+        ("tokens", _p), ("ignore_index", ctypes.c_int64), ("top_k", ctypes.c_int64),
+        ("out_logprob", _p), ("out_entropy", _p), ("out_lse", _p), ("out_rank", _p),
+        ("out_top_ids", _p), ("out_top_logprobs", _p), ("out_saved", _p),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+class ScoreGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32),
+        ("logits", _p), ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("ld", ctypes.c_int64),
+        ("tokens", _p), ("ignore_index", ctypes.c_int64), ("saved", _p),
+        ("grad_logprob", _p), ("grad_entropy", _p), ("grad_lse", _p),
+        ("out_grad", _p), ("out_ld", ctypes.c_int64),
+    ]
+
+
+class NormArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("wdtype", ctypes.c_int32), ("eps", ctypes.c_float),
+        ("x", _p), ("rows", ctypes.c_int64), ("dim", ctypes.c_int64), ("ld", ctypes.c_int64),
+        ("weight", _p), ("bias", _p), ("out", _p), ("out_ld", ctypes.c_int64), ("out_mean", _p), ("out_rstd", _p),
+    ]
+
+
+class NormGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("wdtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("x", _p), ("rows", ctypes.c_int64), ("dim", ctypes.c_int64), ("ld", ctypes.c_int64),
+        ("weight", _p), ("grad", _p), ("grad_ld", ctypes.c_int64), ("mean", _p), ("rstd", _p),
+        ("out_dx", _p), ("out_ld", ctypes.c_int64), ("out_dweight", _p), ("out_dbias", _p),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+FL_NORM_MAX_DIM = 16384
+FL_SCORE_MAX_TOPK = 64
 FL_LM_HEAD_MAX_BATCH = 64
 FL_LM_HEAD_MAX_TOPK = 64
 FL_LM_HEAD_MAX_CAND = 4096
@@ -158,6 +199,19 @@ def lib() -> ctypes.CDLL:
     handle.fl_lm_head_workspace_bytes.restype = ctypes.c_int
     handle.fl_row_stats.argtypes = [ctypes.POINTER(RowStatsArgs), _p]
     handle.fl_row_stats.restype = ctypes.c_int
+    handle.fl_score_tokens.argtypes = [ctypes.POINTER(ScoreArgs), _p]
+    handle.fl_score_tokens.restype = ctypes.c_int
+    handle.fl_score_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)]
+    handle.fl_score_workspace_bytes.restype = ctypes.c_int
+    handle.fl_score_tokens_grad.argtypes = [ctypes.POINTER(ScoreGradArgs), _p]
+    handle.fl_score_tokens_grad.restype = ctypes.c_int
+    handle.fl_layer_norm.argtypes = [ctypes.POINTER(NormArgs), _p]
+    handle.fl_layer_norm.restype = ctypes.c_int
+    handle.fl_layer_norm_grad.argtypes = [ctypes.POINTER(NormGradArgs), _p]
+    handle.fl_layer_norm_grad.restype = ctypes.c_int
+    handle.fl_layer_norm_grad_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
+                                                          ctypes.POINTER(ctypes.c_size_t)]
+    handle.fl_layer_norm_grad_workspace_bytes.restype = ctypes.c_int
     _lib = handle
     return handle
 
@@ -185,6 +239,20 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def call(fn, args: ctypes.Structure, device: torch.device, what: str) -> None:
+    """fn(args) on the device's current stream; the device is made the current
+    one for the launch if another is."""
+    if device.index is None or torch.cuda.current_device() == device.index:
+        rc = fn(ctypes.byref(args), stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(ctypes.byref(args), stream_handle(device))
+    if rc:
+        check(rc, what)
+
+
 EXPORTED_SYMBOLS = ("fl_sample", "fl_sample_exact", "fl_fill_rows", "fl_apply_filter", "fl_spec_verify", "fl_spec_verify_static",
                     "fl_spec_workspace_bytes", "fl_spec_cache_workspace_bytes", "fl_lm_head_sample", "fl_lm_head_workspace_bytes", "fl_row_stats",
+                    "fl_score_tokens", "fl_score_workspace_bytes", "fl_score_tokens_grad",
+                    "fl_layer_norm", "fl_layer_norm_grad", "fl_layer_norm_grad_workspace_bytes",
                     "fl_last_error", "fl_abi_version")

@@ -31,6 +31,35 @@ int check_launch(hipError_t e, const char* what) {
   return ok();
 }
 
+// Work-groups of 256 threads in one launch: a grid's work-items stay below 2^32.
+constexpr int64_t MAX_BLOCKS_256 = (1ll << 24) - 1;
+
+// Logits rows of the score calls; 0 = go on.
+int validate_rows(const char* fn, int32_t dtype, int64_t rows, int64_t vocab, int64_t ld) {
+  if (dtype != FL_DTYPE_F32 && dtype != FL_DTYPE_BF16 && dtype != FL_DTYPE_F16)
+    return fail(FL_EINVAL, "%s: unknown dtype %d", fn, dtype);
+  if (rows < 0 || vocab < 1 || ld < vocab)
+    return fail(FL_EINVAL, "%s: bad shape rows=%lld vocab=%lld ld=%lld", fn, static_cast<long long>(rows),
+                static_cast<long long>(vocab), static_cast<long long>(ld));
+  if (vocab > FL_MAX_VOCAB_F32 || rows > MAX_BLOCKS_256)
+    return fail(FL_ENOTSUP, "%s: vocab %lld or rows %lld beyond the library's limits", fn,
+                static_cast<long long>(vocab), static_cast<long long>(rows));
+  return 0;
+}
+
+// The layer norm calls; 0 = go on.
+int validate_norm(const char* fn, int32_t dtype, int32_t wdtype, int64_t rows, int64_t dim) {
+  if (dtype != FL_DTYPE_F32 && dtype != FL_DTYPE_BF16 && dtype != FL_DTYPE_F16)
+    return fail(FL_EINVAL, "%s: unknown dtype %d", fn, dtype);
+  if (wdtype != dtype && wdtype != FL_DTYPE_F32)
+    return fail(FL_EINVAL, "%s: wdtype %d is neither dtype %d nor float32", fn, wdtype, dtype);
+  if (rows < 0 || dim < 1)
+    return fail(FL_EINVAL, "%s: bad shape rows=%lld dim=%lld", fn, static_cast<long long>(rows), static_cast<long long>(dim));
+  if (dim > FL_NORM_MAX_DIM)
+    return fail(FL_ENOTSUP, "%s: dim %lld beyond the library's limit %d", fn, static_cast<long long>(dim), FL_NORM_MAX_DIM);
+  return 0;
+}
+
 int validate_sample(const fl_sample_args* a, const char* fn) {
   if (a == nullptr) return fail(FL_EINVAL, "%s: args is NULL", fn);
   if (a->struct_size != sizeof(fl_sample_args))
@@ -246,6 +275,93 @@ int fl_spec_cache_workspace_bytes(int64_t batch, int64_t vocab, size_t* out_byte
                 static_cast<long long>(vocab));
   *out_bytes = fl::spec_cache_workspace_bytes(batch, vocab);
   return ok();
+}
+
+int fl_score_workspace_bytes(int64_t rows, int64_t vocab, int64_t top_k, size_t* out_bytes) {
+  const char* fn = "fl_score_workspace_bytes";
+  if (out_bytes == nullptr) return fail(FL_EINVAL, "%s: out_bytes is NULL", fn);
+  if (const int rc = validate_rows(fn, FL_DTYPE_F32, rows, vocab, vocab)) return rc;
+  if (top_k < 0) return fail(FL_EINVAL, "%s: top_k %lld < 0", fn, static_cast<long long>(top_k));
+  if (top_k > FL_SCORE_MAX_TOPK)
+    return fail(FL_ENOTSUP, "%s: top_k %lld beyond the library's limit %d", fn, static_cast<long long>(top_k),
+                FL_SCORE_MAX_TOPK);
+  *out_bytes = fl::score_workspace_bytes(rows, vocab, top_k);
+  return ok();
+}
+
+int fl_score_tokens(const fl_score_args* a, void* stream) {
+  const char* fn = "fl_score_tokens";
+  if (a == nullptr) return fail(FL_EINVAL, "%s: args is NULL", fn);
+  if (a->struct_size != sizeof(fl_score_args)) return fail(FL_EINVAL, "%s: struct_size mismatch", fn);
+  if (const int rc = validate_rows(fn, a->dtype, a->rows, a->vocab, a->ld)) return rc;
+  if (a->top_k < 0 || a->top_k > a->vocab)
+    return fail(FL_EINVAL, "%s: top_k %lld outside 0 .. vocab %lld", fn, static_cast<long long>(a->top_k),
+                static_cast<long long>(a->vocab));
+  if (a->top_k > FL_SCORE_MAX_TOPK || fl::score_blocks(a->rows, a->vocab) > MAX_BLOCKS_256)
+    return fail(FL_ENOTSUP, "%s: top_k %lld or rows %lld beyond the library's limits", fn,
+                static_cast<long long>(a->top_k), static_cast<long long>(a->rows));
+  if ((a->out_logprob || a->out_rank) && !a->tokens) return fail(FL_EINVAL, "%s: logprob and rank need tokens", fn);
+  if (a->rows == 0) return ok();
+  if (!a->logits) return fail(FL_EINVAL, "%s: logits is NULL", fn);
+  const size_t need = fl::score_workspace_bytes(a->rows, a->vocab, a->top_k);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < 0 || static_cast<size_t>(a->workspace_bytes) < need))
+    return fail(FL_EINVAL, "%s: workspace of %lld bytes, %zu needed", fn, static_cast<long long>(a->workspace_bytes), need);
+  if ((reinterpret_cast<uintptr_t>(a->workspace) & 7u) != 0) return fail(FL_EINVAL, "%s: workspace not 8-byte aligned", fn);
+  return check_launch(fl::launch_score(*a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int fl_score_tokens_grad(const fl_score_grad_args* a, void* stream) {
+  const char* fn = "fl_score_tokens_grad";
+  if (a == nullptr) return fail(FL_EINVAL, "%s: args is NULL", fn);
+  if (a->struct_size != sizeof(fl_score_grad_args)) return fail(FL_EINVAL, "%s: struct_size mismatch", fn);
+  if (const int rc = validate_rows(fn, a->dtype, a->rows, a->vocab, a->ld)) return rc;
+  if (a->out_ld < a->vocab) return fail(FL_EINVAL, "%s: out_ld %lld < vocab", fn, static_cast<long long>(a->out_ld));
+  if (fl::score_grad_blocks(a->rows, a->vocab, a->dtype) > MAX_BLOCKS_256)
+    return fail(FL_ENOTSUP, "%s: rows %lld beyond the library's limits", fn, static_cast<long long>(a->rows));
+  if (a->grad_logprob && !a->tokens) return fail(FL_EINVAL, "%s: grad_logprob needs tokens", fn);
+  if (a->rows == 0) return ok();
+  if (!a->logits || !a->saved || !a->out_grad) return fail(FL_EINVAL, "%s: a required pointer is NULL", fn);
+  return check_launch(fl::launch_score_grad(*a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int fl_layer_norm(const fl_norm_args* a, void* stream) {
+  const char* fn = "fl_layer_norm";
+  if (a == nullptr) return fail(FL_EINVAL, "%s: args is NULL", fn);
+  if (a->struct_size != sizeof(fl_norm_args)) return fail(FL_EINVAL, "%s: struct_size mismatch", fn);
+  if (const int rc = validate_norm(fn, a->dtype, a->wdtype, a->rows, a->dim)) return rc;
+  if (a->ld < a->dim || a->out_ld < a->dim) return fail(FL_EINVAL, "%s: a row stride below dim", fn);
+  if (!std::isfinite(a->eps) || a->eps < 0.0f) return fail(FL_EINVAL, "%s: eps must be finite and >= 0", fn);
+  if (a->rows == 0) return ok();
+  if (!a->x || !a->out) return fail(FL_EINVAL, "%s: x or out is NULL", fn);
+  return check_launch(fl::launch_norm(*a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int fl_layer_norm_grad_workspace_bytes(int64_t rows, int64_t dim, int32_t dtype, size_t* out_bytes) {
+  const char* fn = "fl_layer_norm_grad_workspace_bytes";
+  if (out_bytes == nullptr) return fail(FL_EINVAL, "%s: out_bytes is NULL", fn);
+  if (const int rc = validate_norm(fn, dtype, dtype, rows, dim)) return rc;
+  *out_bytes = fl::norm_grad_workspace_bytes(rows, dim, dtype);
+  return ok();
+}
+
+int fl_layer_norm_grad(const fl_norm_grad_args* a, void* stream) {
+  const char* fn = "fl_layer_norm_grad";
+  if (a == nullptr) return fail(FL_EINVAL, "%s: args is NULL", fn);
+  if (a->struct_size != sizeof(fl_norm_grad_args)) return fail(FL_EINVAL, "%s: struct_size mismatch", fn);
+  if (a->reserved != 0) return fail(FL_EINVAL, "%s: reserved must be 0", fn);
+  if (const int rc = validate_norm(fn, a->dtype, a->wdtype, a->rows, a->dim)) return rc;
+  if (a->ld < a->dim || a->grad_ld < a->dim || (a->out_dx && a->out_ld < a->dim))
+    return fail(FL_EINVAL, "%s: a row stride below dim", fn);
+  if (a->rows > 0 && (!a->x || !a->grad || !a->mean || !a->rstd))
+    return fail(FL_EINVAL, "%s: a required pointer is NULL", fn);
+  if (a->out_dweight || a->out_dbias) {
+    const size_t need = fl::norm_grad_workspace_bytes(a->rows, a->dim, a->dtype);
+    if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < 0 || static_cast<size_t>(a->workspace_bytes) < need))
+      return fail(FL_EINVAL, "%s: workspace of %lld bytes, %zu needed", fn, static_cast<long long>(a->workspace_bytes), need);
+    if ((reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0)
+      return fail(FL_EINVAL, "%s: workspace not 16-byte aligned", fn);
+  }
+  return check_launch(fl::launch_norm_grad(*a, static_cast<hipStream_t>(stream)), fn);
 }
 
 }  // extern "C"

@@ -97,6 +97,43 @@ __device__ __forceinline__ uint4 buf_load16_once(__amdgpu_buffer_rsrc_t r, uint3
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// A 16-byte chunk of a row's values, and one value by itself (for the last of
+// an odd 16-bit row, whose dword reaches past the buffer's range).
+template <class D>
+struct RowChunk;
+template <>
+struct RowChunk<F32> {
+  static constexpr int N = 4;
+  __device__ static float elem(__amdgpu_buffer_rsrc_t r, int i) {
+    return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, 4 * i, 0, 0));
+  }
+  __device__ static void unpack(const uint4 u, float (&x)[N]) {
+    x[0] = __uint_as_float(u.x);
+    x[1] = __uint_as_float(u.y);
+    x[2] = __uint_as_float(u.z);
+    x[3] = __uint_as_float(u.w);
+  }
+};
+template <class H>
+struct RowChunk16 {
+  static constexpr int N = 8;
+  __device__ static float elem(__amdgpu_buffer_rsrc_t r, int i) {
+    return H::to_f32(__builtin_amdgcn_raw_buffer_load_b16(r, 2 * i, 0, 0));
+  }
+  __device__ static void unpack(const uint4 u, float (&x)[N]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[2 * k] = H::to_f32(w[k] & 0xFFFFu);
+      x[2 * k + 1] = H::to_f32(w[k] >> 16);
+    }
+  }
+};
+template <>
+struct RowChunk<BF16> : RowChunk16<BF16> {};
+template <>
+struct RowChunk<F16> : RowChunk16<F16> {};
+
 // Order index of a 16-bit float pattern: 0 for the largest value (+NaN
 // patterns first), increasing towards the most negative value.
 __device__ __forceinline__ uint32_t order16(uint32_t bits) { return (bits & 0x8000u) ? bits : (0x7FFFu - bits); }

@@ -34,4 +34,17 @@ hipError_t launch_row_stats(const fl_row_stats_args& a, hipStream_t s);
 hipError_t launch_lm_head(const fl_lm_head_args& a, hipStream_t s);
 size_t lm_head_workspace_bytes(int64_t batch, int64_t vocab);
 
+
+// Scores of given tokens, and the logits' gradient.  The blocks of a launch:
+// its work-items have to stay below 2^32.
+hipError_t launch_score(const fl_score_args& a, hipStream_t s);
+size_t score_workspace_bytes(int64_t rows, int64_t vocab, int64_t top_k);
+int64_t score_blocks(int64_t rows, int64_t vocab);
+hipError_t launch_score_grad(const fl_score_grad_args& a, hipStream_t s);
+int64_t score_grad_blocks(int64_t rows, int64_t vocab, int dtype);
+
+hipError_t launch_norm(const fl_norm_args& a, hipStream_t s);
+hipError_t launch_norm_grad(const fl_norm_grad_args& a, hipStream_t s);
+size_t norm_grad_workspace_bytes(int64_t rows, int64_t dim, int dtype);
+
 }  // namespace fl

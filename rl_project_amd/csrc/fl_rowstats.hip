@@ -52,41 +52,6 @@ constexpr float SLACK = 3.5f;
 // any sum, its exponent finite and far below that of any reference in base 2.
 constexpr float PAD = -1.0e38f;
 
-template <class D>
-struct RowChunk;
-template <>
-struct RowChunk<F32> {
-  static constexpr int N = 4;
-  __device__ static float elem(__amdgpu_buffer_rsrc_t r, int i) {
-    return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, 4 * i, 0, 0));
-  }
-  __device__ static void unpack(const uint4 u, float (&x)[N]) {
-    x[0] = __uint_as_float(u.x);
-    x[1] = __uint_as_float(u.y);
-    x[2] = __uint_as_float(u.z);
-    x[3] = __uint_as_float(u.w);
-  }
-};
-template <class H>
-struct RowChunk16 {
-  static constexpr int N = 8;
-  __device__ static float elem(__amdgpu_buffer_rsrc_t r, int i) {
-    return H::to_f32(__builtin_amdgcn_raw_buffer_load_b16(r, 2 * i, 0, 0));
-  }
-  __device__ static void unpack(const uint4 u, float (&x)[N]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[2 * k] = H::to_f32(w[k] & 0xFFFFu);
-      x[2 * k + 1] = H::to_f32(w[k] >> 16);
-    }
-  }
-};
-template <>
-struct RowChunk<BF16> : RowChunk16<BF16> {};
-template <>
-struct RowChunk<F16> : RowChunk16<F16> {};
-
 // Running state of one row for one thread (or a merged set of threads).
 struct Acc {
   float m;    // reference of x, its maximum less at most SLACK (-inf: nothing yet)
