@@ -506,6 +506,73 @@ typedef struct fl_norm_grad_args {
 int fl_layer_norm_grad(const fl_norm_grad_args* args, void* stream);
 int fl_layer_norm_grad_workspace_bytes(int64_t rows, int64_t dim, int32_t dtype, size_t* out_bytes);
 
+/*
+ * Scores of given tokens from hidden states and the lm_head weight, without the
+ * [rows, vocab] logits (the training and evaluation counterpart of
+ * fl_lm_head_sample): with x[r, v] = sum_d hidden[r, d] weight[v, d] in float32
+ * accumulators, out_logprob, out_entropy, out_lse and out_saved are
+ * fl_score_tokens' of x.  hidden [rows, dim] (row stride ld_hidden) and weight
+ * [vocab, dim] (rows contiguous) are bf16, 16-byte aligned (ld_hidden a multiple
+ * of 8), dim a multiple of 64 up to 16384, vocab up to FL_MAX_VOCAB_16, rows up to
+ * FL_HEAD_MAX_ROWS.  workspace (fl_head_workspace_bytes, 256-byte aligned): calls
+ * that overlap in time must not share one.
+ */
+#define FL_HEAD_MAX_ROWS 131072
+typedef struct fl_head_args {
+  uint32_t struct_size;
+  int32_t dtype;               /* FL_DTYPE_BF16 */
+  const void* hidden;
+  const void* weight;
+  int64_t rows;
+  int64_t dim;
+  int64_t vocab;
+  int64_t ld_hidden;
+  const int64_t* tokens;       /* [rows] or NULL */
+  int64_t ignore_index;
+  float* out_logprob;          /* [rows], each may be NULL */
+  float* out_entropy;
+  float* out_lse;
+  float* out_saved;            /* [rows, 4] */
+  void* workspace;
+  int64_t workspace_bytes;
+} fl_head_args;
+
+int fl_head_logprobs(const fl_head_args* args, void* stream);
+int fl_head_workspace_bytes(int64_t rows, int64_t vocab, size_t* out_bytes);
+
+/*
+ * The gradients of fl_head_logprobs for upstream gradients of logprob, entropy
+ * and lse (NULL: 0), each NULL if not asked for: out_dhidden [rows, dim]
+ * (contiguous) and out_dweight [vocab, dim], bf16, summed in float32.  The
+ * logits are computed again, a chunk of the vocabulary at a time; their gradient
+ * (as fl_score_tokens_grad's, zero rows and rows without a distribution
+ * included) passes through the workspace in bf16.  Every sum has a fixed order.
+ */
+typedef struct fl_head_grad_args {
+  uint32_t struct_size;
+  int32_t dtype;               /* FL_DTYPE_BF16 */
+  const void* hidden;
+  const void* weight;
+  int64_t rows;
+  int64_t dim;
+  int64_t vocab;
+  int64_t ld_hidden;
+  const int64_t* tokens;
+  int64_t ignore_index;
+  const float* saved;          /* [rows, 4] of the forward call */
+  const float* grad_logprob;
+  const float* grad_entropy;
+  const float* grad_lse;
+  void* out_dhidden;
+  void* out_dweight;
+  void* workspace;
+  int64_t workspace_bytes;
+} fl_head_grad_args;
+
+int fl_head_logprobs_grad(const fl_head_grad_args* args, void* stream);
+/* dhidden: whether out_dhidden will be asked for (0 or 1) */
+int fl_head_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t vocab, int32_t dhidden, size_t* out_bytes);
+
 /* Thread-local description of the last error returned on this thread. */
 const char* fl_last_error(void);
 

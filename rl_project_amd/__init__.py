@@ -21,6 +21,8 @@ token_logprobs_from_logits, entropy_from_logits, kl_full_distribution, row_stats
 score_tokens, score_tokens_backward
     Log-probabilities of given tokens with entropy, rank and top alternatives, and
     the logits' gradient (models/policy.py, training/common/logprobs.py).
+lm_head_logprobs, lm_head_logprobs_backward
+    The same from hidden states and the lm_head weight, without the [N, V] logits.
 layer_norm, layer_norm_backward
     The norm in front of the head, with its gradients.
 SamplingParams
@@ -36,6 +38,7 @@ from .logprobs import RowStats, entropy_from_logits, kl_full_distribution, row_s
 from .norm import NormStats, layer_norm, layer_norm_backward
 from .scores import TokenScores, score_tokens, score_tokens_backward
 from .lmhead import LmHeadOutput, LmHeadPlan, lm_head_sample
+from .headlp import HeadScores, lm_head_logprobs, lm_head_logprobs_backward
 
 __all__ = [
     "apply_sampling_filters", "sample_from_logits", "generate_tokens",
@@ -44,5 +47,6 @@ __all__ = [
     "BatchedSampler", "row_stats", "RowStats", "token_logprobs_from_logits", "entropy_from_logits", "kl_full_distribution",
     "SamplingParams", "GenerationSettings", "SamplingParamsError",
     "score_tokens", "score_tokens_backward", "TokenScores", "layer_norm", "layer_norm_backward", "NormStats",
+    "lm_head_logprobs", "lm_head_logprobs_backward", "HeadScores",
     "lm_head_sample", "LmHeadPlan", "LmHeadOutput",
 ]

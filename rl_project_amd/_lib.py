@@ -136,6 +136,27 @@ class NormGradArgs(ctypes.Structure):
     ]
 
 
+class HeadArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32),
+        ("hidden", _p), ("weight", _p), ("rows", ctypes.c_int64), ("dim", ctypes.c_int64), ("vocab", ctypes.c_int64),
+        ("ld_hidden", ctypes.c_int64), ("tokens", _p), ("ignore_index", ctypes.c_int64),
+        ("out_logprob", _p), ("out_entropy", _p), ("out_lse", _p), ("out_saved", _p),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+class HeadGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32),
+        ("hidden", _p), ("weight", _p), ("rows", ctypes.c_int64), ("dim", ctypes.c_int64), ("vocab", ctypes.c_int64),
+        ("ld_hidden", ctypes.c_int64), ("tokens", _p), ("ignore_index", ctypes.c_int64), ("saved", _p),
+        ("grad_logprob", _p), ("grad_entropy", _p), ("grad_lse", _p), ("out_dhidden", _p), ("out_dweight", _p),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+FL_HEAD_MAX_ROWS = 131072
 FL_NORM_MAX_DIM = 16384
 FL_SCORE_MAX_TOPK = 64
 FL_LM_HEAD_MAX_BATCH = 64
@@ -212,6 +233,15 @@ def lib() -> ctypes.CDLL:
     handle.fl_layer_norm_grad_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
                                                           ctypes.POINTER(ctypes.c_size_t)]
     handle.fl_layer_norm_grad_workspace_bytes.restype = ctypes.c_int
+    handle.fl_head_logprobs.argtypes = [ctypes.POINTER(HeadArgs), _p]
+    handle.fl_head_logprobs.restype = ctypes.c_int
+    handle.fl_head_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)]
+    handle.fl_head_workspace_bytes.restype = ctypes.c_int
+    handle.fl_head_logprobs_grad.argtypes = [ctypes.POINTER(HeadGradArgs), _p]
+    handle.fl_head_logprobs_grad.restype = ctypes.c_int
+    handle.fl_head_grad_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
+                                                    ctypes.POINTER(ctypes.c_size_t)]
+    handle.fl_head_grad_workspace_bytes.restype = ctypes.c_int
     _lib = handle
     return handle
 
@@ -239,10 +269,14 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def call(fn, args: ctypes.Structure, device: torch.device, what: str) -> None:
     """fn(args) on the device's current stream; the device is made the current
     one for the launch if another is."""
-    if device.index is None or torch.cuda.current_device() == device.index:
+    index = device.index
+    if index is None or _current_device() == index:
         rc = fn(ctypes.byref(args), stream_handle(device))
     else:
         with torch.cuda.device(device):
@@ -255,4 +289,5 @@ EXPORTED_SYMBOLS = ("fl_sample", "fl_sample_exact", "fl_fill_rows", "fl_apply_fi
                     "fl_spec_workspace_bytes", "fl_spec_cache_workspace_bytes", "fl_lm_head_sample", "fl_lm_head_workspace_bytes", "fl_row_stats",
                     "fl_score_tokens", "fl_score_workspace_bytes", "fl_score_tokens_grad",
                     "fl_layer_norm", "fl_layer_norm_grad", "fl_layer_norm_grad_workspace_bytes",
+                    "fl_head_logprobs", "fl_head_workspace_bytes", "fl_head_logprobs_grad", "fl_head_grad_workspace_bytes",
                     "fl_last_error", "fl_abi_version")

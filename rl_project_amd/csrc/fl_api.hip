@@ -60,6 +60,31 @@ int validate_norm(const char* fn, int32_t dtype, int32_t wdtype, int64_t rows, i
   return 0;
 }
 
+// The head calls; 0 = go on.
+int validate_head(const char* fn, int32_t dtype, int64_t rows, int64_t dim, int64_t vocab, int64_t ld) {
+  if (dtype != FL_DTYPE_BF16) return fail(FL_ENOTSUP, "%s: dtype %d (bf16 only)", fn, dtype);
+  if (rows < 0 || vocab < 1 || dim < 64 || dim % 64 != 0 || ld < dim || ld % 8 != 0)
+    return fail(FL_EINVAL, "%s: bad shape rows=%lld dim=%lld vocab=%lld ld_hidden=%lld (dim a multiple of 64, ld_hidden of 8)",
+                fn, static_cast<long long>(rows), static_cast<long long>(dim), static_cast<long long>(vocab),
+                static_cast<long long>(ld));
+  // (the kernels address a tile's rows, at most 256 of hidden or 64, with 31-bit byte offsets)
+  if (rows > FL_HEAD_MAX_ROWS || vocab > FL_MAX_VOCAB_16 || dim > 16384 || ld > (1 << 21))
+    return fail(FL_ENOTSUP, "%s: rows %lld, vocab %lld, dim %lld or ld_hidden %lld beyond the library's limits", fn,
+                static_cast<long long>(rows), static_cast<long long>(vocab), static_cast<long long>(dim),
+                static_cast<long long>(ld));
+  return 0;
+}
+int validate_head_pointers(const char* fn, const void* hidden, const void* weight, const void* ws, int64_t ws_bytes,
+                           size_t need) {
+  if (!hidden || !weight) return fail(FL_EINVAL, "%s: hidden or weight is NULL", fn);
+  if (((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight)) & 15u) != 0)
+    return fail(FL_EINVAL, "%s: hidden and weight must be 16-byte aligned", fn);
+  if (ws == nullptr || ws_bytes < 0 || static_cast<size_t>(ws_bytes) < need)
+    return fail(FL_EINVAL, "%s: workspace of %lld bytes, %zu needed", fn, static_cast<long long>(ws_bytes), need);
+  if ((reinterpret_cast<uintptr_t>(ws) & 255u) != 0) return fail(FL_EINVAL, "%s: workspace not 256-byte aligned", fn);
+  return 0;
+}
+
 int validate_sample(const fl_sample_args* a, const char* fn) {
   if (a == nullptr) return fail(FL_EINVAL, "%s: args is NULL", fn);
   if (a->struct_size != sizeof(fl_sample_args))
@@ -362,6 +387,50 @@ int fl_layer_norm_grad(const fl_norm_grad_args* a, void* stream) {
       return fail(FL_EINVAL, "%s: workspace not 16-byte aligned", fn);
   }
   return check_launch(fl::launch_norm_grad(*a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int fl_head_workspace_bytes(int64_t rows, int64_t vocab, size_t* out_bytes) {
+  const char* fn = "fl_head_workspace_bytes";
+  if (out_bytes == nullptr) return fail(FL_EINVAL, "%s: out_bytes is NULL", fn);
+  if (const int rc = validate_head(fn, FL_DTYPE_BF16, rows, 64, vocab, 64)) return rc;
+  *out_bytes = fl::head_workspace_bytes(rows, vocab);
+  return ok();
+}
+
+int fl_head_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t vocab, int32_t dhidden, size_t* out_bytes) {
+  const char* fn = "fl_head_grad_workspace_bytes";
+  if (out_bytes == nullptr) return fail(FL_EINVAL, "%s: out_bytes is NULL", fn);
+  if (const int rc = validate_head(fn, FL_DTYPE_BF16, rows, dim, vocab, dim)) return rc;
+  *out_bytes = fl::head_grad_workspace_bytes(rows, dim, vocab, dhidden != 0);
+  return ok();
+}
+
+int fl_head_logprobs(const fl_head_args* a, void* stream) {
+  const char* fn = "fl_head_logprobs";
+  if (a == nullptr) return fail(FL_EINVAL, "%s: args is NULL", fn);
+  if (a->struct_size != sizeof(fl_head_args)) return fail(FL_EINVAL, "%s: struct_size mismatch", fn);
+  if (const int rc = validate_head(fn, a->dtype, a->rows, a->dim, a->vocab, a->ld_hidden)) return rc;
+  if (a->out_logprob && !a->tokens) return fail(FL_EINVAL, "%s: out_logprob needs tokens", fn);
+  if (a->rows == 0) return ok();
+  if (const int rc = validate_head_pointers(fn, a->hidden, a->weight, a->workspace, a->workspace_bytes,
+                                            fl::head_workspace_bytes(a->rows, a->vocab))) return rc;
+  return check_launch(fl::launch_head(*a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int fl_head_logprobs_grad(const fl_head_grad_args* a, void* stream) {
+  const char* fn = "fl_head_logprobs_grad";
+  if (a == nullptr) return fail(FL_EINVAL, "%s: args is NULL", fn);
+  if (a->struct_size != sizeof(fl_head_grad_args)) return fail(FL_EINVAL, "%s: struct_size mismatch", fn);
+  if (const int rc = validate_head(fn, a->dtype, a->rows, a->dim, a->vocab, a->ld_hidden)) return rc;
+  if (a->grad_logprob && !a->tokens) return fail(FL_EINVAL, "%s: grad_logprob needs tokens", fn);
+  if (a->rows == 0 || (!a->out_dhidden && !a->out_dweight)) return ok();
+  if (!a->saved) return fail(FL_EINVAL, "%s: saved is NULL", fn);
+  if (const int rc = validate_head_pointers(fn, a->hidden, a->weight, a->workspace, a->workspace_bytes,
+                                            fl::head_grad_workspace_bytes(a->rows, a->dim, a->vocab, a->out_dhidden != nullptr)))
+    return rc;
+  if (((reinterpret_cast<uintptr_t>(a->out_dhidden) | reinterpret_cast<uintptr_t>(a->out_dweight)) & 7u) != 0)
+    return fail(FL_EINVAL, "%s: out_dhidden and out_dweight must be 8-byte aligned", fn);
+  return check_launch(fl::launch_head_grad(*a, static_cast<hipStream_t>(stream)), fn);
 }
 
 }  // extern "C"

@@ -1,0 +1,656 @@
+// Log-probabilities, entropy and log-sum-exp of given tokens from hidden states
+// and the lm_head weight, and their gradients, without the [rows, vocab] logits
+// in memory.  With logits x[n, v] = sum_d hidden[n, d] weight[v, d] (float32
+// accumulators, never rounded to 16 bits) and p = softmax(x[n, :]):
+//
+//   forward   per row the running (max, sum e, sum e (x - max)) of each 128
+//             vocabulary rows from the product's registers, joined per row;
+//   backward  g[n, v] = a (1[v = t] - p) - b p (log p + H) + c p for upstream
+//             a, b, c of logprob, entropy, lse; then
+//             dhidden[n, d] = sum_v g[n, v] weight[v, d],
+//             dweight[v, d] = sum_n g[n, v] hidden[n, d].
+//
+// Four products of one main loop.  The gradient g of a chunk of the vocabulary
+// is written once, in bfloat16 (a rounding of at most 2^-8 relative, independent from
+// entry to entry: a sum of many terms moves by as much relative to its terms'
+// norm, as rounding the result does), the largest chunk that a bounded workspace
+// holds; each product then reads it as its matrix operand.
+#include <algorithm>
+#include <type_traits>
+
+#include "fl_device.h"
+#include "fl_kernels.h"
+
+namespace fl {
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef int int32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float HL_LOG2E = 1.44269504088896340736f;
+
+// ---------------------------------------------------------------- main loop
+// A work-group of 8 waves computes out[j, i] = sum_k A(i, k) B(j, k) for HL_I =
+// 256 values of i and BJ of j, with v_mfma_f32_32x32x16_bf16: lane l holds
+// column j = l % 32 of a 32 x 32 block and its rows i = 8 (r / 4) + 4 (l / 32) +
+// r % 4, r = 0 .. 15, so that a lane's four consecutive results lie side by
+// side along i.  Each operand lies in memory either with k contiguous
+// ("rows": A(i, k) = p[i * ld + k]) or with i (j) contiguous ("cols":
+// p[k * ld + i]).
+//
+// A stage is 64 k of both tiles, loaded straight into LDS (16 bytes a lane) NST -
+// 1 stages ahead.  LDS holds 16-byte granules with an exclusive-or of the row in
+// their place, applied to the address each lane loads from, so that the fragment
+// reads spread over all banks:
+//   rows: granule g (of 8) of row r at r 8 + (g ^ ((r >> 1) & 7)); a lane's 8
+//         k of a 32 x 16 fragment are one ds_read_b128;
+//   cols: granule g (of BJ / 8) of k-row k at k BJ / 8 + (g ^ (4 (k & 3))); a
+//         16-lane group's ds_read_b64_tr_b16 takes 4 k-rows of 16 columns and
+//         leaves each lane 4 k of its column.
+constexpr int HL_I = 256, HL_K = 64, HL_NT = 512, HL_NW = HL_NT / WAVE;
+
+// One operand: a tile's first element, and what may be read from it.
+struct Operand {
+  const uint16_t* p;   // rows: element (row 0 of the tile, k 0); cols: (k 0, column 0)
+  int64_t ld;          // elements
+  int rows;            // rows of the tile that exist (rows), k-rows left (cols)
+  int width;           // rows: k; cols: columns left from column 0
+};
+
+__device__ __forceinline__ int32x4 hl_rsrc(const void* p, uint32_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  int32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(a));
+  r[1] = __builtin_amdgcn_readfirstlane(static_cast<int>(a >> 32) & 0xFFFF);
+  r[2] = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes));
+  r[3] = 0x00020000;
+  return r;
+}
+
+// 16 bytes per lane from r (voff bytes per lane, soff) to LDS at lds + 16 lane.
+// No register is written (m0, which the compiler sets before each use of its own,
+// apart); completion is counted in vmcnt.  m0 is read a wait state after it is set.
+__device__ __forceinline__ void hl_load_lds(int32x4 r, uint32_t voff, uint32_t soff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(lds), "v"(voff), "s"(r), "s"(soff)
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void hl_wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+// bytes from the first element to the end of what may be read (below 2^31:
+// checked by the host for every shape)
+__device__ __forceinline__ uint32_t hl_bytes(int64_t rows, int64_t ld, int64_t width) {
+  return rows <= 0 || width <= 0 ? 0u : static_cast<uint32_t>(2 * ((rows - 1) * ld + width));
+}
+
+// COLS: the layout; T: rows i (j) of the tile
+template <bool COLS, int T>
+struct Loader {
+  static constexpr int LOADS = T * HL_K * 2 / (HL_NT * 16);   // per thread and stage
+  static_assert(LOADS >= 1 && T * HL_K * 2 % (HL_NT * 16) == 0, "whole loads");
+  static constexpr int BYTES = T * HL_K * 2;
+  Operand o;
+  uint32_t voff[LOADS];
+
+  __device__ __forceinline__ void init(const Operand& op) {
+    o = op;
+    const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
+#pragma unroll
+    for (int p = 0; p < LOADS; ++p) {
+      const int q = p * HL_NW + w;   // 1 KiB piece of the tile
+      if constexpr (!COLS) {
+        const int row = q * 8 + (lane >> 3), g = (lane & 7) ^ ((row >> 1) & 7);
+        // (a row that does not exist lies past the range, whatever ld is)
+        voff[p] = row < o.rows ? static_cast<uint32_t>(2 * (row * o.ld + 8 * g)) : 0x80000000u;
+      } else {
+        constexpr int GR = T / 8;                  // granules of a k-row
+        const int k = q * (WAVE / GR) + lane / GR, g = (lane % GR) ^ (4 * (k & 3));
+        voff[p] = static_cast<uint32_t>(2 * (k * o.ld + 8 * g));
+      }
+    }
+  }
+  // stage s into LDS at lds (wave-uniform)
+  __device__ __forceinline__ void load(int s, uint32_t lds) const {
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    if constexpr (!COLS) {
+      const int32x4 r = hl_rsrc(o.p, hl_bytes(o.rows, o.ld, o.width));
+#pragma unroll
+      for (int p = 0; p < LOADS; ++p) hl_load_lds(r, voff[p], static_cast<uint32_t>(2 * HL_K * s), lds + 1024 * (p * HL_NW + w));
+    } else {
+      const int64_t k0 = static_cast<int64_t>(s) * HL_K;
+      const int64_t left = o.rows - k0;
+      const int32x4 r = hl_rsrc(o.p + k0 * o.ld, hl_bytes(left < HL_K ? left : HL_K, o.ld, o.width));
+#pragma unroll
+      for (int p = 0; p < LOADS; ++p) hl_load_lds(r, voff[p], 0u, lds + 1024 * (p * HL_NW + w));
+    }
+  }
+};
+
+// The fragments of 32 rows i0 + 32 f .. of a tile in LDS, 16 k from 16 ks.
+template <bool COLS, int T, int F>
+struct Reader {
+  uint32_t at[COLS ? F : 4];
+  __device__ __forceinline__ void init(int i0) {
+    const int lane = threadIdx.x & (WAVE - 1);
+    if constexpr (!COLS) {
+      const int row = i0 + (lane & 31);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) at[ks] = 16 * (row * 8 + ((2 * ks + (lane >> 5)) ^ ((row >> 1) & 7)));
+    } else {
+      const int j = lane & 15, g = lane >> 4;
+      const int k = 8 * (g >> 1) + (j >> 2);
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        const int col = i0 + 32 * f + 16 * (g & 1) + 4 * (j & 3);
+        at[f] = 16 * (k * (T / 8) + ((col >> 3) ^ (4 * (k & 3)))) + 2 * (col & 7);
+      }
+    }
+  }
+  __device__ __forceinline__ bf16x8 read(const char* tile, int f, int ks) const {
+    if constexpr (!COLS) {
+      return *reinterpret_cast<const bf16x8*>(tile + at[ks] + f * 32 * 128);
+    } else {
+      typedef __attribute__((address_space(3))) short4v* lds4;
+      const char* p = tile + at[f] + ks * 16 * T * 2;
+      const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p));
+      const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * T * 2));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+// Wave grid WI x WJ of FI x FJ blocks of 32 x 32 per wave; NST stages in LDS.
+template <int BJ>
+struct Shape {
+  static constexpr int WJ = BJ / 64, WI = HL_NW / WJ, FI = HL_I / (32 * WI), FJ = 2;
+  static constexpr int STAGE = (HL_I + BJ) * HL_K * 2;
+  static constexpr int NST = BJ == 256 ? 2 : 3;
+  static_assert(NST * STAGE <= 160 * 1024, "LDS");
+};
+
+template <bool ACOLS, bool BCOLS, int BJ>
+__device__ __forceinline__ void hl_product(const Operand& A, const Operand& B, int stages, char* smem,
+                                           floatx16 (&acc)[Shape<BJ>::FI][Shape<BJ>::FJ]) {
+  using S = Shape<BJ>;
+  constexpr int NST = S::NST;
+  Loader<ACOLS, HL_I> la;
+  Loader<BCOLS, BJ> lb;
+  la.init(A);
+  lb.init(B);
+  constexpr int L = Loader<ACOLS, HL_I>::LOADS + Loader<BCOLS, BJ>::LOADS;
+  const int w = threadIdx.x / WAVE;
+  Reader<ACOLS, HL_I, S::FI> ra;
+  Reader<BCOLS, BJ, S::FJ> rb;
+  ra.init((w / S::WJ) * 32 * S::FI);
+  rb.init((w % S::WJ) * 32 * S::FJ);
+  const uint32_t lds = static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(smem)));
+#pragma unroll
+  for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+    for (int j = 0; j < S::FJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+  auto load = [&](int s, int buf) {
+    la.load(s, lds + buf * S::STAGE);
+    lb.load(s, lds + buf * S::STAGE + Loader<ACOLS, HL_I>::BYTES);
+  };
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s)
+    if (s < stages) load(s, s);
+  int buf = 0;
+#pragma unroll 1
+  for (int s = 0; s < stages; ++s) {
+    // stage s has landed for this wave (NST - 2 later ones may be in flight),
+    // then for all, and all have read stage s - 1, whose buffer is loaded next
+    if (NST > 2 && s + NST - 2 < stages) hl_wait_vm<L*(NST - 2)>();
+    else hl_wait_vm<0>();
+    lds_barrier();
+    if (s + NST - 1 < stages) load(s + NST - 1, buf == 0 ? NST - 1 : buf - 1);
+    const char* ta = smem + buf * S::STAGE;
+    const char* tb = ta + Loader<ACOLS, HL_I>::BYTES;
+#pragma unroll
+    for (int ks = 0; ks < HL_K / 16; ++ks) {
+      bf16x8 a[S::FI], b[S::FJ];
+#pragma unroll
+      for (int i = 0; i < S::FI; ++i) a[i] = ra.read(ta, i, ks);
+#pragma unroll
+      for (int j = 0; j < S::FJ; ++j) b[j] = rb.read(tb, j, ks);
+#pragma unroll
+      for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+    }
+    buf = buf == NST - 1 ? 0 : buf + 1;
+  }
+}
+
+// Tile of a work-group: each of the 8 XCDs (work-groups go round them) takes a
+// contiguous range of an order in which 8 j-tiles share each i-tile, so that the
+// work-groups of an XCD read the same few rows through its L2.
+struct TileIdx {
+  int i, j;
+};
+__device__ __forceinline__ TileIdx hl_tile(int b, int ni, int nj) {
+  const int n = ni * nj, x = b % 8, q = b / 8;
+  // XCD x has n / 8 tiles, the first n % 8 of them one more
+  const int t = x * (n / 8) + min(x, n % 8) + q;
+  const int per = 8 * ni, grp = t / per, in = t - grp * per;
+  const int gj = min(8, nj - 8 * grp);
+  return {in / gj, 8 * grp + in % gj};
+}
+
+// ---------------------------------------------------------------- forward
+struct HlArgs {
+  const uint16_t* hidden;   // [rows, dim], ld
+  const uint16_t* weight;   // [vocab, dim]
+  int64_t ld;
+  int rows, dim, vocab;
+  const int64_t* tokens;
+  int64_t ignore_index;
+};
+
+}  // namespace
+
+// part[(2 vocabulary tile + half) rows + n] (for BJ < 256: (waves along i) parts
+// a tile): max, sum e, sum e d2 of the wave's vocabulary rows
+template <int BJ>
+__global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_head_stats(const HlArgs a, float4* part,
+                                                                                               float* xt, int ni, int nj) {
+  using S = Shape<BJ>;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const TileIdx t = hl_tile(blockIdx.x, ni, nj);
+  const int v0 = t.i * HL_I, n0 = t.j * BJ;
+  floatx16 acc[S::FI][S::FJ];
+  hl_product<false, false, BJ>({a.weight + static_cast<int64_t>(v0) * a.dim, a.dim, min(HL_I, a.vocab - v0), a.dim},
+                               {a.hidden + n0 * a.ld, a.ld, min(BJ, a.rows - n0), a.dim}, a.dim / HL_K, smem, acc);
+  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
+  const int wi = w / S::WJ, wj = w % S::WJ;
+  const int vw = v0 + wi * 32 * S::FI + 4 * (lane >> 5);   // the lane's first vocabulary row
+  constexpr float NINF = -__builtin_inff();
+  if (v0 + HL_I > a.vocab) {
+#pragma unroll
+    for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (vw + 32 * i + 8 * (r / 4) + r % 4 >= a.vocab) {
+#pragma unroll
+          for (int j = 0; j < S::FJ; ++j) acc[i][j][r] = NINF;
+        }
+  }
+#pragma unroll
+  for (int j = 0; j < S::FJ; ++j) {
+    const int n = n0 + wj * 32 * S::FJ + 32 * j + (lane & 31);
+    float m = NINF;
+#pragma unroll
+    for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+    m = fmaxf(m, __shfl_xor(m, 32, WAVE));
+    const float ref = m == NINF ? 0.0f : m;
+    float s[2] = {0.0f, 0.0f}, u[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float d2 = (acc[i][j][r] - ref) * HL_LOG2E;
+        const float e = __builtin_amdgcn_exp2f(d2);
+        s[r & 1] += e;
+        u[r & 1] = fmaf(e, fmaxf(d2, -200.0f), u[r & 1]);   // (e is 0 there)
+      }
+    float ss = s[0] + s[1], uu = u[0] + u[1];
+    ss += __shfl_xor(ss, 32, WAVE);
+    uu += __shfl_xor(uu, 32, WAVE);
+    if (n >= a.rows) continue;
+    if (lane < 32) part[static_cast<int64_t>(t.i * S::WI + wi) * a.rows + n] = make_float4(m, ss, uu, 0.0f);
+    // the token's logit, by the lane that has it
+    const int64_t tk = a.tokens ? a.tokens[n] : -1;
+    const int64_t d = tk - vw;
+    if (tk >= 0 && tk < a.vocab && d >= 0 && d < 32 * S::FI) {
+#pragma unroll
+      for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (d == 32 * i + 8 * (r / 4) + r % 4) xt[n] = acc[i][j][r];
+    }
+  }
+}
+
+// The parts of each row joined: 64 rows per work-group, a wave per 16th of the
+// parts, in float64 and in a fixed order.
+constexpr int HJ_W = 16;
+__global__ __launch_bounds__(HJ_W * WAVE) void k_head_join(const fl_head_args a, const float4* part, const float* xt,
+                                                           int parts) {
+  __shared__ double sm[3][HJ_W][WAVE];
+  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * WAVE + lane;
+  const float ninf = -__builtin_inff();
+  float m = ninf;
+  double s = 0.0, u = 0.0;
+  auto merge = [&](float pm, double ps, double pu) {
+    // (u in base 2 relative to its own maximum)
+    if (!(pm <= m)) {   // a larger maximum, or NaN
+      const float d = (m - pm) * HL_LOG2E;
+      const double f = m == ninf ? 0.0 : exp2(static_cast<double>(d));
+      u = (u + (m == ninf ? 0.0 : s * static_cast<double>(fmaxf(d, -1e30f)))) * f + pu;
+      s = s * f + ps;
+      m = pm;
+    } else if (pm != ninf) {
+      const float d = (pm - m) * HL_LOG2E;
+      const double f = exp2(static_cast<double>(d));
+      u += (pu + ps * static_cast<double>(fmaxf(d, -1e30f))) * f;
+      s += ps * f;
+    } else {
+      s += ps;   // (NaN values among -inf)
+    }
+  };
+  if (n < a.rows)
+    for (int p = w; p < parts; p += HJ_W) {
+      const float4 q = part[static_cast<int64_t>(p) * a.rows + n];
+      merge(q.x, q.y, q.z);
+    }
+  sm[0][w][lane] = m;
+  sm[1][w][lane] = s;
+  sm[2][w][lane] = u;
+  __syncthreads();
+  if (w != 0 || n >= a.rows) return;
+  for (int q = 1; q < HJ_W; ++q) merge(static_cast<float>(sm[0][q][lane]), sm[1][q][lane], sm[2][q][lane]);
+  const float nan = __builtin_nanf("");
+  const bool okr = s > 0.0 && s < static_cast<double>(__builtin_inff());
+  const double logs = log(s), ref = static_cast<double>(m);
+  const float ent = okr ? static_cast<float>(logs - u / s / static_cast<double>(HL_LOG2E)) : nan;
+  if (a.out_entropy) a.out_entropy[n] = ent;
+  if (a.out_lse) a.out_lse[n] = okr ? static_cast<float>(ref + logs) : nan;
+  if (a.tokens && a.out_logprob) {
+    const int64_t t = a.tokens[n];
+    const bool bad = t < 0 || t >= a.vocab || !okr;
+    a.out_logprob[n] = t == a.ignore_index ? -0.0f : bad ? nan : static_cast<float>((static_cast<double>(xt[n]) - ref) - logs);
+  }
+  if (a.out_saved) {   // as fl_score_tokens
+    float* sv = a.out_saved + 4 * n;
+    sv[0] = okr ? m : nan;
+    sv[1] = okr ? static_cast<float>(logs) : nan;
+    sv[2] = a.out_entropy ? ent : 0.0f;
+    sv[3] = 0.0f;
+  }
+}
+
+// ---------------------------------------------------------------- backward
+namespace {
+struct HlGrad {
+  const float* saved;
+  const float *ga, *gb, *gc;   // upstream of logprob, entropy, lse (NULL: 0)
+};
+}  // namespace
+
+// g of the vocabulary rows c0 .. c0 + cn - 1 (cn a multiple of 64; those past
+// the vocabulary 0), bfloat16 [rows, cn]
+template <int BJ>
+__global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_head_g(const HlArgs a, const HlGrad gr,
+                                                                                           uint16_t* g, int c0, int cn, int ni,
+                                                                                           int nj) {
+  using S = Shape<BJ>;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const TileIdx t = hl_tile(blockIdx.x, ni, nj);
+  const int v0 = c0 + t.i * HL_I, n0 = t.j * BJ;
+  floatx16 acc[S::FI][S::FJ];
+  hl_product<false, false, BJ>({a.weight + static_cast<int64_t>(v0) * a.dim, a.dim, min(HL_I, a.vocab - v0), a.dim},
+                               {a.hidden + n0 * a.ld, a.ld, min(BJ, a.rows - n0), a.dim}, a.dim / HL_K, smem, acc);
+  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
+  const int wi = w / S::WJ, wj = w % S::WJ;
+  const int vw = v0 + wi * 32 * S::FI + 4 * (lane >> 5);
+#pragma unroll
+  for (int j = 0; j < S::FJ; ++j) {
+    const int n = n0 + wj * 32 * S::FJ + 32 * j + (lane & 31);
+    if (n >= a.rows) continue;
+    const float hi = gr.saved[4 * n], lo = gr.saved[4 * n + 1], H = gr.saved[4 * n + 2];
+    const float gb = gr.gb ? gr.gb[n] : 0.0f, gc = gr.gc ? gr.gc[n] : 0.0f;
+    float ga = gr.ga ? gr.ga[n] : 0.0f;
+    int d = -1;   // the token's place from the lane's first row
+    if (a.tokens) {
+      const int64_t tk = a.tokens[n];
+      if (tk == a.ignore_index) ga = 0.0f;
+      else if (tk < 0 || tk >= a.vocab) ga = ga == 0.0f ? 0.0f : __builtin_nanf("");
+      else d = static_cast<int>(tk) - vw;
+    }
+    const bool zero = ga == 0.0f && gb == 0.0f && gc == 0.0f;
+    const float k0 = gc - ga, h = gb == 0.0f ? 0.0f : H;
+    uint16_t* out = g + static_cast<int64_t>(n) * cn + (vw - c0);
+#pragma unroll
+    for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int at = 32 * i + 8 * q;
+        if (vw - c0 + at >= cn) continue;   // (cn is a multiple of 64: whole fours)
+        uint16_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float l = (acc[i][j][4 * q + e] - hi) - lo;
+          const float p = __builtin_amdgcn_exp2f(l * HL_LOG2E);
+          float v = p * (k0 - gb * (fmaxf(l, -200.0f) + h));
+          if (at + e == d) v += ga;
+          o[e] = zero || vw + at + e >= a.vocab ? 0 : static_cast<uint16_t>(BF16::from_f32(v));
+        }
+        *reinterpret_cast<uint2*>(out + at) =
+            make_uint2(o[0] | (static_cast<uint32_t>(o[1]) << 16), o[2] | (static_cast<uint32_t>(o[3]) << 16));
+      }
+  }
+}
+
+// dweight[c0 + v, d] = sum_n g[n, v] hidden[n, d]: i = d, j = v
+__global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_head_dw(const HlArgs a, const uint16_t* g,
+                                                                                            uint16_t* dw, int c0, int cn, int ni,
+                                                                                            int nj) {
+  constexpr int BJ = 256;
+  using S = Shape<BJ>;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const TileIdx t = hl_tile(blockIdx.x, ni, nj);
+  const int d0 = t.i * HL_I, j0 = t.j * BJ;
+  floatx16 acc[S::FI][S::FJ];
+  hl_product<true, true, BJ>({a.hidden + d0, a.ld, a.rows, a.dim - d0}, {g + j0, cn, a.rows, cn - j0},
+                             (a.rows + HL_K - 1) / HL_K, smem, acc);
+  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
+  const int d = d0 + (w / S::WJ) * 32 * S::FI + 4 * (lane >> 5);
+#pragma unroll
+  for (int j = 0; j < S::FJ; ++j) {
+    const int v = c0 + j0 + (w % S::WJ) * 32 * S::FJ + 32 * j + (lane & 31);
+    if (v >= a.vocab || v >= c0 + cn) continue;
+    uint16_t* out = dw + static_cast<int64_t>(v) * a.dim + d;
+#pragma unroll
+    for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (d + 32 * i + 8 * q >= a.dim) continue;   // (dim is a multiple of 64)
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = BF16::from_f32(acc[i][j][4 * q + e]);
+        *reinterpret_cast<uint2*>(out + 32 * i + 8 * q) = make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
+      }
+  }
+}
+
+// dhidden's part z: sum over the z-th of `splits` ranges of the chunk's
+// vocabulary rows of g[n, v] weight[c0 + v, d]: i = d, j = n.  first: the part is
+// written, else added to.
+__global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_head_dh(const HlArgs a, const uint16_t* g,
+                                                                                            float* acc_out, int c0, int cn,
+                                                                                            int ni, int nj, int per, int first) {
+  constexpr int BJ = 256;
+  using S = Shape<BJ>;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const TileIdx t = hl_tile(blockIdx.x, ni, nj);
+  const int d0 = t.i * HL_I, n0 = t.j * BJ, z = blockIdx.y;
+  const int s0 = z * per, stages = max(0, min(cn / HL_K - s0, per));   // (cn is a multiple of 64)
+  const int k0 = s0 * HL_K;
+  floatx16 acc[S::FI][S::FJ];
+  hl_product<true, false, BJ>(
+      {a.weight + static_cast<int64_t>(c0 + k0) * a.dim + d0, a.dim, min(stages * HL_K, a.vocab - c0 - k0), a.dim - d0},
+      {g + static_cast<int64_t>(n0) * cn + k0, cn, min(BJ, a.rows - n0), stages * HL_K}, stages, smem, acc);
+  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
+  const int d = d0 + (w / S::WJ) * 32 * S::FI + 4 * (lane >> 5);
+#pragma unroll
+  for (int j = 0; j < S::FJ; ++j) {
+    const int n = n0 + (w % S::WJ) * 32 * S::FJ + 32 * j + (lane & 31);
+    if (n >= a.rows) continue;
+    float* out = acc_out + (static_cast<int64_t>(z) * a.rows + n) * a.dim + d;
+#pragma unroll
+    for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (d + 32 * i + 8 * q >= a.dim) continue;
+        float4* o = reinterpret_cast<float4*>(out + 32 * i + 8 * q);
+        float4 v = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+        if (!first) {
+          const float4 b = *o;
+          v = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
+        }
+        *o = v;
+      }
+  }
+}
+
+// dhidden = the parts' sum, rounded once; four values per thread
+__global__ __launch_bounds__(256) void k_head_dh_join(const float4* part, uint2* out, int64_t n4, int splits) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n4) return;
+  float4 v = part[i];
+  for (int z = 1; z < splits; ++z) {
+    const float4 b = part[z * n4 + i];
+    v = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
+  }
+  out[i] = make_uint2(BF16::from_f32(v.x) | (BF16::from_f32(v.y) << 16), BF16::from_f32(v.z) | (BF16::from_f32(v.w) << 16));
+}
+
+// ---------------------------------------------------------------- launches
+namespace {
+
+int cdiv(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
+size_t al(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+
+// j-tile of the products over rows: the rows' own size up to 128, so that a few
+// rows do not pay for 256
+int hl_bj(int64_t rows) { return rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+int hl_parts(int64_t rows, int64_t vocab) { return cdiv(vocab, HL_I) * (HL_NW / (hl_bj(rows) / 64)); }
+
+// Vocabulary rows of a backward chunk: g's bytes stay within HL_G_BYTES, but a
+// chunk has at least HL_CHUNK rows, so that the products of many rows have k
+// enough beside the sums they read and write.
+constexpr int64_t HL_G_BYTES = 512ll << 20, HL_CHUNK = 16384;
+int hl_chunk(int64_t rows, int64_t vocab) {
+  const int64_t fit = std::max<int64_t>(HL_CHUNK, HL_G_BYTES / (2 * std::max<int64_t>(rows, 1)) / HL_I * HL_I);
+  const int64_t all = (vocab + HL_K - 1) / HL_K * HL_K;
+  if (all <= fit) return static_cast<int>(all);
+  // chunks of about one size
+  const int64_t n = (all + fit - 1) / fit;
+  return static_cast<int>(std::min(all, ((all + n - 1) / n + HL_I - 1) / HL_I * HL_I));
+}
+// Ranges of a chunk's vocabulary rows that dhidden's product is split into: as
+// many as give every CU a tile, of 8 stages or more.
+constexpr int HL_CUS = 256;
+int hl_splits(int64_t rows, int64_t dim, int64_t chunk) {
+  const int64_t tiles = static_cast<int64_t>(cdiv(rows, 256)) * cdiv(dim, HL_I);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(HL_CUS / std::max<int64_t>(tiles, 1), chunk / HL_K / 8)));
+}
+
+HlArgs hl_args(const void* hidden, const void* weight, int64_t ld, int64_t rows, int64_t dim, int64_t vocab,
+               const int64_t* tokens, int64_t ignore_index) {
+  return {static_cast<const uint16_t*>(hidden), static_cast<const uint16_t*>(weight), ld, static_cast<int>(rows),
+          static_cast<int>(dim), static_cast<int>(vocab), tokens, ignore_index};
+}
+
+// f(BJ) for the rows' tile
+template <class F>
+void hl_by_rows(int64_t rows, F&& f) {
+  const int bj = hl_bj(rows);
+  if (bj == 64) f(std::integral_constant<int, 64>{});
+  else if (bj == 128) f(std::integral_constant<int, 128>{});
+  else f(std::integral_constant<int, 256>{});
+}
+
+template <int BJ>
+constexpr int hl_lds() {
+  return Shape<BJ>::NST * Shape<BJ>::STAGE;
+}
+// (above 64 KiB a kernel's dynamic LDS has to be asked for)
+template <class K>
+hipError_t hl_allow(K k, int bytes) {
+  return hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+}  // namespace
+
+size_t head_workspace_bytes(int64_t rows, int64_t vocab) {
+  const size_t R = static_cast<size_t>(rows);
+  return al(16 * R * static_cast<size_t>(hl_parts(rows, vocab))) + al(4 * R);
+}
+
+size_t head_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t vocab, bool dhidden) {
+  const int64_t cn = hl_chunk(rows, vocab);
+  const size_t R = static_cast<size_t>(rows);
+  return al(2 * R * static_cast<size_t>(cn)) +
+         (dhidden ? al(4 * R * static_cast<size_t>(dim) * static_cast<size_t>(hl_splits(rows, dim, cn))) : 0);
+}
+
+hipError_t launch_head(const fl_head_args& a, hipStream_t s) {
+  const HlArgs h = hl_args(a.hidden, a.weight, a.ld_hidden, a.rows, a.dim, a.vocab, a.tokens, a.ignore_index);
+  float4* part = static_cast<float4*>(a.workspace);
+  const int parts = hl_parts(a.rows, a.vocab);
+  float* xt = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + al(16 * static_cast<size_t>(a.rows) * parts));
+  hipError_t e = hipSuccess;
+  hl_by_rows(a.rows, [&](auto bj) {
+    constexpr int BJ = decltype(bj)::value;
+    const int ni = cdiv(a.vocab, HL_I), nj = cdiv(a.rows, BJ);
+    e = hl_allow(k_head_stats<BJ>, hl_lds<BJ>());
+    if (e == hipSuccess)
+      hipLaunchKernelGGL(k_head_stats<BJ>, dim3(static_cast<unsigned>(ni) * nj), dim3(HL_NT), hl_lds<BJ>(), s, h, part, xt, ni, nj);
+  });
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(k_head_join, dim3(cdiv(a.rows, WAVE)), dim3(HJ_W * WAVE), 0, s, a, part, xt, parts);
+  return hipGetLastError();
+}
+
+hipError_t launch_head_grad(const fl_head_grad_args& a, hipStream_t s) {
+  const HlArgs h = hl_args(a.hidden, a.weight, a.ld_hidden, a.rows, a.dim, a.vocab, a.tokens, a.ignore_index);
+  const HlGrad gr = {a.saved, a.grad_logprob, a.grad_entropy, a.grad_lse};
+  const int chunk = hl_chunk(a.rows, a.vocab), splits = hl_splits(a.rows, a.dim, chunk);
+  uint16_t* g = static_cast<uint16_t*>(a.workspace);
+  float* acc = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + al(2 * static_cast<size_t>(a.rows) * chunk));
+  const int nd = cdiv(a.dim, HL_I), nr = cdiv(a.rows, 256);
+  hipError_t e = hl_allow(k_head_dw, hl_lds<256>());
+  if (e == hipSuccess) e = hl_allow(k_head_dh, hl_lds<256>());
+  if (e != hipSuccess) return e;
+  for (int c0 = 0; c0 < a.vocab; c0 += chunk) {
+    const int cn = static_cast<int>(std::min<int64_t>(chunk, (a.vocab - c0 + HL_K - 1) / HL_K * HL_K));
+    const int nc = cdiv(cn, HL_I);
+    hl_by_rows(a.rows, [&](auto bj) {
+      constexpr int BJ = decltype(bj)::value;
+      const int nj = cdiv(a.rows, BJ);
+      e = hl_allow(k_head_g<BJ>, hl_lds<BJ>());
+      if (e == hipSuccess)
+        hipLaunchKernelGGL(k_head_g<BJ>, dim3(static_cast<unsigned>(nc) * nj), dim3(HL_NT), hl_lds<BJ>(), s, h, gr, g, c0, cn, nc, nj);
+    });
+    if (e != hipSuccess) return e;
+    if (a.out_dweight)
+      hipLaunchKernelGGL(k_head_dw, dim3(static_cast<unsigned>(nd) * nc), dim3(HL_NT), hl_lds<256>(), s, h, g,
+                         static_cast<uint16_t*>(a.out_dweight), c0, cn, nd, nc);
+    if (a.out_dhidden)
+      hipLaunchKernelGGL(k_head_dh, dim3(static_cast<unsigned>(nd) * nr, splits), dim3(HL_NT), hl_lds<256>(), s, h, g, acc, c0, cn,
+                         nd, nr, cdiv(cn / HL_K, splits), c0 == 0 ? 1 : 0);
+  }
+  if (a.out_dhidden) {
+    const int64_t n4 = a.rows * a.dim / 4;
+    hipLaunchKernelGGL(k_head_dh_join, dim3(static_cast<unsigned>(cdiv(n4, 256))), dim3(256), 0, s,
+                       reinterpret_cast<const float4*>(acc), static_cast<uint2*>(a.out_dhidden), n4, splits);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace fl

@@ -47,4 +47,10 @@ hipError_t launch_norm(const fl_norm_args& a, hipStream_t s);
 hipError_t launch_norm_grad(const fl_norm_grad_args& a, hipStream_t s);
 size_t norm_grad_workspace_bytes(int64_t rows, int64_t dim, int dtype);
 
+// Head log-probabilities and their gradients.
+hipError_t launch_head(const fl_head_args& a, hipStream_t s);
+size_t head_workspace_bytes(int64_t rows, int64_t vocab);
+hipError_t launch_head_grad(const fl_head_grad_args& a, hipStream_t s);
+size_t head_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t vocab, bool dhidden);
+
 }  // namespace fl

@@ -30,6 +30,7 @@ import torch
 
 from . import _lib
 from ._lib import LmHeadArgs, check, lib, ptr
+from .norm import layer_norm
 from .sampling import PerRow, _history_tensor, _per_row, _raise_on_status, sample_tokens
 
 
@@ -129,13 +130,24 @@ class LmHeadPlan:
         return LmHeadOutput(self.tokens, self.status, self.logprob, self.logits)
 
 
+def _normed(hidden: torch.Tensor, norm) -> torch.Tensor:
+    """``hidden`` after the model's final layer norm, ``norm = (weight, bias,
+    eps)`` (weight and bias may be None)."""
+    if norm is None:
+        return hidden
+    weight, bias, eps = norm
+    return layer_norm(hidden, weight, bias, eps)
+
+
 def lm_head_sample(hidden: torch.Tensor, weight: torch.Tensor, *, temperature: PerRow = 1.0, top_k: PerRow = 50,
                    top_p: PerRow = None, min_p: PerRow = None, repetition_penalty: PerRow = None, history=None,
                    softcap: float = 0.0, uniforms: Optional[torch.Tensor] = None,
                    generator: Optional[torch.Generator] = None, return_logprobs: bool = False,
                    return_logits: bool = False, check_status: bool = True,
-                   fused: Optional[bool] = None) -> LmHeadOutput:
+                   fused: Optional[bool] = None, norm=None) -> LmHeadOutput:
     """One decode step's ``lm_head`` and sampling (one token per row).
+    ``norm=(weight, bias, eps)`` applies ``layer_norm`` to the hidden states
+    first (the model's final norm).
 
     ``fused`` None picks the faster path for the shape (``fused_is_faster``):
     today always ``torch.nn.functional.linear`` followed by ``sample_tokens``,
@@ -144,6 +156,7 @@ def lm_head_sample(hidden: torch.Tensor, weight: torch.Tensor, *, temperature: P
     are sampled by ``fl_sample`` over the GEMM's logits, with the same
     uniforms, and batches above 64 rows run in groups of 64.  Any other row
     status raises ``SamplingError`` (unless ``check_status`` is off)."""
+    hidden = _normed(hidden, norm)
     B = hidden.size(0)
     if fused is None:
         fused = fused_is_faster(B, hidden.size(-1), weight.size(0))

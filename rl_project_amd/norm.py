@@ -4,6 +4,7 @@ uses it (``lm_head_sample`` and ``lm_head_logprobs`` take one as ``norm=``)."""
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -28,6 +29,8 @@ def _x_rows(x: torch.Tensor, name: str) -> torch.Tensor:
         raise NotImplementedError(f"{name} dtype {x.dtype} is not supported (float32, bfloat16, float16)")
     if x.dim() < 1 or x.size(-1) < 1:
         raise ValueError(f"{name} must have a last dimension of at least 1")
+    if x.dim() == 2 and x.is_contiguous():
+        return x
     x2 = x.reshape(-1, x.size(-1))
     if (x2.size(1) > 1 and x2.stride(1) != 1) or (x2.size(0) > 1 and x2.stride(0) < x2.size(1)):
         x2 = x2.contiguous()
@@ -76,16 +79,21 @@ class _LayerNorm(torch.autograd.Function):
         x2 = _x_rows(x.detach(), "x")
         w, b = _affine(weight, x, "weight"), _affine(bias, x, "bias")
         y, mean, rstd = _forward(x2, x.shape, w, b, eps, True)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        ctx.save_for_backward(x, weight)
+        # (mean and rstd are this node's own: no caller sees or changes them)
+        ctx.stats = (mean, rstd)
+        need = ctx.needs_input_grad
+        ctx.types = (weight.dtype if need[1] else None, bias.dtype if need[2] else None)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dw, db = layer_norm_backward(grad, x, weight, bias, NormStats(mean, rstd), need_dx=need[0],
-                                         need_dweight=need[1], need_dbias=need[2])
+        x, weight = ctx.saved_tensors
+        # (the engine has checked the gradient's shape, type and device)
+        dx, dw, db = _backward(_x_rows(grad, "grad"), _x_rows(x, "x"), x.shape,
+                               None if weight is None else weight.contiguous(), *ctx.types, *ctx.stats,
+                               ctx.needs_input_grad[0])
         return dx, dw, db, None
 
 
@@ -132,23 +140,40 @@ def layer_norm_backward(grad: torch.Tensor, x: torch.Tensor, weight: Optional[to
             if t.shape != (R,) or t.dtype != torch.float32 or t.device != dev or not t.is_contiguous():
                 raise ValueError(f"stats must be the forward call's: two float32 [{R}] tensors")
         w, b = _affine(weight, x, "weight"), _affine(bias, x, "bias")
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_dx else None
-        dw = torch.empty_like(w) if need_dweight and w is not None else None
-        db = torch.empty_like(b) if need_dbias and b is not None else None
-        a = NormGradArgs()
-        a.struct_size = ctypes.sizeof(NormGradArgs)
-        a.dtype, a.wdtype = _DTYPES[x2.dtype], _wdtype(x2, w, b)
-        a.x, a.rows, a.dim, a.ld = x2.data_ptr(), R, D, x2.stride(0) if R > 1 else D
-        a.weight, a.grad, a.grad_ld = ptr(w), g2.data_ptr(), g2.stride(0) if R > 1 else D
-        a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
-        a.out_dx, a.out_ld, a.out_dweight, a.out_dbias = ptr(dx), D, ptr(dw), ptr(db)
-        ws = None
-        if dw is not None or db is not None:
-            n = ctypes.c_size_t(0)
-            _lib.check(lib().fl_layer_norm_grad_workspace_bytes(R, D, a.dtype, ctypes.byref(n)),
-                       "fl_layer_norm_grad_workspace_bytes")
-            ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-            a.workspace, a.workspace_bytes = ptr(ws), n.value
-        if dx is not None or ws is not None:
-            call(lib().fl_layer_norm_grad, a, dev, "fl_layer_norm_grad")
-        return dx, dw, db
+        _wdtype(x2, w, b)
+        return _backward(g2, x2, x.shape, w, w.dtype if need_dweight and w is not None else None,
+                         b.dtype if need_dbias and b is not None else None, mean, rstd, need_dx)
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(rows: int, dim: int, dtype: int) -> int:
+    n = ctypes.c_size_t(0)
+    _lib.check(lib().fl_layer_norm_grad_workspace_bytes(rows, dim, dtype, ctypes.byref(n)),
+               "fl_layer_norm_grad_workspace_bytes")
+    return n.value
+
+
+def _backward(g2, x2, shape, w, dw_type, db_type, mean, rstd, need_dx: bool):
+    """The launches; dw_type, db_type: None where not asked for."""
+    R, D = x2.shape
+    dev = x2.device
+    dx = torch.empty(shape, dtype=x2.dtype, device=dev) if need_dx else None
+    dw = torch.empty(D, dtype=dw_type, device=dev) if dw_type is not None else None
+    db = torch.empty(D, dtype=db_type, device=dev) if db_type is not None else None
+    a = NormGradArgs()
+    a.struct_size = ctypes.sizeof(NormGradArgs)
+    a.dtype = _DTYPES[x2.dtype]
+    a.wdtype = _DTYPES[w.dtype if w is not None else db_type if db_type is not None else x2.dtype]
+    a.x, a.rows, a.dim, a.ld = x2.data_ptr(), R, D, x2.stride(0) if R > 1 else D
+    a.weight, a.grad, a.grad_ld = ptr(w), g2.data_ptr(), g2.stride(0) if R > 1 else D
+    a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
+    a.out_dx, a.out_ld, a.out_dweight, a.out_dbias = ptr(dx), D, ptr(dw), ptr(db)
+    L = lib()
+    ws = None
+    if dw is not None or db is not None:
+        n = _workspace_bytes(R, D, a.dtype)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    if dx is not None or ws is not None:
+        call(L.fl_layer_norm_grad, a, dev, "fl_layer_norm_grad")
+    return dx, dw, db

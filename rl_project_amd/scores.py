@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -69,6 +70,13 @@ def _check_range(tokens: torch.Tensor, vocab: int, ignore_index: int) -> None:
         raise IndexError(f"token {int(tokens[bad][0])} is out of bounds for {vocab} classes")
 
 
+@lru_cache(maxsize=256)
+def _workspace_bytes(rows: int, vocab: int, top_k: int) -> int:
+    n = ctypes.c_size_t(0)
+    _lib.check(lib().fl_score_workspace_bytes(rows, vocab, top_k, ctypes.byref(n)), "fl_score_workspace_bytes")
+    return n.value
+
+
 def _forward(x: torch.Tensor, lead, tok: Optional[torch.Tensor], top_k: int, entropy: bool, lse: bool, rank: bool,
              ignore_index: int, save: bool):
     """The launch; (logprob, entropy, lse, rank, top_ids, top_logprobs, saved)."""
@@ -93,10 +101,9 @@ def _forward(x: torch.Tensor, lead, tok: Optional[torch.Tensor], top_k: int, ent
     a.out_top_ids, a.out_top_logprobs, a.out_saved = ptr(o_ids), ptr(o_top), ptr(saved)
     ws = None
     if V > 16384 and R > 0:   # (rows of one slice need none)
-        n = ctypes.c_size_t(0)
-        _lib.check(L.fl_score_workspace_bytes(R, V, top_k, ctypes.byref(n)), "fl_score_workspace_bytes")
-        ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
+        n = _workspace_bytes(R, V, top_k)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), n
     call(L.fl_score_tokens, a, dev, "fl_score_tokens")
     return o_lp, o_h, o_lse, o_rank, o_ids, o_top, saved
 
@@ -107,18 +114,21 @@ class _Score(torch.autograd.Function):
         x = _rows(logits.detach(), "logits")
         out = _forward(x, logits.shape[:-1], tok, top_k, entropy, lse, rank, ignore_index, True)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, out[6])
-        ctx.tok, ctx.ignore_index = tok, ignore_index
+        ctx.save_for_backward(logits) if tok is None else ctx.save_for_backward(logits, tok)
+        # (this node's own: no caller sees or changes it)
+        ctx.saved, ctx.ignore_index = out[6], ignore_index
         ctx.mark_non_differentiable(*(t for t in out[3:6] if t is not None))
         return out[:6]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_lp, g_h, g_lse, *_):
-        logits, saved = ctx.saved_tensors
+        logits, *tok = ctx.saved_tensors
         if g_lp is None and g_h is None and g_lse is None:
             return (None,) * 7
-        d = score_tokens_backward(logits, ctx.tok, saved, g_lp, g_h, g_lse, ignore_index=ctx.ignore_index)
+        # (the engine has checked the gradients' shapes, types and device)
+        d = _backward(_rows(logits, "logits"), logits.shape, tok[0] if tok else None, ctx.saved,
+                      *(None if g is None else g.contiguous() for g in (g_lp, g_h, g_lse)), ctx.ignore_index)
         return d, None, None, None, None, None, None
 
 
@@ -192,14 +202,19 @@ def score_tokens_backward(logits: torch.Tensor, tokens: Optional[torch.Tensor], 
         gc = _upstream(grad_lse, lead, dev, "grad_lse")
         if ga is not None and tok is None:
             raise ValueError("grad_logprob needs tokens")
-        out = torch.empty(logits.shape, dtype=x.dtype, device=dev)
-        a = ScoreGradArgs()
-        a.struct_size = ctypes.sizeof(ScoreGradArgs)
-        a.dtype = _DTYPES[x.dtype]
-        a.logits = x.data_ptr()
-        a.rows, a.vocab, a.ld = R, V, x.stride(0) if R > 1 else V
-        a.tokens, a.ignore_index, a.saved = ptr(tok), int(ignore_index), saved.data_ptr()
-        a.grad_logprob, a.grad_entropy, a.grad_lse = ptr(ga), ptr(gb), ptr(gc)
-        a.out_grad, a.out_ld = out.data_ptr(), V
-        call(lib().fl_score_tokens_grad, a, dev, "fl_score_tokens_grad")
-        return out
+        return _backward(x, logits.shape, tok, saved, ga, gb, gc, int(ignore_index))
+
+
+def _backward(x, shape, tok, saved, ga, gb, gc, ignore_index: int) -> torch.Tensor:
+    R, V = x.shape
+    out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    a = ScoreGradArgs()
+    a.struct_size = ctypes.sizeof(ScoreGradArgs)
+    a.dtype = _DTYPES[x.dtype]
+    a.logits = x.data_ptr()
+    a.rows, a.vocab, a.ld = R, V, x.stride(0) if R > 1 else V
+    a.tokens, a.ignore_index, a.saved = ptr(tok), ignore_index, saved.data_ptr()
+    a.grad_logprob, a.grad_entropy, a.grad_lse = ptr(ga), ptr(gb), ptr(gc)
+    a.out_grad, a.out_ld = out.data_ptr(), V
+    call(lib().fl_score_tokens_grad, a, x.device, "fl_score_tokens_grad")
+    return out
