@@ -260,8 +260,8 @@ struct HlArgs {
 
 }  // namespace
 
-// part[(2 vocabulary tile + half) rows + n] (for BJ < 256: (waves along i) parts
-// a tile): max, sum e, sum e d2 of the wave's vocabulary rows
+// part[tile rows + n]: max, sum e, sum e d2 of the tile's vocabulary rows, in the
+// order rows run so that a join's loads are coalesced
 template <int BJ>
 __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_head_stats(const HlArgs a, float4* part,
                                                                                                float* xt, int ni, int nj) {
@@ -276,6 +276,8 @@ __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   const int wi = w / S::WJ, wj = w % S::WJ;
   const int vw = v0 + wi * 32 * S::FI + 4 * (lane >> 5);   // the lane's first vocabulary row
   constexpr float NINF = -__builtin_inff();
+  float* wave_part = reinterpret_cast<float*>(smem);   // [WI][BJ][3]
+  lds_barrier();
   if (v0 + HL_I > a.vocab) {
 #pragma unroll
     for (int i = 0; i < S::FI; ++i)
@@ -309,8 +311,13 @@ __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     float ss = s[0] + s[1], uu = u[0] + u[1];
     ss += __shfl_xor(ss, 32, WAVE);
     uu += __shfl_xor(uu, 32, WAVE);
+    if (lane < 32) {   // (the product's stages are read: LDS is free)
+      float* wp = wave_part + 3 * (wi * BJ + wj * 32 * S::FJ + 32 * j + lane);
+      wp[0] = m;
+      wp[1] = ss;
+      wp[2] = uu;
+    }
     if (n >= a.rows) continue;
-    if (lane < 32) part[static_cast<int64_t>(t.i * S::WI + wi) * a.rows + n] = make_float4(m, ss, uu, 0.0f);
     // the token's logit, by the lane that has it
     const int64_t tk = a.tokens ? a.tokens[n] : -1;
     const int64_t d = tk - vw;
@@ -322,47 +329,82 @@ __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
           if (d == 32 * i + 8 * (r / 4) + r % 4) xt[n] = acc[i][j][r];
     }
   }
+  __syncthreads();
+  // the tile's part of each row: the waves' joined
+  for (int q = threadIdx.x; q < BJ && n0 + q < a.rows; q += HL_NT) {
+    float m = NINF, s = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S::WI; ++i) m = fmaxf(m, wave_part[3 * (i * BJ + q)]);
+    const float ref = m == NINF ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < S::WI; ++i) {
+      const float* wp = wave_part + 3 * (i * BJ + q);
+      const float d = (wp[0] - ref) * HL_LOG2E, f = __builtin_amdgcn_exp2f(d);
+      s = fmaf(wp[1], f, s);
+      u = fmaf(fmaf(wp[1], fmaxf(d, -200.0f), wp[2]), f, u);
+    }
+    part[static_cast<int64_t>(t.i) * a.rows + n0 + q] = make_float4(m, s, u, 0.0f);
+  }
 }
 
-// The parts of each row joined: 64 rows per work-group, a wave per 16th of the
-// parts, in float64 and in a fixed order.
-constexpr int HJ_W = 16;
-__global__ __launch_bounds__(HJ_W * WAVE) void k_head_join(const fl_head_args a, const float4* part, const float* xt,
+// The parts of each row joined: 8 rows per work-group, 32 threads each, in
+// float64 and in a fixed order.
+constexpr int HJ_R = 8, HJ_P = 32;
+__global__ __launch_bounds__(HJ_R * HJ_P) void k_head_join(const fl_head_args a, const float4* part, const float* xt,
                                                            int parts) {
-  __shared__ double sm[3][HJ_W][WAVE];
-  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * WAVE + lane;
+  __shared__ float sm[HJ_P / 8][HJ_R];
+  __shared__ double ss[HJ_P / 8][HJ_R], su[HJ_P / 8][HJ_R];
+  const int r = threadIdx.x % HJ_R, p0 = threadIdx.x / HJ_R, w = threadIdx.x / WAVE;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * HJ_R + r;
+  const bool on = n < a.rows;
   const float ninf = -__builtin_inff();
+  // (a thread's parts relative to its own maximum; of -inf alone m stays -inf,
+  // and a NaN sum stays NaN)
   float m = ninf;
   double s = 0.0, u = 0.0;
-  auto merge = [&](float pm, double ps, double pu) {
-    // (u in base 2 relative to its own maximum)
-    if (!(pm <= m)) {   // a larger maximum, or NaN
-      const float d = (m - pm) * HL_LOG2E;
-      const double f = m == ninf ? 0.0 : exp2(static_cast<double>(d));
-      u = (u + (m == ninf ? 0.0 : s * static_cast<double>(fmaxf(d, -1e30f)))) * f + pu;
-      s = s * f + ps;
-      m = pm;
-    } else if (pm != ninf) {
-      const float d = (pm - m) * HL_LOG2E;
-      const double f = exp2(static_cast<double>(d));
-      u += (pu + ps * static_cast<double>(fmaxf(d, -1e30f))) * f;
-      s += ps * f;
-    } else {
-      s += ps;   // (NaN values among -inf)
-    }
-  };
-  if (n < a.rows)
-    for (int p = w; p < parts; p += HJ_W) {
+  if (on) {
+#pragma unroll 4
+    for (int p = p0; p < parts; p += HJ_P) {
       const float4 q = part[static_cast<int64_t>(p) * a.rows + n];
-      merge(q.x, q.y, q.z);
+      const float nm = fmaxf(m, q.x), ref = nm == ninf ? 0.0f : nm;
+      const float d0 = (m - ref) * HL_LOG2E, d1 = (q.x - ref) * HL_LOG2E;
+      const double f0 = __builtin_amdgcn_exp2f(d0), f1 = __builtin_amdgcn_exp2f(d1);
+      u = (u + s * static_cast<double>(fmaxf(d0, -200.0f))) * f0 + (static_cast<double>(q.z) + q.y * fmaxf(d1, -200.0f)) * f1;
+      s = s * f0 + q.y * f1;
+      m = nm;
     }
-  sm[0][w][lane] = m;
-  sm[1][w][lane] = s;
-  sm[2][w][lane] = u;
+  }
+  float M = m;
+  for (int x = HJ_R; x < WAVE; x <<= 1) M = fmaxf(M, __shfl_xor(M, x, WAVE));
+  if ((threadIdx.x & (WAVE - 1)) < HJ_R) sm[w][r] = M;
   __syncthreads();
-  if (w != 0 || n >= a.rows) return;
-  for (int q = 1; q < HJ_W; ++q) merge(static_cast<float>(sm[0][q][lane]), sm[1][q][lane], sm[2][q][lane]);
+  M = sm[0][r];
+#pragma unroll
+  for (int i = 1; i < HJ_P / 8; ++i) M = fmaxf(M, sm[i][r]);
+  {
+    const float ref = M == ninf ? 0.0f : M, d = (m - ref) * HL_LOG2E;
+    const double f = __builtin_amdgcn_exp2f(d);
+    u = (u + s * static_cast<double>(fmaxf(d, -200.0f))) * f;
+    s *= f;
+  }
+  for (int x = HJ_R; x < WAVE; x <<= 1) {
+    s += __shfl_xor(s, x, WAVE);
+    u += __shfl_xor(u, x, WAVE);
+  }
+  if ((threadIdx.x & (WAVE - 1)) < HJ_R) {
+    ss[w][r] = s;
+    su[w][r] = u;
+  }
+  __syncthreads();
+  if (p0 != 0 || !on) return;
+  m = M;
+  s = ss[0][r];
+  u = su[0][r];
+#pragma unroll
+  for (int i = 1; i < HJ_P / 8; ++i) {
+    s += ss[i][r];
+    u += su[i][r];
+  }
   const float nan = __builtin_nanf("");
   const bool okr = s > 0.0 && s < static_cast<double>(__builtin_inff());
   const double logs = log(s), ref = static_cast<double>(m);
@@ -538,7 +580,7 @@ size_t al(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 // j-tile of the products over rows: the rows' own size up to 128, so that a few
 // rows do not pay for 256
 int hl_bj(int64_t rows) { return rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
-int hl_parts(int64_t rows, int64_t vocab) { return cdiv(vocab, HL_I) * (HL_NW / (hl_bj(rows) / 64)); }
+int hl_parts(int64_t vocab) { return cdiv(vocab, HL_I); }
 
 // Vocabulary rows of a backward chunk: g's bytes stay within HL_G_BYTES, but a
 // chunk has at least HL_CHUNK rows, so that the products of many rows have k
@@ -589,7 +631,7 @@ hipError_t hl_allow(K k, int bytes) {
 
 size_t head_workspace_bytes(int64_t rows, int64_t vocab) {
   const size_t R = static_cast<size_t>(rows);
-  return al(16 * R * static_cast<size_t>(hl_parts(rows, vocab))) + al(4 * R);
+  return al(16 * R * static_cast<size_t>(hl_parts(vocab))) + al(4 * R);
 }
 
 size_t head_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t vocab, bool dhidden) {
@@ -602,7 +644,7 @@ size_t head_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t vocab, bool 
 hipError_t launch_head(const fl_head_args& a, hipStream_t s) {
   const HlArgs h = hl_args(a.hidden, a.weight, a.ld_hidden, a.rows, a.dim, a.vocab, a.tokens, a.ignore_index);
   float4* part = static_cast<float4*>(a.workspace);
-  const int parts = hl_parts(a.rows, a.vocab);
+  const int parts = hl_parts(a.vocab);
   float* xt = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + al(16 * static_cast<size_t>(a.rows) * parts));
   hipError_t e = hipSuccess;
   hl_by_rows(a.rows, [&](auto bj) {
@@ -613,7 +655,7 @@ hipError_t launch_head(const fl_head_args& a, hipStream_t s) {
       hipLaunchKernelGGL(k_head_stats<BJ>, dim3(static_cast<unsigned>(ni) * nj), dim3(HL_NT), hl_lds<BJ>(), s, h, part, xt, ni, nj);
   });
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(k_head_join, dim3(cdiv(a.rows, WAVE)), dim3(HJ_W * WAVE), 0, s, a, part, xt, parts);
+  hipLaunchKernelGGL(k_head_join, dim3(cdiv(a.rows, HJ_R)), dim3(HJ_R * HJ_P), 0, s, a, part, xt, parts);
   return hipGetLastError();
 }
 

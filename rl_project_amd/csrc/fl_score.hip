@@ -156,89 +156,164 @@ __global__ __launch_bounds__(SC_NT) void k_score_slice(const fl_score_args a, co
     if (t >= 0 && t < V && t != a.ignore_index)
       xt = C::elem(row_rsrc(row, static_cast<uint32_t>(V * ESZ)), static_cast<int>(t));
   }
-  // -inf past the row; the last value of an odd 16-bit row by itself (the range
-  // check goes by dwords)
-  auto pad = [&](uint4 v, int k) {
+  // Past the slice's values a chunk takes the pattern `fill`; the last value of
+  // an odd 16-bit row by itself (the range check goes by dwords).
+  const bool part = nval < SC_SLICE;
+  constexpr uint32_t NINF = D::id == FL_DTYPE_F32 ? 0xFF800000u : D::id == FL_DTYPE_BF16 ? 0xFF80u : 0xFC00u;
+  uint32_t last = 0;
+  if (D::id != FL_DTYPE_F32 && part && (nval & 1))
+    last = static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(rs, 2 * (nval - 1), 0, 0));
+  auto pad = [&](uint4 v, int k, uint32_t fill) {
     uint32_t wd[4] = {v.x, v.y, v.z, v.w};
     const int f = N * (tid + k * SC_NT);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if constexpr (D::id == FL_DTYPE_F32) {
-        if (f + j >= nval) wd[j] = 0xFF800000u;
+        wd[j] = f + j >= nval ? fill : wd[j];
       } else {
-        constexpr uint32_t NINF = 0x8000u | D::INF_BITS;
-        const int i = f + 2 * j;
-        if (i >= nval) wd[j] = NINF | (NINF << 16);
-        else if (i + 1 >= nval)
-          wd[j] = static_cast<uint32_t>(static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(rs, 2 * i, 0, 0))) | (NINF << 16);
+        wd[j] = f + 2 * j + 1 == nval ? (last | (fill << 16)) : wd[j];
+        wd[j] = f + 2 * j >= nval ? (fill | (fill << 16)) : wd[j];
       }
     }
     return make_uint4(wd[0], wd[1], wd[2], wd[3]);
   };
-  if (nval < SC_SLICE) {
+  auto pad_all = [&](uint32_t fill) {
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) q[k] = pad(q[k], k);
-  }
+    for (int k = 0; k < NCH; ++k) q[k] = pad(q[k], k, fill);
+  };
+  if (part) pad_all(NINF);
+  // (chunk k from memory again, for the rare paths: rolled loops, small code)
+  auto fetch = [&](float (&x)[N], int k) {
+    C::unpack(pad(buf_load16(rs, 16u * static_cast<uint32_t>(tid + k * SC_NT), 0u), k, NINF), x);
+  };
   // (the steps below unpack the values again each, rather than hold both forms)
   auto fence = [&]() {
 #pragma unroll
     for (int k = 0; k < NCH; ++k) asm volatile("" : "+v"(q[k].x), "+v"(q[k].y), "+v"(q[k].z), "+v"(q[k].w));
   };
 
-  // maxima: chunk, thread, slice
-  float cm[NCH], tm = -__builtin_inff();
+  // Maxima: chunk, thread, slice.  Of the values' bits as signed integers, two
+  // 16-bit values at a time: right as soon as one value is not negative, else
+  // it finds the one farthest from 0 (a value of the chunk still).  Only where
+  // that matters are they taken again as floats: a slice of negative values,
+  // or fewer than K threads with one that is not.
+  float cm[NCH];
+  int tb = -0x7FFFFFFF - 1;
 #pragma unroll
   for (int k = 0; k < NCH; ++k) {
-    float x[N];
-    C::unpack(q[k], x);
-    float c = x[0];
-#pragma unroll
-    for (int e = 1; e < N; ++e) c = fmaxf(c, x[e]);
-    cm[k] = c;
-    tm = fmaxf(tm, c);
+    int c;
+    if constexpr (D::id == FL_DTYPE_F32) {
+      c = max(max(static_cast<int>(q[k].x), static_cast<int>(q[k].y)), max(static_cast<int>(q[k].z), static_cast<int>(q[k].w)));
+      cm[k] = __uint_as_float(static_cast<uint32_t>(c));
+    } else {
+      typedef short short2v __attribute__((ext_vector_type(2)));
+      const short2v m2 = __builtin_elementwise_max(
+          __builtin_elementwise_max(__builtin_bit_cast(short2v, q[k].x), __builtin_bit_cast(short2v, q[k].y)),
+          __builtin_elementwise_max(__builtin_bit_cast(short2v, q[k].z), __builtin_bit_cast(short2v, q[k].w)));
+      const uint32_t b = __builtin_bit_cast(uint32_t, m2);
+      c = max(static_cast<int>(b << 16), static_cast<int>(b & 0xFFFF0000u));
+      cm[k] = D::to_f32(static_cast<uint32_t>(c) >> 16);
+    }
+    tb = max(tb, c);
   }
-  fence();
+  auto as_float = [](int b) {
+    if constexpr (D::id == FL_DTYPE_F32) return __uint_as_float(static_cast<uint32_t>(b));
+    else return D::to_f32(static_cast<uint32_t>(b) >> 16);
+  };
+  auto exact_maxima = [&]() {   // (of the thread)
+    fence();
+    float t = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      float x[N];
+      C::unpack(q[k], x);
+      float c = x[0];
+#pragma unroll
+      for (int e = 1; e < N; ++e) c = fmaxf(c, x[e]);
+      cm[k] = c;
+      t = fmaxf(t, c);
+    }
+    fence();
+    return t;
+  };
   if (tid == 0) s_n = 0u;
-  tkey[tid] = f32_key(tm + 0.0f);
-  const float wm = wave_reduce(tm, OpMax());
-  if (lane == 0) red[w] = wm;
+  tkey[tid] = f32_key(as_float(tb) + 0.0f);
+  const int wb = wave_reduce(tb, OpMax());
+  if (lane == 0) red[w] = as_float(wb);
   __syncthreads();
   float m = red[0];
 #pragma unroll
   for (int i = 1; i < SC_NW; ++i) m = fmaxf(m, red[i]);
+  // (a wave of negative values alone left a lower one: no matter beside a
+  // wave that has one which is not)
+  bool exact = !(m >= 0.0f);
+  if (exact) {   // (for the whole work-group)
+    const float t = exact_maxima();
+    const float wm = wave_reduce(t, OpMax());
+    __syncthreads();
+    tkey[tid] = f32_key(t + 0.0f);
+    if (lane == 0) red[w] = wm;
+    __syncthreads();
+    m = red[0];
+#pragma unroll
+    for (int i = 1; i < SC_NW; ++i) m = fmaxf(m, red[i]);
+  }
   m = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(m)));
+  fence();
 
   // Sums relative to the slice's maximum, exponents in base 2.  d2 =
   // fma(x, log2(e), -mb) has one rounding; it is relative to mb / log2(e),
   // which is what `ref` says.  From |mb| = 2^31 on (a mask of the type's lowest
   // value) that would not do, and d2 = (x - m) log2(e).  A term of the entropy
-  // is e max(d2, -200): 0 where e is, -inf values and those the exponent
-  // leaves the float range for among them.
+  // is e d2, which for a -inf value, or one the exponent leaves the float range
+  // for, is 0 * -inf: a wave that finds a NaN takes its sums again with
+  // e max(d2, -200), 0 there.
   const float mb = m == -__builtin_inff() ? 0.0f : m * SC_LOG2E;
-  const bool plain = __builtin_fabsf(mb) < 0x1p31f;
+  // Past the slice's values a finite fill far below m, so that the fast sums of
+  // a row's last slice have no NaN (float16 has none below a mask of its lowest).
+  constexpr uint32_t FILL = D::id == FL_DTYPE_F32 ? 0xF149F2CAu : D::id == FL_DTYPE_BF16 ? 0xF149u : 0xFBFFu;   // -1e30; -65504
+  const bool plain = __builtin_fabsf(mb) < 0x1p31f && !(D::id == FL_DTYPE_F16 && part && m < -60000.0f);
+  if (part && plain) pad_all(FILL);
   const double ref = m == -__builtin_inff() ? static_cast<double>(m)
                      : plain                ? static_cast<double>(mb) * SC_INV_LOG2E
-                                            : static_cast<double>(m);
+                                            : static_cast<double>(m);   // (as the sums below take it)
   float fs[2] = {0.0f, 0.0f}, fu[2] = {0.0f, 0.0f};
   uint32_t above = 0;
-  auto sums = [&](auto&& d2_of) {
+  if (plain) {
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       float x[N];
       C::unpack(q[k], x);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float d2 = d2_of(x[e]);
+        const float d2 = fmaf(x[e], SC_LOG2E, -mb);
+        const float ex = __builtin_amdgcn_exp2f(d2);
+        fs[e & 1] += ex;
+        if (ENT) fu[e & 1] = fmaf(ex, d2, fu[e & 1]);
+        if (RANK) above += static_cast<uint32_t>(__popcll(__ballot(x[e] > xt)));
+      }
+      __builtin_amdgcn_sched_barrier(0);   // (one chunk's comparisons live at a time)
+    }
+  }
+  const float u0 = fu[0] + fu[1];
+  if (!plain || (ENT && __any(u0 != u0))) {   // (for the whole wave)
+    const float ref0 = m == -__builtin_inff() ? 0.0f : m;
+    fs[0] = fs[1] = fu[0] = fu[1] = 0.0f;
+    above = 0;
+#pragma unroll 1
+    for (int k = 0; k < NCH; ++k) {
+      float x[N];
+      fetch(x, k);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float d2 = plain ? fmaf(x[e], SC_LOG2E, -mb) : (x[e] - ref0) * SC_LOG2E;
         const float ex = __builtin_amdgcn_exp2f(d2);
         fs[e & 1] += ex;
         if (ENT) fu[e & 1] = fmaf(ex, fmaxf(d2, -200.0f), fu[e & 1]);
         if (RANK) above += static_cast<uint32_t>(__popcll(__ballot(x[e] > xt)));
       }
-      __builtin_amdgcn_sched_barrier(0);   // (one chunk's comparisons live at a time)
     }
-  };
-  if (plain) sums([&](float x) { return fmaf(x, SC_LOG2E, -mb); });
-  else sums([&](float x) { return (x - m) * SC_LOG2E; });
+  }
   const float ws_s = wave_reduce(fs[0] + fs[1], OpAdd());
   const float ws_u = ENT ? wave_reduce(fu[0] + fu[1], OpAdd()) : 0.0f;
   if (lane == 0) {
@@ -246,7 +321,7 @@ __global__ __launch_bounds__(SC_NT) void k_score_slice(const fl_score_args a, co
     red_u[w] = ws_u;
     red_c[w] = above;
   }
-  if (K > 0 && w == 0) {
+  auto bound = [&]() {
     // the K-th largest of the threads' maxima: K values of the slice reach it
     // (past the slice's values the maxima are -inf)
     uint32_t kk[SC_NW];
@@ -263,7 +338,8 @@ __global__ __launch_bounds__(SC_NT) void k_score_slice(const fl_score_args a, co
     }
     if (LOW > 0 && !(T & 0x80000000u)) T |= (1u << LOW) - 1u;
     if (lane == 0) s_key = T;
-  }
+  };
+  if (K > 0 && w == 0) bound();
   __syncthreads();
   if (tid == 0) {
     double s = 0.0, u = 0.0;
@@ -282,6 +358,14 @@ __global__ __launch_bounds__(SC_NT) void k_score_slice(const fl_score_args a, co
 
   // ---- the slice's K largest values
   fence();
+  if (!exact && s_key < 0x80000000u) {   // (a negative bound, by integer maxima)
+    __syncthreads();
+    if (part) pad_all(NINF);
+    tkey[tid] = f32_key(exact_maxima() + 0.0f);
+    __syncthreads();
+    if (w == 0) bound();
+    __syncthreads();
+  }
   float tf = f32_of_key(s_key);
   auto append = [&](const float (&x)[N], int k, auto&& in) {
 #pragma unroll
@@ -308,11 +392,7 @@ __global__ __launch_bounds__(SC_NT) void k_score_slice(const fl_score_args a, co
     // Many values at or above the bound.  The exact K-th largest value: the
     // bound itself if fewer than K values are above it (many equal values: a
     // mask), else by bisection over the keys.  Then the values above it, and of
-    // those equal to it the first ones.  From memory again, chunk by chunk: the
-    // path is rare, and its code small.
-    auto fetch = [&](float (&x)[N], int k) {
-      C::unpack(pad(buf_load16(rs, 16u * static_cast<uint32_t>(tid + k * SC_NT), 0u), k), x);
-    };
+    // those equal to it the first ones.
     auto count = [&](auto&& in) {   // (over the slice; the same for every thread)
       uint32_t c = 0;
 #pragma unroll 1
@@ -405,6 +485,13 @@ __global__ __launch_bounds__(SC_NT) void k_score_join(const fl_score_args a, con
   const int S = ws.S, K = static_cast<int>(a.top_k);
   const int64_t r = blockIdx.x;
   const uint64_t* list = ws.list + r * S * K;
+  if (tid == 0) s_n = 0u;
+  // (the list's loads beside the statistics)
+  const uint64_t kth = K > 0 && (tid & (WAVE - 1)) < S ? list[(tid & (WAVE - 1)) * K + K - 1] : 0u;
+  constexpr int PER = SC_CAP / SC_NT;
+  uint64_t mine[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) mine[i] = tid + i * SC_NT < S * K ? list[tid + i * SC_NT] : 0u;
   if (tid < WAVE) {
     constexpr int G = SC_MAX_SLICES;   // lanes of the fixed tree
     static_assert(G <= WAVE && (G & (G - 1)) == 0, "one lane per slice");
@@ -419,27 +506,16 @@ __global__ __launch_bounds__(SC_NT) void k_score_join(const fl_score_args a, con
     const double s = wave_reduce<double, OpAdd, G>(on ? p.s * f : p.s, OpAdd());
     const double u = wave_reduce<double, OpAdd, G>(on ? (p.u + p.s * (f > 0.0 ? d : 0.0)) * f : p.u, OpAdd());
     const int c = wave_reduce<int, OpAdd, G>(p.rank, OpAdd());
-    if (tid == 0) {
-      s_row = sc_finish(a, r, R, s, u, p.xt, c);
-      s_n = 0u;
-    }
+    if (tid == 0) s_row = sc_finish(a, r, R, s, u, p.xt, c);
   }
   if (K == 0) return;   // (one wave)
   __syncthreads();
   const ScRow rw = s_row;
   // the largest of the lists' K-th entries: the row's K-th value reaches it
-  uint64_t bound = 0;
-  for (int i = 0; i < S; ++i) {
-    const uint64_t e = list[i * K + K - 1];
-    bound = e > bound ? e : bound;
-  }
-  for (int i = tid; i < S * K; i += SC_NT) {
-    const uint64_t e = list[i];
-    if (e >= bound && e != 0u) {
-      const uint32_t slot = atomicAdd(&s_n, 1u);
-      cand[slot] = e;   // (at most S K <= SC_CAP)
-    }
-  }
+  const uint64_t bound = wave_reduce(kth, OpMax());   // (every wave's the same)
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (mine[i] >= bound && mine[i] != 0u) cand[atomicAdd(&s_n, 1u)] = mine[i];   // (at most S K <= SC_CAP)
   __syncthreads();
   const int n = static_cast<int>(s_n);
   sc_place(cand, n, K, [&](int p, uint64_t key) { sc_emit(a, r, p, key, rw); });
