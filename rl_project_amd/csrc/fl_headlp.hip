@@ -77,7 +77,7 @@ __device__ __forceinline__ int32x4 hl_rsrc(const void* p, uint32_t bytes) {
 __device__ __forceinline__ void hl_load_lds(int32x4 r, uint32_t voff, uint32_t soff, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
-               : "s"(lds), "v"(voff), "s"(r), "s"(soff)
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(r), "s"(__builtin_amdgcn_readfirstlane(soff))
                : "memory");
 }
 template <int N>
@@ -167,25 +167,63 @@ struct Reader {
   }
 };
 
-// Wave grid WI x WJ of FI x FJ blocks of 32 x 32 per wave; NST stages in LDS.
-template <int BJ>
+// Wave grid WI x WJ of FI x FJ blocks of 32 x 32 per wave; NST stages in LDS, and
+// beside them an area for the epilogues.
+template <int BJ_>
 struct Shape {
-  static constexpr int WJ = BJ / 64, WI = HL_NW / WJ, FI = HL_I / (32 * WI), FJ = 2;
+  static constexpr int BJ = BJ_, WJ = BJ / 64, WI = HL_NW / WJ, FI = HL_I / (32 * WI), FJ = 2;
   static constexpr int STAGE = (HL_I + BJ) * HL_K * 2;
   static constexpr int NST = BJ == 256 ? 2 : 3;
-  static_assert(NST * STAGE <= 160 * 1024, "LDS");
+  static constexpr int AREA_W = BJ == 128 ? 2048 : 4096;   // per wave
+  static constexpr int LDS = NST * STAGE + HL_NW * AREA_W;
+  static_assert(LDS <= 160 * 1024, "LDS");
 };
 
-template <bool ACOLS, bool BCOLS, int BJ>
-__device__ __forceinline__ void hl_product(const Operand& A, const Operand& B, int stages, char* smem,
-                                           floatx16 (&acc)[Shape<BJ>::FI][Shape<BJ>::FJ]) {
-  using S = Shape<BJ>;
-  constexpr int NST = S::NST;
-  Loader<ACOLS, HL_I> la;
-  Loader<BCOLS, BJ> lb;
-  la.init(A);
-  lb.init(B);
-  constexpr int L = Loader<ACOLS, HL_I>::LOADS + Loader<BCOLS, BJ>::LOADS;
+// Tiles of a launch: ni of 256 along i, nj of BJ along j, nz ranges of k.  Work-group
+// b of a grid of at most one per CU takes every (grid / 8)-th tile of its XCD's
+// share (work-groups go round the 8 XCDs): a contiguous range of an order in
+// which 8 j-tiles share each i-tile, so that the work-groups of an XCD read the
+// same few rows through its L2.
+struct Tiles {
+  int ni, nj, nz;
+  __device__ __forceinline__ int count() const { return ni * nj * nz; }
+  __device__ __forceinline__ void at(int t, int& i, int& j, int& z) const {
+    z = t / (ni * nj);
+    t -= z * ni * nj;
+    const int per = 8 * ni, grp = t / per, in = t - grp * per, gj = min(8, nj - 8 * grp);
+    i = in / gj;
+    j = 8 * grp + in % gj;
+  }
+};
+// The tiles of one work-group: first, first + step, ... below end.
+struct Share {
+  int t, end, step;
+};
+__device__ __forceinline__ Share hl_share(const Tiles& ts) {
+  const int n = ts.count(), x = blockIdx.x % 8, q = blockIdx.x / 8;
+  const int lo = x * (n / 8) + min(x, n % 8);
+  // (work-groups of XCD x in the grid)
+  const int step = (static_cast<int>(gridDim.x) - x + 7) / 8;
+  return {lo + q, lo + n / 8 + (x < n % 8 ? 1 : 0), step};
+}
+
+// The products of a work-group's tiles, one after another without a gap in the
+// loads: operands(t, A, B) says what tile t reads and returns its stages (one or
+// more); epilogue(t, acc) takes its results.  A stage's last fragments are in
+// registers when the work-group meets (all have read the stage, the next has
+// landed); the next stage's first fragments are read, and the loads into the
+// stage's place issued, ahead of the last quarter of its matrix instructions.
+// While an epilogue runs, the next tile's first stages are on their way: it calls
+// hl_wait_vm<0>() before its first store, so that no later wait for a load waits
+// for a store.
+template <bool ACOLS, bool BCOLS, class S, class OPS, class EPI>
+__device__ __forceinline__ void hl_products(const Tiles& ts, char* smem, OPS&& operands, EPI&& epilogue) {
+  constexpr int NST = S::NST, BJ = S::BJ;
+  using LA = Loader<ACOLS, HL_I>;
+  using LB = Loader<BCOLS, BJ>;
+  constexpr int L = LA::LOADS + LB::LOADS;
+  const Share sh = hl_share(ts);
+  if (sh.t >= sh.end) return;
   const int w = threadIdx.x / WAVE;
   Reader<ACOLS, HL_I, S::FI> ra;
   Reader<BCOLS, BJ, S::FJ> rb;
@@ -193,59 +231,128 @@ __device__ __forceinline__ void hl_product(const Operand& A, const Operand& B, i
   rb.init((w % S::WJ) * 32 * S::FJ);
   const uint32_t lds = static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(smem)));
-#pragma unroll
-  for (int i = 0; i < S::FI; ++i)
-#pragma unroll
-    for (int j = 0; j < S::FJ; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-  auto load = [&](int s, int buf) {
-    la.load(s, lds + buf * S::STAGE);
-    lb.load(s, lds + buf * S::STAGE + Loader<ACOLS, HL_I>::BYTES);
+
+  // the load cursor: tile lt, its next stage ls of ln, into buffer lbuf
+  LA la;
+  LB lb;
+  int lt = sh.t, ls = 0, ln = 0, lbuf = 0;
+  auto open = [&]() {
+    Operand A, B;
+    ln = operands(lt, A, B);
+    la.init(A);
+    lb.init(B);
+    ls = 0;
   };
-#pragma unroll
-  for (int s = 0; s < NST - 1; ++s)
-    if (s < stages) load(s, s);
-  int buf = 0;
-#pragma unroll 1
-  for (int s = 0; s < stages; ++s) {
-    // stage s has landed for this wave (NST - 2 later ones may be in flight),
-    // then for all, and all have read stage s - 1, whose buffer is loaded next
-    if (NST > 2 && s + NST - 2 < stages) hl_wait_vm<L*(NST - 2)>();
-    else hl_wait_vm<0>();
-    lds_barrier();
-    if (s + NST - 1 < stages) load(s + NST - 1, buf == 0 ? NST - 1 : buf - 1);
-    const char* ta = smem + buf * S::STAGE;
-    const char* tb = ta + Loader<ACOLS, HL_I>::BYTES;
-#pragma unroll
-    for (int ks = 0; ks < HL_K / 16; ++ks) {
-      bf16x8 a[S::FI], b[S::FJ];
-#pragma unroll
-      for (int i = 0; i < S::FI; ++i) a[i] = ra.read(ta, i, ks);
-#pragma unroll
-      for (int j = 0; j < S::FJ; ++j) b[j] = rb.read(tb, j, ks);
-#pragma unroll
-      for (int i = 0; i < S::FI; ++i)
-#pragma unroll
-        for (int j = 0; j < S::FJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+  auto issue = [&]() {   // returns whether there was a stage
+    if (lt >= sh.end) return 0;
+    la.load(ls, lds + lbuf * S::STAGE);
+    lb.load(ls, lds + lbuf * S::STAGE + LA::BYTES);
+    lbuf = lbuf == NST - 1 ? 0 : lbuf + 1;
+    if (++ls == ln) {
+      lt += sh.step;
+      if (lt < sh.end) open();
     }
-    buf = buf == NST - 1 ? 0 : buf + 1;
+    return 1;
+  };
+  open();
+  int stages = ln;     // of the current tile
+  int ahead = 0;       // stages issued past the current one ...
+  int landed = 0;      // ... and how many of them this wave has waited for
+  issue();
+  hl_wait_vm<0>();
+#pragma unroll
+  for (int s = 1; s < NST; ++s) ahead += issue();
+  lds_barrier();
+
+  bf16x8 fa[2][S::FI], fb[2][S::FJ];
+  int buf = 0;
+  auto read = [&](int slot, int b, int ks) {
+    const char* ta = smem + b * S::STAGE;
+    const char* tb = ta + LA::BYTES;
+#pragma unroll
+    for (int i = 0; i < S::FI; ++i) fa[slot][i] = ra.read(ta, i, ks);
+#pragma unroll
+    for (int j = 0; j < S::FJ; ++j) fb[slot][j] = rb.read(tb, j, ks);
+  };
+#pragma unroll 1
+  for (int t = sh.t; t < sh.end; t += sh.step) {
+    floatx16 acc[S::FI][S::FJ];
+#pragma unroll
+    for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    read(0, buf, 0);
+#pragma unroll 1
+    for (int s = 0; s < stages; ++s) {
+#pragma unroll
+      for (int ks = 0; ks < HL_K / 16; ++ks) {
+        if (ks < HL_K / 16 - 1) {
+          read((ks + 1) & 1, buf, ks + 1);
+        } else if (ahead > 0) {
+          if (landed > 0) --landed;
+          else if (NST > 2 && ahead > 1) hl_wait_vm<L>();   // (the newest stage may be on its way)
+          else hl_wait_vm<0>();
+          lds_barrier();
+          ahead += issue() - 1;
+          buf = buf == NST - 1 ? 0 : buf + 1;
+          if (s + 1 < stages) read(0, buf, 0);   // (a tile's first ones after the epilogue, which needs the registers)
+        }
+#pragma unroll
+        for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+          for (int j = 0; j < S::FJ; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[ks & 1][i], fb[ks & 1][j], acc[i][j], 0, 0, 0);
+      }
+    }
+    epilogue(t, acc);
+    landed = ahead;
+    if (t + sh.step < sh.end) {
+      Operand A, B;
+      stages = operands(t + sh.step, A, B);
+    }
   }
 }
 
-// Tile of a work-group: each of the 8 XCDs (work-groups go round them) takes a
-// contiguous range of an order in which 8 j-tiles share each i-tile, so that the
-// work-groups of an XCD read the same few rows through its L2.
-struct TileIdx {
-  int i, j;
-};
-__device__ __forceinline__ TileIdx hl_tile(int b, int ni, int nj) {
-  const int n = ni * nj, x = b % 8, q = b / 8;
-  // XCD x has n / 8 tiles, the first n % 8 of them one more
-  const int t = x * (n / 8) + min(x, n % 8) + q;
-  const int per = 8 * ni, grp = t / per, in = t - grp * per;
-  const int gj = min(8, nj - 8 * grp);
-  return {in / gj, 8 * grp + in % gj};
+// A wave's results as bfloat16 rows: out[j, i0 ...] for its 32 x 32 blocks,
+// through its area of LDS, so that every store is 16 bytes of rows of 64 or 128.
+// row(j) is the row's first element of the wave's i range, NULL for none; left: the
+// elements of the range that exist, a multiple of 8.  Called by whole waves.
+template <class S, class ROW>
+__device__ __forceinline__ void hl_store_rows(const floatx16 (&acc)[S::FI][S::FJ], char* area, int left, ROW&& row) {
+  constexpr int PI = S::FI < S::AREA_W / 2048 ? S::FI : S::AREA_W / 2048;   // i-blocks of a turn: rows of 64 PI bytes
+  constexpr int GR = 4 * PI;                  // 16-byte granules of a row
+  static_assert(32 * GR * 16 <= S::AREA_W, "the wave's area");
+  int lane = threadIdx.x & (WAVE - 1);
+  asm volatile("" : "+v"(lane));   // (what follows from it is not kept over the product's loop)
+  const int r = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int j = 0; j < S::FJ; ++j)
+#pragma unroll
+    for (int ib = 0; ib < S::FI; ib += PI) {
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < PI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = BF16::from_f32(acc[ib + i][j][4 * q + e]);
+          const int g = (4 * i + q) ^ (r & (GR - 1));
+          *reinterpret_cast<uint2*>(area + 16 * (r * GR + g) + 8 * h) = make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
+        }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int p = 0; p < 32 * GR / WAVE; ++p) {
+        const int rr = p * (WAVE / GR) + lane / GR, g = lane % GR;
+        const uint4 v = *reinterpret_cast<const uint4*>(area + 16 * (rr * GR + (g ^ (rr & (GR - 1)))));
+        uint16_t* out = row(32 * j + rr);
+        const int i = 32 * ib + 8 * g;
+        if (out != nullptr && i < left) *reinterpret_cast<uint4*>(out + i) = v;
+        __builtin_amdgcn_sched_barrier(0);   // (one address live at a time)
+      }
+    }
 }
 
 // ---------------------------------------------------------------- forward
@@ -258,93 +365,115 @@ struct HlArgs {
   int64_t ignore_index;
 };
 
+// Operands of the logits' product: vocabulary rows v0 .., rows n0 ..; the stages.
+template <int BJ>
+__device__ __forceinline__ int hl_logits_operands(const HlArgs& a, int v0, int n0, Operand& A, Operand& B) {
+  A = {a.weight + static_cast<int64_t>(v0) * a.dim, a.dim, min(HL_I, a.vocab - v0), a.dim};
+  B = {a.hidden + n0 * a.ld, a.ld, min(BJ, a.rows - n0), a.dim};
+  return a.dim / HL_K;
+}
+
 }  // namespace
 
 // part[tile rows + n]: max, sum e, sum e d2 of the tile's vocabulary rows, in the
 // order rows run so that a join's loads are coalesced
 template <int BJ>
 __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_head_stats(const HlArgs a, float4* part,
-                                                                                               float* xt, int ni, int nj) {
+                                                                                               float* xt, const Tiles ts) {
   using S = Shape<BJ>;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  const TileIdx t = hl_tile(blockIdx.x, ni, nj);
-  const int v0 = t.i * HL_I, n0 = t.j * BJ;
-  floatx16 acc[S::FI][S::FJ];
-  hl_product<false, false, BJ>({a.weight + static_cast<int64_t>(v0) * a.dim, a.dim, min(HL_I, a.vocab - v0), a.dim},
-                               {a.hidden + n0 * a.ld, a.ld, min(BJ, a.rows - n0), a.dim}, a.dim / HL_K, smem, acc);
+  float* wave_part = reinterpret_cast<float*>(smem + S::NST * S::STAGE);   // [WI][BJ][3]
+  static_assert(S::WI * BJ * 12 <= HL_NW * S::AREA_W, "the area");
   const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
   const int wi = w / S::WJ, wj = w % S::WJ;
-  const int vw = v0 + wi * 32 * S::FI + 4 * (lane >> 5);   // the lane's first vocabulary row
   constexpr float NINF = -__builtin_inff();
-  float* wave_part = reinterpret_cast<float*>(smem);   // [WI][BJ][3]
-  lds_barrier();
-  if (v0 + HL_I > a.vocab) {
+  hl_products<false, false, S>(
+      ts, smem,
+      [&](int t, Operand& A, Operand& B) {
+        int i, j, z;
+        ts.at(t, i, j, z);
+        return hl_logits_operands<BJ>(a, i * HL_I, j * BJ, A, B);
+      },
+      [&](int t, floatx16 (&acc)[S::FI][S::FJ]) {
+        int ti, tj, z;
+        ts.at(t, ti, tj, z);
+        const int v0 = ti * HL_I, n0 = tj * BJ;
+        const int vw = v0 + wi * 32 * S::FI + 4 * (lane >> 5);   // the lane's first vocabulary row
+        lds_barrier();   // (the last tile's parts are read)
+        if (v0 + HL_I > a.vocab) {
 #pragma unroll
-    for (int i = 0; i < S::FI; ++i)
+          for (int i = 0; i < S::FI; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (vw + 32 * i + 8 * (r / 4) + r % 4 >= a.vocab) {
+            for (int r = 0; r < 16; ++r)
+              if (vw + 32 * i + 8 * (r / 4) + r % 4 >= a.vocab) {
 #pragma unroll
-          for (int j = 0; j < S::FJ; ++j) acc[i][j][r] = NINF;
+                for (int j = 0; j < S::FJ; ++j) acc[i][j][r] = NINF;
+              }
         }
-  }
 #pragma unroll
-  for (int j = 0; j < S::FJ; ++j) {
-    const int n = n0 + wj * 32 * S::FJ + 32 * j + (lane & 31);
-    float m = NINF;
+        for (int j = 0; j < S::FJ; ++j) {
+          float m = NINF;
 #pragma unroll
-    for (int i = 0; i < S::FI; ++i)
+          for (int i = 0; i < S::FI; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
-    m = fmaxf(m, __shfl_xor(m, 32, WAVE));
-    const float ref = m == NINF ? 0.0f : m;
-    float s[2] = {0.0f, 0.0f}, u[2] = {0.0f, 0.0f};
+            for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+          m = fmaxf(m, __shfl_xor(m, 32, WAVE));
+          const float ref = m == NINF ? 0.0f : m;
+          float s[2] = {0.0f, 0.0f}, u[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < S::FI; ++i)
+          for (int i = 0; i < S::FI; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float d2 = (acc[i][j][r] - ref) * HL_LOG2E;
-        const float e = __builtin_amdgcn_exp2f(d2);
-        s[r & 1] += e;
-        u[r & 1] = fmaf(e, fmaxf(d2, -200.0f), u[r & 1]);   // (e is 0 there)
-      }
-    float ss = s[0] + s[1], uu = u[0] + u[1];
-    ss += __shfl_xor(ss, 32, WAVE);
-    uu += __shfl_xor(uu, 32, WAVE);
-    if (lane < 32) {   // (the product's stages are read: LDS is free)
-      float* wp = wave_part + 3 * (wi * BJ + wj * 32 * S::FJ + 32 * j + lane);
-      wp[0] = m;
-      wp[1] = ss;
-      wp[2] = uu;
-    }
-    if (n >= a.rows) continue;
-    // the token's logit, by the lane that has it
-    const int64_t tk = a.tokens ? a.tokens[n] : -1;
-    const int64_t d = tk - vw;
-    if (tk >= 0 && tk < a.vocab && d >= 0 && d < 32 * S::FI) {
+            for (int r = 0; r < 16; ++r) {
+              const float d2 = (acc[i][j][r] - ref) * HL_LOG2E;
+              const float e = __builtin_amdgcn_exp2f(d2);
+              s[r & 1] += e;
+              u[r & 1] = fmaf(e, fmaxf(d2, -200.0f), u[r & 1]);   // (e is 0 there)
+            }
+          float ss = s[0] + s[1], uu = u[0] + u[1];
+          ss += __shfl_xor(ss, 32, WAVE);
+          uu += __shfl_xor(uu, 32, WAVE);
+          if (lane < 32) {
+            float* wp = wave_part + 3 * (wi * BJ + wj * 32 * S::FJ + 32 * j + lane);
+            wp[0] = m;
+            wp[1] = ss;
+            wp[2] = uu;
+          }
+        }
+        hl_wait_vm<0>();
+        // the tokens' logits, by the lanes that have them
 #pragma unroll
-      for (int i = 0; i < S::FI; ++i)
+        for (int j = 0; j < S::FJ; ++j) {
+          const int n = n0 + wj * 32 * S::FJ + 32 * j + (lane & 31);
+          const int64_t tk = a.tokens && n < a.rows ? a.tokens[n] : -1;
+          const int64_t d = tk - vw;
+          if (tk >= 0 && tk < a.vocab && d >= 0 && d < 32 * S::FI) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (d == 32 * i + 8 * (r / 4) + r % 4) xt[n] = acc[i][j][r];
-    }
-  }
-  __syncthreads();
-  // the tile's part of each row: the waves' joined
-  for (int q = threadIdx.x; q < BJ && n0 + q < a.rows; q += HL_NT) {
-    float m = NINF, s = 0.0f, u = 0.0f;
+            for (int i = 0; i < S::FI; ++i)
 #pragma unroll
-    for (int i = 0; i < S::WI; ++i) m = fmaxf(m, wave_part[3 * (i * BJ + q)]);
-    const float ref = m == NINF ? 0.0f : m;
+              for (int r = 0; r < 16; ++r) {
+                if (d == 32 * i + 8 * (r / 4) + r % 4) xt[n] = acc[i][j][r];
+                __builtin_amdgcn_sched_barrier(0);   // (one comparison live at a time)
+              }
+          }
+        }
+        lds_barrier();
+        // the tile's part of each row: the waves' joined
+        const int q = threadIdx.x;
+        if (q < BJ && n0 + q < a.rows) {
+          float m = NINF, s = 0.0f, u = 0.0f;
 #pragma unroll
-    for (int i = 0; i < S::WI; ++i) {
-      const float* wp = wave_part + 3 * (i * BJ + q);
-      const float d = (wp[0] - ref) * HL_LOG2E, f = __builtin_amdgcn_exp2f(d);
-      s = fmaf(wp[1], f, s);
-      u = fmaf(fmaf(wp[1], fmaxf(d, -200.0f), wp[2]), f, u);
-    }
-    part[static_cast<int64_t>(t.i) * a.rows + n0 + q] = make_float4(m, s, u, 0.0f);
-  }
+          for (int i = 0; i < S::WI; ++i) m = fmaxf(m, wave_part[3 * (i * BJ + q)]);
+          const float ref = m == NINF ? 0.0f : m;
+#pragma unroll
+          for (int i = 0; i < S::WI; ++i) {
+            const float* wp = wave_part + 3 * (i * BJ + q);
+            const float d = (wp[0] - ref) * HL_LOG2E, f = __builtin_amdgcn_exp2f(d);
+            s = fmaf(wp[1], f, s);
+            u = fmaf(fmaf(wp[1], fmaxf(d, -200.0f), wp[2]), f, u);
+          }
+          part[static_cast<int64_t>(ti) * a.rows + n0 + q] = make_float4(m, s, u, 0.0f);
+        }
+      });
 }
 
 // The parts of each row joined: 8 rows per work-group, 32 threads each, in
@@ -437,126 +566,145 @@ struct HlGrad {
 // the vocabulary 0), bfloat16 [rows, cn]
 template <int BJ>
 __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_head_g(const HlArgs a, const HlGrad gr,
-                                                                                           uint16_t* g, int c0, int cn, int ni,
-                                                                                           int nj) {
+                                                                                           uint16_t* g, int c0, int cn,
+                                                                                           const Tiles ts) {
   using S = Shape<BJ>;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  const TileIdx t = hl_tile(blockIdx.x, ni, nj);
-  const int v0 = c0 + t.i * HL_I, n0 = t.j * BJ;
-  floatx16 acc[S::FI][S::FJ];
-  hl_product<false, false, BJ>({a.weight + static_cast<int64_t>(v0) * a.dim, a.dim, min(HL_I, a.vocab - v0), a.dim},
-                               {a.hidden + n0 * a.ld, a.ld, min(BJ, a.rows - n0), a.dim}, a.dim / HL_K, smem, acc);
   const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
   const int wi = w / S::WJ, wj = w % S::WJ;
-  const int vw = v0 + wi * 32 * S::FI + 4 * (lane >> 5);
+  char* area = smem + S::NST * S::STAGE + w * S::AREA_W;
+  hl_products<false, false, S>(
+      ts, smem,
+      [&](int t, Operand& A, Operand& B) {
+        int i, j, z;
+        ts.at(t, i, j, z);
+        return hl_logits_operands<BJ>(a, c0 + i * HL_I, j * BJ, A, B);
+      },
+      [&](int t, floatx16 (&acc)[S::FI][S::FJ]) {
+        int ti, tj, z;
+        ts.at(t, ti, tj, z);
+        const int i0 = ti * HL_I + wi * 32 * S::FI, n0 = tj * BJ + wj * 32 * S::FJ;   // of the wave
+        const int vw = c0 + i0 + 4 * (lane >> 5);                                     // the lane's first vocabulary row
 #pragma unroll
-  for (int j = 0; j < S::FJ; ++j) {
-    const int n = n0 + wj * 32 * S::FJ + 32 * j + (lane & 31);
-    if (n >= a.rows) continue;
-    const float hi = gr.saved[4 * n], lo = gr.saved[4 * n + 1], H = gr.saved[4 * n + 2];
-    const float gb = gr.gb ? gr.gb[n] : 0.0f, gc = gr.gc ? gr.gc[n] : 0.0f;
-    float ga = gr.ga ? gr.ga[n] : 0.0f;
-    int d = -1;   // the token's place from the lane's first row
-    if (a.tokens) {
-      const int64_t tk = a.tokens[n];
-      if (tk == a.ignore_index) ga = 0.0f;
-      else if (tk < 0 || tk >= a.vocab) ga = ga == 0.0f ? 0.0f : __builtin_nanf("");
-      else d = static_cast<int>(tk) - vw;
-    }
-    const bool zero = ga == 0.0f && gb == 0.0f && gc == 0.0f;
-    const float k0 = gc - ga, h = gb == 0.0f ? 0.0f : H;
-    uint16_t* out = g + static_cast<int64_t>(n) * cn + (vw - c0);
+        for (int j = 0; j < S::FJ; ++j) {
+          const int n = min(n0 + 32 * j + (lane & 31), a.rows - 1);   // (rows past the last are not stored)
+          const float hi = gr.saved[4 * n], lo = gr.saved[4 * n + 1], H = gr.saved[4 * n + 2];
+          const float gb = gr.gb ? gr.gb[n] : 0.0f, gc = gr.gc ? gr.gc[n] : 0.0f;
+          float ga = gr.ga ? gr.ga[n] : 0.0f;
+          int d = -1;   // the token's place from the lane's first row
+          if (a.tokens) {
+            const int64_t tk = a.tokens[n];
+            if (tk == a.ignore_index) ga = 0.0f;
+            else if (tk < 0 || tk >= a.vocab) ga = ga == 0.0f ? 0.0f : __builtin_nanf("");
+            else d = static_cast<int>(tk) - vw;
+          }
+          const bool zero = ga == 0.0f && gb == 0.0f && gc == 0.0f;
+          const float k0 = gc - ga, h = gb == 0.0f ? 0.0f : H;
 #pragma unroll
-    for (int i = 0; i < S::FI; ++i)
+          for (int i = 0; i < S::FI; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int at = 32 * i + 8 * q;
-        if (vw - c0 + at >= cn) continue;   // (cn is a multiple of 64: whole fours)
-        uint16_t o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float l = (acc[i][j][4 * q + e] - hi) - lo;
-          const float p = __builtin_amdgcn_exp2f(l * HL_LOG2E);
-          float v = p * (k0 - gb * (fmaxf(l, -200.0f) + h));
-          if (at + e == d) v += ga;
-          o[e] = zero || vw + at + e >= a.vocab ? 0 : static_cast<uint16_t>(BF16::from_f32(v));
+            for (int r = 0; r < 16; ++r) {
+              const int at = 32 * i + 8 * (r / 4) + r % 4;
+              const float l = (acc[i][j][r] - hi) - lo;
+              const float p = __builtin_amdgcn_exp2f(l * HL_LOG2E);
+              float v = p * (k0 - gb * (fmaxf(l, -200.0f) + h));
+              if (at == d) v += ga;
+              acc[i][j][r] = zero || vw + at >= a.vocab ? 0.0f : v;
+              if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (four results' temporaries live at a time)
+            }
         }
-        *reinterpret_cast<uint2*>(out + at) =
-            make_uint2(o[0] | (static_cast<uint32_t>(o[1]) << 16), o[2] | (static_cast<uint32_t>(o[3]) << 16));
-      }
-  }
+        hl_wait_vm<0>();
+        uint16_t* out = g + static_cast<int64_t>(n0) * cn + i0;
+        const int rows = a.rows - n0;
+        hl_store_rows<S>(acc, area, cn - i0, [&](int q) { return q < rows ? out + static_cast<int64_t>(q) * cn : nullptr; });
+      });
 }
 
 // dweight[c0 + v, d] = sum_n g[n, v] hidden[n, d]: i = d, j = v
 __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_head_dw(const HlArgs a, const uint16_t* g,
-                                                                                            uint16_t* dw, int c0, int cn, int ni,
-                                                                                            int nj) {
-  constexpr int BJ = 256;
-  using S = Shape<BJ>;
+                                                                                            uint16_t* dw, int c0, int cn,
+                                                                                            const Tiles ts) {
+  using S = Shape<256>;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  const TileIdx t = hl_tile(blockIdx.x, ni, nj);
-  const int d0 = t.i * HL_I, j0 = t.j * BJ;
-  floatx16 acc[S::FI][S::FJ];
-  hl_product<true, true, BJ>({a.hidden + d0, a.ld, a.rows, a.dim - d0}, {g + j0, cn, a.rows, cn - j0},
-                             (a.rows + HL_K - 1) / HL_K, smem, acc);
-  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
-  const int d = d0 + (w / S::WJ) * 32 * S::FI + 4 * (lane >> 5);
-#pragma unroll
-  for (int j = 0; j < S::FJ; ++j) {
-    const int v = c0 + j0 + (w % S::WJ) * 32 * S::FJ + 32 * j + (lane & 31);
-    if (v >= a.vocab || v >= c0 + cn) continue;
-    uint16_t* out = dw + static_cast<int64_t>(v) * a.dim + d;
-#pragma unroll
-    for (int i = 0; i < S::FI; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (d + 32 * i + 8 * q >= a.dim) continue;   // (dim is a multiple of 64)
-        uint32_t o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = BF16::from_f32(acc[i][j][4 * q + e]);
-        *reinterpret_cast<uint2*>(out + 32 * i + 8 * q) = make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
-      }
-  }
+  const int w = threadIdx.x / WAVE;
+  char* area = smem + S::NST * S::STAGE + w * S::AREA_W;
+  hl_products<true, true, S>(
+      ts, smem,
+      [&](int t, Operand& A, Operand& B) {
+        int i, j, z;
+        ts.at(t, i, j, z);
+        A = {a.hidden + i * HL_I, a.ld, a.rows, a.dim - i * HL_I};
+        B = {g + j * S::BJ, cn, a.rows, cn - j * S::BJ};
+        return (a.rows + HL_K - 1) / HL_K;
+      },
+      [&](int t, floatx16 (&acc)[S::FI][S::FJ]) {
+        int ti, tj, z;
+        ts.at(t, ti, tj, z);
+        const int d0 = ti * HL_I + (w / S::WJ) * 32 * S::FI, v0 = c0 + tj * S::BJ + (w % S::WJ) * 32 * S::FJ;
+        uint16_t* out = dw + static_cast<int64_t>(v0) * a.dim + d0;
+        const int rows = min(a.vocab, c0 + cn) - v0;
+        hl_wait_vm<0>();
+        hl_store_rows<S>(acc, area, a.dim - d0, [&](int q) { return q < rows ? out + static_cast<int64_t>(q) * a.dim : nullptr; });
+      });
 }
 
-// dhidden's part z: sum over the z-th of `splits` ranges of the chunk's
-// vocabulary rows of g[n, v] weight[c0 + v, d]: i = d, j = n.  first: the part is
-// written, else added to.
+// dhidden's part z: sum over the z-th of nz ranges of the chunk's vocabulary
+// rows of g[n, v] weight[c0 + v, d]: i = d, j = n.  The part is written, or (for a
+// chunk after the first) added to; DIRECT: one part in all, rounded into dhidden.
+template <int BJ, bool DIRECT>
 __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_head_dh(const HlArgs a, const uint16_t* g,
-                                                                                            float* acc_out, int c0, int cn,
-                                                                                            int ni, int nj, int per, int first) {
-  constexpr int BJ = 256;
+                                                                                            float* sum, uint16_t* dh, int c0,
+                                                                                            int cn, const Tiles ts, int per,
+                                                                                            int first) {
   using S = Shape<BJ>;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  const TileIdx t = hl_tile(blockIdx.x, ni, nj);
-  const int d0 = t.i * HL_I, n0 = t.j * BJ, z = blockIdx.y;
-  const int s0 = z * per, stages = max(0, min(cn / HL_K - s0, per));   // (cn is a multiple of 64)
-  const int k0 = s0 * HL_K;
-  floatx16 acc[S::FI][S::FJ];
-  hl_product<true, false, BJ>(
-      {a.weight + static_cast<int64_t>(c0 + k0) * a.dim + d0, a.dim, min(stages * HL_K, a.vocab - c0 - k0), a.dim - d0},
-      {g + static_cast<int64_t>(n0) * cn + k0, cn, min(BJ, a.rows - n0), stages * HL_K}, stages, smem, acc);
   const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
-  const int d = d0 + (w / S::WJ) * 32 * S::FI + 4 * (lane >> 5);
+  char* area = smem + S::NST * S::STAGE + w * S::AREA_W;
+  hl_products<true, false, S>(
+      ts, smem,
+      [&](int t, Operand& A, Operand& B) {
+        int i, j, z;
+        ts.at(t, i, j, z);
+        // (the host's nz leaves no range empty)
+        const int k0 = z * per * HL_K, stages = min(cn / HL_K - z * per, per);
+        A = {a.weight + static_cast<int64_t>(c0 + k0) * a.dim + i * HL_I, a.dim, min(stages * HL_K, a.vocab - c0 - k0),
+             a.dim - i * HL_I};
+        B = {g + static_cast<int64_t>(j) * BJ * cn + k0, cn, min(BJ, a.rows - j * BJ), stages * HL_K};
+        return stages;
+      },
+      [&](int t, floatx16 (&acc)[S::FI][S::FJ]) {
+        int ti, tj, z;
+        ts.at(t, ti, tj, z);
+        const int d0 = ti * HL_I + (w / S::WJ) * 32 * S::FI, n0 = tj * BJ + (w % S::WJ) * 32 * S::FJ;
+        const int rows = a.rows - n0;
+        hl_wait_vm<0>();
+        if constexpr (DIRECT) {
+          uint16_t* out = dh + static_cast<int64_t>(n0) * a.dim + d0;
+          hl_store_rows<S>(acc, area, a.dim - d0,
+                           [&](int q) { return q < rows ? out + static_cast<int64_t>(q) * a.dim : nullptr; });
+        } else {
+          const int d = d0 + 4 * (lane >> 5);
 #pragma unroll
-  for (int j = 0; j < S::FJ; ++j) {
-    const int n = n0 + (w % S::WJ) * 32 * S::FJ + 32 * j + (lane & 31);
-    if (n >= a.rows) continue;
-    float* out = acc_out + (static_cast<int64_t>(z) * a.rows + n) * a.dim + d;
+          for (int j = 0; j < S::FJ; ++j) {
+            const int n = 32 * j + (lane & 31);
+            if (n >= rows) continue;
+            float* out = sum + (static_cast<int64_t>(z) * a.rows + n0 + n) * a.dim + d;
 #pragma unroll
-    for (int i = 0; i < S::FI; ++i)
+            for (int i = 0; i < S::FI; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (d + 32 * i + 8 * q >= a.dim) continue;
-        float4* o = reinterpret_cast<float4*>(out + 32 * i + 8 * q);
-        float4 v = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-        if (!first) {
-          const float4 b = *o;
-          v = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
+              for (int q = 0; q < 4; ++q) {
+                if (d + 32 * i + 8 * q >= a.dim) continue;   // (dim is a multiple of 64)
+                float4* o = reinterpret_cast<float4*>(out + 32 * i + 8 * q);
+                float4 v = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+                if (!first) {
+                  const float4 b = *o;
+                  v = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
+                }
+                *o = v;
+              }
+          }
         }
-        *o = v;
-      }
-  }
+      });
 }
 
 // dhidden = the parts' sum, rounded once; four values per thread
@@ -595,11 +743,17 @@ int hl_chunk(int64_t rows, int64_t vocab) {
   return static_cast<int>(std::min(all, ((all + n - 1) / n + HL_I - 1) / HL_I * HL_I));
 }
 // Ranges of a chunk's vocabulary rows that dhidden's product is split into: as
-// many as give every CU a tile, of 8 stages or more.
+// many as give every CU a tile, of 8 stages or more; each but the last `per`
+// stages, none empty.
 constexpr int HL_CUS = 256;
-int hl_splits(int64_t rows, int64_t dim, int64_t chunk) {
-  const int64_t tiles = static_cast<int64_t>(cdiv(rows, 256)) * cdiv(dim, HL_I);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(HL_CUS / std::max<int64_t>(tiles, 1), chunk / HL_K / 8)));
+struct Split {
+  int nz, per;
+};
+Split hl_split(int64_t rows, int64_t dim, int64_t chunk) {
+  const int64_t tiles = std::max<int64_t>(1, static_cast<int64_t>(cdiv(rows, hl_bj(rows))) * cdiv(dim, HL_I));
+  const int64_t st = chunk / HL_K, want = std::max<int64_t>(1, std::min(HL_CUS / tiles, st / 8));
+  const int per = cdiv(st, want);
+  return {cdiv(st, per), per};
 }
 
 HlArgs hl_args(const void* hidden, const void* weight, int64_t ld, int64_t rows, int64_t dim, int64_t vocab,
@@ -617,14 +771,15 @@ void hl_by_rows(int64_t rows, F&& f) {
   else f(std::integral_constant<int, 256>{});
 }
 
-template <int BJ>
-constexpr int hl_lds() {
-  return Shape<BJ>::NST * Shape<BJ>::STAGE;
-}
-// (above 64 KiB a kernel's dynamic LDS has to be asked for)
-template <class K>
-hipError_t hl_allow(K k, int bytes) {
-  return hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+// Launch of a persistent kernel over the tiles: a work-group per CU at most (each
+// fills a CU's LDS).  Above 64 KiB a kernel's dynamic LDS has to be asked for.
+template <class S, class K, class... A>
+hipError_t hl_launch(K k, const Tiles& ts, hipStream_t s, A... args) {
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
+  if (e != hipSuccess) return e;
+  const int64_t n = static_cast<int64_t>(ts.ni) * ts.nj * ts.nz;
+  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(std::min<int64_t>(n, HL_CUS))), dim3(HL_NT), S::LDS, s, args...);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -638,7 +793,7 @@ size_t head_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t vocab, bool 
   const int64_t cn = hl_chunk(rows, vocab);
   const size_t R = static_cast<size_t>(rows);
   return al(2 * R * static_cast<size_t>(cn)) +
-         (dhidden ? al(4 * R * static_cast<size_t>(dim) * static_cast<size_t>(hl_splits(rows, dim, cn))) : 0);
+         (dhidden ? al(4 * R * static_cast<size_t>(dim) * static_cast<size_t>(hl_split(rows, dim, cn).nz)) : 0);
 }
 
 hipError_t launch_head(const fl_head_args& a, hipStream_t s) {
@@ -649,10 +804,8 @@ hipError_t launch_head(const fl_head_args& a, hipStream_t s) {
   hipError_t e = hipSuccess;
   hl_by_rows(a.rows, [&](auto bj) {
     constexpr int BJ = decltype(bj)::value;
-    const int ni = cdiv(a.vocab, HL_I), nj = cdiv(a.rows, BJ);
-    e = hl_allow(k_head_stats<BJ>, hl_lds<BJ>());
-    if (e == hipSuccess)
-      hipLaunchKernelGGL(k_head_stats<BJ>, dim3(static_cast<unsigned>(ni) * nj), dim3(HL_NT), hl_lds<BJ>(), s, h, part, xt, ni, nj);
+    const Tiles ts = {cdiv(a.vocab, HL_I), cdiv(a.rows, BJ), 1};
+    e = hl_launch<Shape<BJ>>(k_head_stats<BJ>, ts, s, h, part, xt, ts);
   });
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(k_head_join, dim3(cdiv(a.rows, HJ_R)), dim3(HJ_R * HJ_P), 0, s, a, part, xt, parts);
@@ -662,35 +815,39 @@ hipError_t launch_head(const fl_head_args& a, hipStream_t s) {
 hipError_t launch_head_grad(const fl_head_grad_args& a, hipStream_t s) {
   const HlArgs h = hl_args(a.hidden, a.weight, a.ld_hidden, a.rows, a.dim, a.vocab, a.tokens, a.ignore_index);
   const HlGrad gr = {a.saved, a.grad_logprob, a.grad_entropy, a.grad_lse};
-  const int chunk = hl_chunk(a.rows, a.vocab), splits = hl_splits(a.rows, a.dim, chunk);
+  const int chunk = hl_chunk(a.rows, a.vocab), nd = cdiv(a.dim, HL_I);
   uint16_t* g = static_cast<uint16_t*>(a.workspace);
-  float* acc = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + al(2 * static_cast<size_t>(a.rows) * chunk));
-  const int nd = cdiv(a.dim, HL_I), nr = cdiv(a.rows, 256);
-  hipError_t e = hl_allow(k_head_dw, hl_lds<256>());
-  if (e == hipSuccess) e = hl_allow(k_head_dh, hl_lds<256>());
-  if (e != hipSuccess) return e;
-  for (int c0 = 0; c0 < a.vocab; c0 += chunk) {
+  float* sum = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + al(2 * static_cast<size_t>(a.rows) * chunk));
+  uint16_t* dh = static_cast<uint16_t*>(a.out_dhidden);
+  const bool direct = chunk >= a.vocab && hl_split(a.rows, a.dim, chunk).nz == 1;
+  hipError_t e = hipSuccess;
+  for (int c0 = 0; c0 < a.vocab && e == hipSuccess; c0 += chunk) {
     const int cn = static_cast<int>(std::min<int64_t>(chunk, (a.vocab - c0 + HL_K - 1) / HL_K * HL_K));
     const int nc = cdiv(cn, HL_I);
     hl_by_rows(a.rows, [&](auto bj) {
       constexpr int BJ = decltype(bj)::value;
-      const int nj = cdiv(a.rows, BJ);
-      e = hl_allow(k_head_g<BJ>, hl_lds<BJ>());
-      if (e == hipSuccess)
-        hipLaunchKernelGGL(k_head_g<BJ>, dim3(static_cast<unsigned>(nc) * nj), dim3(HL_NT), hl_lds<BJ>(), s, h, gr, g, c0, cn, nc, nj);
+      using S = Shape<BJ>;
+      const Tiles tg = {nc, cdiv(a.rows, BJ), 1};
+      e = hl_launch<S>(k_head_g<BJ>, tg, s, h, gr, g, c0, cn, tg);
+      if (e != hipSuccess || dh == nullptr) return;
+      // (ranges of the first chunk's size, so that a later one has no more of them:
+      // every part that it adds to was written)
+      const Split sp = hl_split(a.rows, a.dim, chunk);
+      const Tiles td = {nd, cdiv(a.rows, BJ), cdiv(cn / HL_K, sp.per)};
+      if (direct) e = hl_launch<S>(k_head_dh<BJ, true>, td, s, h, g, sum, dh, c0, cn, td, sp.per, 1);
+      else e = hl_launch<S>(k_head_dh<BJ, false>, td, s, h, g, sum, dh, c0, cn, td, sp.per, c0 == 0 ? 1 : 0);
     });
-    if (e != hipSuccess) return e;
-    if (a.out_dweight)
-      hipLaunchKernelGGL(k_head_dw, dim3(static_cast<unsigned>(nd) * nc), dim3(HL_NT), hl_lds<256>(), s, h, g,
-                         static_cast<uint16_t*>(a.out_dweight), c0, cn, nd, nc);
-    if (a.out_dhidden)
-      hipLaunchKernelGGL(k_head_dh, dim3(static_cast<unsigned>(nd) * nr, splits), dim3(HL_NT), hl_lds<256>(), s, h, g, acc, c0, cn,
-                         nd, nr, cdiv(cn / HL_K, splits), c0 == 0 ? 1 : 0);
+    if (e == hipSuccess && a.out_dweight) {
+      const Tiles tw = {nd, nc, 1};
+      e = hl_launch<Shape<256>>(k_head_dw, tw, s, h, g, static_cast<uint16_t*>(a.out_dweight), c0, cn, tw);
+    }
   }
-  if (a.out_dhidden) {
+  if (e != hipSuccess) return e;
+  if (dh != nullptr && !direct) {
     const int64_t n4 = a.rows * a.dim / 4;
     hipLaunchKernelGGL(k_head_dh_join, dim3(static_cast<unsigned>(cdiv(n4, 256))), dim3(256), 0, s,
-                       reinterpret_cast<const float4*>(acc), static_cast<uint2*>(a.out_dhidden), n4, splits);
+                       reinterpret_cast<const float4*>(sum), reinterpret_cast<uint2*>(dh), n4,
+                       hl_split(a.rows, a.dim, chunk).nz);
   }
   return hipGetLastError();
 }
