@@ -109,28 +109,31 @@ struct Loader {
       if constexpr (!COLS) {
         const int row = q * 8 + (lane >> 3), g = (lane & 7) ^ ((row >> 1) & 7);
         // (a row that does not exist lies past the range, whatever ld is)
-        voff[p] = row < o.rows ? static_cast<uint32_t>(2 * (row * o.ld + 8 * g)) : 0x80000000u;
+        const uint32_t v = 2u * (static_cast<uint32_t>(row) * static_cast<uint32_t>(o.ld) + 8u * g);
+        voff[p] = row < o.rows ? v : 0x80000000u;
       } else {
         constexpr int GR = T / 8;                  // granules of a k-row
         const int k = q * (WAVE / GR) + lane / GR, g = (lane % GR) ^ (4 * (k & 3));
-        voff[p] = static_cast<uint32_t>(2 * (k * o.ld + 8 * g));
+        voff[p] = 2u * (static_cast<uint32_t>(k) * static_cast<uint32_t>(o.ld) + 8u * g);
       }
     }
   }
-  // stage s into LDS at lds (wave-uniform)
-  __device__ __forceinline__ void load(int s, uint32_t lds) const {
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  // what stage s's loads have in common
+  struct Stage {
+    int32x4 r;
+    uint32_t soff;
+  };
+  __device__ __forceinline__ Stage stage(int s) const {
     if constexpr (!COLS) {
-      const int32x4 r = hl_rsrc(o.p, hl_bytes(o.rows, o.ld, o.width));
-#pragma unroll
-      for (int p = 0; p < LOADS; ++p) hl_load_lds(r, voff[p], static_cast<uint32_t>(2 * HL_K * s), lds + 1024 * (p * HL_NW + w));
+      return {hl_rsrc(o.p, hl_bytes(o.rows, o.ld, o.width)), static_cast<uint32_t>(2 * HL_K * s)};
     } else {
-      const int64_t k0 = static_cast<int64_t>(s) * HL_K;
-      const int64_t left = o.rows - k0;
-      const int32x4 r = hl_rsrc(o.p + k0 * o.ld, hl_bytes(left < HL_K ? left : HL_K, o.ld, o.width));
-#pragma unroll
-      for (int p = 0; p < LOADS; ++p) hl_load_lds(r, voff[p], 0u, lds + 1024 * (p * HL_NW + w));
+      const int64_t k0 = static_cast<int64_t>(s) * HL_K, left = o.rows - k0;
+      return {hl_rsrc(o.p + k0 * o.ld, hl_bytes(left < HL_K ? left : HL_K, o.ld, o.width)), 0u};
     }
+  }
+  // load p of the stage into the tile in LDS at lds + 1024 times the wave
+  __device__ __forceinline__ void load(const Stage& st, int p, uint32_t lds) const {
+    hl_load_lds(st.r, voff[p], st.soff, lds + 1024 * p * HL_NW);
   }
 };
 
@@ -171,7 +174,7 @@ struct Reader {
 // beside them an area for the epilogues.
 template <int BJ_>
 struct Shape {
-  static constexpr int BJ = BJ_, WJ = BJ / 64, WI = HL_NW / WJ, FI = HL_I / (32 * WI), FJ = 2;
+  static constexpr int BJ = BJ_, WJ = BJ / 64, WI = HL_NW / WJ, FI = HL_I / (32 * WI), FJ = BJ / (32 * WJ);
   static constexpr int STAGE = (HL_I + BJ) * HL_K * 2;
   static constexpr int NST = BJ == 256 ? 2 : 3;
   static constexpr int AREA_W = BJ == 128 ? 2048 : 4096;   // per wave
@@ -243,25 +246,40 @@ __device__ __forceinline__ void hl_products(const Tiles& ts, char* smem, OPS&& o
     lb.init(B);
     ls = 0;
   };
-  auto issue = [&]() {   // returns whether there was a stage
-    if (lt >= sh.end) return 0;
-    la.load(ls, lds + lbuf * S::STAGE);
-    lb.load(ls, lds + lbuf * S::STAGE + LA::BYTES);
+  typename LA::Stage sa;
+  typename LB::Stage sb;
+  uint32_t to = 0;
+  auto aim = [&](bool on) {   // at the cursor's stage; past the last, at nothing (zeros into a free place)
+    sa = la.stage(ls);
+    sb = lb.stage(ls);
+    sa.r[2] = on ? sa.r[2] : 0;
+    sb.r[2] = on ? sb.r[2] : 0;
+    to = lds + lbuf * S::STAGE + 1024 * __builtin_amdgcn_readfirstlane(w);
+  };
+  auto load = [&](int p) {
+    if (p < LA::LOADS) la.load(sa, p, to);
+    else lb.load(sb, p - LA::LOADS, to + LA::BYTES);
+  };
+  auto advance = [&]() {
     lbuf = lbuf == NST - 1 ? 0 : lbuf + 1;
     if (++ls == ln) {
       lt += sh.step;
       if (lt < sh.end) open();
     }
-    return 1;
   };
   open();
   int stages = ln;     // of the current tile
   int ahead = 0;       // stages issued past the current one ...
   int landed = 0;      // ... and how many of them this wave has waited for
-  issue();
-  hl_wait_vm<0>();
+#pragma unroll 1
+  for (int s = 0; s < NST && lt < sh.end; ++s) {
+    aim(true);
 #pragma unroll
-  for (int s = 1; s < NST; ++s) ahead += issue();
+    for (int p = 0; p < L; ++p) load(p);
+    advance();
+    if (s == 0) hl_wait_vm<0>();
+    else ++ahead;
+  }
   lds_barrier();
 
   bf16x8 fa[2][S::FI], fb[2][S::FJ];
@@ -274,6 +292,7 @@ __device__ __forceinline__ void hl_products(const Tiles& ts, char* smem, OPS&& o
 #pragma unroll
     for (int j = 0; j < S::FJ; ++j) fb[slot][j] = rb.read(tb, j, ks);
   };
+  constexpr int M = S::FI * S::FJ, KS = HL_K / 16;
 #pragma unroll 1
   for (int t = sh.t; t < sh.end; t += sh.step) {
     floatx16 acc[S::FI][S::FJ];
@@ -283,27 +302,47 @@ __device__ __forceinline__ void hl_products(const Tiles& ts, char* smem, OPS&& o
       for (int j = 0; j < S::FJ; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    auto mfma = [&](int slot, int m) {
+      const int i = m / S::FJ, j = m % S::FJ;
+      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[slot][i], fb[slot][j], acc[i][j], 0, 0, 0);
+    };
     read(0, buf, 0);
 #pragma unroll 1
     for (int s = 0; s < stages; ++s) {
 #pragma unroll
-      for (int ks = 0; ks < HL_K / 16; ++ks) {
-        if (ks < HL_K / 16 - 1) {
-          read((ks + 1) & 1, buf, ks + 1);
-        } else if (ahead > 0) {
-          if (landed > 0) --landed;
-          else if (NST > 2 && ahead > 1) hl_wait_vm<L>();   // (the newest stage may be on its way)
-          else hl_wait_vm<0>();
-          lds_barrier();
-          ahead += issue() - 1;
-          buf = buf == NST - 1 ? 0 : buf + 1;
-          if (s + 1 < stages) read(0, buf, 0);   // (a tile's first ones after the epilogue, which needs the registers)
-        }
+      for (int ks = 0; ks < KS - 1; ++ks) {
+        // (the next fragments are on their way while these are multiplied)
+        read((ks + 1) & 1, buf, ks + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < S::FI; ++i)
+        for (int m = 0; m < M; ++m) mfma(ks & 1, m);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      constexpr int last = (KS - 1) & 1;
+      if (ahead > 0) {
+        if (landed > 0) --landed;
+        else if (NST > 2 && ahead > 1) hl_wait_vm<L>();   // (the newest stage may be on its way)
+        else hl_wait_vm<0>();
+        lds_barrier();
+        --ahead;
+        buf = buf == NST - 1 ? 0 : buf + 1;
+        if (s + 1 < stages) read(0, buf, 0);   // (a tile's first ones after the epilogue, which needs the registers)
+      }
+      // (also past the last stage, without a branch: into the place of one that
+      // every wave has read)
+      const bool more = lt < sh.end;
+      aim(more);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int j = 0; j < S::FJ; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[ks & 1][i], fb[ks & 1][j], acc[i][j], 0, 0, 0);
+      for (int m = 0; m < M; ++m) {
+        mfma(last, m);
+#pragma unroll
+        for (int p = m * L / M; p < (m + 1) * L / M; ++p) load(p);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (more) {
+        advance();
+        ++ahead;
       }
     }
     epilogue(t, acc);
@@ -620,7 +659,8 @@ __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       });
 }
 
-// dweight[c0 + v, d] = sum_n g[n, v] hidden[n, d]: i = d, j = v
+// dweight[c0 + v, d] = sum_n g[n, v] hidden[n, d]: i = d, j = v.  (Tiles of 128 or
+// 64 vocabulary rows are slower for few rows too: 255x1024x50257 58, 61, 73 us.)
 __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_head_dw(const HlArgs a, const uint16_t* g,
                                                                                             uint16_t* dw, int c0, int cn,
                                                                                             const Tiles ts) {
@@ -742,6 +782,13 @@ int hl_chunk(int64_t rows, int64_t vocab) {
   const int64_t n = (all + fit - 1) / fit;
   return static_cast<int>(std::min(all, ((all + n - 1) / n + HL_I - 1) / HL_I * HL_I));
 }
+// j-tile of dhidden's product: few tiles mean many parts, 4 bytes a value each
+// written and read, so smaller ones where they are fewer than 32 (255x1024x50257:
+// 4 tiles of 256 in 61 parts 64 us with their sum, 16 of 64 in 16 parts 47 us).
+int hl_dh_bj(int64_t rows, int64_t dim) {
+  const int64_t nd = cdiv(dim, HL_I);
+  return rows > 128 && cdiv(rows, 256) * nd >= 32 ? 256 : rows > 64 && cdiv(rows, 128) * nd >= 32 ? 128 : 64;
+}
 // Ranges of a chunk's vocabulary rows that dhidden's product is split into: as
 // many as give every CU a tile, of 8 stages or more; each but the last `per`
 // stages, none empty.
@@ -750,7 +797,7 @@ struct Split {
   int nz, per;
 };
 Split hl_split(int64_t rows, int64_t dim, int64_t chunk) {
-  const int64_t tiles = std::max<int64_t>(1, static_cast<int64_t>(cdiv(rows, hl_bj(rows))) * cdiv(dim, HL_I));
+  const int64_t tiles = std::max<int64_t>(1, static_cast<int64_t>(cdiv(rows, hl_dh_bj(rows, dim))) * cdiv(dim, HL_I));
   const int64_t st = chunk / HL_K, want = std::max<int64_t>(1, std::min(HL_CUS / tiles, st / 8));
   const int per = cdiv(st, want);
   return {cdiv(st, per), per};
@@ -762,10 +809,9 @@ HlArgs hl_args(const void* hidden, const void* weight, int64_t ld, int64_t rows,
           static_cast<int>(dim), static_cast<int>(vocab), tokens, ignore_index};
 }
 
-// f(BJ) for the rows' tile
+// f(bj) as a constant
 template <class F>
-void hl_by_rows(int64_t rows, F&& f) {
-  const int bj = hl_bj(rows);
+void hl_by(int bj, F&& f) {
   if (bj == 64) f(std::integral_constant<int, 64>{});
   else if (bj == 128) f(std::integral_constant<int, 128>{});
   else f(std::integral_constant<int, 256>{});
@@ -802,7 +848,7 @@ hipError_t launch_head(const fl_head_args& a, hipStream_t s) {
   const int parts = hl_parts(a.vocab);
   float* xt = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + al(16 * static_cast<size_t>(a.rows) * parts));
   hipError_t e = hipSuccess;
-  hl_by_rows(a.rows, [&](auto bj) {
+  hl_by(hl_bj(a.rows), [&](auto bj) {
     constexpr int BJ = decltype(bj)::value;
     const Tiles ts = {cdiv(a.vocab, HL_I), cdiv(a.rows, BJ), 1};
     e = hl_launch<Shape<BJ>>(k_head_stats<BJ>, ts, s, h, part, xt, ts);
@@ -824,19 +870,23 @@ hipError_t launch_head_grad(const fl_head_grad_args& a, hipStream_t s) {
   for (int c0 = 0; c0 < a.vocab && e == hipSuccess; c0 += chunk) {
     const int cn = static_cast<int>(std::min<int64_t>(chunk, (a.vocab - c0 + HL_K - 1) / HL_K * HL_K));
     const int nc = cdiv(cn, HL_I);
-    hl_by_rows(a.rows, [&](auto bj) {
+    hl_by(hl_bj(a.rows), [&](auto bj) {
       constexpr int BJ = decltype(bj)::value;
       using S = Shape<BJ>;
       const Tiles tg = {nc, cdiv(a.rows, BJ), 1};
       e = hl_launch<S>(k_head_g<BJ>, tg, s, h, gr, g, c0, cn, tg);
-      if (e != hipSuccess || dh == nullptr) return;
-      // (ranges of the first chunk's size, so that a later one has no more of them:
-      // every part that it adds to was written)
-      const Split sp = hl_split(a.rows, a.dim, chunk);
-      const Tiles td = {nd, cdiv(a.rows, BJ), cdiv(cn / HL_K, sp.per)};
-      if (direct) e = hl_launch<S>(k_head_dh<BJ, true>, td, s, h, g, sum, dh, c0, cn, td, sp.per, 1);
-      else e = hl_launch<S>(k_head_dh<BJ, false>, td, s, h, g, sum, dh, c0, cn, td, sp.per, c0 == 0 ? 1 : 0);
     });
+    if (e == hipSuccess && dh != nullptr)
+      hl_by(hl_dh_bj(a.rows, a.dim), [&](auto bj) {
+        constexpr int BJ = decltype(bj)::value;
+        using S = Shape<BJ>;
+        // (ranges of the first chunk's size, so that a later one has no more of them:
+        // every part that it adds to was written)
+        const Split sp = hl_split(a.rows, a.dim, chunk);
+        const Tiles td = {nd, cdiv(a.rows, BJ), cdiv(cn / HL_K, sp.per)};
+        if (direct) e = hl_launch<S>(k_head_dh<BJ, true>, td, s, h, g, sum, dh, c0, cn, td, sp.per, 1);
+        else e = hl_launch<S>(k_head_dh<BJ, false>, td, s, h, g, sum, dh, c0, cn, td, sp.per, c0 == 0 ? 1 : 0);
+      });
     if (e == hipSuccess && a.out_dweight) {
       const Tiles tw = {nd, nc, 1};
       e = hl_launch<Shape<256>>(k_head_dw, tw, s, h, g, static_cast<uint16_t*>(a.out_dweight), c0, cn, tw);

@@ -111,24 +111,27 @@ def _forward(x: torch.Tensor, lead, tok: Optional[torch.Tensor], top_k: int, ent
 class _Score(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tok, top_k, entropy, lse, rank, ignore_index):
-        x = _rows(logits.detach(), "logits")
+        x = _rows(logits, "logits")
         out = _forward(x, logits.shape[:-1], tok, top_k, entropy, lse, rank, ignore_index, True)
         ctx.set_materialize_grads(False)
+        # (checked in backward for changes in place)
         ctx.save_for_backward(logits) if tok is None else ctx.save_for_backward(logits, tok)
-        # (this node's own: no caller sees or changes it)
-        ctx.saved, ctx.ignore_index = out[6], ignore_index
+        # What the backward launch needs, made here: the engine runs backward on a
+        # thread of its own, where the same Python takes twice the time.  The saved
+        # statistics are this node's own: no caller sees or changes them.
+        ctx.args = _grad_args(x, tok, out[6], ignore_index)
+        ctx.keep = (x, out[6])
         ctx.mark_non_differentiable(*(t for t in out[3:6] if t is not None))
         return out[:6]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_lp, g_h, g_lse, *_):
-        logits, *tok = ctx.saved_tensors
+        logits = ctx.saved_tensors[0]
         if g_lp is None and g_h is None and g_lse is None:
             return (None,) * 7
         # (the engine has checked the gradients' shapes, types and device)
-        d = _backward(_rows(logits, "logits"), logits.shape, tok[0] if tok else None, ctx.saved,
-                      *(None if g is None else g.contiguous() for g in (g_lp, g_h, g_lse)), ctx.ignore_index)
+        d = _backward(ctx.args, logits, *(None if g is None else g.contiguous() for g in (g_lp, g_h, g_lse)))
         return d, None, None, None, None, None, None
 
 
@@ -202,19 +205,23 @@ def score_tokens_backward(logits: torch.Tensor, tokens: Optional[torch.Tensor], 
         gc = _upstream(grad_lse, lead, dev, "grad_lse")
         if ga is not None and tok is None:
             raise ValueError("grad_logprob needs tokens")
-        return _backward(x, logits.shape, tok, saved, ga, gb, gc, int(ignore_index))
+        return _backward(_grad_args(x, tok, saved, int(ignore_index)), logits, ga, gb, gc)
 
 
-def _backward(x, shape, tok, saved, ga, gb, gc, ignore_index: int) -> torch.Tensor:
+def _grad_args(x, tok, saved, ignore_index: int) -> ScoreGradArgs:
+    """The arguments that do not depend on the upstream gradients."""
     R, V = x.shape
-    out = torch.empty(shape, dtype=x.dtype, device=x.device)
     a = ScoreGradArgs()
     a.struct_size = ctypes.sizeof(ScoreGradArgs)
     a.dtype = _DTYPES[x.dtype]
     a.logits = x.data_ptr()
     a.rows, a.vocab, a.ld = R, V, x.stride(0) if R > 1 else V
-    a.tokens, a.ignore_index, a.saved = ptr(tok), ignore_index, saved.data_ptr()
-    a.grad_logprob, a.grad_entropy, a.grad_lse = ptr(ga), ptr(gb), ptr(gc)
-    a.out_grad, a.out_ld = out.data_ptr(), V
-    call(lib().fl_score_tokens_grad, a, x.device, "fl_score_tokens_grad")
+    a.tokens, a.ignore_index, a.saved, a.out_ld = ptr(tok), ignore_index, saved.data_ptr(), V
+    return a
+
+
+def _backward(a: ScoreGradArgs, logits, ga, gb, gc) -> torch.Tensor:
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    a.grad_logprob, a.grad_entropy, a.grad_lse, a.out_grad = ptr(ga), ptr(gb), ptr(gc), out.data_ptr()
+    call(lib().fl_score_tokens_grad, a, out.device, "fl_score_tokens_grad")
     return out
