@@ -246,6 +246,36 @@ def lib() -> ctypes.CDLL:
     return handle
 
 
+AUTOGRAD_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "_fl_autograd.so")
+_AUTOGRAD_ENTRIES = ("fl_last_error", "fl_score_tokens", "fl_score_workspace_bytes", "fl_score_tokens_grad", "fl_layer_norm",
+                     "fl_layer_norm_grad", "fl_layer_norm_grad_workspace_bytes", "fl_head_logprobs", "fl_head_workspace_bytes",
+                     "fl_head_logprobs_grad", "fl_head_grad_workspace_bytes")
+_autograd = None
+
+
+def autograd():
+    """The extension with the differentiable calls' autograd nodes (loaded once),
+    bound to this library's entry points."""
+    global _autograd
+    if _autograd is not None:
+        return _autograd
+    handle = lib()
+    if not os.path.exists(AUTOGRAD_PATH):
+        raise SamplerLibraryError(f"{AUTOGRAD_PATH} is missing: build it with `python -m rl_project_amd.build`")
+    from importlib.machinery import ExtensionFileLoader
+    from importlib.util import module_from_spec, spec_from_file_location
+
+    spec = spec_from_file_location("_fl_autograd", AUTOGRAD_PATH, loader=ExtensionFileLoader("_fl_autograd", AUTOGRAD_PATH))
+    try:
+        module = module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except ImportError as exc:
+        raise SamplerLibraryError(f"cannot load {AUTOGRAD_PATH}: {exc}") from exc
+    module.bind([ctypes.cast(getattr(handle, n), ctypes.c_void_p).value for n in _AUTOGRAD_ENTRIES])
+    _autograd = module
+    return module
+
+
 def check(rc: int, what: str) -> None:
     if rc != FL_OK:
         msg = lib().fl_last_error().decode(errors="replace")

@@ -1,4 +1,5 @@
-"""Build libflsampler.so in-tree from ``rl_project_amd/csrc/*.hip`` for gfx950.
+"""Build libflsampler.so in-tree from ``rl_project_amd/csrc/*.hip`` for gfx950, and
+the autograd nodes over it (``csrc/fl_autograd.cpp``, a torch extension).
 
     python -m rl_project_amd.build [-v]
 
@@ -21,6 +22,7 @@ CSRC = os.path.join(PKG, "csrc")
 OBJ_DIR = os.path.join(PKG, "_build")
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libflsampler.so")
+AUTOGRAD_PATH = os.path.join(LIB_DIR, "_fl_autograd.so")
 ARCH = os.environ.get("FL_OFFLOAD_ARCH", "gfx950")
 
 # Correctly rounded float32 division (the reference's x / T is IEEE division),
@@ -78,14 +80,41 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _build_autograd(verbose: bool) -> str:
+    """Compile and link csrc/fl_autograd.cpp (host code alone) against the installed torch."""
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    tmp = AUTOGRAD_PATH + ".tmp"
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1",
+           "-DUSE_ROCM=1", "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_fl_autograd",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{p}" for p in (f"{root}/include", f"{root}/include/torch/csrc/api/include", "/opt/rocm/include",
+                                      sysconfig.get_paths()["include"])),
+           os.path.join(CSRC, "fl_autograd.cpp"), f"-L{root}/lib", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch",
+           "-ltorch_python", "-o", tmp]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"the autograd extension failed to build:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, AUTOGRAD_PATH)
+    return AUTOGRAD_PATH
+
+
 def build(verbose: bool = False, jobs: int = 0) -> str:
-    """Compile every kernel source and link the shared library; returns its path."""
+    """Compile every kernel source and link the shared library, and the autograd
+    extension; returns the library's path."""
     os.makedirs(OBJ_DIR, exist_ok=True)
     os.makedirs(LIB_DIR, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
     jobs = jobs or min(len(srcs), max(1, (os.cpu_count() or 2) // 2), 8)
     with ThreadPoolExecutor(max_workers=jobs) as ex:
+        ext = ex.submit(_build_autograd, verbose)
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
+        ext.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp]
     if verbose:

@@ -1,0 +1,330 @@
+// Autograd nodes of the differentiable calls (score_tokens, layer_norm,
+// lm_head_logprobs) as a torch extension over the C ABI (include/fl_sampler.h).
+// The kernels are the library's; what is here is what a torch.autograd.Function
+// would do in Python, which costs more than the small calls' kernels: the
+// engine runs backward on a thread of its own, where a Python node waits for the
+// interpreter as well (layer_norm 255x1025, forward and gradients: 110 us of host
+// time as a Python node).
+//
+// The Python callers have checked every argument; the entry points come from the
+// library that Python loaded (bind).
+#include <torch/extension.h>
+
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
+#include <optional>
+#include <string>
+#include <vector>
+
+#include "../../include/fl_sampler.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<Tensor>;
+
+struct Entry {
+  decltype(&fl_last_error) last_error = nullptr;
+  decltype(&fl_score_tokens) score = nullptr;
+  decltype(&fl_score_workspace_bytes) score_ws = nullptr;
+  decltype(&fl_score_tokens_grad) score_grad = nullptr;
+  decltype(&fl_layer_norm) norm = nullptr;
+  decltype(&fl_layer_norm_grad) norm_grad = nullptr;
+  decltype(&fl_layer_norm_grad_workspace_bytes) norm_ws = nullptr;
+  decltype(&fl_head_logprobs) head = nullptr;
+  decltype(&fl_head_workspace_bytes) head_ws = nullptr;
+  decltype(&fl_head_logprobs_grad) head_grad = nullptr;
+  decltype(&fl_head_grad_workspace_bytes) head_grad_ws = nullptr;
+} L;
+
+void bind(const std::vector<uintptr_t>& p) {
+  TORCH_CHECK(p.size() == 11, "fl_autograd: 11 entry points expected");
+  auto at = [&](size_t i, auto& f) { f = reinterpret_cast<std::decay_t<decltype(f)>>(p[i]); };
+  at(0, L.last_error), at(1, L.score), at(2, L.score_ws), at(3, L.score_grad), at(4, L.norm), at(5, L.norm_grad),
+      at(6, L.norm_ws), at(7, L.head), at(8, L.head_ws), at(9, L.head_grad), at(10, L.head_grad_ws);
+}
+
+void check(int rc, const char* what) {
+  if (rc == FL_OK) return;
+  const std::string msg = std::string(what) + " failed (" + std::to_string(rc) + "): " + L.last_error();
+  if (rc == FL_EINVAL) C10_THROW_ERROR(ValueError, msg);
+  if (rc == FL_ENOTSUP) C10_THROW_ERROR(NotImplementedError, msg);
+  C10_THROW_ERROR(Error, msg);
+}
+
+int dtype_of(at::ScalarType t) {
+  return t == at::kFloat ? FL_DTYPE_F32 : t == at::kBFloat16 ? FL_DTYPE_BF16 : FL_DTYPE_F16;
+}
+
+// [rows, n] with contiguous rows (a copy where they are not)
+Tensor rows_of(const Tensor& x) {
+  if (x.dim() == 2 && x.is_contiguous()) return x;
+  Tensor r = x.reshape({-1, x.size(-1)});
+  if ((r.size(1) > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < r.size(1))) r = r.contiguous();
+  return r;
+}
+// The head's: rows that 16-byte loads can take, and an offset of their stride
+Tensor hidden_rows(const Tensor& x) {
+  Tensor h = x.reshape({-1, x.size(-1)});
+  if (h.stride(1) != 1 || (h.size(0) > 1 && (h.stride(0) < h.size(1) || h.stride(0) % 8 != 0 || h.stride(0) > (1 << 21))))
+    h = h.contiguous();
+  if (reinterpret_cast<uintptr_t>(h.data_ptr()) % 16 != 0) h = h.clone(at::MemoryFormat::Contiguous);
+  return h;
+}
+int64_t row_stride(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+template <class T = void>
+T* ptr(const Tensor& t) {
+  return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
+}
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+Tensor floats(at::IntArrayRef shape, const Tensor& like) { return at::empty(shape, like.options().dtype(at::kFloat)); }
+Tensor bytes(size_t n, const Tensor& like) {
+  return at::empty({static_cast<int64_t>(n)}, like.options().dtype(at::kByte));
+}
+
+// Results of a backward pass that has none of its own: one that is asked to
+// record its graph returns results that raise when differentiated.
+variable_list once(variable_list out) {
+  if (!at::GradMode::is_enabled()) return out;
+  auto e = std::make_shared<torch::autograd::DelayedError>(
+      "this call is differentiable once: its gradients have no gradients", static_cast<int>(out.size()));
+  return (*e)(std::move(out));
+}
+
+Tensor upstream(const Tensor& g) { return g.defined() ? g.contiguous() : g; }
+
+// ---------------------------------------------------------------- layer norm
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+    const Tensor x2 = rows_of(x);
+    const Tensor w = weight ? weight->contiguous() : Tensor(), b = bias ? bias->contiguous() : Tensor();
+    const Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+    const Tensor stats = floats({2, x2.size(0)}, x);
+    fl_norm_args a = {};
+    a.struct_size = sizeof(a);
+    a.dtype = dtype_of(x.scalar_type());
+    a.wdtype = w.defined() ? dtype_of(w.scalar_type()) : b.defined() ? dtype_of(b.scalar_type()) : a.dtype;
+    a.eps = static_cast<float>(eps);
+    a.x = x2.data_ptr();
+    a.rows = x2.size(0), a.dim = x2.size(1), a.ld = row_stride(x2);
+    a.weight = ptr(w), a.bias = ptr(b);
+    a.out = y.data_ptr(), a.out_ld = a.dim;
+    a.out_mean = ptr<float>(stats), a.out_rstd = a.out_mean + a.rows;
+    const c10::DeviceGuard guard(x.device());
+    check(L.norm(&a, stream_of(x)), "fl_layer_norm");
+    ctx->save_for_backward({x, weight ? *weight : Tensor()});
+    ctx->saved_data["stats"] = stats;   // (this node's own: no caller sees or changes it)
+    ctx->saved_data["bias"] = bias ? static_cast<int64_t>(bias->scalar_type()) : int64_t{-1};
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor stats = ctx->saved_data["stats"].toTensor();
+    const int64_t btype = ctx->saved_data["bias"].toInt();
+    variable_list out(4);
+    {
+      const at::NoGradGuard no_grad;
+      const Tensor& x = saved[0];
+      const Tensor x2 = rows_of(x), g2 = rows_of(grads[0]), w = saved[1].defined() ? saved[1].contiguous() : Tensor();
+      const int64_t D = x2.size(1);
+      if (ctx->needs_input_grad(0)) out[0] = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+      if (w.defined() && ctx->needs_input_grad(1)) out[1] = at::empty({D}, w.options());
+      // (the edges are those of the tensors given: without a weight the bias is the second)
+      if (btype >= 0 && ctx->needs_input_grad(w.defined() ? 2 : 1)) out[2] = at::empty({D}, x.options().dtype(static_cast<at::ScalarType>(btype)));
+      fl_norm_grad_args a = {};
+      a.struct_size = sizeof(a);
+      a.dtype = dtype_of(x.scalar_type());
+      a.wdtype = w.defined() ? dtype_of(w.scalar_type()) : btype >= 0 ? dtype_of(static_cast<at::ScalarType>(btype)) : a.dtype;
+      a.x = x2.data_ptr();
+      a.rows = x2.size(0), a.dim = D, a.ld = row_stride(x2);
+      a.weight = ptr(w);
+      a.grad = g2.data_ptr(), a.grad_ld = row_stride(g2);
+      a.mean = ptr<float>(stats), a.rstd = a.mean + a.rows;
+      a.out_dx = ptr(out[0]), a.out_ld = D;
+      a.out_dweight = ptr(out[1]), a.out_dbias = ptr(out[2]);
+      Tensor ws;
+      if (a.out_dweight != nullptr || a.out_dbias != nullptr) {
+        size_t n = 0;
+        check(L.norm_ws(a.rows, D, a.dtype, &n), "fl_layer_norm_grad_workspace_bytes");
+        ws = bytes(n, x);
+        a.workspace = ws.data_ptr(), a.workspace_bytes = static_cast<int64_t>(n);
+      }
+      const c10::DeviceGuard guard(x.device());
+      check(L.norm_grad(&a, stream_of(x)), "fl_layer_norm_grad");
+    }
+    return once(std::move(out));
+  }
+};
+
+// ---------------------------------------------------------------- scores
+// Results: those asked for, in the order logprob, entropy, lse, rank, top ids,
+// top logprobs.
+struct Score : torch::autograd::Function<Score> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const OptTensor& tokens, int64_t top_k, bool entropy,
+                               bool lse, bool rank, int64_t ignore_index) {
+    const Tensor x = rows_of(logits);
+    const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+    std::vector<int64_t> top(lead.begin(), lead.end());
+    top.push_back(top_k);
+    const auto opt = logits.options();
+    Tensor lp, ent, ls, rk, ids, tl;
+    if (tokens) lp = floats(lead, x);
+    if (entropy) ent = floats(lead, x);
+    if (lse) ls = floats(lead, x);
+    if (rank) rk = at::empty(lead, opt.dtype(at::kInt));
+    if (top_k > 0) {
+      ids = at::empty(top, opt.dtype(at::kLong));
+      tl = floats(top, x);
+    }
+    const Tensor saved = floats({x.size(0), 4}, x);
+    fl_score_args a = {};
+    a.struct_size = sizeof(a);
+    a.dtype = dtype_of(x.scalar_type());
+    a.logits = x.data_ptr();
+    a.rows = x.size(0), a.vocab = x.size(1), a.ld = row_stride(x);
+    a.tokens = tokens ? ptr<int64_t>(*tokens) : nullptr;
+    a.ignore_index = ignore_index, a.top_k = top_k;
+    a.out_logprob = ptr<float>(lp), a.out_entropy = ptr<float>(ent), a.out_lse = ptr<float>(ls), a.out_rank = ptr<int32_t>(rk);
+    a.out_top_ids = ptr<int64_t>(ids), a.out_top_logprobs = ptr<float>(tl), a.out_saved = ptr<float>(saved);
+    size_t n = 0;
+    check(L.score_ws(a.rows, a.vocab, top_k, &n), "fl_score_workspace_bytes");
+    const Tensor ws = bytes(n, x);
+    a.workspace = ws.data_ptr(), a.workspace_bytes = static_cast<int64_t>(n);
+    const c10::DeviceGuard guard(x.device());
+    check(L.score(&a, stream_of(x)), "fl_score_tokens");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, tokens ? *tokens : Tensor()});
+    ctx->saved_data["saved"] = saved;   // (this node's own: no caller sees or changes it)
+    ctx->saved_data["has"] = (tokens ? 1 : 0) | (entropy ? 2 : 0) | (lse ? 4 : 0);
+    ctx->saved_data["ignore"] = ignore_index;
+    variable_list out, plain;
+    for (const Tensor& t : {lp, ent, ls}) if (t.defined()) out.push_back(t);
+    for (const Tensor& t : {rk, ids, tl}) if (t.defined()) plain.push_back(t);
+    ctx->mark_non_differentiable(plain);
+    out.insert(out.end(), plain.begin(), plain.end());
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto kept = ctx->get_saved_variables();
+    const int64_t has = ctx->saved_data["has"].toInt();
+    Tensor g[3];
+    for (size_t i = 0, k = 0; i < 3; ++i)
+      if (has & (1 << i)) g[i] = upstream(grads[k++]);
+    variable_list out(7);
+    if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return out;
+    {
+      const at::NoGradGuard no_grad;
+      const Tensor& logits = kept[0];
+      const Tensor x = rows_of(logits), saved = ctx->saved_data["saved"].toTensor();
+      out[0] = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
+      fl_score_grad_args a = {};
+      a.struct_size = sizeof(a);
+      a.dtype = dtype_of(x.scalar_type());
+      a.logits = x.data_ptr();
+      a.rows = x.size(0), a.vocab = x.size(1), a.ld = row_stride(x);
+      a.tokens = ptr<int64_t>(kept[1]);
+      a.ignore_index = ctx->saved_data["ignore"].toInt();
+      a.saved = ptr<float>(saved);
+      a.grad_logprob = ptr<float>(g[0]), a.grad_entropy = ptr<float>(g[1]), a.grad_lse = ptr<float>(g[2]);
+      a.out_grad = out[0].data_ptr(), a.out_ld = a.vocab;
+      const c10::DeviceGuard guard(x.device());
+      check(L.score_grad(&a, stream_of(x)), "fl_score_tokens_grad");
+    }
+    return once(std::move(out));
+  }
+};
+
+// ---------------------------------------------------------------- head
+// Results: those asked for, in the order logprob, entropy, lse.
+struct Head : torch::autograd::Function<Head> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const OptTensor& tokens,
+                               bool entropy, bool lse, int64_t ignore_index) {
+    const Tensor h = hidden_rows(hidden);
+    const auto lead = hidden.sizes().slice(0, hidden.dim() - 1);
+    Tensor lp, ent, ls;
+    if (tokens) lp = floats(lead, h);
+    if (entropy) ent = floats(lead, h);
+    if (lse) ls = floats(lead, h);
+    const Tensor saved = floats({h.size(0), 4}, h);
+    fl_head_args a = {};
+    a.struct_size = sizeof(a);
+    a.dtype = FL_DTYPE_BF16;
+    a.hidden = h.data_ptr(), a.weight = weight.data_ptr();
+    a.rows = h.size(0), a.dim = h.size(1), a.vocab = weight.size(0), a.ld_hidden = row_stride(h);
+    a.tokens = tokens ? ptr<int64_t>(*tokens) : nullptr;
+    a.ignore_index = ignore_index;
+    a.out_logprob = ptr<float>(lp), a.out_entropy = ptr<float>(ent), a.out_lse = ptr<float>(ls), a.out_saved = ptr<float>(saved);
+    size_t n = 0;
+    check(L.head_ws(a.rows, a.vocab, &n), "fl_head_workspace_bytes");
+    const Tensor ws = bytes(n, h);
+    a.workspace = ws.data_ptr(), a.workspace_bytes = static_cast<int64_t>(n);
+    const c10::DeviceGuard guard(h.device());
+    check(L.head(&a, stream_of(h)), "fl_head_logprobs");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({hidden, weight, tokens ? *tokens : Tensor()});
+    ctx->saved_data["saved"] = saved;   // (this node's own: no caller sees or changes it)
+    ctx->saved_data["has"] = (tokens ? 1 : 0) | (entropy ? 2 : 0) | (lse ? 4 : 0);
+    ctx->saved_data["ignore"] = ignore_index;
+    variable_list out;
+    for (const Tensor& t : {lp, ent, ls}) if (t.defined()) out.push_back(t);
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto kept = ctx->get_saved_variables();
+    const int64_t has = ctx->saved_data["has"].toInt();
+    Tensor g[3];
+    for (size_t i = 0, k = 0; i < 3; ++i)
+      if (has & (1 << i)) g[i] = upstream(grads[k++]);
+    variable_list out(6);
+    if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return out;
+    {
+      const at::NoGradGuard no_grad;
+      const Tensor &hidden = kept[0], &weight = kept[1];
+      const Tensor h = hidden_rows(hidden), saved = ctx->saved_data["saved"].toTensor();
+      if (ctx->needs_input_grad(0))
+        out[0] = at::empty(hidden.sizes(), hidden.options().memory_format(at::MemoryFormat::Contiguous));
+      if (ctx->needs_input_grad(1))   // (no rows: no sums)
+        out[1] = h.size(0) == 0 ? at::zeros(weight.sizes(), weight.options()) : at::empty(weight.sizes(), weight.options());
+      fl_head_grad_args a = {};
+      a.struct_size = sizeof(a);
+      a.dtype = FL_DTYPE_BF16;
+      a.hidden = h.data_ptr(), a.weight = weight.data_ptr();
+      a.rows = h.size(0), a.dim = h.size(1), a.vocab = weight.size(0), a.ld_hidden = row_stride(h);
+      a.tokens = ptr<int64_t>(kept[2]);
+      a.ignore_index = ctx->saved_data["ignore"].toInt();
+      a.saved = ptr<float>(saved);
+      a.grad_logprob = ptr<float>(g[0]), a.grad_entropy = ptr<float>(g[1]), a.grad_lse = ptr<float>(g[2]);
+      a.out_dhidden = ptr(out[0]), a.out_dweight = ptr(out[1]);
+      size_t n = 0;
+      check(L.head_grad_ws(a.rows, a.dim, a.vocab, out[0].defined() ? 1 : 0, &n), "fl_head_grad_workspace_bytes");
+      const Tensor ws = bytes(n, h);
+      a.workspace = ws.data_ptr(), a.workspace_bytes = static_cast<int64_t>(n);
+      const c10::DeviceGuard guard(h.device());
+      check(L.head_grad(&a, stream_of(h)), "fl_head_logprobs_grad");
+    }
+    return once(std::move(out));
+  }
+};
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("bind", &bind);
+  m.def("layer_norm", [](const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) { return LayerNorm::apply(x, w, b, eps); },
+        py::call_guard<py::gil_scoped_release>());
+  m.def("score", [](const Tensor& x, const OptTensor& t, int64_t k, bool e, bool l, bool r, int64_t ii) {
+    return Score::apply(x, t, k, e, l, r, ii);
+  }, py::call_guard<py::gil_scoped_release>());
+  m.def("head", [](const Tensor& h, const Tensor& w, const OptTensor& t, bool e, bool l, int64_t ii) {
+    return Head::apply(h, w, t, e, l, ii);
+  }, py::call_guard<py::gil_scoped_release>());
+}

@@ -117,28 +117,6 @@ def _backward(h, shape, weight, tok, saved, ga, gb, gc, ignore_index: int, need_
     return dh, dw
 
 
-class _HeadLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, tok, entropy, lse, ignore_index):
-        out = _forward(_hidden_rows(hidden.detach()), hidden.shape[:-1], weight.detach(), tok, entropy, lse, ignore_index, True)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(*(t for t in (hidden, weight, tok) if t is not None))
-        # (this node's own: no caller sees or changes it)
-        ctx.saved, ctx.ignore_index = out[3], ignore_index
-        return out[:3]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_lp, g_h, g_lse):
-        hidden, weight, *tok = ctx.saved_tensors
-        if g_lp is None and g_h is None and g_lse is None:
-            return (None,) * 6
-        dh, dw = _backward(_hidden_rows(hidden), hidden.shape, weight, tok[0] if tok else None, ctx.saved,
-                           *(None if g is None else g.contiguous() for g in (g_lp, g_h, g_lse)), ctx.ignore_index,
-                           *ctx.needs_input_grad[:2])
-        return dh, dw, None, None, None, None
-
-
 def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optional[torch.Tensor] = None, *,
                      entropy: bool = False, lse: bool = False, norm=None, ignore_index: int = IGNORE_INDEX,
                      check_tokens: bool = False, return_saved: bool = False):
@@ -170,7 +148,10 @@ def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optiona
         if return_saved:
             raise ValueError("return_saved is for calls under torch.no_grad()")
         _no_autograd_under_capture("lm_head_logprobs")
-        return HeadScores(*_HeadLogprobs.apply(hidden, weight, tok, bool(entropy), bool(lse), int(ignore_index)))
+        if tok is None and not entropy and not lse:
+            raise ValueError("nothing is asked for: give tokens, entropy=True or lse=True")
+        out = iter(_lib.autograd().head(hidden, weight, tok, bool(entropy), bool(lse), int(ignore_index)))
+        return HeadScores(*(next(out) if on else None for on in (tok is not None, entropy, lse)))
     out = _forward(_hidden_rows(hidden), lead, weight, tok, entropy, lse, int(ignore_index), return_saved)
     s = HeadScores(*out[:3])
     return (s, out[3]) if return_saved else s

@@ -73,30 +73,6 @@ def _forward(x2, lead_shape, weight, bias, eps: float, stats: bool):
     return y, mean, rstd
 
 
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        x2 = _x_rows(x, "x")
-        w, b = _affine(weight, x, "weight"), _affine(bias, x, "bias")
-        y, mean, rstd = _forward(x2, x.shape, w, b, eps, True)
-        ctx.save_for_backward(x, weight)   # (checked there for changes in place)
-        # What the backward launch needs, made here: the engine runs backward on a
-        # thread of its own, where the same Python takes twice the time.  mean and
-        # rstd are this node's own: no caller sees or changes them.
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
-        ctx.args = _grad_args(x2, w, b, mean, rstd)
-        ctx.keep = (x2, w, mean, rstd)
-        ctx.out = (need_x, w.dtype if need_w else None, b.dtype if need_b else None)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        x, _ = ctx.saved_tensors
-        # (the engine has checked the gradient's shape, type and device)
-        return (*_backward(ctx.args, _x_rows(grad, "grad"), x.shape, *ctx.out), None)
-
-
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5, *, return_stats: bool = False):
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of
@@ -114,7 +90,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         if return_stats:
             raise ValueError("return_stats is for calls under torch.no_grad()")
         _no_autograd_under_capture("layer_norm", "return_stats")
-        return _LayerNorm.apply(x, weight, bias, eps)
+        _wdtype(x, _affine(weight, x, "weight"), _affine(bias, x, "bias"))
+        return _lib.autograd().layer_norm(x, weight, bias, eps)
     y, mean, rstd = _forward(x2, x.shape, _affine(weight, x, "weight"), _affine(bias, x, "bias"), eps, return_stats)
     return (y, NormStats(mean, rstd)) if return_stats else y
 
@@ -140,9 +117,24 @@ def layer_norm_backward(grad: torch.Tensor, x: torch.Tensor, weight: Optional[to
             if t.shape != (R,) or t.dtype != torch.float32 or t.device != dev or not t.is_contiguous():
                 raise ValueError(f"stats must be the forward call's: two float32 [{R}] tensors")
         w, b = _affine(weight, x, "weight"), _affine(bias, x, "bias")
-        return _backward(_grad_args(x2, w, b, mean, rstd), g2, x.shape, need_dx,
-                         w.dtype if need_dweight and w is not None else None,
-                         b.dtype if need_dbias and b is not None else None)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_dx else None
+        dw = torch.empty_like(w) if need_dweight and w is not None else None
+        db = torch.empty_like(b) if need_dbias and b is not None else None
+        a = NormGradArgs()
+        a.struct_size = ctypes.sizeof(NormGradArgs)
+        a.dtype, a.wdtype = _DTYPES[x2.dtype], _wdtype(x2, w, b)
+        a.x, a.rows, a.dim, a.ld = x2.data_ptr(), R, D, x2.stride(0) if R > 1 else D
+        a.weight, a.grad, a.grad_ld = ptr(w), g2.data_ptr(), g2.stride(0) if R > 1 else D
+        a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
+        a.out_dx, a.out_ld, a.out_dweight, a.out_dbias = ptr(dx), D, ptr(dw), ptr(db)
+        ws = None
+        if dw is not None or db is not None:
+            n = _workspace_bytes(R, D, a.dtype)
+            ws = torch.empty(n, dtype=torch.uint8, device=dev)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), n
+        if dx is not None or ws is not None:
+            call(lib().fl_layer_norm_grad, a, dev, "fl_layer_norm_grad")
+        return dx, dw, db
 
 
 @lru_cache(maxsize=256)
@@ -151,32 +143,3 @@ def _workspace_bytes(rows: int, dim: int, dtype: int) -> int:
     _lib.check(lib().fl_layer_norm_grad_workspace_bytes(rows, dim, dtype, ctypes.byref(n)),
                "fl_layer_norm_grad_workspace_bytes")
     return n.value
-
-
-def _grad_args(x2, w, b, mean, rstd) -> NormGradArgs:
-    """The arguments that do not depend on the upstream gradient."""
-    a = NormGradArgs()
-    a.struct_size = ctypes.sizeof(NormGradArgs)
-    a.dtype, a.wdtype = _DTYPES[x2.dtype], _wdtype(x2, w, b)
-    R, D = x2.shape
-    a.x, a.rows, a.dim, a.ld = x2.data_ptr(), R, D, x2.stride(0) if R > 1 else D
-    a.weight, a.mean, a.rstd, a.out_ld = ptr(w), mean.data_ptr(), rstd.data_ptr(), D
-    return a
-
-
-def _backward(a: NormGradArgs, g2, shape, need_dx: bool, dw_type, db_type):
-    """The launches; dw_type, db_type: None where not asked for."""
-    D, dev = a.dim, g2.device
-    dx = torch.empty(shape, dtype=g2.dtype, device=dev) if need_dx else None
-    dw = torch.empty(D, dtype=dw_type, device=dev) if dw_type is not None else None
-    db = torch.empty(D, dtype=db_type, device=dev) if db_type is not None else None
-    a.grad, a.grad_ld = g2.data_ptr(), g2.stride(0) if a.rows > 1 else D
-    a.out_dx, a.out_dweight, a.out_dbias = ptr(dx), ptr(dw), ptr(db)
-    ws = None
-    if dw is not None or db is not None:
-        n = _workspace_bytes(a.rows, D, a.dtype)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), n
-    if dx is not None or ws is not None:
-        call(lib().fl_layer_norm_grad, a, dev, "fl_layer_norm_grad")
-    return dx, dw, db

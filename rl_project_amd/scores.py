@@ -108,33 +108,6 @@ def _forward(x: torch.Tensor, lead, tok: Optional[torch.Tensor], top_k: int, ent
     return o_lp, o_h, o_lse, o_rank, o_ids, o_top, saved
 
 
-class _Score(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tok, top_k, entropy, lse, rank, ignore_index):
-        x = _rows(logits, "logits")
-        out = _forward(x, logits.shape[:-1], tok, top_k, entropy, lse, rank, ignore_index, True)
-        ctx.set_materialize_grads(False)
-        # (checked in backward for changes in place)
-        ctx.save_for_backward(logits) if tok is None else ctx.save_for_backward(logits, tok)
-        # What the backward launch needs, made here: the engine runs backward on a
-        # thread of its own, where the same Python takes twice the time.  The saved
-        # statistics are this node's own: no caller sees or changes them.
-        ctx.args = _grad_args(x, tok, out[6], ignore_index)
-        ctx.keep = (x, out[6])
-        ctx.mark_non_differentiable(*(t for t in out[3:6] if t is not None))
-        return out[:6]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_lp, g_h, g_lse, *_):
-        logits = ctx.saved_tensors[0]
-        if g_lp is None and g_h is None and g_lse is None:
-            return (None,) * 7
-        # (the engine has checked the gradients' shapes, types and device)
-        d = _backward(ctx.args, logits, *(None if g is None else g.contiguous() for g in (g_lp, g_h, g_lse)))
-        return d, None, None, None, None, None, None
-
-
 def score_tokens(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top_k: int = 0,
                  entropy: bool = False, lse: bool = False, rank: bool = False, ignore_index: int = IGNORE_INDEX,
                  check_tokens: bool = False, return_saved: bool = False):
@@ -171,7 +144,11 @@ def score_tokens(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *,
         if return_saved:
             raise ValueError("return_saved is for calls under torch.no_grad()")
         _no_autograd_under_capture("score_tokens")
-        return TokenScores(*_Score.apply(logits, tok, top_k, bool(entropy), bool(lse), bool(rank), int(ignore_index)))
+        if top_k > _lib.FL_SCORE_MAX_TOPK:
+            raise NotImplementedError(f"top_k {top_k} beyond the library's limit {_lib.FL_SCORE_MAX_TOPK}")
+        out = iter(_lib.autograd().score(logits, tok, top_k, bool(entropy), bool(lse), bool(rank), int(ignore_index)))
+        asked = (tok is not None, entropy, lse, rank, top_k, top_k)
+        return TokenScores(*(next(out) if on else None for on in asked))
     out = _forward(x, lead, tok, top_k, entropy, lse, rank, int(ignore_index), return_saved)
     s = TokenScores(*out[:6])
     return (s, out[6]) if return_saved else s
@@ -205,23 +182,14 @@ def score_tokens_backward(logits: torch.Tensor, tokens: Optional[torch.Tensor], 
         gc = _upstream(grad_lse, lead, dev, "grad_lse")
         if ga is not None and tok is None:
             raise ValueError("grad_logprob needs tokens")
-        return _backward(_grad_args(x, tok, saved, int(ignore_index)), logits, ga, gb, gc)
-
-
-def _grad_args(x, tok, saved, ignore_index: int) -> ScoreGradArgs:
-    """The arguments that do not depend on the upstream gradients."""
-    R, V = x.shape
-    a = ScoreGradArgs()
-    a.struct_size = ctypes.sizeof(ScoreGradArgs)
-    a.dtype = _DTYPES[x.dtype]
-    a.logits = x.data_ptr()
-    a.rows, a.vocab, a.ld = R, V, x.stride(0) if R > 1 else V
-    a.tokens, a.ignore_index, a.saved, a.out_ld = ptr(tok), ignore_index, saved.data_ptr(), V
-    return a
-
-
-def _backward(a: ScoreGradArgs, logits, ga, gb, gc) -> torch.Tensor:
-    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    a.grad_logprob, a.grad_entropy, a.grad_lse, a.out_grad = ptr(ga), ptr(gb), ptr(gc), out.data_ptr()
-    call(lib().fl_score_tokens_grad, a, out.device, "fl_score_tokens_grad")
-    return out
+        out = torch.empty(logits.shape, dtype=x.dtype, device=dev)
+        a = ScoreGradArgs()
+        a.struct_size = ctypes.sizeof(ScoreGradArgs)
+        a.dtype = _DTYPES[x.dtype]
+        a.logits = x.data_ptr()
+        a.rows, a.vocab, a.ld = R, V, x.stride(0) if R > 1 else V
+        a.tokens, a.ignore_index, a.saved = ptr(tok), int(ignore_index), saved.data_ptr()
+        a.grad_logprob, a.grad_entropy, a.grad_lse = ptr(ga), ptr(gb), ptr(gc)
+        a.out_grad, a.out_ld = out.data_ptr(), V
+        call(lib().fl_score_tokens_grad, a, dev, "fl_score_tokens_grad")
+        return out
