@@ -11,6 +11,7 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
@@ -97,6 +98,14 @@ variable_list once(variable_list out) {
   return (*e)(std::move(out));
 }
 
+// A backward pass under stream capture is refused, as the forward calls refuse to
+// record their graph there: the engine synchronises with the streams that the
+// leaves' other graphs ran on.
+void refuse_capture(const char* functional) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+    C10_THROW_ERROR(Error, std::string("backward under stream capture: call ") + functional);
+}
+
 Tensor upstream(const Tensor& g) { return g.defined() ? g.contiguous() : g; }
 
 // ---------------------------------------------------------------- layer norm
@@ -125,6 +134,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_capture("layer_norm_backward");
     const auto saved = ctx->get_saved_variables();
     const Tensor stats = ctx->saved_data["stats"].toTensor();
     const int64_t btype = ctx->saved_data["bias"].toInt();
@@ -213,6 +223,7 @@ struct Score : torch::autograd::Function<Score> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_capture("score_tokens_backward");
     const auto kept = ctx->get_saved_variables();
     const int64_t has = ctx->saved_data["has"].toInt();
     Tensor g[3];
@@ -279,6 +290,7 @@ struct Head : torch::autograd::Function<Head> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_capture("lm_head_logprobs_backward");
     const auto kept = ctx->get_saved_variables();
     const int64_t has = ctx->saved_data["has"].toInt();
     Tensor g[3];
