@@ -35,7 +35,7 @@ from .sampling import (SampleOutput, SamplerPlan, SamplingError, apply_sampling_
 from .speculative import MTPSpeculativeGenerator, SpeculativeGenerator, SpecOutput, SpecPlan, speculative_verify
 from .engine import BatchedSampler
 from .logprobs import RowStats, entropy_from_logits, kl_full_distribution, row_stats, token_logprobs_from_logits
-from .norm import NormStats, layer_norm, layer_norm_backward
+from .norm import layer_norm, layer_norm_backward
 from .scores import TokenScores, score_tokens, score_tokens_backward
 from .lmhead import LmHeadOutput, LmHeadPlan, lm_head_sample
 from .headlp import HeadScores, lm_head_logprobs, lm_head_logprobs_backward
@@ -46,7 +46,7 @@ __all__ = [
     "speculative_verify", "SpeculativeGenerator", "MTPSpeculativeGenerator", "SpecOutput", "SpecPlan",
     "BatchedSampler", "row_stats", "RowStats", "token_logprobs_from_logits", "entropy_from_logits", "kl_full_distribution",
     "SamplingParams", "GenerationSettings", "SamplingParamsError",
-    "score_tokens", "score_tokens_backward", "TokenScores", "layer_norm", "layer_norm_backward", "NormStats",
+    "score_tokens", "score_tokens_backward", "TokenScores", "layer_norm", "layer_norm_backward",
     "lm_head_logprobs", "lm_head_logprobs_backward", "HeadScores",
     "lm_head_sample", "LmHeadPlan", "LmHeadOutput",
 ]

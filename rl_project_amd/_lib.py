@@ -254,8 +254,8 @@ _autograd = None
 
 
 def autograd():
-    """The extension with the differentiable calls' autograd nodes (loaded once),
-    bound to this library's entry points."""
+    """The extension that launches score_tokens, layer_norm and lm_head_logprobs and
+    holds their autograd nodes (loaded once), bound to this library's entry points."""
     global _autograd
     if _autograd is not None:
         return _autograd
@@ -297,22 +297,6 @@ def stream_handle(device: torch.device) -> int:
         idx = device.index if device.index is not None else torch.cuda.current_device()
         return _raw_stream(idx)
     return torch.cuda.current_stream(device).cuda_stream
-
-
-_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-
-
-def call(fn, args: ctypes.Structure, device: torch.device, what: str) -> None:
-    """fn(args) on the device's current stream; the device is made the current
-    one for the launch if another is."""
-    index = device.index
-    if index is None or _current_device() == index:
-        rc = fn(ctypes.byref(args), stream_handle(device))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(ctypes.byref(args), stream_handle(device))
-    if rc:
-        check(rc, what)
 
 
 EXPORTED_SYMBOLS = ("fl_sample", "fl_sample_exact", "fl_fill_rows", "fl_apply_filter", "fl_spec_verify", "fl_spec_verify_static",

@@ -1,5 +1,5 @@
 """Build libflsampler.so in-tree from ``rl_project_amd/csrc/*.hip`` for gfx950, and
-the autograd nodes over it (``csrc/fl_autograd.cpp``, a torch extension).
+the torch extension over it (``csrc/fl_autograd.cpp``).
 
     python -m rl_project_amd.build [-v]
 
