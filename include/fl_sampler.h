@@ -385,7 +385,7 @@ int fl_lm_head_workspace_bytes(int64_t batch, int64_t vocab, size_t* out_bytes);
  * A row without a distribution (a NaN or +inf logit, or -inf alone) has NaN in
  * every float output (lse: -inf for -inf alone), rank -1 and top_ids -1.
  * out_saved (float [rows, 4]) is what fl_score_tokens_grad reads: lse in two
- * floats, and the entropy if out_entropy is asked for.  top_k: 0 (none) to
+ * floats, and the entropy (NaN unless out_entropy is asked for).  top_k: 0 (none) to
  * min(vocab, FL_SCORE_MAX_TOPK); vocab up to FL_MAX_VOCAB_F32.  workspace
  * (fl_score_workspace_bytes, 8-byte aligned; 0 bytes for vocab <= 16384): calls
  * that overlap in time must not share one.  A row's results are a function of

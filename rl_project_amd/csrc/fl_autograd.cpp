@@ -93,6 +93,8 @@ Tensor bytes(size_t n, const Tensor& like) {
 // record its graph returns results that raise when differentiated.
 variable_list once(variable_list out) {
   if (!at::GradMode::is_enabled()) return out;
+  for (Tensor& t : out)   // (results of leaves that need no gradient would get no node)
+    if (t.defined()) t.requires_grad_(true);
   auto e = std::make_shared<torch::autograd::DelayedError>(
       "this call is differentiable once: its gradients have no gradients", static_cast<int>(out.size()));
   return (*e)(std::move(out));

@@ -588,7 +588,7 @@ __global__ __launch_bounds__(HJ_R * HJ_P) void k_head_join(const fl_head_args a,
     float* sv = a.out_saved + 4 * n;
     sv[0] = okr ? m : nan;
     sv[1] = okr ? static_cast<float>(logs) : nan;
-    sv[2] = a.out_entropy ? ent : 0.0f;
+    sv[2] = a.out_entropy ? ent : nan;
     sv[3] = 0.0f;
   }
 }

@@ -94,7 +94,7 @@ __device__ __forceinline__ ScRow sc_finish(const fl_score_args& a, int64_t r, do
     const float hi = static_cast<float>(ref);
     sv[0] = out.ok ? hi : nan;
     sv[1] = out.ok ? static_cast<float>((ref - static_cast<double>(hi)) + logs) : nan;
-    sv[2] = a.out_entropy ? ent : 0.0f;
+    sv[2] = a.out_entropy ? ent : nan;   // (a gradient of it without it is NaN, not another number)
     sv[3] = 0.0f;
   }
   return out;

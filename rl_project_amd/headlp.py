@@ -53,7 +53,8 @@ def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optiona
     logits are float32 sums, not rounded to bfloat16 as ``linear``'s are.
     ``norm=(weight, bias, eps)`` applies ``layer_norm`` to the hidden states
     first (the model's final norm).  Ignored and out-of-range tokens as in
-    ``score_tokens``; up to 131072 rows.
+    ``score_tokens``; up to 131072 rows.  (The gradient of ``weight`` is a product
+    over all rows: a NaN in the hidden states of an ignored row is in it too.)
 
     Differentiable (once) in ``hidden`` and ``weight`` (and through ``norm``), except
     under stream capture: a captured step takes ``return_saved=True``, which
@@ -71,12 +72,11 @@ def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optiona
     if grad and norm is not None and return_saved and any(isinstance(t, torch.Tensor) and t.requires_grad for t in norm[:2]):
         raise ValueError("return_saved is for calls under torch.no_grad()")
     hidden = _normed(hidden, norm)
-    if grad and (hidden.requires_grad or weight.requires_grad):
+    # (a call that asks for no result has no graph)
+    if grad and (hidden.requires_grad or weight.requires_grad) and (tok is not None or entropy or lse or return_saved):
         if return_saved:
             raise ValueError("return_saved is for calls under torch.no_grad()")
         _no_autograd_under_capture("lm_head_logprobs")
-        if tok is None and not entropy and not lse:
-            raise ValueError("nothing is asked for: give tokens, entropy=True or lse=True")
         out = iter(_lib.autograd().head(hidden, weight, tok, entropy, lse, ignore_index))
         return HeadScores(*(next(out) if on else None for on in (tok is not None, entropy, lse)))
     out = _lib.autograd().head_forward(hidden, weight, tok, entropy, lse, ignore_index, return_saved)

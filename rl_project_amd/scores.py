@@ -104,7 +104,8 @@ def score_tokens(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *,
             _check_range(tok, V, ignore_index)
     elif rank:
         raise ValueError("rank needs tokens")
-    if logits.requires_grad and torch.is_grad_enabled():
+    # (a call that asks for no result with a gradient has no graph)
+    if logits.requires_grad and torch.is_grad_enabled() and (tok is not None or entropy or lse or return_saved):
         if return_saved:
             raise ValueError("return_saved is for calls under torch.no_grad()")
         _no_autograd_under_capture("score_tokens")
