@@ -62,6 +62,19 @@ def test_norm_of_one_row_and_of_many_dimensions(D):
     _same(ds, layer_norm_backward(torch.ones_like(x), x, w, b, stats, need_dweight=False, need_dbias=False)[0])
 
 
+@pytest.mark.parametrize("D", [3, 768, 2048, 4096, 8192, 10001])
+def test_a_norm_row_is_a_function_of_the_row_alone(D):
+    x, dy = torch.randn(2, 1100, D, device="cuda").bfloat16()
+    w = torch.randn(D, device="cuda")
+    want, stats = layer_norm(x, w, None, return_stats=True)
+    dx = layer_norm_backward(dy, x, w, None, stats, need_dweight=False)[0]
+    for rows in (slice(0, 1), slice(7, 71), slice(500, 1013)):
+        got, st = layer_norm(x[rows], w, None, return_stats=True)
+        _same(got, want[rows])
+        _same(st, stats[:, rows].contiguous())
+        _same(layer_norm_backward(dy[rows], x[rows], w, None, st)[0], dx[rows])
+
+
 def test_head_of_one_row_and_of_many_dimensions():
     h, w, tok = _head()
     want = lm_head_logprobs(h, w, tok, entropy=True, lse=True)
