@@ -15,7 +15,14 @@
 // and a row's results are a function of the row alone.  A thread holds its 64
 // values of the slice in registers, so every step (maximum, sums, rank count,
 // the largest values) reads HBM once; the join of a row's slices is a second
-// kernel (none for a row of one slice).
+// kernel (none for a row of one slice).  bf16 4096x128256 (1.05 GB), whole calls:
+// 171 us for the log-probability (6.1 TB/s), 179 with the entropy, 200 with 5
+// alternatives, 208 to 223 with the rank too: bound by HBM, and past that by the
+// vector instructions and the meetings of the search.  12x128256 with 20
+// alternatives and the rank: 11.9 us + 4.9 us for the join, a chain of a load, eight
+// barriers and the list; 1x50257: 8 + 4 us.  (Fewer registers for 7 or 8 waves
+// per SIMD spill: 238 us with the entropy; slices streamed by one work-group per
+// row: 289 us with 5 alternatives.)
 #include <type_traits>
 
 #include "fl_device.h"
@@ -110,13 +117,13 @@ __device__ __forceinline__ void sc_emit(const fl_score_args& a, int64_t r, int q
 
 // n candidates to their places by counting the greater ones (they are
 // distinct), eight a turn; put(place, key) for places below k.  Called by the
-// whole work-group, cand written and met on.
-template <class P>
+// whole work-group of NT threads, cand written and met on.
+template <int NT, class P>
 __device__ __forceinline__ void sc_place(uint64_t* cand, int n, int k, P&& put) {
   const int n8 = (n + 7) & ~7;
   if (static_cast<int>(threadIdx.x) < n8 - n) cand[n + threadIdx.x] = 0u;
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += SC_NT) {
+  for (int i = threadIdx.x; i < n; i += NT) {
     const uint64_t mine = cand[i];
     int above = 0;
     for (int j = 0; j < n8; j += 8) {
@@ -475,20 +482,23 @@ __global__ __launch_bounds__(SC_NT) void k_score_slice(const fl_score_args a, co
   }
   if (S == 1) {
     const ScRow rw = s_row;
-    sc_place(cand, n, K, [&](int p, uint64_t key) { sc_emit(a, r, p, key, rw); });
+    sc_place<SC_NT>(cand, n, K, [&](int p, uint64_t key) { sc_emit(a, r, p, key, rw); });
     // (fewer than K values found: NaN values, whose row has no distribution)
     for (int p = n + tid; p < K; p += SC_NT) sc_emit(a, r, p, 0u, rw);
   } else {
     uint64_t* out = ws.list + (r * S + sl) * static_cast<int64_t>(K);
-    sc_place(cand, n, K, [&](int p, uint64_t key) { out[p] = key; });
+    sc_place<SC_NT>(cand, n, K, [&](int p, uint64_t key) { out[p] = key; });
     for (int p = n + tid; p < K; p += SC_NT) out[p] = 0u;
   }
 }
 
-// A row's slices joined; one work-group per row (of one wave if no list is
-// asked for).
-__global__ __launch_bounds__(SC_NT) void k_score_join(const fl_score_args a, const ScWs ws) {
-  __shared__ __attribute__((aligned(16))) uint64_t cand[SC_CAP];
+// A row's slices joined; one work-group per row: of one wave where its lists hold
+// no more than an entry a lane (bf16 4096x128256, K = 5: 8.8 us, 13.5 of four
+// waves), else of SC_NT threads (12x128256, K = 20, 160 entries: 4.9 us, 6.3 of one
+// wave).
+template <int NT>
+__global__ __launch_bounds__(NT) void k_score_join(const fl_score_args a, const ScWs ws) {
+  __shared__ __attribute__((aligned(16))) uint64_t cand[NT == SC_NT ? SC_CAP : NT];
   __shared__ ScRow s_row;
   __shared__ uint32_t s_n;
   const int tid = threadIdx.x;
@@ -505,10 +515,10 @@ __global__ __launch_bounds__(SC_NT) void k_score_join(const fl_score_args a, con
   const bool has = K > 0 && sl < S;
   const int nth = static_cast<int>((static_cast<int64_t>(K) * min(SC_SLICE, V - sl * SC_SLICE) + V - 1) / V);
   const uint64_t kth = has ? list[sl * K + K - 1] : 0u, share = has ? list[sl * K + nth - 1] : ~0ull;
-  constexpr int PER = SC_CAP / SC_NT;
+  constexpr int PER = NT == SC_NT ? SC_CAP / SC_NT : 1;   // (the host's choice of NT)
   uint64_t mine[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) mine[i] = tid + i * SC_NT < S * K ? list[tid + i * SC_NT] : 0u;
+  for (int i = 0; i < PER; ++i) mine[i] = tid + i * NT < S * K ? list[tid + i * NT] : 0u;
   if (tid < WAVE) {
     constexpr int G = SC_MAX_SLICES;   // lanes of the fixed tree
     static_assert(G <= WAVE && (G & (G - 1)) == 0, "one lane per slice");
@@ -525,22 +535,23 @@ __global__ __launch_bounds__(SC_NT) void k_score_join(const fl_score_args a, con
     const int c = wave_reduce<int, OpAdd, G>(p.rank, OpAdd());
     if (tid == 0) s_row = sc_finish(a, r, R, s, u, p.xt, c);
   }
-  if (K == 0) return;   // (one wave)
+  if (K == 0) return;
   __syncthreads();
   const ScRow rw = s_row;
   const uint64_t bound = max(wave_reduce(kth, OpMax()), wave_reduce(share, OpMin()));   // (every wave's the same)
 #pragma unroll
   for (int i = 0; i < PER; ++i)
-    if (mine[i] >= bound && mine[i] != 0u) cand[atomicAdd(&s_n, 1u)] = mine[i];   // (at most S K <= SC_CAP)
+    if (mine[i] >= bound && mine[i] != 0u) cand[atomicAdd(&s_n, 1u)] = mine[i];   // (at most S K)
   __syncthreads();
   const int n = static_cast<int>(s_n);
-  sc_place(cand, n, K, [&](int p, uint64_t key) { sc_emit(a, r, p, key, rw); });
-  for (int p = n + tid; p < K; p += SC_NT) sc_emit(a, r, p, 0u, rw);
+  sc_place<NT>(cand, n, K, [&](int p, uint64_t key) { sc_emit(a, r, p, key, rw); });
+  for (int p = n + tid; p < K; p += NT) sc_emit(a, r, p, 0u, rw);
 }
 
 // ---------------------------------------------------------------- gradient
 // Element by element: a read and a write of every value, which HBM bounds.
-// One work-group per piece of GR_NT x GR_U chunks of a row.
+// One work-group per piece of GR_NT x GR_U chunks of a row.  bf16 4096x128256 (2.1
+// GB): 385 to 419 us, 5.0 to 5.5 TB/s; f32 255x50257 (103 MB): 18.4 us.
 namespace {
 constexpr int GR_NT = 256, GR_U = 4;
 }
@@ -658,8 +669,11 @@ hipError_t launch_score(const fl_score_args& a, hipStream_t s) {
   if (a.dtype == FL_DTYPE_F32) run(F32{});
   else if (a.dtype == FL_DTYPE_BF16) run(BF16{});
   else run(F16{});
-  if (ws.S > 1)
-    hipLaunchKernelGGL(k_score_join, dim3(static_cast<unsigned>(a.rows)), dim3(a.top_k > 0 ? SC_NT : WAVE), 0, s, a, ws);
+  if (ws.S > 1) {
+    const dim3 rows(static_cast<unsigned>(a.rows));
+    if (ws.S * a.top_k <= WAVE) hipLaunchKernelGGL(k_score_join<WAVE>, rows, dim3(WAVE), 0, s, a, ws);
+    else hipLaunchKernelGGL(k_score_join<SC_NT>, rows, dim3(SC_NT), 0, s, a, ws);
+  }
   return hipGetLastError();
 }
 
