@@ -3,7 +3,7 @@
 // in memory.  With logits x[n, v] = sum_d hidden[n, d] weight[v, d] (float32
 // accumulators, never rounded to 16 bits) and p = softmax(x[n, :]):
 //
-//   forward   per row the running (max, sum e, sum e (x - max)) of each 128
+//   forward   per row (max, sum e, sum e (x - max)) of each tile of 256
 //             vocabulary rows from the product's registers, joined per row;
 //   backward  g[n, v] = a (1[v = t] - p) - b p (log p + H) + c p for upstream
 //             a, b, c of logprob, entropy, lse; then
@@ -15,6 +15,19 @@
 // entry to entry: a sum of many terms moves by as much relative to its terms'
 // norm, as rounding the result does), the largest chunk that a bounded workspace
 // holds; each product then reads it as its matrix operand.
+//
+// What bounds them: with few rows the weight's bytes (64x4096x128256: 170 to 217 us
+// for 1.05 GB, 6.2 to 4.8 TB/s, by the clock the card holds), with many LDS: the
+// fragments of a stage (64 k) of a 256 x 256 tile are 192 KiB read beside 64 KiB
+// written, 2048 cycles at 128 bytes a cycle, as many as its matrix instructions
+// take.  4096x4096x128256, per product of 4.3 TFLOP: statistics 3.51 ms, g 3.83,
+// dhidden 3.48, dweight 3.75 ms (1.12 to 1.24 PFLOP/s; the matrix units busy for 57
+// to 65 % of the cycles, LDS without bank conflicts but for the stores' 2 %); a
+// library product of that shape, which writes the logits, reaches 1.41 PFLOP/s.
+// Tried and slower: 4 waves of 128 x 128, which read a third less of LDS (dweight
+// 4.4 ms, dhidden 4.0, g 4.8; the statistics spill); s_setprio around the matrix
+// instructions (no change).  255x1024x50257: 35, 42, 47 and 52 us; 197 tiles of 256
+// vocabulary rows leave 59 CUs idle (128 columns a tile: 39 us for the first).
 #include <algorithm>
 #include <type_traits>
 
