@@ -511,10 +511,10 @@ int fl_layer_norm_grad_workspace_bytes(int64_t rows, int64_t dim, int32_t dtype,
  * [rows, vocab] logits (the training and evaluation counterpart of
  * fl_lm_head_sample): with x[r, v] = sum_d hidden[r, d] weight[v, d] in float32
  * accumulators, out_logprob, out_entropy, out_lse and out_saved are
- * fl_score_tokens' of x.  hidden [rows, dim] (row stride ld_hidden) and weight
- * [vocab, dim] (rows contiguous) are bf16, 16-byte aligned (ld_hidden a multiple
- * of 8), dim a multiple of 64 up to 16384, vocab up to FL_MAX_VOCAB_16, rows up to
- * FL_HEAD_MAX_ROWS.  workspace (fl_head_workspace_bytes, 256-byte aligned): calls
+ * fl_score_tokens' of x (and x_r[t] in out_saved's last column).  hidden [rows,
+ * dim] (row stride ld_hidden) and weight [vocab, dim] (rows contiguous) are bf16,
+ * 16-byte aligned (ld_hidden a multiple of 8), dim a multiple of 64 up to 16384,
+ * vocab up to FL_MAX_VOCAB_16, rows up to FL_HEAD_MAX_ROWS.  workspace (fl_head_workspace_bytes, 256-byte aligned): calls
  * that overlap in time must not share one.
  */
 #define FL_HEAD_MAX_ROWS 131072

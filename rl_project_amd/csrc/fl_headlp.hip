@@ -11,10 +11,14 @@
 //             dweight[v, d] = sum_n g[n, v] hidden[n, d].
 //
 // Four products of one main loop.  The gradient g of a chunk of the vocabulary
-// is written once, in bfloat16 (a rounding of at most 2^-8 relative, independent from
-// entry to entry: a sum of many terms moves by as much relative to its terms'
-// norm, as rounding the result does), the largest chunk that a bounded workspace
-// holds; each product then reads it as its matrix operand.
+// is written once, in bfloat16, the largest chunk that a bounded workspace holds;
+// each product then reads it as its matrix operand.  Its rounding, of at most 2^-8
+// relative, is independent from entry to entry, so that a sum of many terms moves
+// by as much relative to its terms' norm as rounding the result does; but a row's
+// largest entry is its token's, most of the row's dhidden and of that token's
+// dweight.  What the rounding took of it is kept in float32 and added to both sums
+// (a training step of few rows: distance from 64 bits up to 2.3 times that of
+// rounding the results alone without it, 1.0 to 1.2 times with it).
 //
 // What bounds them: with few rows the weight's bytes (64x4096x128256: 170 to 217 us
 // for 1.05 GB, 6.2 to 4.8 TB/s, by the clock the card holds), with many LDS: the
@@ -26,7 +30,7 @@
 // library product of that shape, which writes the logits, reaches 1.41 PFLOP/s.
 // Tried and slower: 4 waves of 128 x 128, which read a third less of LDS (dweight
 // 4.4 ms, dhidden 4.0, g 4.8; the statistics spill); s_setprio around the matrix
-// instructions (no change).  255x1024x50257: 35, 42, 47 and 52 us; 197 tiles of 256
+// instructions (no change).  255x1024x50257: 35, 42, 49 and 56 us; 197 tiles of 256
 // vocabulary rows leave 59 CUs idle (128 columns a tile: 39 us for the first).
 #include <algorithm>
 #include <type_traits>
@@ -602,7 +606,8 @@ __global__ __launch_bounds__(HJ_R * HJ_P) void k_head_join(const fl_head_args a,
     sv[0] = okr ? m : nan;
     sv[1] = okr ? static_cast<float>(logs) : nan;
     sv[2] = a.out_entropy ? ent : nan;
-    sv[3] = 0.0f;
+    const int64_t t = a.tokens ? a.tokens[n] : -1;
+    sv[3] = t >= 0 && t < a.vocab ? xt[n] : nan;   // (0 there)
   }
 }
 
@@ -612,6 +617,32 @@ struct HlGrad {
   const float* saved;
   const float *ga, *gb, *gc;   // upstream of logprob, entropy, lse (NULL: 0)
 };
+// What rounding took of g at a row's token v, if that lies in a chunk that was
+// written (else -1).
+struct HlFix {
+  int v;
+  float r;
+};
+// acc += r x for a lane's column of a wave's blocks and the bf16 x[first ...] of
+// width elements (those past it go to results that nobody stores; all loads ahead
+// of the first use).
+template <int FI>
+__device__ __forceinline__ void hl_add(floatx16 (&acc)[FI], float r, const uint16_t* x, int first, int width) {
+  uint2 w[FI][4];
+#pragma unroll
+  for (int i = 0; i < FI; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) w[i][q] = *reinterpret_cast<const uint2*>(x + min(first + 32 * i + 8 * q, width - 4));
+#pragma unroll
+  for (int i = 0; i < FI; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t u[2] = {w[i][q].x, w[i][q].y};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        acc[i][4 * q + e] = fmaf(r, BF16::to_f32(e % 2 == 0 ? u[e / 2] & 0xFFFFu : u[e / 2] >> 16), acc[i][4 * q + e]);
+    }
+}
 }  // namespace
 
 // g of the vocabulary rows c0 .. c0 + cn - 1 (cn a multiple of 64; those past
@@ -672,11 +703,63 @@ __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       });
 }
 
+// What rounding took of g at the rows' tokens in a chunk: g in float32 from the
+// token's logit that the forward pass left, less what k_head_g wrote.  No more than
+// a rounding: of a forward call with other tokens it is 0 or as small.  A wave takes
+// 64 vocabulary rows and looks for them among the tokens: fix by row, for dhidden,
+// and list by vocabulary row, for dweight: the 64 first rows with such a token, v
+// their number times 64 and the place, 0 behind the last.
+// 255x1024x50257 5 us, 4096x4096x128256 13 us for each of two chunks; what dweight
+// does with the list is 4 of its 56 us there, nothing here.
+constexpr int HL_LIST = 64;
+__global__ __launch_bounds__(256) void k_head_fix(const HlArgs a, const HlGrad gr, const uint16_t* g, HlFix* fix, HlFix* list,
+                                                  int c0, int cn) {
+  const int lane = threadIdx.x & (WAVE - 1), bin = blockIdx.x * (256 / WAVE) + threadIdx.x / WAVE;
+  if (bin >= cn / HL_LIST) return;
+  const int v0 = c0 + bin * HL_LIST, v1 = min(a.vocab, v0 + HL_LIST);
+  int count = 0;
+  constexpr int U = 8;
+#pragma unroll 1
+  for (int nb = 0; nb < a.rows; nb += U * WAVE) {
+    int64_t tk[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) tk[u] = a.tokens ? a.tokens[min(nb + u * WAVE + lane, a.rows - 1)] : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int n = nb + u * WAVE + lane;
+      // (the first wave of the first chunk: rows whose token lies in no chunk yet have none)
+      if (c0 == 0 && bin == 0 && n < a.rows && (tk[u] < 0 || tk[u] >= min(a.vocab, cn))) fix[n] = HlFix{-1, 0.0f};
+      const bool in = n < a.rows && tk[u] >= v0 && tk[u] < v1;
+      const uint64_t hits = __ballot(in);
+      if (hits == 0) continue;
+      if (in) {
+        const float ga = gr.ga && tk[u] != a.ignore_index ? gr.ga[n] : 0.0f;
+        const float gb = gr.gb ? gr.gb[n] : 0.0f, gc = gr.gc ? gr.gc[n] : 0.0f;
+        const float4 sv = reinterpret_cast<const float4*>(gr.saved)[n];
+        const float l = (sv.w - sv.x) - sv.y, p = __builtin_amdgcn_exp2f(l * HL_LOG2E);
+        const float v = p * (gc - ga - gb * (fmaxf(l, -200.0f) + (gb == 0.0f ? 0.0f : sv.z))) + ga;
+        const float was = BF16::to_f32(g[static_cast<int64_t>(n) * cn + (tk[u] - c0)]), lost = v - was;
+        const float r = __builtin_fabsf(lost) <= __builtin_fabsf(was) * 0x1.02p-8f ? lost : 0.0f;   // (NaN: 0)
+        fix[n] = HlFix{static_cast<int>(tk[u]), r};
+        const int at = count + __popcll(hits & ((1ull << lane) - 1ull));
+        if (at < HL_LIST) list[bin * HL_LIST + at] = HlFix{n * HL_LIST + static_cast<int>(tk[u] - v0), r};
+      }
+      count += __popcll(hits);
+    }
+  }
+  if (lane >= count) list[bin * HL_LIST + lane] = HlFix{0, 0.0f};
+}
+
 // dweight[c0 + v, d] = sum_n g[n, v] hidden[n, d]: i = d, j = v.  (Tiles of 128 or
 // 64 vocabulary rows are slower for few rows too: 255x1024x50257 58, 61, 73 us.)
+// What rounding took of g at the rows' tokens comes to the sums of the tokens'
+// rows: a wave's 64 vocabulary rows take one row's part each at a time, in the
+// order of the rows, in HL_FIXES turns at most, which bounds the time where many
+// rows have one token (more rows' roundings are as independent as any).
+constexpr int HL_FIXES = 16;
 __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_head_dw(const HlArgs a, const uint16_t* g,
-                                                                                            uint16_t* dw, int c0, int cn,
-                                                                                            const Tiles ts) {
+                                                                                            const HlFix* list, uint16_t* dw,
+                                                                                            int c0, int cn, const Tiles ts) {
   using S = Shape<256>;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int w = threadIdx.x / WAVE;
@@ -696,7 +779,46 @@ __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
         const int d0 = ti * HL_I + (w / S::WJ) * 32 * S::FI, v0 = c0 + tj * S::BJ + (w % S::WJ) * 32 * S::FJ;
         uint16_t* out = dw + static_cast<int64_t>(v0) * a.dim + d0;
         const int rows = min(a.vocab, c0 + cn) - v0;
+        const int lane = threadIdx.x & (WAVE - 1);
+        static_assert(32 * S::FJ == HL_LIST, "a wave's vocabulary rows are a list's");
+        const HlFix f = rows > 0 ? list[v0 - c0 + lane] : HlFix{0, 0.0f};   // (beside the next tile's loads)
         hl_wait_vm<0>();
+        int qn[2] = {0, 0}, turns = 0;
+        float qr[2] = {0.0f, 0.0f};   // the lane's columns' parts that wait; 0: none
+        uint64_t wait = 0;            // the columns that have one
+        uint64_t hits = __ballot(f.r != 0.0f);
+#pragma unroll 1
+        while ((hits | wait) != 0 && turns < HL_FIXES) {   // (the same way for the whole wave)
+          const bool end = hits == 0;
+          const int b = end ? 0 : __builtin_ctzll(hits);
+          const int e = __builtin_amdgcn_readlane(f.v, b), v = e % HL_LIST;
+          if (end || (wait >> v & 1)) {
+#pragma unroll
+            for (int j = 0; j < S::FJ; ++j) {
+              if (qr[j] != 0.0f) {
+                floatx16 col[S::FI];
+#pragma unroll
+                for (int i = 0; i < S::FI; ++i) col[i] = acc[i][j];
+                hl_add<S::FI>(col, qr[j], a.hidden + qn[j] * a.ld, d0 + 4 * (lane >> 5), a.dim);
+#pragma unroll
+                for (int i = 0; i < S::FI; ++i) acc[i][j] = col[i];
+              }
+              qr[j] = 0.0f;
+            }
+            wait = 0;
+            ++turns;
+          } else {
+            hits &= hits - 1;
+            wait |= 1ull << v;
+            const float r = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f.r), b));
+#pragma unroll
+            for (int j = 0; j < S::FJ; ++j)
+              if (v - 32 * j == (lane & 31)) {
+                qn[j] = e / HL_LIST;
+                qr[j] = r;
+              }
+          }
+        }
         hl_store_rows<S>(acc, area, a.dim - d0, [&](int q) { return q < rows ? out + static_cast<int64_t>(q) * a.dim : nullptr; });
       });
 }
@@ -706,9 +828,9 @@ __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 // chunk after the first) added to; DIRECT: one part in all, rounded into dhidden.
 template <int BJ, bool DIRECT>
 __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_head_dh(const HlArgs a, const uint16_t* g,
-                                                                                            float* sum, uint16_t* dh, int c0,
-                                                                                            int cn, const Tiles ts, int per,
-                                                                                            int first) {
+                                                                                            const HlFix* fix, float* sum,
+                                                                                            uint16_t* dh, int c0, int cn,
+                                                                                            const Tiles ts, int per, int first) {
   using S = Shape<BJ>;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
@@ -732,6 +854,18 @@ __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
         const int rows = a.rows - n0;
         hl_wait_vm<0>();
         if constexpr (DIRECT) {
+#pragma unroll
+          for (int j = 0; j < S::FJ; ++j) {
+            const int n = 32 * j + (lane & 31), d = d0 + 4 * (lane >> 5);
+            const HlFix f = fix[n0 + min(n, rows - 1)];
+            if (f.v < 0 || n >= rows) continue;
+            floatx16 col[S::FI];
+#pragma unroll
+            for (int i = 0; i < S::FI; ++i) col[i] = acc[i][j];
+            hl_add<S::FI>(col, f.r, a.weight + static_cast<int64_t>(f.v) * a.dim, d, a.dim);
+#pragma unroll
+            for (int i = 0; i < S::FI; ++i) acc[i][j] = col[i];
+          }
           uint16_t* out = dh + static_cast<int64_t>(n0) * a.dim + d0;
           hl_store_rows<S>(acc, area, a.dim - d0,
                            [&](int q) { return q < rows ? out + static_cast<int64_t>(q) * a.dim : nullptr; });
@@ -760,14 +894,23 @@ __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       });
 }
 
-// dhidden = the parts' sum, rounded once; four values per thread
-__global__ __launch_bounds__(256) void k_head_dh_join(const float4* part, uint2* out, int64_t n4, int splits) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+// dhidden = the parts' sum and what rounding took of g at the row's token times the
+// token's weights, rounded once; four values per thread (of dim / 4 a row)
+__global__ __launch_bounds__(256) void k_head_dh_join(const HlArgs a, const HlFix* fix, const float4* part, uint2* out,
+                                                      int splits) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, n4 = static_cast<int64_t>(a.rows) * (a.dim / 4);
   if (i >= n4) return;
+  const int64_t n = i / (a.dim / 4);
+  const HlFix f = fix[n];
   float4 v = part[i];
   for (int z = 1; z < splits; ++z) {
     const float4 b = part[z * n4 + i];
     v = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
+  }
+  if (f.v >= 0) {
+    const uint2 w = *reinterpret_cast<const uint2*>(a.weight + static_cast<int64_t>(f.v) * a.dim + 4 * (i - n * (a.dim / 4)));
+    v = make_float4(fmaf(f.r, BF16::to_f32(w.x & 0xFFFFu), v.x), fmaf(f.r, BF16::to_f32(w.x >> 16), v.y),
+                    fmaf(f.r, BF16::to_f32(w.y & 0xFFFFu), v.z), fmaf(f.r, BF16::to_f32(w.y >> 16), v.w));
   }
   out[i] = make_uint2(BF16::from_f32(v.x) | (BF16::from_f32(v.y) << 16), BF16::from_f32(v.z) | (BF16::from_f32(v.w) << 16));
 }
@@ -851,7 +994,7 @@ size_t head_workspace_bytes(int64_t rows, int64_t vocab) {
 size_t head_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t vocab, bool dhidden) {
   const int64_t cn = hl_chunk(rows, vocab);
   const size_t R = static_cast<size_t>(rows);
-  return al(2 * R * static_cast<size_t>(cn)) +
+  return al(2 * R * static_cast<size_t>(cn)) + al(sizeof(HlFix) * R) + al(sizeof(HlFix) * static_cast<size_t>(cn)) +
          (dhidden ? al(4 * R * static_cast<size_t>(dim) * static_cast<size_t>(hl_split(rows, dim, cn).nz)) : 0);
 }
 
@@ -876,7 +1019,10 @@ hipError_t launch_head_grad(const fl_head_grad_args& a, hipStream_t s) {
   const HlGrad gr = {a.saved, a.grad_logprob, a.grad_entropy, a.grad_lse};
   const int chunk = hl_chunk(a.rows, a.vocab), nd = cdiv(a.dim, HL_I);
   uint16_t* g = static_cast<uint16_t*>(a.workspace);
-  float* sum = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + al(2 * static_cast<size_t>(a.rows) * chunk));
+  char* behind = static_cast<char*>(a.workspace) + al(2 * static_cast<size_t>(a.rows) * chunk);
+  HlFix* fix = reinterpret_cast<HlFix*>(behind);
+  HlFix* list = reinterpret_cast<HlFix*>(behind + al(sizeof(HlFix) * static_cast<size_t>(a.rows)));
+  float* sum = reinterpret_cast<float*>(reinterpret_cast<char*>(list) + al(sizeof(HlFix) * static_cast<size_t>(chunk)));
   uint16_t* dh = static_cast<uint16_t*>(a.out_dhidden);
   const bool direct = chunk >= a.vocab && hl_split(a.rows, a.dim, chunk).nz == 1;
   hipError_t e = hipSuccess;
@@ -889,6 +1035,9 @@ hipError_t launch_head_grad(const fl_head_grad_args& a, hipStream_t s) {
       const Tiles tg = {nc, cdiv(a.rows, BJ), 1};
       e = hl_launch<S>(k_head_g<BJ>, tg, s, h, gr, g, c0, cn, tg);
     });
+    if (e != hipSuccess) break;
+    hipLaunchKernelGGL(k_head_fix, dim3(cdiv(cn / HL_LIST, 256 / WAVE)), dim3(256), 0, s, h, gr, g, fix, list, c0, cn);
+    e = hipGetLastError();
     if (e == hipSuccess && dh != nullptr)
       hl_by(hl_dh_bj(a.rows, a.dim), [&](auto bj) {
         constexpr int BJ = decltype(bj)::value;
@@ -897,19 +1046,19 @@ hipError_t launch_head_grad(const fl_head_grad_args& a, hipStream_t s) {
         // every part that it adds to was written)
         const Split sp = hl_split(a.rows, a.dim, chunk);
         const Tiles td = {nd, cdiv(a.rows, BJ), cdiv(cn / HL_K, sp.per)};
-        if (direct) e = hl_launch<S>(k_head_dh<BJ, true>, td, s, h, g, sum, dh, c0, cn, td, sp.per, 1);
-        else e = hl_launch<S>(k_head_dh<BJ, false>, td, s, h, g, sum, dh, c0, cn, td, sp.per, c0 == 0 ? 1 : 0);
+        if (direct) e = hl_launch<S>(k_head_dh<BJ, true>, td, s, h, g, fix, sum, dh, c0, cn, td, sp.per, 1);
+        else e = hl_launch<S>(k_head_dh<BJ, false>, td, s, h, g, fix, sum, dh, c0, cn, td, sp.per, c0 == 0 ? 1 : 0);
       });
     if (e == hipSuccess && a.out_dweight) {
       const Tiles tw = {nd, nc, 1};
-      e = hl_launch<Shape<256>>(k_head_dw, tw, s, h, g, static_cast<uint16_t*>(a.out_dweight), c0, cn, tw);
+      e = hl_launch<Shape<256>>(k_head_dw, tw, s, h, g, list, static_cast<uint16_t*>(a.out_dweight), c0, cn, tw);
     }
   }
   if (e != hipSuccess) return e;
   if (dh != nullptr && !direct) {
     const int64_t n4 = a.rows * a.dim / 4;
-    hipLaunchKernelGGL(k_head_dh_join, dim3(static_cast<unsigned>(cdiv(n4, 256))), dim3(256), 0, s,
-                       reinterpret_cast<const float4*>(sum), reinterpret_cast<uint2*>(dh), n4,
+    hipLaunchKernelGGL(k_head_dh_join, dim3(static_cast<unsigned>(cdiv(n4, 256))), dim3(256), 0, s, h, fix,
+                       reinterpret_cast<const float4*>(sum), reinterpret_cast<uint2*>(dh),
                        hl_split(a.rows, a.dim, chunk).nz);
   }
   return hipGetLastError();
