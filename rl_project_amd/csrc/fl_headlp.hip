@@ -65,7 +65,8 @@ constexpr float HL_LOG2E = 1.44269504088896340736f;
 // reads spread over all banks:
 //   rows: granule g (of 8) of row r at r 8 + (g ^ ((r >> 1) & 7)); a lane's 8
 //         k of a 32 x 16 fragment are one ds_read_b128;
-//   cols: granule g (of BJ / 8) of k-row k at k BJ / 8 + (g ^ (4 (k & 3))); a
+//   cols: granule g (of BJ / 8) of k-row k at k BJ / 8 + (g ^ (4 (k & 3))), of 8
+//         granules 4 (k & 1); a
 //         16-lane group's ds_read_b64_tr_b16 takes 4 k-rows of 16 columns and
 //         leaves each lane 4 k of its column.
 constexpr int HL_I = 256, HL_K = 64, HL_NT = 512, HL_NW = HL_NT / WAVE;
@@ -130,7 +131,7 @@ struct Loader {
         voff[p] = row < o.rows ? v : 0x80000000u;
       } else {
         constexpr int GR = T / 8;                  // granules of a k-row
-        const int k = q * (WAVE / GR) + lane / GR, g = (lane % GR) ^ (4 * (k & 3));
+        const int k = q * (WAVE / GR) + lane / GR, g = (lane % GR) ^ (4 * (k & 3) & (GR - 1));
         voff[p] = 2u * (static_cast<uint32_t>(k) * static_cast<uint32_t>(o.ld) + 8u * g);
       }
     }
@@ -170,7 +171,7 @@ struct Reader {
 #pragma unroll
       for (int f = 0; f < F; ++f) {
         const int col = i0 + 32 * f + 16 * (g & 1) + 4 * (j & 3);
-        at[f] = 16 * (k * (T / 8) + ((col >> 3) ^ (4 * (k & 3)))) + 2 * (col & 7);
+        at[f] = 16 * (k * (T / 8) + ((col >> 3) ^ (4 * (k & 3) & (T / 8 - 1)))) + 2 * (col & 7);
       }
     }
   }
@@ -751,16 +752,19 @@ __global__ __launch_bounds__(256) void k_head_fix(const HlArgs a, const HlGrad g
 }
 
 // dweight[c0 + v, d] = sum_n g[n, v] hidden[n, d]: i = d, j = v.  (Tiles of 128 or
-// 64 vocabulary rows are slower for few rows too: 255x1024x50257 58, 61, 73 us.)
+// 64 vocabulary rows are slower where those of 256 fill the CUs, also for few rows:
+// 255x1024x50257 58, 61, 73 us.)
 // What rounding took of g at the rows' tokens comes to the sums of the tokens'
 // rows: a wave's 64 vocabulary rows take one row's part each at a time, in the
 // order of the rows, in HL_FIXES turns at most, which bounds the time where many
-// rows have one token (more rows' roundings are as independent as any).
+// rows have one token (more rows' roundings are as independent as any; 4096 rows
+// of one token in a vocabulary of 64 would be 4096 turns of about a microsecond).
 constexpr int HL_FIXES = 16;
+template <int BJ>
 __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_head_dw(const HlArgs a, const uint16_t* g,
                                                                                             const HlFix* list, uint16_t* dw,
                                                                                             int c0, int cn, const Tiles ts) {
-  using S = Shape<256>;
+  using S = Shape<BJ>;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int w = threadIdx.x / WAVE;
   char* area = smem + S::NST * S::STAGE + w * S::AREA_W;
@@ -858,7 +862,7 @@ __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
           for (int j = 0; j < S::FJ; ++j) {
             const int n = 32 * j + (lane & 31), d = d0 + 4 * (lane >> 5);
             const HlFix f = fix[n0 + min(n, rows - 1)];
-            if (f.v < 0 || n >= rows) continue;
+            if (f.r == 0.0f || n >= rows) continue;
             floatx16 col[S::FI];
 #pragma unroll
             for (int i = 0; i < S::FI; ++i) col[i] = acc[i][j];
@@ -907,7 +911,7 @@ __global__ __launch_bounds__(256) void k_head_dh_join(const HlArgs a, const HlFi
     const float4 b = part[z * n4 + i];
     v = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
   }
-  if (f.v >= 0) {
+  if (f.r != 0.0f) {
     const uint2 w = *reinterpret_cast<const uint2*>(a.weight + static_cast<int64_t>(f.v) * a.dim + 4 * (i - n * (a.dim / 4)));
     v = make_float4(fmaf(f.r, BF16::to_f32(w.x & 0xFFFFu), v.x), fmaf(f.r, BF16::to_f32(w.x >> 16), v.y),
                     fmaf(f.r, BF16::to_f32(w.y & 0xFFFFu), v.z), fmaf(f.r, BF16::to_f32(w.y >> 16), v.w));
@@ -921,9 +925,16 @@ namespace {
 int cdiv(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 size_t al(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
-// j-tile of the products over rows: the rows' own size up to 128, so that a few
-// rows do not pay for 256
-int hl_bj(int64_t rows) { return rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+// j-tile of the logits' products: the rows' own size up to 128, so that a few rows
+// do not pay for 256, and smaller while that leaves half the CUs or more idle
+// (calls, 4096x4096x1000: 93 us with 64 tiles of 256, 54 with 256 of 64; 255x768x32000
+// 32 and, 250 of 128, 24).
+constexpr int HL_CUS = 256;
+int hl_few(int64_t ni, int64_t nj, int bj = 256) {
+  while (bj > 64 && 2 * ni * cdiv(nj, bj) <= HL_CUS) bj /= 2;
+  return bj;
+}
+int hl_bj(int64_t rows, int64_t vocab) { return hl_few(cdiv(vocab, HL_I), rows, rows <= 64 ? 64 : rows <= 128 ? 128 : 256); }
 int hl_parts(int64_t vocab) { return cdiv(vocab, HL_I); }
 
 // Vocabulary rows of a backward chunk: g's bytes stay within HL_G_BYTES, but a
@@ -948,7 +959,6 @@ int hl_dh_bj(int64_t rows, int64_t dim) {
 // Ranges of a chunk's vocabulary rows that dhidden's product is split into: as
 // many as give every CU a tile, of 8 stages or more; each but the last `per`
 // stages, none empty.
-constexpr int HL_CUS = 256;
 struct Split {
   int nz, per;
 };
@@ -1004,7 +1014,7 @@ hipError_t launch_head(const fl_head_args& a, hipStream_t s) {
   const int parts = hl_parts(a.vocab);
   float* xt = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + al(16 * static_cast<size_t>(a.rows) * parts));
   hipError_t e = hipSuccess;
-  hl_by(hl_bj(a.rows), [&](auto bj) {
+  hl_by(hl_bj(a.rows, a.vocab), [&](auto bj) {
     constexpr int BJ = decltype(bj)::value;
     const Tiles ts = {cdiv(a.vocab, HL_I), cdiv(a.rows, BJ), 1};
     e = hl_launch<Shape<BJ>>(k_head_stats<BJ>, ts, s, h, part, xt, ts);
@@ -1029,7 +1039,7 @@ hipError_t launch_head_grad(const fl_head_grad_args& a, hipStream_t s) {
   for (int c0 = 0; c0 < a.vocab && e == hipSuccess; c0 += chunk) {
     const int cn = static_cast<int>(std::min<int64_t>(chunk, (a.vocab - c0 + HL_K - 1) / HL_K * HL_K));
     const int nc = cdiv(cn, HL_I);
-    hl_by(hl_bj(a.rows), [&](auto bj) {
+    hl_by(hl_bj(a.rows, cn), [&](auto bj) {
       constexpr int BJ = decltype(bj)::value;
       using S = Shape<BJ>;
       const Tiles tg = {nc, cdiv(a.rows, BJ), 1};
@@ -1049,10 +1059,11 @@ hipError_t launch_head_grad(const fl_head_grad_args& a, hipStream_t s) {
         if (direct) e = hl_launch<S>(k_head_dh<BJ, true>, td, s, h, g, fix, sum, dh, c0, cn, td, sp.per, 1);
         else e = hl_launch<S>(k_head_dh<BJ, false>, td, s, h, g, fix, sum, dh, c0, cn, td, sp.per, c0 == 0 ? 1 : 0);
       });
-    if (e == hipSuccess && a.out_dweight) {
-      const Tiles tw = {nd, nc, 1};
-      e = hl_launch<Shape<256>>(k_head_dw, tw, s, h, g, list, static_cast<uint16_t*>(a.out_dweight), c0, cn, tw);
-    }
+    if (e == hipSuccess && a.out_dweight) hl_by(hl_few(nd, cn), [&](auto bj) {
+      constexpr int BJ = decltype(bj)::value;
+      const Tiles tw = {nd, cdiv(cn, BJ), 1};
+      e = hl_launch<Shape<BJ>>(k_head_dw<BJ>, tw, s, h, g, list, static_cast<uint16_t*>(a.out_dweight), c0, cn, tw);
+    });
   }
   if (e != hipSuccess) return e;
   if (dh != nullptr && !direct) {
