@@ -32,3 +32,31 @@ def test_each_tile_against_float64(N, D, V):
     dh, dw = torch.autograd.grad((a * s.logprob + b * s.entropy + c * s.lse).sum(), (hd, wd))
     _near(dh, ref["dh"], ref["t_dh"], "dh")
     _near(dw, ref["dw"], ref["t_dw"], "dw")
+
+
+def test_an_ignored_token_inside_the_vocabulary():
+    h, w, tok, ups = _inputs(90, 128, 400, 3)
+    tok = torch.where(tok < 0, torch.full_like(tok, 7), tok)
+    tok[1] = 6
+    ref = _ref(h, w, tok, ups, ignore=7)
+    hd, wd = h.cuda().requires_grad_(), w.cuda().requires_grad_()
+    s = lm_head_logprobs(hd, wd, tok.cuda(), entropy=True, lse=True, ignore_index=7)
+    _near(s.logprob, ref["logprob"], ref["t_logprob"], "logprob")
+    assert bool((s.logprob.detach().cpu()[tok == 7] == 0).all())
+    dh, dw = torch.autograd.grad((s.logprob, s.entropy, s.lse), (hd, wd), [u.cuda() for u in ups])
+    _near(dh, ref["dh"], ref["t_dh"], "dh")
+    _near(dw, ref["dw"], ref["t_dw"], "dw")
+
+
+def test_rows_past_the_lists_of_a_vocabulary_row():
+    """More rows of one token than are made good one by one, beside a row of
+    another: the same bounds as without that."""
+    h, w, tok, ups = _inputs(200, 128, 90, 5, scale=1.0)
+    tok = torch.full_like(tok, 33)
+    tok[150], tok[199] = 34, 89
+    ref = _ref(h, w, tok, ups)
+    hd, wd = h.cuda().requires_grad_(), w.cuda().requires_grad_()
+    s = lm_head_logprobs(hd, wd, tok.cuda(), entropy=True, lse=True)
+    dh, dw = torch.autograd.grad((s.logprob, s.entropy, s.lse), (hd, wd), [u.cuda() for u in ups])
+    _near(dh, ref["dh"], ref["t_dh"], "dh")
+    _near(dw, ref["dw"], ref["t_dw"], "dw")
