@@ -711,7 +711,7 @@ __global__ __launch_bounds__(HL_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 // and list by vocabulary row, for dweight: the 64 first rows with such a token, v
 // their number times 64 and the place, 0 behind the last.
 // 255x1024x50257 5 us, 4096x4096x128256 13 us for each of two chunks; what dweight
-// does with the list is 4 of its 56 us there, nothing here.
+// does with the list is 4 of its 56 us at the first size and not seen at the second.
 constexpr int HL_LIST = 64;
 __global__ __launch_bounds__(256) void k_head_fix(const HlArgs a, const HlGrad gr, const uint16_t* g, HlFix* fix, HlFix* list,
                                                   int c0, int cn) {
