@@ -213,7 +213,8 @@ __global__ __launch_bounds__(SC_NT) void k_score_slice(const fl_score_args a, co
   // 16-bit values at a time: right as soon as one value is not negative, else
   // it finds the one farthest from 0 (a value of the chunk still).  Only where
   // that matters are they taken again as floats: a slice of negative values,
-  // or fewer than K threads with one that is not.
+  // fewer than K threads with one that is not, or a K-th value of 0 (-0, which
+  // is equal to it, is the least of the integers).
   float cm[NCH];
   int tb = -0x7FFFFFFF - 1;
 #pragma unroll
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(SC_NT) void k_score_slice(const fl_score_args a, co
 
   // ---- the slice's K largest values
   fence();
-  if (!exact && s_key < 0x80000000u) {   // (a negative bound, by integer maxima)
+  if (!exact && s_key <= 0x80000000u) {   // (a negative bound, or 0, by integer maxima)
     __syncthreads();
     if (part) pad_all(NINF);
     tkey[tid] = f32_key(exact_maxima() + 0.0f);
