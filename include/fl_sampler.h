@@ -543,7 +543,7 @@ int fl_head_workspace_bytes(int64_t rows, int64_t vocab, size_t* out_bytes);
 /*
  * The gradients of fl_head_logprobs for upstream gradients of logprob, entropy
  * and lse (NULL: 0), each NULL if not asked for: out_dhidden [rows, dim]
- * (contiguous) and out_dweight [vocab, dim], bf16, summed in float32.  The
+ * (contiguous) and out_dweight [vocab, dim], bf16, 8-byte aligned, summed in float32.  The
  * logits are computed again, a chunk of the vocabulary at a time; their gradient
  * (as fl_score_tokens_grad's, zero rows and rows without a distribution
  * included) passes through the workspace in bf16.  Every sum has a fixed order.
