@@ -597,7 +597,7 @@ __global__ __launch_bounds__(HJ_R * HJ_P) void k_head_join(const fl_head_args a,
   const double logs = log(s), ref = static_cast<double>(m);
   const float ent = okr ? static_cast<float>(logs - u / s / static_cast<double>(HL_LOG2E)) : nan;
   if (a.out_entropy) a.out_entropy[n] = ent;
-  if (a.out_lse) a.out_lse[n] = okr ? static_cast<float>(ref + logs) : nan;
+  if (a.out_lse) a.out_lse[n] = okr ? static_cast<float>(ref + logs) : s == 0.0 ? ninf : nan;
   if (a.tokens && a.out_logprob) {
     const int64_t t = a.tokens[n];
     const bool bad = t < 0 || t >= a.vocab || !okr;
