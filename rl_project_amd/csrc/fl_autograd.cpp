@@ -10,6 +10,7 @@
 // library that Python loaded (bind).
 #include <torch/extension.h>
 
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -108,6 +109,19 @@ void refuse_capture(const char* functional) {
     C10_THROW_ERROR(Error, std::string("backward under stream capture: call ") + functional);
 }
 
+// No call has a forward-mode derivative: an input with a tangent is refused, not
+// taken without it.
+bool dual(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool dual(const OptTensor& t) { return t && dual(*t); }
+template <class... T>
+void refuse_tangents(const char* what, const T&... t) {
+  if ((dual(t) || ...) && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    C10_THROW_ERROR(NotImplementedError, std::string(what) + " has no forward-mode derivative");
+}
+void refuse_tangents(const char* what, const variable_list& v) {
+  for (const Tensor& t : v) refuse_tangents(what, t);
+}
+
 Tensor upstream(const Tensor& g) { return g.defined() ? g.contiguous() : g; }
 
 // ---------------------------------------------------------------- layer norm
@@ -180,6 +194,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_capture("layer_norm_backward");
+    refuse_tangents("layer_norm_backward", grads);
     const auto saved = ctx->get_saved_variables();
     const int64_t b = ctx->saved_data["bias"].toInt();
     const auto btype = b >= 0 ? std::optional<at::ScalarType>(static_cast<at::ScalarType>(b)) : std::nullopt;
@@ -298,6 +313,7 @@ struct Score : torch::autograd::Function<Score> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_capture("score_tokens_backward");
+    refuse_tangents("score_tokens_backward", grads);
     const auto kept = ctx->get_saved_variables();
     Tensor g[3];
     variable_list out(7);
@@ -383,6 +399,7 @@ struct Head : torch::autograd::Function<Head> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_capture("lm_head_logprobs_backward");
+    refuse_tangents("lm_head_logprobs_backward", grads);
     const auto kept = ctx->get_saved_variables();
     Tensor g[3];
     if (!upstreams(ctx, grads, g)) return variable_list(6);
@@ -411,41 +428,51 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   using release = py::call_guard<py::gil_scoped_release>;
   m.def("bind", &bind);
   // (differentiable)
-  m.def("layer_norm", [](const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) { return LayerNorm::apply(x, w, b, eps); },
-        release());
+  m.def("layer_norm", [](const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
+    refuse_tangents("layer_norm", x, w, b);
+    return LayerNorm::apply(x, w, b, eps);
+  }, release());
   m.def("score", [](const Tensor& x, const OptTensor& t, int64_t k, bool e, bool l, bool r, int64_t ii) {
+    refuse_tangents("score_tokens", x);
     return Score::apply(x, t, k, e, l, r, ii);
   }, release());
   m.def("head", [](const Tensor& h, const Tensor& w, const OptTensor& t, bool e, bool l, int64_t ii) {
+    refuse_tangents("lm_head_logprobs", h, w);
     return Head::apply(h, w, t, e, l, ii);
   }, release());
   // (the launches alone)
   m.def("norm_forward", [](const Tensor& x, const OptTensor& w, const OptTensor& b, double eps, bool keep) {
+    refuse_tangents("layer_norm", x, w, b);
     const at::NoGradGuard no_grad;
     auto [y, stats] = norm_forward(x, w, b, eps, keep);
     return or_none({y, stats});
   }, release());
   m.def("norm_backward", [](const Tensor& g, const Tensor& x, const OptTensor& w, const OptTensor& b, const Tensor& stats, bool nx,
                             bool nw, bool nb) {
+    refuse_tangents("layer_norm_backward", g, x, w, stats);
     const at::NoGradGuard no_grad;
     return or_none(norm_backward(g, x, or_undefined(w), stats, nx, nw && w, w ? type_of(w) : type_of(b),
                                  nb ? type_of(b) : std::nullopt));
   }, release());
   m.def("score_forward", [](const Tensor& x, const OptTensor& t, int64_t k, bool e, bool l, bool r, int64_t ii, bool save) {
+    refuse_tangents("score_tokens", x);
     const at::NoGradGuard no_grad;
     return or_none(score_forward(x, t, k, e, l, r, ii, save));
   }, release());
   m.def("score_backward", [](const Tensor& x, const OptTensor& t, const Tensor& saved, const OptTensor& ga, const OptTensor& gb,
                              const OptTensor& gc, int64_t ii) {
+    refuse_tangents("score_tokens_backward", x, saved, ga, gb, gc);
     const at::NoGradGuard no_grad;
     return score_backward(x, or_undefined(t), saved, or_undefined(ga), or_undefined(gb), or_undefined(gc), ii);
   }, release());
   m.def("head_forward", [](const Tensor& h, const Tensor& w, const OptTensor& t, bool e, bool l, int64_t ii, bool save) {
+    refuse_tangents("lm_head_logprobs", h, w);
     const at::NoGradGuard no_grad;
     return or_none(head_forward(h, w, t, e, l, ii, save));
   }, release());
   m.def("head_backward", [](const Tensor& h, const Tensor& w, const OptTensor& t, const Tensor& saved, const OptTensor& ga,
                             const OptTensor& gb, const OptTensor& gc, int64_t ii, bool nh, bool nw) {
+    refuse_tangents("lm_head_logprobs_backward", h, w, saved, ga, gb, gc);
     const at::NoGradGuard no_grad;
     return or_none(head_backward(h, w, or_undefined(t), saved, or_undefined(ga), or_undefined(gb), or_undefined(gc), ii, nh, nw));
   }, release());

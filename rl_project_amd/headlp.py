@@ -56,10 +56,10 @@ def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optiona
     ``score_tokens``; up to 131072 rows.  (The gradient of ``weight`` is a product
     over all rows: a NaN in the hidden states of an ignored row is in it too.)
 
-    Differentiable (once) in ``hidden`` and ``weight`` (and through ``norm``), except
-    under stream capture: a captured step takes ``return_saved=True``, which
-    returns ``(scores, saved)``, under ``torch.no_grad()``, and
-    ``lm_head_logprobs_backward``.  The backward pass holds the logits' gradient
+    Differentiable (once, in reverse mode) in ``hidden`` and ``weight`` (and through
+    ``norm``), except under stream capture: a captured step takes
+    ``return_saved=True``, which returns ``(scores, saved)``, under
+    ``torch.no_grad()``, and ``lm_head_logprobs_backward``.  The backward pass holds the logits' gradient
     of a chunk of the vocabulary in bfloat16 (512 MiB, or 32 KiB a row)."""
     _check(hidden, weight)
     lead = hidden.shape[:-1]

@@ -42,8 +42,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     dtype; mean and variance (over D, not D - 1) in float32.  ``weight`` and
     ``bias`` (``[D]``, either may be None) share one dtype, ``x``'s or float32.
 
-    Differentiable (once) in all three, except under stream capture: a captured
-    step takes ``return_stats=True``, which returns ``(y, stats)``, under
+    Differentiable (once, in reverse mode) in all three, except under stream
+    capture: a captured step takes ``return_stats=True``, which returns ``(y, stats)``, under
     ``torch.no_grad()``, and ``layer_norm_backward``."""
     _check_x(x, "x")
     _check_affine(x, weight, bias)

@@ -87,8 +87,8 @@ def score_tokens(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *,
     -inf alone, has NaN results and ids -1; a -inf logit is a masked value, with
     probability and gradient 0.
 
-    Differentiable (once) in ``logits``, except under stream capture: a captured step
-    takes ``return_saved=True``, which returns ``(scores, saved)``, under
+    Differentiable (once, in reverse mode) in ``logits``, except under stream capture: a
+    captured step takes ``return_saved=True``, which returns ``(scores, saved)``, under
     ``torch.no_grad()``, and ``score_tokens_backward``.  Nothing here waits for
     the device unless ``check_tokens`` is set."""
     _check_logits(logits)
@@ -122,7 +122,7 @@ def _upstream(g: Optional[torch.Tensor], lead, dev: torch.device, name: str) -> 
         return None
     if g.shape != lead or g.device != dev:
         raise ValueError(f"{name} must be {tuple(lead)} on {dev}")
-    return g.detach().to(torch.float32).contiguous()
+    return g.to(torch.float32).contiguous()
 
 
 def score_tokens_backward(logits: torch.Tensor, tokens: Optional[torch.Tensor], saved: torch.Tensor,
