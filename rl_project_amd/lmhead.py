@@ -147,7 +147,8 @@ def lm_head_sample(hidden: torch.Tensor, weight: torch.Tensor, *, temperature: P
                    fused: Optional[bool] = None, norm=None) -> LmHeadOutput:
     """One decode step's ``lm_head`` and sampling (one token per row).
     ``norm=(weight, bias, eps)`` applies ``layer_norm`` to the hidden states
-    first (the model's final norm).
+    first (the model's final norm; its gradient graph is recorded only where
+    ``return_logits`` asks for the logits).
 
     ``fused`` None picks the faster path for the shape (``fused_is_faster``):
     today always ``torch.nn.functional.linear`` followed by ``sample_tokens``,
@@ -156,7 +157,10 @@ def lm_head_sample(hidden: torch.Tensor, weight: torch.Tensor, *, temperature: P
     are sampled by ``fl_sample`` over the GEMM's logits, with the same
     uniforms, and batches above 64 rows run in groups of 64.  Any other row
     status raises ``SamplingError`` (unless ``check_status`` is off)."""
-    hidden = _normed(hidden, norm)
+    # (a sampled token has no gradient: a model's own parameters as the norm's, and
+    # outside torch.no_grad(), are no reason to record a graph, nor to refuse capture)
+    with torch.set_grad_enabled(torch.is_grad_enabled() and return_logits):
+        hidden = _normed(hidden, norm)
     B = hidden.size(0)
     if fused is None:
         fused = fused_is_faster(B, hidden.size(-1), weight.size(0))
