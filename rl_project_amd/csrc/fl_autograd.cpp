@@ -327,6 +327,38 @@ struct Score : torch::autograd::Function<Score> {
   }
 };
 
+// The gradient of a statistic that another kernel computed: value (float32, the
+// logits' leading dimensions) is passed on, bit for bit, as the tokens'
+// log-probability or, without tokens, as the entropy.  The backward pass takes
+// the softmax's statistics by itself (one more read of the logits).
+struct Stat : torch::autograd::Function<Stat> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& value, const OptTensor& tokens,
+                        int64_t ignore_index) {
+    ctx->save_for_backward({logits, tokens ? *tokens : Tensor()});
+    ctx->saved_data["ignore"] = ignore_index;
+    if (!tokens) ctx->saved_data["entropy"] = value.clone();   // (the result may be changed)
+    return value.detach();
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_capture("score_tokens_backward");
+    refuse_tangents("score_tokens_backward", grads);
+    const auto kept = ctx->get_saved_variables();
+    const Tensor &x = kept[0], &tokens = kept[1], none;
+    const int64_t ignore = ctx->saved_data["ignore"].toInt();
+    const bool lp = tokens.defined();
+    variable_list out(4);
+    {
+      const at::NoGradGuard no_grad;
+      const Tensor g = upstream(grads[0]), saved = score_forward(x, std::nullopt, 0, !lp, false, false, ignore, true)[6];
+      // (the value's own entropy: NaN, and so the gradient, where a logit is -inf)
+      if (!lp) saved.select(1, 2).copy_(ctx->saved_data["entropy"].toTensor().reshape({-1}));
+      out[0] = score_backward(x, tokens, saved, lp ? g : none, lp ? none : g, none, ignore);
+    }
+    return once(std::move(out));
+  }
+};
+
 // ---------------------------------------------------------------- head
 // logprob, entropy, lse, saved: undefined where not asked for
 variable_list head_forward(const Tensor& hidden, const Tensor& weight, const OptTensor& tokens, bool entropy, bool lse,
@@ -436,6 +468,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     refuse_tangents("score_tokens", x);
     return Score::apply(x, t, k, e, l, r, ii);
   }, release());
+  m.def("stat", [](const Tensor& x, const Tensor& value, const OptTensor& t, int64_t ii) { return Stat::apply(x, value, t, ii); },
+        release());
   m.def("head", [](const Tensor& h, const Tensor& w, const OptTensor& t, bool e, bool l, int64_t ii) {
     refuse_tangents("lm_head_logprobs", h, w);
     return Head::apply(h, w, t, e, l, ii);

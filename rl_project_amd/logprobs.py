@@ -10,7 +10,8 @@ Drop-ins with the reference's signatures and results (float32, shapes
 * ``kl_full_distribution(new_logits, ref_logits)`` -- ``training/common/logprobs.py:58-62``
 
 ``row_stats`` returns any combination of them (plus log-sum-exp) from one
-read of the logits.  A row's results are a function of the row alone: the same
+read of the logits, without a gradient; the first two drop-ins have one where
+their logits require it.  A row's results are a function of the row alone: the same
 bits in a call of any number of rows.  Logits must be on the ROCm device; there
 is no CPU path.
 """
@@ -101,19 +102,34 @@ def row_stats(logits: torch.Tensor, labels: Optional[torch.Tensor] = None, ref_l
     return RowStats(shape(o_lp), shape(o_h), shape(o_kl), shape(o_lse))
 
 
+def _with_graph(logits: torch.Tensor, value: torch.Tensor, labels: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``value`` as a result that ``logits`` have a gradient of, where they
+    require one (not under stream capture, which records no backward pass)."""
+    if not (logits.requires_grad and torch.is_grad_enabled()) or torch.cuda.is_current_stream_capturing():
+        return value
+    if labels is not None:
+        labels = labels.to(device=logits.device, dtype=torch.int64).contiguous()
+    return _lib.autograd().stat(logits, value, labels, IGNORE_INDEX)
+
+
 def token_logprobs_from_logits(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
     """Per-token ``log p(label)`` of ``logits [B, T, V]``, ``labels [B, T]``
-    (``-cross_entropy`` of the float32 logits; reference ``policy.py:47-50``)."""
-    return row_stats(logits, labels).logprob
+    (``-cross_entropy`` of the float32 logits; reference ``policy.py:47-50``).
+    Differentiable (once, in reverse mode; two reads of the logits and a write,
+    where ``score_tokens`` needs one read), except under stream capture."""
+    return _with_graph(logits, row_stats(logits, labels).logprob, labels)
 
 
 def entropy_from_logits(logits: torch.Tensor) -> torch.Tensor:
     """Per-position entropy ``[B, T]`` of the full distribution (reference
-    ``training/common/logprobs.py:65-68``)."""
-    return row_stats(logits, entropy=True).entropy
+    ``training/common/logprobs.py:65-68``).  Differentiable as
+    ``token_logprobs_from_logits`` is; a -inf logit makes value and gradient NaN,
+    as the reference's ``0 * -inf`` does (``score_tokens`` takes it as masked)."""
+    return _with_graph(logits, row_stats(logits, entropy=True).entropy)
 
 
 def kl_full_distribution(new_logits: torch.Tensor, ref_logits: torch.Tensor) -> torch.Tensor:
     """Exact per-token ``KL(new || ref)`` from full-vocabulary logits ``[B, T, V]``
-    (reference ``training/common/logprobs.py:58-62``)."""
+    (reference ``training/common/logprobs.py:58-62``); the result has no
+    gradient."""
     return row_stats(new_logits, ref_logits=ref_logits).kl
