@@ -47,7 +47,8 @@ typedef short short4v __attribute__((ext_vector_type(4)));
 typedef short short8v __attribute__((ext_vector_type(8)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef int int32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4_8 __attribute__((ext_vector_type(4), aligned(8)));   // (what a caller's results are aligned to)
+typedef uint32_t u32x4_8 __attribute__((ext_vector_type(4), aligned(8)));   // (what a caller's results are aligned to,
+typedef float floatx4_4 __attribute__((ext_vector_type(4), aligned(4)));    // and `saved`)
 
 constexpr float HL_LOG2E = 1.44269504088896340736f;
 
@@ -737,9 +738,9 @@ __global__ __launch_bounds__(256) void k_head_fix(const HlArgs a, const HlGrad g
       if (in) {
         const float ga = gr.ga && tk[u] != a.ignore_index ? gr.ga[n] : 0.0f;
         const float gb = gr.gb ? gr.gb[n] : 0.0f, gc = gr.gc ? gr.gc[n] : 0.0f;
-        const float* sv = gr.saved + 4 * static_cast<int64_t>(n);
-        const float l = (sv[3] - sv[0]) - sv[1], p = __builtin_amdgcn_exp2f(l * HL_LOG2E);
-        const float v = p * (gc - ga - gb * (fmaxf(l, -200.0f) + (gb == 0.0f ? 0.0f : sv[2]))) + ga;
+        const floatx4_4 sv = reinterpret_cast<const floatx4_4*>(gr.saved)[n];
+        const float l = (sv.w - sv.x) - sv.y, p = __builtin_amdgcn_exp2f(l * HL_LOG2E);
+        const float v = p * (gc - ga - gb * (fmaxf(l, -200.0f) + (gb == 0.0f ? 0.0f : sv.z))) + ga;
         const float was = BF16::to_f32(g[static_cast<int64_t>(n) * cn + (tk[u] - c0)]), lost = v - was;
         const float r = __builtin_fabsf(lost) <= __builtin_fabsf(was) * 0x1.02p-8f ? lost : 0.0f;   // (NaN: 0)
         fix[n] = HlFix{static_cast<int>(tk[u]), r};
