@@ -290,9 +290,6 @@ __global__ __launch_bounds__(SC_NT) void k_score_slice(const fl_score_args a, co
   // Past the slice's values a finite fill far below m, so that the fast sums of
   // a row's last slice have no NaN (float16 has none below a mask of its lowest).
   constexpr uint32_t FILL = D::id == FL_DTYPE_F32 ? 0xF149F2CAu : D::id == FL_DTYPE_BF16 ? 0xF149u : 0xFBFFu;   // -1e30; -65504
-  // (a token below the fill, a masked one, would count those places as greater:
-  // its slice is summed again below with -inf there, which no value is below)
-  const bool low = RANK && part && xt < as_float(static_cast<int>(D::id == FL_DTYPE_F32 ? FILL : FILL << 16));
   const bool plain = __builtin_fabsf(mb) < 0x1p31f && !(D::id == FL_DTYPE_F16 && part && m < -60000.0f);
   if (part && plain) pad_all(FILL);
   const double ref = m == -__builtin_inff() ? static_cast<double>(m)
@@ -315,9 +312,17 @@ __global__ __launch_bounds__(SC_NT) void k_score_slice(const fl_score_args a, co
       }
       __builtin_amdgcn_sched_barrier(0);   // (one chunk's comparisons live at a time)
     }
+    // (a token below the fill, a masked one, has counted the wave's places past
+    // the slice; summing its slice again instead, with -inf there: 318 us for
+    // bf16 4096x128256 with every token masked, 190 of other tokens)
+    if (RANK && part && xt < as_float(static_cast<int>(D::id == FL_DTYPE_F32 ? FILL : FILL << 16))) {
+#pragma unroll 1
+      for (int k = 0; k < NCH; ++k)
+        above -= static_cast<uint32_t>(min(max(N * (tid - lane + WAVE + k * SC_NT) - nval, 0), N * WAVE));
+    }
   }
   const float u0 = fu[0] + fu[1];
-  if (!plain || low || (ENT && __any(u0 != u0))) {   // (for the whole wave)
+  if (!plain || (ENT && __any(u0 != u0))) {   // (for the whole wave)
     const float ref0 = m == -__builtin_inff() ? 0.0f : m;
     fs[0] = fs[1] = fu[0] = fu[1] = 0.0f;
     above = 0;
