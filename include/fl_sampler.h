@@ -421,7 +421,8 @@ int fl_score_workspace_bytes(int64_t rows, int64_t vocab, int64_t top_k, size_t*
  * logprob, entropy and lse ([rows] each, NULL: 0):
  *   out_grad[r, i] = a (1[i == t] - p_i) - b p_i (log p_i + entropy) + c p_i
  * rounded once to the logits' dtype.  a counts as 0 where the token is ignored.
- * A masked value's gradient is 0, and so is a row's whose a, b and c are 0; else
+ * A masked value's gradient is 0 (a at the row's own token, also a masked one), and
+ * so is a row's whose a, b and c are 0; else
  * a row without a distribution has NaN.  saved and the logits are the forward
  * call's (its out_entropy asked for if grad_entropy is given).
  */
@@ -546,7 +547,10 @@ int fl_head_workspace_bytes(int64_t rows, int64_t vocab, size_t* out_bytes);
  * (contiguous) and out_dweight [vocab, dim], bf16, 8-byte aligned, summed in float32.  The
  * logits are computed again, a chunk of the vocabulary at a time; their gradient
  * (as fl_score_tokens_grad's, zero rows and rows without a distribution
- * included) passes through the workspace in bf16.  Every sum has a fixed order.
+ * included) passes through the workspace in bf16: an entry g loses at most 2^-8 of
+ * itself, except a row's own token's, whose loss is made good in float32 (in dweight
+ * for the first rows of a token, in 16 turns for 64 tokens at most).  Every sum has
+ * a fixed order.
  */
 typedef struct fl_head_grad_args {
   uint32_t struct_size;

@@ -11,9 +11,9 @@
 // their way meanwhile (the sums' barriers and the loads took turns before:
 // backward of bf16 4096x4096 32.5 us, 22.6 so).  Statistics and sums in
 // float32; one rounding to the type of x (dw, db: of the weight) at the end.
-// bf16 4096x4096: forward 15.0 us (4.5 TB/s of 67 MB), backward 22.6 us (4.5 TB/s
-// of 101 MB) and 3.9 us for the partial sums; 64x4096: 3.9 us, a launch's
-// length.
+// bf16 4096x4096: forward 15.0 to 16.5 us (4.5 to 4.1 TB/s of 67 MB), backward 22.6
+// to 23.9 us (4.5 to 4.2 TB/s of 101 MB) and 3.9 us for the partial sums; 64x4096:
+// 3.9 to 4.3 us, a launch's length.
 #include <algorithm>
 #include <type_traits>
 

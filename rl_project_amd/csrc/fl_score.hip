@@ -16,13 +16,15 @@
 // values of the slice in registers, so every step (maximum, sums, rank count,
 // the largest values) reads HBM once; the join of a row's slices is a second
 // kernel (none for a row of one slice).  bf16 4096x128256 (1.05 GB), whole calls:
-// 171 us for the log-probability (6.1 TB/s), 179 with the entropy, 200 with 5
-// alternatives, 208 to 223 with the rank too: bound by HBM, and past that by the
-// vector instructions and the meetings of the search.  12x128256 with 20
-// alternatives and the rank: 11.9 us + 4.9 us for the join, a chain of a load, eight
-// barriers and the list; 1x50257: 8 + 4 us.  (Fewer registers for 7 or 8 waves
-// per SIMD spill: 238 us with the entropy; slices streamed by one work-group per
-// row: 289 us with 5 alternatives.)
+// 170 us for the log-probability (6.2 TB/s), 179 with the entropy, 201 with 5
+// alternatives too, 203 with all that and the rank: bound by HBM, and past that by
+// the vector instructions and the meetings of the search.  12x128256 with 20
+// alternatives and the rank: 12.0 us + 4.7 us for the join, a chain of a load, eight
+// barriers and the list; 1x50257: 7.6 + 3.5 us.  A slice costs the instructions of
+// 16384 values whatever it holds: 4096 bf16 rows of 512, 4099, 8192 and 16384 take
+// 26, 28, 26 and 22 us with the entropy, for 4 to 134 MB.  (Fewer registers for 7
+// or 8 waves per SIMD spill: 238 us with the entropy; slices streamed by one
+// work-group per row: 289 us with 5 alternatives.)
 #include <type_traits>
 
 #include "fl_device.h"
@@ -560,7 +562,7 @@ __global__ __launch_bounds__(NT) void k_score_join(const fl_score_args a, const 
 // ---------------------------------------------------------------- gradient
 // Element by element: a read and a write of every value, which HBM bounds.
 // One work-group per piece of GR_NT x GR_U chunks of a row.  bf16 4096x128256 (2.1
-// GB): 385 to 419 us, 5.0 to 5.5 TB/s; f32 255x50257 (103 MB): 18.4 us.
+// GB): 355 to 419 us, 5.0 to 5.9 TB/s; f32 255x50257 (103 MB): 18.5 to 20 us.
 namespace {
 constexpr int GR_NT = 256, GR_U = 4;
 }

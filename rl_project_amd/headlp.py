@@ -59,8 +59,18 @@ def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optiona
     Differentiable (once, in reverse mode) in ``hidden`` and ``weight`` (and through
     ``norm``), except under stream capture: a captured step takes
     ``return_saved=True``, which returns ``(scores, saved)``, under
-    ``torch.no_grad()``, and ``lm_head_logprobs_backward``.  The backward pass holds the logits' gradient
-    of a chunk of the vocabulary in bfloat16 (512 MiB, or 32 KiB a row)."""
+    ``torch.no_grad()``, and ``lm_head_logprobs_backward``.
+
+    The backward pass holds the logits' gradient g of a chunk of the vocabulary in
+    bfloat16 (512 MiB, or 32 KiB a row).  An entry loses at most 2^-8 of itself, as
+    every entry does that a linear layer in bfloat16 is handed, so ``hidden``'s
+    gradient is off by at most 2^-8 of ``sum_v |g| |weight|`` and ``weight``'s by 2^-8
+    of ``sum_n |g| |hidden|``; the loss at a row's own token, the largest entry of
+    most rows, is made good.  Against the rounding of the results themselves: 1.00
+    to 1.07 times as far from 64 bits in random batches of 4099 tokens or more, up to
+    1.35 times with 64 to 512, up to 2.4 times for rows whose probability sits on
+    another token.  Where that matters, ``score_tokens`` over float32 logits keeps g
+    in float32."""
     _check(hidden, weight)
     lead = hidden.shape[:-1]
     tok = None
