@@ -62,6 +62,24 @@ def test_masked_rows_have_the_reference_s_nan():
     assert not bool(torch.isnan(d).any()) and float(d[1, 7]) == 0.0
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_masked_with_the_lowest_value(dtype):
+    """Finite in the reference: the entropy and both gradients are those of the values left."""
+    V = 9001
+    g = torch.Generator().manual_seed(5)
+    x = (2.5 * torch.randn(4, V, generator=g)).to(dtype)
+    x[:3].masked_fill_(torch.rand(3, V, generator=g) < torch.tensor([[0.5], [0.9], [0.999]]), torch.finfo(dtype).min)
+    tok = x.float().argmax(1)
+    a, b, zero = torch.randn(4, generator=g), torch.randn(4, generator=g), torch.zeros(4)
+    xd = x.cuda().requires_grad_()
+    ref = _reference(x, tok, 0)
+    (d1,) = torch.autograd.grad(token_logprobs_from_logits(xd, tok.cuda()), xd, a.cuda())
+    (d2,) = torch.autograd.grad(entropy_from_logits(xd), xd, b.cuda())
+    for d, ups in ((d1, (a, zero)), (d2, (zero, b))):
+        want, tol = _want_grad(ref, tok, *ups, zero, dtype)
+        _near(d, want, tol, "masked")
+
+
 def test_calls_without_a_gradient_are_as_ever():
     x = torch.randn(4, 300, device="cuda", requires_grad=True)
     tok = torch.zeros(4, dtype=torch.int64, device="cuda")
