@@ -40,9 +40,9 @@
 extern "C" {
 #endif
 
-#define FL_ABI_VERSION 7
+#define FL_ABI_VERSION 8
 
-enum fl_dtype { FL_DTYPE_F32 = 0, FL_DTYPE_BF16 = 1, FL_DTYPE_F16 = 2 };
+enum fl_dtype { FL_DTYPE_F32 = 0, FL_DTYPE_BF16 = 1, FL_DTYPE_F16 = 2, FL_DTYPE_E4M3 = 3 /* caches alone */ };
 
 enum fl_result { FL_OK = 0, FL_EIO = -5, FL_EINVAL = -22, FL_ENOTSUP = -95 };
 
@@ -576,6 +576,190 @@ typedef struct fl_head_grad_args {
 int fl_head_logprobs_grad(const fl_head_grad_args* args, void* stream);
 /* dhidden: whether out_dhidden will be asked for (0 or 1) */
 int fl_head_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t vocab, int32_t dhidden, size_t* out_bytes);
+
+/*
+ * Norms of queries and keys for each head, and their rotation by position:
+ *   y   = x weight / sqrt(mean(x^2) + eps)       (norm != 0; the mean over dim)
+ *   out = y, its first `rotated` values turned pair by pair: pair p by the angle
+ *         a = position * inv_freq[p], (y_i, y_j) -> gain (y_i cos a - y_j sin a,
+ *         y_i sin a + y_j cos a), i = p, j = p + rotated / 2, or with
+ *         FL_ROPE_INTERLEAVED i = 2 p, j = 2 p + 1
+ * for every head of every token.  q [tokens, heads, dim] and k [tokens, kv_heads,
+ * dim] have dtype and strides of their own (the last dimension contiguous); the
+ * weights ([dim], contiguous, NULL: 1) have wdtype, which is dtype or
+ * FL_DTYPE_F32; out_q and out_k are contiguous.  Sums in float32, angles in
+ * float64 (positions up to 2^40 keep 12 digits), one rounding at the end.  dim is
+ * even, up to FL_ROPE_MAX_DIM; rotated is even, 0 to dim.  kv_heads may be 0.
+ */
+#define FL_ROPE_MAX_DIM 512
+#define FL_ROPE_INTERLEAVED 1   /* pairs side by side */
+#define FL_ROPE_POSITIONS32 2   /* positions are int32, not int64 */
+typedef struct fl_rope_args {
+  uint32_t struct_size;
+  int32_t dtype;
+  int32_t wdtype;
+  int32_t flags;
+  const void* q;
+  const void* k;
+  int64_t tokens;
+  int64_t heads;
+  int64_t kv_heads;
+  int64_t dim;
+  int64_t rotated;
+  int64_t q_ld;                /* elements from token to token */
+  int64_t q_hs;                /* elements from head to head */
+  int64_t k_ld;
+  int64_t k_hs;
+  const void* positions;       /* [tokens] */
+  const double* inv_freq;      /* [rotated / 2] */
+  const void* q_weight;
+  const void* k_weight;
+  float eps;                   /* >= 0, finite */
+  float gain;
+  int32_t norm;
+  int32_t reserved;            /* 0 */
+  void* out_q;                 /* [tokens, heads, dim] */
+  void* out_k;
+} fl_rope_args;
+
+int fl_qk_norm_rope(const fl_rope_args* args, void* stream);
+
+/*
+ * The gradients of fl_qk_norm_rope for the upstream gradients grad_q and grad_k
+ * (contiguous, dtype; NULL: 0): out_q and out_k of `fwd` receive dq and dk,
+ * out_dwq and out_dwk ([dim], wdtype, summed over tokens and heads in a fixed
+ * order) the weights' (each NULL if not asked for).  The other fields of `fwd` are
+ * the forward call's.  workspace (fl_qk_norm_rope_grad_workspace_bytes, 16-byte
+ * aligned): calls that overlap in time must not share one; not needed without
+ * out_dwq and out_dwk.
+ */
+typedef struct fl_rope_grad_args {
+  uint32_t struct_size;
+  int32_t reserved;            /* 0 */
+  fl_rope_args fwd;
+  const void* grad_q;
+  const void* grad_k;
+  void* out_dwq;
+  void* out_dwk;
+  void* workspace;
+  int64_t workspace_bytes;
+} fl_rope_grad_args;
+
+int fl_qk_norm_rope_grad(const fl_rope_grad_args* args, void* stream);
+int fl_qk_norm_rope_grad_workspace_bytes(int64_t tokens, int64_t dim, size_t* out_bytes);
+
+/*
+ * A layer's keys and values in pages of page_size (16, 32, 64 or 128) tokens:
+ *   k [pages, heads, page_size, dim],  v [pages, heads, dim, page_size]
+ * contiguous, 16-byte aligned (a page's values lie as the matrix cores take them:
+ * a channel's tokens side by side).  dim is a multiple of 8 up to
+ * FL_CACHE_MAX_DIM.  dtype is FL_DTYPE_BF16, FL_DTYPE_F16 or FL_DTYPE_E4M3; the
+ * last holds a token's row x of one head as e4m3(x 2^-e), e the least integer
+ * (within -96 .. 120; 0 for a row of zeros) with max|x| 2^-e <= 448, and e + 127 in
+ * k_scale / v_scale ([pages, heads, page_size], 16-byte aligned): the scale itself
+ * rounds nothing.  A NaN or infinity becomes NaN; the maximum is the finite values'.
+ */
+#define FL_CACHE_MAX_DIM 256
+typedef struct fl_cache {
+  void* k;
+  void* v;
+  uint8_t* k_scale;            /* FL_DTYPE_E4M3 alone */
+  uint8_t* v_scale;
+  int64_t pages;               /* 1 .. 2^31 - 1 */
+  int64_t heads;
+  int64_t page_size;
+  int64_t dim;
+  int32_t dtype;
+  int32_t reserved;            /* 0 */
+} fl_cache;
+
+/*
+ * The tokens of a call on a cache: of sequence b the newest n_b of the lengths[b]
+ * it has (these among them), at positions lengths[b] - n_b up, and in rows
+ * starts[b] .. starts[b + 1] - 1 of the call's tensors.  starts (NULL: every
+ * sequence has tokens / seqs new tokens) ascends from 0; rows at starts[seqs] or
+ * behind are neither read nor written.  Position t of sequence b is slot t %
+ * page_size of page table[b * table_ld + t / page_size].  table, lengths and starts
+ * are read on the device: a token whose position is negative does not exist, and one
+ * whose page is missing (the number outside 0 .. pages - 1, or the position past the
+ * table) is never read or written in the cache.
+ */
+typedef struct fl_cache_rows {
+  const int32_t* table;        /* [seqs, table_width], row stride table_ld */
+  const int32_t* lengths;      /* [seqs] */
+  const int32_t* starts;       /* [seqs + 1] or NULL */
+  int64_t seqs;
+  int64_t tokens;              /* rows of the call's tensors */
+  int64_t table_width;
+  int64_t table_ld;
+} fl_cache_rows;
+
+/*
+ * fl_cache_write: k and v ([tokens, heads, dim], dtype, strides of their own, the
+ * last dimension contiguous) into the cache.  dtype is the cache's, or any of
+ * F32, BF16 and F16 for FL_DTYPE_E4M3.  A token without a page is left out.
+ * fl_cache_read: the tokens' values from the cache into k and v (dtype F32, BF16
+ * or F16, rounded once): 0 for a token that does not exist, NaN without a page.
+ * Sequences that share a page may read it together; where several write one slot
+ * in a call, any of them may be the last.
+ */
+typedef struct fl_cache_args {
+  uint32_t struct_size;
+  int32_t dtype;
+  fl_cache cache;
+  fl_cache_rows rows;
+  void* k;
+  void* v;
+  int64_t k_ld;                /* elements from token to token */
+  int64_t k_hs;                /* elements from head to head */
+  int64_t v_ld;
+  int64_t v_hs;
+} fl_cache_args;
+
+int fl_cache_write(const fl_cache_args* args, void* stream);
+int fl_cache_read(const fl_cache_args* args, void* stream);
+
+/*
+ * Attention of each sequence's newest tokens over its pages, each token's query
+ * heads / cache.heads of every cached head:
+ *   s_t = scale q . k_t, cap tanh(s / cap) with softcap > 0
+ *   out = sum_t softmax(s)_t v_t,   out_lse = log sum_t exp(s_t)
+ * over the positions t that token p sees: t <= p and, with window > 0, t > p -
+ * window or t < sinks.  The new tokens' own keys and values are in the cache (write
+ * first).  A token that sees nothing (its position negative) has out 0 and lse -inf;
+ * one that would see a token without a page has NaN; what a masked slot holds, NaN
+ * or infinity among it, does not matter.  q [tokens, q_heads, dim] and out have
+ * dtype (BF16 or F16; a 16-bit cache's own) and strides of their own, the last
+ * dimension contiguous: q 16-byte aligned with strides in multiples of 8 elements,
+ * out 8-byte with multiples of 4.  Scores, sums and results in float32; the weights
+ * exp(s - max) are rounded to dtype for the product with v.  A token's results
+ * depend on the shapes of the call (how its keys are split), not on other tokens.
+ * workspace (fl_paged_attention_workspace_bytes for the same args, 16-byte aligned):
+ * calls that overlap in time must not share one.
+ */
+typedef struct fl_attn_args {
+  uint32_t struct_size;
+  int32_t dtype;
+  fl_cache cache;
+  fl_cache_rows rows;
+  const void* q;
+  int64_t q_heads;
+  int64_t q_ld;
+  int64_t q_hs;
+  void* out;
+  int64_t out_ld;
+  int64_t out_hs;
+  float* out_lse;              /* [tokens, q_heads] or NULL */
+  float scale;
+  float softcap;               /* 0: none */
+  int64_t window;              /* 0: none */
+  int64_t sinks;
+  void* workspace;
+  int64_t workspace_bytes;
+} fl_attn_args;
+
+int fl_paged_attention(const fl_attn_args* args, void* stream);
+int fl_paged_attention_workspace_bytes(const fl_attn_args* args, size_t* out_bytes);
 
 /* Thread-local description of the last error returned on this thread. */
 const char* fl_last_error(void);

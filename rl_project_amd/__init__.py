@@ -25,6 +25,12 @@ lm_head_logprobs, lm_head_logprobs_backward
     The same from hidden states and the lm_head weight, without the [N, V] logits.
 layer_norm, layer_norm_backward
     The norm in front of the head, with its gradients.
+qk_norm_rope, qk_norm_rope_backward, rotary_frequencies
+    Norms of queries and keys for each head and their rotation by position, with
+    gradients.
+PagedCache, cache_write, cache_read, paged_attention
+    A paged key / value cache (16 bits, or 8 with scales) and attention of a decode
+    or verify step's, or a prompt's, new tokens over it.
 SamplingParams
     Per-request parameters with the reference's validation (inference/requests.py).
 """
@@ -35,6 +41,8 @@ from .sampling import (SampleOutput, SamplerPlan, SamplingError, apply_sampling_
 from .speculative import MTPSpeculativeGenerator, SpeculativeGenerator, SpecOutput, SpecPlan, speculative_verify
 from .engine import BatchedSampler
 from .logprobs import RowStats, entropy_from_logits, kl_full_distribution, row_stats, token_logprobs_from_logits
+from .cache import PagedCache, cache_read, cache_write, paged_attention
+from .rotary import qk_norm_rope, qk_norm_rope_backward, rotary_frequencies
 from .norm import layer_norm, layer_norm_backward
 from .scores import TokenScores, score_tokens, score_tokens_backward
 from .lmhead import LmHeadOutput, LmHeadPlan, lm_head_sample
@@ -49,4 +57,6 @@ __all__ = [
     "score_tokens", "score_tokens_backward", "TokenScores", "layer_norm", "layer_norm_backward",
     "lm_head_logprobs", "lm_head_logprobs_backward", "HeadScores",
     "lm_head_sample", "LmHeadPlan", "LmHeadOutput",
+    "qk_norm_rope", "qk_norm_rope_backward", "rotary_frequencies",
+    "PagedCache", "cache_write", "cache_read", "paged_attention",
 ]

@@ -18,8 +18,8 @@ import torch  # noqa: F401  (loads the HIP runtime the library binds to)
 LIB_PATH = os.environ.get("FL_SAMPLER_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib",
                                                             "libflsampler.so")
 
-FL_ABI_VERSION = 7
-FL_DTYPE_F32, FL_DTYPE_BF16, FL_DTYPE_F16 = 0, 1, 2
+FL_ABI_VERSION = 8
+FL_DTYPE_F32, FL_DTYPE_BF16, FL_DTYPE_F16, FL_DTYPE_E4M3 = 0, 1, 2, 3
 FL_OK, FL_EIO, FL_EINVAL, FL_ENOTSUP = 0, -5, -22, -95
 FL_ROW_OK, FL_ROW_NAN, FL_ROW_INF, FL_ROW_BAD_HISTORY, FL_ROW_LIMIT, FL_ROW_ALL_MASKED = 0, 1, 2, 4, 8, 16
 FL_FLAG_NO_SELECT = 1
@@ -156,6 +156,60 @@ class HeadGradArgs(ctypes.Structure):
     ]
 
 
+class RopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("wdtype", ctypes.c_int32), ("flags", ctypes.c_int32),
+        ("q", _p), ("k", _p), ("tokens", ctypes.c_int64), ("heads", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+        ("dim", ctypes.c_int64), ("rotated", ctypes.c_int64),
+        ("q_ld", ctypes.c_int64), ("q_hs", ctypes.c_int64), ("k_ld", ctypes.c_int64), ("k_hs", ctypes.c_int64),
+        ("positions", _p), ("inv_freq", _p), ("q_weight", _p), ("k_weight", _p),
+        ("eps", ctypes.c_float), ("gain", ctypes.c_float), ("norm", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("out_q", _p), ("out_k", _p),
+    ]
+
+
+class RopeGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("reserved", ctypes.c_int32), ("fwd", RopeArgs),
+        ("grad_q", _p), ("grad_k", _p), ("out_dwq", _p), ("out_dwk", _p), ("workspace", _p), ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+class Cache(ctypes.Structure):
+    _fields_ = [
+        ("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p),
+        ("pages", ctypes.c_int64), ("heads", ctypes.c_int64), ("page_size", ctypes.c_int64), ("dim", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class CacheRows(ctypes.Structure):
+    _fields_ = [
+        ("table", _p), ("lengths", _p), ("starts", _p),
+        ("seqs", ctypes.c_int64), ("tokens", ctypes.c_int64), ("table_width", ctypes.c_int64), ("table_ld", ctypes.c_int64),
+    ]
+
+
+class CacheArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("cache", Cache), ("rows", CacheRows),
+        ("k", _p), ("v", _p), ("k_ld", ctypes.c_int64), ("k_hs", ctypes.c_int64), ("v_ld", ctypes.c_int64), ("v_hs", ctypes.c_int64),
+    ]
+
+
+class AttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("cache", Cache), ("rows", CacheRows),
+        ("q", _p), ("q_heads", ctypes.c_int64), ("q_ld", ctypes.c_int64), ("q_hs", ctypes.c_int64),
+        ("out", _p), ("out_ld", ctypes.c_int64), ("out_hs", ctypes.c_int64), ("out_lse", _p),
+        ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("window", ctypes.c_int64), ("sinks", ctypes.c_int64),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+FL_ROPE_MAX_DIM = 512
+FL_ROPE_INTERLEAVED, FL_ROPE_POSITIONS32 = 1, 2
+FL_CACHE_MAX_DIM = 256
 FL_HEAD_MAX_ROWS = 131072
 FL_NORM_MAX_DIM = 16384
 FL_SCORE_MAX_TOPK = 64
@@ -242,6 +296,14 @@ def lib() -> ctypes.CDLL:
     handle.fl_head_grad_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
                                                     ctypes.POINTER(ctypes.c_size_t)]
     handle.fl_head_grad_workspace_bytes.restype = ctypes.c_int
+    for name, args in (("fl_qk_norm_rope", RopeArgs), ("fl_qk_norm_rope_grad", RopeGradArgs), ("fl_cache_write", CacheArgs),
+                       ("fl_cache_read", CacheArgs), ("fl_paged_attention", AttnArgs)):
+        getattr(handle, name).argtypes = [ctypes.POINTER(args), _p]
+        getattr(handle, name).restype = ctypes.c_int
+    handle.fl_qk_norm_rope_grad_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)]
+    handle.fl_qk_norm_rope_grad_workspace_bytes.restype = ctypes.c_int
+    handle.fl_paged_attention_workspace_bytes.argtypes = [ctypes.POINTER(AttnArgs), ctypes.POINTER(ctypes.c_size_t)]
+    handle.fl_paged_attention_workspace_bytes.restype = ctypes.c_int
     _lib = handle
     return handle
 
@@ -249,13 +311,15 @@ def lib() -> ctypes.CDLL:
 AUTOGRAD_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "_fl_autograd.so")
 _AUTOGRAD_ENTRIES = ("fl_last_error", "fl_score_tokens", "fl_score_workspace_bytes", "fl_score_tokens_grad", "fl_layer_norm",
                      "fl_layer_norm_grad", "fl_layer_norm_grad_workspace_bytes", "fl_head_logprobs", "fl_head_workspace_bytes",
-                     "fl_head_logprobs_grad", "fl_head_grad_workspace_bytes")
+                     "fl_head_logprobs_grad", "fl_head_grad_workspace_bytes",
+                     "fl_qk_norm_rope", "fl_qk_norm_rope_grad", "fl_qk_norm_rope_grad_workspace_bytes", "fl_cache_write",
+                     "fl_cache_read", "fl_paged_attention", "fl_paged_attention_workspace_bytes")
 _autograd = None
 
 
 def autograd():
-    """The extension that launches score_tokens, layer_norm and lm_head_logprobs and
-    holds their autograd nodes (loaded once), bound to this library's entry points."""
+    """The extension that launches score_tokens, layer_norm, lm_head_logprobs,
+    qk_norm_rope and the calls on a paged cache, and holds their autograd nodes (loaded once), bound to this library's entry points."""
     global _autograd
     if _autograd is not None:
         return _autograd
@@ -304,4 +368,6 @@ EXPORTED_SYMBOLS = ("fl_sample", "fl_sample_exact", "fl_fill_rows", "fl_apply_fi
                     "fl_score_tokens", "fl_score_workspace_bytes", "fl_score_tokens_grad",
                     "fl_layer_norm", "fl_layer_norm_grad", "fl_layer_norm_grad_workspace_bytes",
                     "fl_head_logprobs", "fl_head_workspace_bytes", "fl_head_logprobs_grad", "fl_head_grad_workspace_bytes",
+                    "fl_qk_norm_rope", "fl_qk_norm_rope_grad", "fl_qk_norm_rope_grad_workspace_bytes",
+                    "fl_cache_write", "fl_cache_read", "fl_paged_attention", "fl_paged_attention_workspace_bytes",
                     "fl_last_error", "fl_abi_version")

@@ -85,6 +85,97 @@ int validate_head_pointers(const char* fn, const void* hidden, const void* weigh
   return 0;
 }
 
+// The rotation calls; 0 = go on.
+int validate_rope(const char* fn, const fl_rope_args& a) {
+  if (a.dtype != FL_DTYPE_F32 && a.dtype != FL_DTYPE_BF16 && a.dtype != FL_DTYPE_F16)
+    return fail(FL_EINVAL, "%s: unknown dtype %d", fn, a.dtype);
+  if (a.wdtype != a.dtype && a.wdtype != FL_DTYPE_F32)
+    return fail(FL_EINVAL, "%s: wdtype %d is neither dtype %d nor float32", fn, a.wdtype, a.dtype);
+  if (a.tokens < 0 || a.heads < 0 || a.kv_heads < 0 || a.dim < 2 || a.dim % 2 != 0 || a.rotated < 0 || a.rotated > a.dim ||
+      a.rotated % 2 != 0)
+    return fail(FL_EINVAL, "%s: bad shape tokens=%lld heads=%lld kv_heads=%lld dim=%lld rotated=%lld (dim and rotated even)", fn,
+                static_cast<long long>(a.tokens), static_cast<long long>(a.heads), static_cast<long long>(a.kv_heads),
+                static_cast<long long>(a.dim), static_cast<long long>(a.rotated));
+  if (a.dim > FL_ROPE_MAX_DIM || a.tokens > MAX_BLOCKS_256 || a.heads > 65536 || a.kv_heads > 65536)
+    return fail(FL_ENOTSUP, "%s: dim %lld, tokens %lld or heads beyond the library's limits", fn, static_cast<long long>(a.dim),
+                static_cast<long long>(a.tokens));
+  if ((a.flags & ~(FL_ROPE_INTERLEAVED | FL_ROPE_POSITIONS32)) != 0 || a.reserved != 0)
+    return fail(FL_EINVAL, "%s: unknown flags 0x%x or reserved not 0", fn, static_cast<unsigned>(a.flags));
+  if (!std::isfinite(a.eps) || a.eps < 0.0f || !std::isfinite(a.gain))
+    return fail(FL_EINVAL, "%s: eps must be finite and >= 0, gain finite", fn);
+  if (a.q_ld < 0 || a.q_hs < 0 || a.k_ld < 0 || a.k_hs < 0) return fail(FL_EINVAL, "%s: a negative stride", fn);
+  if (a.tokens > 0 && a.rotated > 0 && (!a.positions || !a.inv_freq))
+    return fail(FL_EINVAL, "%s: positions or inv_freq is NULL", fn);
+  return 0;
+}
+
+// The calls on a paged cache; 0 = go on.
+int validate_cache(const char* fn, const fl_cache& c, const fl_cache_rows& r) {
+  if (c.dtype != FL_DTYPE_BF16 && c.dtype != FL_DTYPE_F16 && c.dtype != FL_DTYPE_E4M3)
+    return fail(FL_EINVAL, "%s: cache dtype %d (bf16, f16 or e4m3)", fn, c.dtype);
+  if (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128)
+    return fail(FL_EINVAL, "%s: page_size %lld (16, 32, 64 or 128)", fn, static_cast<long long>(c.page_size));
+  if (c.pages < 1 || c.heads < 1 || c.dim < 8 || c.dim % 8 != 0 || c.reserved != 0 || r.seqs < 0 || r.tokens < 0 ||
+      r.table_width < 0 || (r.seqs > 1 && r.table_ld < r.table_width))
+    return fail(FL_EINVAL, "%s: bad shape pages=%lld heads=%lld dim=%lld (a multiple of 8) seqs=%lld tokens=%lld table %lld wide", fn,
+                static_cast<long long>(c.pages), static_cast<long long>(c.heads), static_cast<long long>(c.dim),
+                static_cast<long long>(r.seqs), static_cast<long long>(r.tokens), static_cast<long long>(r.table_width));
+  if (c.dim > FL_CACHE_MAX_DIM || c.pages > 0x7fffffff || c.heads > 65536 || r.seqs > 0x7fffff || r.tokens > 0x7fffff ||
+      r.table_width > 0x7fffffff / c.page_size)
+    return fail(FL_ENOTSUP, "%s: dim %lld, pages %lld, seqs %lld, tokens %lld or a table %lld wide beyond the library's limits", fn,
+                static_cast<long long>(c.dim), static_cast<long long>(c.pages), static_cast<long long>(r.seqs),
+                static_cast<long long>(r.tokens), static_cast<long long>(r.table_width));
+  if (r.starts == nullptr && r.seqs > 0 && r.tokens % r.seqs != 0)
+    return fail(FL_EINVAL, "%s: %lld tokens are not as many for each of %lld sequences (starts)", fn,
+                static_cast<long long>(r.tokens), static_cast<long long>(r.seqs));
+  if (r.tokens == 0 || r.seqs == 0) return 0;
+  if (!c.k || !c.v || !r.lengths || (r.table_width > 0 && !r.table)) return fail(FL_EINVAL, "%s: a required pointer is NULL", fn);
+  if (c.dtype == FL_DTYPE_E4M3 && (!c.k_scale || !c.v_scale)) return fail(FL_EINVAL, "%s: an e4m3 cache needs its scales", fn);
+  uintptr_t bits = reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v);
+  if (c.dtype == FL_DTYPE_E4M3) bits |= reinterpret_cast<uintptr_t>(c.k_scale) | reinterpret_cast<uintptr_t>(c.v_scale);
+  if ((bits & 15u) != 0) return fail(FL_EINVAL, "%s: the cache must be 16-byte aligned", fn);
+  return 0;
+}
+int validate_cache_call(const char* fn, const fl_cache_args* a, bool write) {
+  if (a == nullptr) return fail(FL_EINVAL, "%s: args is NULL", fn);
+  if (a->struct_size != sizeof(fl_cache_args)) return fail(FL_EINVAL, "%s: struct_size mismatch", fn);
+  if (a->dtype != FL_DTYPE_F32 && a->dtype != FL_DTYPE_BF16 && a->dtype != FL_DTYPE_F16)
+    return fail(FL_EINVAL, "%s: unknown dtype %d", fn, a->dtype);
+  if (const int rc = validate_cache(fn, a->cache, a->rows)) return rc;
+  if (write && a->cache.dtype != FL_DTYPE_E4M3 && a->dtype != a->cache.dtype)
+    return fail(FL_EINVAL, "%s: dtype %d is not the cache's %d", fn, a->dtype, a->cache.dtype);
+  if (a->k_ld < 0 || a->k_hs < 0 || a->v_ld < 0 || a->v_hs < 0) return fail(FL_EINVAL, "%s: a negative stride", fn);
+  if (fl::cache_blocks(*a) > MAX_BLOCKS_256)
+    return fail(FL_ENOTSUP, "%s: tokens %lld by heads %lld beyond the library's limits", fn, static_cast<long long>(a->rows.tokens),
+                static_cast<long long>(a->cache.heads));
+  if (a->rows.tokens > 0 && a->rows.seqs > 0 && (!a->k || !a->v)) return fail(FL_EINVAL, "%s: k or v is NULL", fn);
+  return 0;
+}
+int validate_attn(const char* fn, const fl_attn_args* a) {
+  if (a == nullptr) return fail(FL_EINVAL, "%s: args is NULL", fn);
+  if (a->struct_size != sizeof(fl_attn_args)) return fail(FL_EINVAL, "%s: struct_size mismatch", fn);
+  if (a->dtype != FL_DTYPE_BF16 && a->dtype != FL_DTYPE_F16) return fail(FL_ENOTSUP, "%s: dtype %d (bf16 or f16)", fn, a->dtype);
+  if (const int rc = validate_cache(fn, a->cache, a->rows)) return rc;
+  if (a->cache.dtype != FL_DTYPE_E4M3 && a->dtype != a->cache.dtype)
+    return fail(FL_EINVAL, "%s: dtype %d is not the cache's %d", fn, a->dtype, a->cache.dtype);
+  if (a->q_heads < 1 || a->q_heads % a->cache.heads != 0)
+    return fail(FL_EINVAL, "%s: %lld query heads over %lld cached", fn, static_cast<long long>(a->q_heads),
+                static_cast<long long>(a->cache.heads));
+  if (a->q_heads > 65536 || a->rows.tokens * a->q_heads > 0x7fffffff)
+    return fail(FL_ENOTSUP, "%s: tokens %lld by query heads %lld beyond the library's limits", fn,
+                static_cast<long long>(a->rows.tokens), static_cast<long long>(a->q_heads));
+  if (!std::isfinite(a->scale) || !std::isfinite(a->softcap) || a->softcap < 0.0f)
+    return fail(FL_EINVAL, "%s: scale must be finite, softcap finite and >= 0", fn);
+  if (a->window < 0 || a->sinks < 0) return fail(FL_EINVAL, "%s: window and sinks must be >= 0", fn);
+  if (a->q_ld < 0 || a->q_hs < 0 || a->out_ld < 0 || a->out_hs < 0 || ((a->q_ld | a->q_hs) & 7) != 0 ||
+      ((a->out_ld | a->out_hs) & 3) != 0)
+    return fail(FL_EINVAL, "%s: strides of q must be multiples of 8 elements, of out of 4", fn);
+  if (fl::attn_blocks(*a) > MAX_BLOCKS_256)
+    return fail(FL_ENOTSUP, "%s: tokens %lld by cached heads %lld beyond the library's limits", fn,
+                static_cast<long long>(a->rows.tokens), static_cast<long long>(a->cache.heads));
+  return 0;
+}
+
 int validate_sample(const fl_sample_args* a, const char* fn) {
   if (a == nullptr) return fail(FL_EINVAL, "%s: args is NULL", fn);
   if (a->struct_size != sizeof(fl_sample_args))
@@ -431,6 +522,84 @@ int fl_head_logprobs_grad(const fl_head_grad_args* a, void* stream) {
   if (((reinterpret_cast<uintptr_t>(a->out_dhidden) | reinterpret_cast<uintptr_t>(a->out_dweight)) & 7u) != 0)
     return fail(FL_EINVAL, "%s: out_dhidden and out_dweight must be 8-byte aligned", fn);
   return check_launch(fl::launch_head_grad(*a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int fl_qk_norm_rope(const fl_rope_args* a, void* stream) {
+  const char* fn = "fl_qk_norm_rope";
+  if (a == nullptr) return fail(FL_EINVAL, "%s: args is NULL", fn);
+  if (a->struct_size != sizeof(fl_rope_args)) return fail(FL_EINVAL, "%s: struct_size mismatch", fn);
+  if (const int rc = validate_rope(fn, *a)) return rc;
+  if (a->tokens == 0 || (a->heads == 0 && a->kv_heads == 0)) return ok();
+  if ((a->heads > 0 && (!a->q || !a->out_q)) || (a->kv_heads > 0 && (!a->k || !a->out_k)))
+    return fail(FL_EINVAL, "%s: a required pointer is NULL", fn);
+  return check_launch(fl::launch_rope(*a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int fl_qk_norm_rope_grad_workspace_bytes(int64_t tokens, int64_t dim, size_t* out_bytes) {
+  const char* fn = "fl_qk_norm_rope_grad_workspace_bytes";
+  if (out_bytes == nullptr) return fail(FL_EINVAL, "%s: out_bytes is NULL", fn);
+  if (tokens < 0 || dim < 2 || dim % 2 != 0 || dim > FL_ROPE_MAX_DIM || tokens > MAX_BLOCKS_256)
+    return fail(FL_EINVAL, "%s: bad tokens %lld or dim %lld", fn, static_cast<long long>(tokens), static_cast<long long>(dim));
+  *out_bytes = static_cast<size_t>(fl::rope_grad_parts(tokens)) * 2 * static_cast<size_t>(dim) * sizeof(float);
+  return ok();
+}
+
+int fl_qk_norm_rope_grad(const fl_rope_grad_args* a, void* stream) {
+  const char* fn = "fl_qk_norm_rope_grad";
+  if (a == nullptr) return fail(FL_EINVAL, "%s: args is NULL", fn);
+  if (a->struct_size != sizeof(fl_rope_grad_args) || a->fwd.struct_size != sizeof(fl_rope_args))
+    return fail(FL_EINVAL, "%s: struct_size mismatch", fn);
+  if (a->reserved != 0) return fail(FL_EINVAL, "%s: reserved must be 0", fn);
+  const fl_rope_args& f = a->fwd;
+  if (const int rc = validate_rope(fn, f)) return rc;
+  const bool weights = a->out_dwq || a->out_dwk;
+  if (weights && !f.norm) return fail(FL_EINVAL, "%s: weight gradients without a norm", fn);
+  if (!weights && (f.tokens == 0 || (!f.out_q && !f.out_k))) return ok();
+  if (f.norm && f.tokens > 0 && ((f.heads > 0 && !f.q) || (f.kv_heads > 0 && !f.k)))
+    return fail(FL_EINVAL, "%s: q or k is NULL", fn);
+  if (weights) {
+    const size_t need = static_cast<size_t>(fl::rope_grad_parts(f.tokens)) * 2 * static_cast<size_t>(f.dim) * sizeof(float);
+    if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < 0 || static_cast<size_t>(a->workspace_bytes) < need))
+      return fail(FL_EINVAL, "%s: workspace of %lld bytes, %zu needed", fn, static_cast<long long>(a->workspace_bytes), need);
+    if ((reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0) return fail(FL_EINVAL, "%s: workspace not 16-byte aligned", fn);
+  }
+  return check_launch(fl::launch_rope_grad(*a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int fl_cache_write(const fl_cache_args* a, void* stream) {
+  const char* fn = "fl_cache_write";
+  if (const int rc = validate_cache_call(fn, a, true)) return rc;
+  if (a->rows.tokens == 0 || a->rows.seqs == 0) return ok();
+  return check_launch(fl::launch_cache_write(*a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int fl_cache_read(const fl_cache_args* a, void* stream) {
+  const char* fn = "fl_cache_read";
+  if (const int rc = validate_cache_call(fn, a, false)) return rc;
+  if (a->rows.tokens == 0 || a->rows.seqs == 0) return ok();
+  return check_launch(fl::launch_cache_read(*a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int fl_paged_attention_workspace_bytes(const fl_attn_args* a, size_t* out_bytes) {
+  const char* fn = "fl_paged_attention_workspace_bytes";
+  if (out_bytes == nullptr) return fail(FL_EINVAL, "%s: out_bytes is NULL", fn);
+  if (const int rc = validate_attn(fn, a)) return rc;
+  *out_bytes = fl::attn_workspace_bytes(*a);
+  return ok();
+}
+
+int fl_paged_attention(const fl_attn_args* a, void* stream) {
+  const char* fn = "fl_paged_attention";
+  if (const int rc = validate_attn(fn, a)) return rc;
+  if (a->rows.tokens == 0 || a->rows.seqs == 0) return ok();
+  if (!a->q || !a->out) return fail(FL_EINVAL, "%s: q or out is NULL", fn);
+  if ((reinterpret_cast<uintptr_t>(a->q) & 15u) != 0 || (reinterpret_cast<uintptr_t>(a->out) & 7u) != 0)
+    return fail(FL_EINVAL, "%s: q must be 16-byte aligned, out 8-byte", fn);
+  const size_t need = fl::attn_workspace_bytes(*a);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < 0 || static_cast<size_t>(a->workspace_bytes) < need))
+    return fail(FL_EINVAL, "%s: workspace of %lld bytes, %zu needed", fn, static_cast<long long>(a->workspace_bytes), need);
+  if ((reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0) return fail(FL_EINVAL, "%s: workspace not 16-byte aligned", fn);
+  return check_launch(fl::launch_attn(*a, static_cast<hipStream_t>(stream)), fn);
 }
 
 }  // extern "C"

@@ -1,0 +1,85 @@
+// What the attention kernels share: types of the matrix instructions' operands, the
+// keys that a tile of queries sees, how they are split, and the partial results.
+#pragma once
+
+#include "fl_kernels.h"
+#include "fl_paged.h"
+
+namespace fl {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// 16-bit operands: 8 values of a lane as a uint4.
+struct OpBF16 {
+  using D = BF16;
+  typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+  typedef __bf16 x2 __attribute__((ext_vector_type(2)));
+  static constexpr uint32_t EXP = 0x7F80u, ONE = 0x0080u;   // the exponent's bits and its lowest
+  __device__ static __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+  }
+  __device__ static __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+  }
+  __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, x2));
+  }
+  // 4 e4m3 values as two dwords: exact (both types hold every e4m3 value)
+  __device__ static __forceinline__ uint2 widen(uint32_t q) {
+    return make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, 1.0f, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, 1.0f, true)));
+  }
+};
+struct OpF16 {
+  using D = F16;
+  typedef _Float16 x8 __attribute__((ext_vector_type(8)));
+  typedef _Float16 x2 __attribute__((ext_vector_type(2)));
+  static constexpr uint32_t EXP = 0x7C00u, ONE = 0x0400u;
+  __device__ static __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+  }
+  __device__ static __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+  }
+  __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, x2));
+  }
+  __device__ static __forceinline__ uint2 widen(uint32_t q) {
+    return make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q, 1.0f, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q, 1.0f, true)));
+  }
+};
+
+// The bits of 0x8000 where a 16-bit value of a dword is NaN or infinite.
+template <class Op>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  return ((w & (Op::EXP * 0x10001u)) + Op::ONE * 0x10001u) & 0x80008000u;
+}
+template <class Op>
+__device__ __forceinline__ uint32_t not_finite(uint4 q) {
+  return not_finite<Op>(q.x) | not_finite<Op>(q.y) | not_finite<Op>(q.z) | not_finite<Op>(q.w);
+}
+// ... and the dword with 0 for those.
+template <class Op>
+__device__ __forceinline__ uint32_t finite_or_0(uint32_t w) {
+  const uint32_t bad = not_finite<Op>(w);
+  return w & ~((bad >> 15) * 0xFFFFu);
+}
+template <class Op>
+__device__ __forceinline__ uint4 finite_or_0(uint4 q) {
+  return make_uint4(finite_or_0<Op>(q.x), finite_or_0<Op>(q.y), finite_or_0<Op>(q.z), finite_or_0<Op>(q.w));
+}
+
+constexpr float AT_LAZY = 8.0f;     // how far, in powers of two, scores may pass the maximum in use
+
+// One score's soft-cap, in powers of two afterwards.  tanh x = 1 - 2 / (e^2x + 1):
+// off by 2^-23 of 1, i.e. by cap 2^-23 in the score, far below the rounding of q k.
+__device__ __forceinline__ float attn_cap(float s, float to_z, float cap2) {
+  const float e = __builtin_amdgcn_exp2f(s * to_z);   // to_z = 2 log2(e) scale / cap
+  return cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(e + 1.0f);   // cap2 = cap log2(e)
+}
+
+
+}  // namespace fl

@@ -1,5 +1,5 @@
-// score_tokens, layer_norm and lm_head_logprobs as a torch extension over the C
-// ABI (include/fl_sampler.h): the launches with their allocations, and the
+// score_tokens, layer_norm, lm_head_logprobs, qk_norm_rope and the calls on a paged
+// cache as a torch extension over the C ABI (include/fl_sampler.h): the launches with their allocations, and the
 // autograd nodes.  The kernels are the library's; what is here would cost more
 // than the small calls' kernels in Python.  (Host time of layer_norm 255x1025,
 // forward and gradients: 110 us with a Python node, which waits for the
@@ -41,13 +41,22 @@ struct Entry {
   decltype(&fl_head_workspace_bytes) head_ws = nullptr;
   decltype(&fl_head_logprobs_grad) head_grad = nullptr;
   decltype(&fl_head_grad_workspace_bytes) head_grad_ws = nullptr;
+  decltype(&fl_qk_norm_rope) rope = nullptr;
+  decltype(&fl_qk_norm_rope_grad) rope_grad = nullptr;
+  decltype(&fl_qk_norm_rope_grad_workspace_bytes) rope_grad_ws = nullptr;
+  decltype(&fl_cache_write) cache_write = nullptr;
+  decltype(&fl_cache_read) cache_read = nullptr;
+  decltype(&fl_paged_attention) attn = nullptr;
+  decltype(&fl_paged_attention_workspace_bytes) attn_ws = nullptr;
 } L;
 
 void bind(const std::vector<uintptr_t>& p) {
-  TORCH_CHECK(p.size() == 11, "fl_autograd: 11 entry points expected");
+  TORCH_CHECK(p.size() == 18, "fl_autograd: 18 entry points expected");
   auto at = [&](size_t i, auto& f) { f = reinterpret_cast<std::decay_t<decltype(f)>>(p[i]); };
   at(0, L.last_error), at(1, L.score), at(2, L.score_ws), at(3, L.score_grad), at(4, L.norm), at(5, L.norm_grad),
-      at(6, L.norm_ws), at(7, L.head), at(8, L.head_ws), at(9, L.head_grad), at(10, L.head_grad_ws);
+      at(6, L.norm_ws), at(7, L.head), at(8, L.head_ws), at(9, L.head_grad), at(10, L.head_grad_ws),
+      at(11, L.rope), at(12, L.rope_grad), at(13, L.rope_grad_ws), at(14, L.cache_write), at(15, L.cache_read), at(16, L.attn),
+      at(17, L.attn_ws);
 }
 
 void check(int rc, const char* what) {
@@ -446,6 +455,181 @@ struct Head : torch::autograd::Function<Head> {
   }
 };
 
+// ---------------------------------------------------------------- norms and rotation
+// [tokens, heads, dim] whose last dimension is contiguous (a copy where it is not,
+// or where the leading dimensions do not fold)
+Tensor heads_of(const Tensor& x) {
+  Tensor r = x.dim() == 3 ? x : x.reshape({-1, x.size(-2), x.size(-1)});
+  bool fine = r.size(2) <= 1 || r.stride(2) == 1;
+  for (int i = 0; i < 2; ++i) fine = fine && (r.size(i) <= 1 || r.stride(i) >= 0);
+  return fine ? r : r.contiguous();
+}
+
+struct RopeSettings {
+  double eps, gain;
+  bool norm, interleaved;
+};
+
+// The arguments that both passes share; q2, k2: [tokens, heads, dim], or undefined
+// for a side that has no part in the call.
+fl_rope_args rope_args(const Tensor& q2, const Tensor& k2, const Tensor& qw, const Tensor& kw, const Tensor& positions,
+                       const Tensor& inv_freq, const RopeSettings& s) {
+  const Tensor& any = q2.defined() ? q2 : k2;
+  fl_rope_args a = {};
+  a.struct_size = sizeof(a);
+  a.dtype = dtype_of(any.scalar_type());
+  a.wdtype = qw.defined() ? dtype_of(qw.scalar_type()) : kw.defined() ? dtype_of(kw.scalar_type()) : a.dtype;
+  a.flags = (s.interleaved ? FL_ROPE_INTERLEAVED : 0) | (positions.scalar_type() == at::kInt ? FL_ROPE_POSITIONS32 : 0);
+  a.tokens = any.size(0), a.dim = any.size(2), a.rotated = 2 * inv_freq.size(0);
+  if (q2.defined()) a.q = q2.data_ptr(), a.heads = q2.size(1), a.q_ld = q2.stride(0), a.q_hs = q2.stride(1);
+  if (k2.defined()) a.k = k2.data_ptr(), a.kv_heads = k2.size(1), a.k_ld = k2.stride(0), a.k_hs = k2.stride(1);
+  a.positions = positions.data_ptr();
+  a.inv_freq = ptr<double>(inv_freq);
+  a.q_weight = ptr(qw), a.k_weight = ptr(kw);
+  a.eps = static_cast<float>(s.eps), a.gain = static_cast<float>(s.gain), a.norm = s.norm ? 1 : 0;
+  return a;
+}
+
+variable_list rope_forward(const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw, const Tensor& positions,
+                           const Tensor& inv_freq, const RopeSettings& s) {
+  const Tensor q2 = heads_of(q), k2 = heads_of(k), w1 = qw ? qw->contiguous() : Tensor(), w2 = kw ? kw->contiguous() : Tensor();
+  variable_list out{at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous)),
+                    at::empty(k.sizes(), k.options().memory_format(at::MemoryFormat::Contiguous))};
+  fl_rope_args a = rope_args(q2, k2, w1, w2, positions, inv_freq, s);
+  a.out_q = out[0].data_ptr(), a.out_k = out[1].data_ptr();
+  const c10::DeviceGuard guard(q.device());
+  check(L.rope(&a, stream_of(q)), "fl_qk_norm_rope");
+  return out;
+}
+
+// dq, dk, dwq, dwk: undefined where not asked for, and for a side without an
+// upstream gradient
+variable_list rope_backward(const Tensor& gq, const Tensor& gk, const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
+                            const Tensor& positions, const Tensor& inv_freq, const RopeSettings& s, const bool (&need)[4]) {
+  variable_list out(4);
+  Tensor q2, k2, g1, g2;
+  if (gq.defined() && (need[0] || need[2])) q2 = heads_of(q), g1 = gq.contiguous();
+  if (gk.defined() && (need[1] || need[3])) k2 = heads_of(k), g2 = gk.contiguous();
+  if (!q2.defined() && !k2.defined()) return out;
+  const Tensor w1 = qw.defined() ? qw.contiguous() : Tensor(), w2 = kw.defined() ? kw.contiguous() : Tensor();
+  fl_rope_grad_args a = {};
+  a.struct_size = sizeof(a);
+  a.fwd = rope_args(q2, k2, w1, w2, positions, inv_freq, s);
+  const auto like = [](const Tensor& x) { return at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous)); };
+  if (q2.defined() && need[0]) out[0] = like(q);
+  if (k2.defined() && need[1]) out[1] = like(k);
+  if (q2.defined() && need[2]) out[2] = at::empty({a.fwd.dim}, w1.options());
+  if (k2.defined() && need[3]) out[3] = at::empty({a.fwd.dim}, w2.options());
+  a.grad_q = ptr(g1), a.grad_k = ptr(g2);
+  a.fwd.out_q = ptr(out[0]), a.fwd.out_k = ptr(out[1]), a.out_dwq = ptr(out[2]), a.out_dwk = ptr(out[3]);
+  Tensor ws;
+  if (out[2].defined() || out[3].defined()) {
+    size_t n = 0;
+    check(L.rope_grad_ws(a.fwd.tokens, a.fwd.dim, &n), "fl_qk_norm_rope_grad_workspace_bytes");
+    ws = bytes(n, positions);
+    a.workspace = ws.data_ptr(), a.workspace_bytes = static_cast<int64_t>(n);
+  }
+  const c10::DeviceGuard guard(positions.device());
+  check(L.rope_grad(&a, stream_of(positions)), "fl_qk_norm_rope_grad");
+  return out;
+}
+
+struct Rope : torch::autograd::Function<Rope> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw,
+                               const Tensor& positions, const Tensor& inv_freq, double eps, double gain, bool norm, bool interleaved) {
+    const variable_list out = rope_forward(q, k, qw, kw, positions, inv_freq, {eps, gain, norm, interleaved});
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({q, k, qw ? *qw : Tensor(), kw ? *kw : Tensor(), positions, inv_freq});
+    ctx->saved_data["eps"] = eps, ctx->saved_data["gain"] = gain;
+    ctx->saved_data["norm"] = norm, ctx->saved_data["interleaved"] = interleaved;
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_capture("qk_norm_rope_backward");
+    refuse_tangents("qk_norm_rope_backward", grads);
+    const auto kept = ctx->get_saved_variables();
+    auto& d = ctx->saved_data;
+    // (the edges are those of the tensors given)
+    const bool has1 = kept[2].defined(), has2 = kept[3].defined();
+    const bool need[4] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), has1 && ctx->needs_input_grad(2),
+                          has2 && ctx->needs_input_grad(has1 ? 3 : 2)};
+    variable_list out;
+    {
+      const at::NoGradGuard no_grad;
+      out = rope_backward(grads[0], grads[1], kept[0], kept[1], kept[2], kept[3], kept[4], kept[5],
+                          {d["eps"].toDouble(), d["gain"].toDouble(), d["norm"].toBool(), d["interleaved"].toBool()}, need);
+    }
+    out.resize(10);
+    return once(std::move(out));
+  }
+};
+
+// ---------------------------------------------------------------- the paged cache
+struct CacheTensors {
+  Tensor k, v;
+  OptTensor k_scale, v_scale;
+};
+
+void set_cache(fl_cache& c, const CacheTensors& t) {
+  c.k = t.k.data_ptr(), c.v = t.v.data_ptr();
+  c.k_scale = t.k_scale ? ptr<uint8_t>(*t.k_scale) : nullptr, c.v_scale = t.v_scale ? ptr<uint8_t>(*t.v_scale) : nullptr;
+  c.pages = t.k.size(0), c.heads = t.k.size(1), c.page_size = t.k.size(2), c.dim = t.k.size(3);
+  c.dtype = t.k.scalar_type() == at::kFloat8_e4m3fn ? FL_DTYPE_E4M3 : dtype_of(t.k.scalar_type());
+}
+void set_rows(fl_cache_rows& r, const Tensor& table, const Tensor& lengths, const OptTensor& starts, int64_t tokens) {
+  r.table = ptr<int32_t>(table), r.lengths = ptr<int32_t>(lengths), r.starts = starts ? ptr<int32_t>(*starts) : nullptr;
+  r.seqs = lengths.size(0), r.tokens = tokens, r.table_width = table.size(1), r.table_ld = table.stride(0);
+}
+
+void cache_call(const CacheTensors& c, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths,
+                const OptTensor& starts, bool write) {
+  const Tensor k2 = write ? heads_of(k) : k, v2 = write ? heads_of(v) : v;
+  fl_cache_args a = {};
+  a.struct_size = sizeof(a);
+  a.dtype = dtype_of(k2.scalar_type());
+  set_cache(a.cache, c);
+  set_rows(a.rows, table, lengths, starts, k2.size(0));
+  a.k = k2.data_ptr(), a.v = v2.data_ptr();
+  a.k_ld = k2.stride(0), a.k_hs = k2.stride(1), a.v_ld = v2.stride(0), a.v_hs = v2.stride(1);
+  const c10::DeviceGuard guard(k2.device());
+  if (write) check(L.cache_write(&a, stream_of(k2)), "fl_cache_write");
+  else check(L.cache_read(&a, stream_of(k2)), "fl_cache_read");
+}
+
+// out, lse (undefined if not asked for); `into`: where out goes
+variable_list attention(const CacheTensors& c, const Tensor& q, const Tensor& table, const Tensor& lengths, const OptTensor& starts,
+                        double scale, double softcap, int64_t window, int64_t sinks, const OptTensor& into, bool want_lse) {
+  Tensor q2 = heads_of(q);
+  const bool odd = reinterpret_cast<uintptr_t>(q2.data_ptr()) % 16 != 0 || (q2.size(0) > 1 && q2.stride(0) % 8 != 0) ||
+                   (q2.size(1) > 1 && q2.stride(1) % 8 != 0);
+  if (odd) q2 = q2.clone(at::MemoryFormat::Contiguous);
+  variable_list out(2);
+  out[0] = into ? *into : at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  const Tensor o2 = into ? *into : out[0].view({q2.size(0), q2.size(1), q2.size(2)});
+  if (want_lse) out[1] = floats(q.sizes().slice(0, q.dim() - 1), q);
+  fl_attn_args a = {};
+  a.struct_size = sizeof(a);
+  a.dtype = dtype_of(q.scalar_type());
+  set_cache(a.cache, c);
+  set_rows(a.rows, table, lengths, starts, q2.size(0));
+  const auto stride = [](const Tensor& t, int i) { return t.size(i) > 1 ? t.stride(i) : int64_t{0}; };
+  a.q = q2.data_ptr(), a.q_heads = q2.size(1), a.q_ld = stride(q2, 0), a.q_hs = stride(q2, 1);
+  a.out = o2.data_ptr(), a.out_ld = stride(o2, 0), a.out_hs = stride(o2, 1);
+  a.out_lse = ptr<float>(out[1]);
+  a.scale = static_cast<float>(scale), a.softcap = static_cast<float>(softcap), a.window = window, a.sinks = sinks;
+  size_t n = 0;
+  check(L.attn_ws(&a, &n), "fl_paged_attention_workspace_bytes");
+  const c10::DeviceGuard guard(q.device());
+  Tensor ws;
+  if (n > 0) {
+    ws = bytes(n, q);
+    a.workspace = ws.data_ptr(), a.workspace_bytes = static_cast<int64_t>(n);
+  }
+  check(L.attn(&a, stream_of(q)), "fl_paged_attention");
+  return out;
+}
+
 // Undefined tensors as None
 std::vector<OptTensor> or_none(const variable_list& v) {
   std::vector<OptTensor> out;
@@ -509,5 +693,38 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     refuse_tangents("lm_head_logprobs_backward", h, w, saved, ga, gb, gc);
     const at::NoGradGuard no_grad;
     return or_none(head_backward(h, w, or_undefined(t), saved, or_undefined(ga), or_undefined(gb), or_undefined(gc), ii, nh, nw));
+  }, release());
+  m.def("rope", [](const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw, const Tensor& pos, const Tensor& f,
+                   double eps, double gain, bool norm, bool inter) {
+    refuse_tangents("qk_norm_rope", q, k, qw, kw);
+    return Rope::apply(q, k, qw, kw, pos, f, eps, gain, norm, inter);
+  }, release());
+  m.def("rope_forward", [](const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw, const Tensor& pos,
+                           const Tensor& f, double eps, double gain, bool norm, bool inter) {
+    refuse_tangents("qk_norm_rope", q, k, qw, kw);
+    const at::NoGradGuard no_grad;
+    return rope_forward(q, k, qw, kw, pos, f, {eps, gain, norm, inter});
+  }, release());
+  m.def("rope_backward", [](const OptTensor& gq, const OptTensor& gk, const Tensor& q, const Tensor& k, const OptTensor& qw,
+                            const OptTensor& kw, const Tensor& pos, const Tensor& f, double eps, double gain, bool norm, bool inter,
+                            bool weights) {
+    refuse_tangents("qk_norm_rope_backward", gq, gk, q, k, qw, kw);
+    const at::NoGradGuard no_grad;
+    const bool need[4] = {true, true, weights && qw, weights && kw};
+    return or_none(rope_backward(or_undefined(gq), or_undefined(gk), q, k, or_undefined(qw), or_undefined(kw), pos, f,
+                                 {eps, gain, norm, inter}, need));
+  }, release());
+  m.def("cache_call", [](const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& k, const Tensor& v,
+                         const Tensor& table, const Tensor& lengths, const OptTensor& starts, bool write) {
+    refuse_tangents("cache_write", k, v);
+    const at::NoGradGuard no_grad;
+    cache_call({ck, cv, ks, vs}, k, v, table, lengths, starts, write);
+  }, release());
+  m.def("attention", [](const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& q, const Tensor& table,
+                        const Tensor& lengths, const OptTensor& starts, double scale, double softcap, int64_t window, int64_t sinks,
+                        const OptTensor& into, bool lse) {
+    refuse_tangents("paged_attention", q);
+    const at::NoGradGuard no_grad;
+    return or_none(attention({ck, cv, ks, vs}, q, table, lengths, starts, scale, softcap, window, sinks, into, lse));
   }, release());
 }

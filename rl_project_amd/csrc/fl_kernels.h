@@ -53,4 +53,18 @@ size_t head_workspace_bytes(int64_t rows, int64_t vocab);
 hipError_t launch_head_grad(const fl_head_grad_args& a, hipStream_t s);
 size_t head_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t vocab, bool dhidden);
 
+// Norms and rotation of queries and keys, and their gradients (parts: of the
+// weights' sums).
+hipError_t launch_rope(const fl_rope_args& a, hipStream_t s);
+hipError_t launch_rope_grad(const fl_rope_grad_args& a, hipStream_t s);
+int64_t rope_grad_parts(int64_t tokens);
+
+// A paged cache: new tokens in, tokens out, attention over it (blocks: of a launch).
+hipError_t launch_cache_write(const fl_cache_args& a, hipStream_t s);
+hipError_t launch_cache_read(const fl_cache_args& a, hipStream_t s);
+int64_t cache_blocks(const fl_cache_args& a);
+hipError_t launch_attn(const fl_attn_args& a, hipStream_t s);
+size_t attn_workspace_bytes(const fl_attn_args& a);
+int64_t attn_blocks(const fl_attn_args& a);
+
 }  // namespace fl

@@ -1,0 +1,155 @@
+// Which tokens, keys and pages a work-group of a call on a paged cache works on: the
+// arithmetic alone, for the device and for a host's checks.
+#pragma once
+
+#include <stdint.h>
+
+#include "../../include/fl_sampler.h"
+
+#ifdef __HIPCC__
+#define FL_HD __host__ __device__ __forceinline__
+#else
+#define FL_HD inline
+#endif
+
+namespace fl {
+
+FL_HD int64_t least(int64_t a, int64_t b) { return a < b ? a : b; }
+FL_HD int64_t most(int64_t a, int64_t b) { return a < b ? b : a; }
+
+// A work-group's sequence: its rows row .. row + n - 1 hold the tokens at positions
+// pos .. pos + n - 1, and `tile` is the work-group's number among the sequence's.
+struct PagedSeq {
+  int b, n, tile;
+  int64_t row;
+  int64_t pos;
+};
+
+// Tiles of a launch, `per` of the sequences' rows x mul each: sequence b's begin at
+// starts[b] mul / per + extra b, which leaves it floor(n mul / per) + extra of them at
+// least.  (The host has checked that tokens x mul and the tiles stay below 2^31.)
+FL_HD int64_t paged_tiles(const fl_cache_rows& r, int64_t mul, int64_t per, int64_t extra, int64_t each) {
+  return r.starts == nullptr ? r.seqs * each : r.tokens * mul / per + extra * r.seqs;
+}
+
+// The sequence of tile x (`each`: tiles of every sequence where all have the same
+// number of tokens).  What starts and lengths hold cannot lead outside the rows.
+FL_HD PagedSeq paged_seq(const fl_cache_rows& r, int x, uint32_t mul, uint32_t per, int extra, int each) {
+  PagedSeq s;
+  int lo, hi;
+  const int tokens = static_cast<int>(r.tokens), seqs = static_cast<int>(r.seqs);
+  if (r.starts == nullptr) {
+    s.b = x / each;
+    s.tile = x - s.b * each;
+    const int n = tokens / seqs;
+    lo = n * s.b;
+    hi = lo + n;
+  } else {
+    // (unsigned: what starts holds is below 2^31 / mul, or no matter)
+    const auto base = [&](int m) { return static_cast<int>(static_cast<uint32_t>(r.starts[m]) * mul / per + extra * m); };
+    int a = 0, z = seqs - 1;
+    while (a < z) {   // the last sequence whose tiles begin at x or before
+      const int m = (a + z + 1) / 2;
+      if (base(m) <= x) a = m;
+      else z = m - 1;
+    }
+    s.b = a;
+    lo = static_cast<int>(least(most(r.starts[a], 0), tokens));
+    hi = static_cast<int>(least(most(r.starts[a + 1], lo), tokens));
+    s.tile = static_cast<int>(most(x - base(a), 0));
+  }
+  s.row = lo;
+  s.n = hi - lo;
+  s.pos = static_cast<int64_t>(r.lengths[s.b]) - s.n;
+  return s;
+}
+
+// The page of position t (0 <= t), or -1.
+FL_HD int paged_page(const fl_cache_rows& r, const fl_cache& c, int b, int64_t t) {
+  const int64_t i = t >> __builtin_ctzll(c.page_size);   // (a power of two)
+  if (i >= r.table_width) return -1;
+  const int p = r.table[b * r.table_ld + i];
+  return p >= 0 && p < c.pages ? p : -1;
+}
+
+// What a work-group of a write or a read works on: 16 neighbouring slots of one page
+// (or -1), slot up, aligned; those from t0 to t1 - 1 hold tokens of the call, slot + t
+// the one of row row0 + t.
+constexpr int KV_T = 16;
+struct KvTile {
+  int page, slot, t0, t1;
+  int64_t row0;
+};
+FL_HD int64_t kv_tiles(const fl_cache_rows& r, int* each) {
+  // (n tokens touch at most (n + 14) / 16 + 1 aligned runs of 16)
+  *each = static_cast<int>((r.tokens / r.seqs + KV_T - 2) / KV_T + 1);
+  return paged_tiles(r, 1, KV_T, 2, *each);
+}
+FL_HD bool kv_tile(const fl_cache_rows& r, const fl_cache& c, const PagedSeq& s, KvTile& t) {
+  const int64_t first = most(s.pos, 0), base = first / KV_T * KV_T + static_cast<int64_t>(s.tile) * KV_T;
+  const int64_t end = s.pos + s.n;
+  if (base >= end) return false;
+  t.t0 = static_cast<int>(most(first - base, 0));
+  t.t1 = static_cast<int>(least(end - base, KV_T));
+  t.row0 = s.row + (base - s.pos);
+  t.page = paged_page(r, c, s.b, base);
+  t.slot = static_cast<int>(base & (c.page_size - 1));
+  return true;
+}
+
+constexpr int AT_BLK = 64;          // keys of a step
+constexpr int AT_MIN_BLKS = 4;      // steps of a split, at least
+constexpr int AT_MAX_SPLITS = 64;
+
+// A launch's plan.  Rows of a sequence and cached head: (token, head of the group),
+// r = token * group + head; tiles of `tr` rows.
+struct AttnPlan {
+  int group;          // query heads per cached head
+  int tr;             // rows of a tile
+  int splits;         // parts that a tile's keys may be split into
+  int min_rows;       // sequences of fewer rows, or
+  int max_rows;       // more rows, are another launch's
+  int each;           // tiles of a sequence where all have the same number of tokens
+  int64_t tiles;
+  float* part;        // [tokens * q_heads][splits][dim], then
+  float* stat;        // [tokens * q_heads][splits][2]: maximum (powers of two) and sum
+};
+
+// The keys that a tile's tokens see, in steps of 64: those of the first `sink` steps
+// and of the steps from `low` on, `blocks` in all; and how many splits they make.
+struct AttnSpan {
+  int64_t pmin, pmax;   // positions of the tile's first and last token
+  int64_t end;          // keys end here
+  int sink, blocks, splits;
+  int64_t low;
+  FL_HD int64_t key(int i) const {   // the first key of step i
+    return static_cast<int64_t>(AT_BLK) * (i < sink ? i : low + (i - sink));
+  }
+};
+
+FL_HD AttnSpan attn_span(const fl_attn_args& a, const AttnPlan& p, const PagedSeq& s, int tile) {
+  AttnSpan v;
+  const int r0 = tile * p.tr, r1 = static_cast<int>(least(r0 + p.tr, s.n * p.group)) - 1;
+  v.pmin = s.pos + r0 / p.group;
+  v.pmax = s.pos + r1 / p.group;
+  // (a position past the table is no key's: its query is given NaN)
+  v.end = least(most(v.pmax + 1, 0), a.rows.table_width * a.cache.page_size);
+  v.low = 0;
+  v.sink = 0;
+  if (a.window > 0) {
+    v.low = most(v.pmin - a.window + 1, 0) / AT_BLK;
+    v.sink = static_cast<int>(least((least(a.sinks, v.end) + AT_BLK - 1) / AT_BLK, v.low));
+  }
+  const int64_t last = (v.end + AT_BLK - 1) / AT_BLK;
+  v.blocks = static_cast<int>(v.sink + most(last - v.low, 0));
+  v.splits = static_cast<int>(most(1, least(p.splits, (v.blocks + AT_MIN_BLKS - 1) / AT_MIN_BLKS)));
+  return v;
+}
+
+// Whether every key of the step is seen by every token of the tile.
+FL_HD bool attn_whole(const fl_attn_args& a, const AttnSpan& v, int64_t t0) {
+  const int64_t t1 = t0 + AT_BLK - 1;
+  return t1 <= v.pmin && (a.window == 0 || t0 > v.pmax - a.window || t1 < a.sinks);
+}
+
+}  // namespace fl

@@ -1,0 +1,398 @@
+// Norms of queries and keys for each head, and their rotation by position.
+//
+//   y   = x r w,  r = 1 / sqrt(sum x^2 / D + eps)
+//   out = R y:    (y_i, y_j) -> (y_i c - y_j s, y_i s + y_j c) for each pair,
+//         c = gain cos a, s = gain sin a, a = position inv_freq
+// and the gradients for an upstream g:
+//   u  = R^T g    (the same with -s)
+//   dw = sum over tokens and heads of u x r
+//   dx = r (u w - x r^2 mean(u w x))
+//
+// HBM bounds both passes: every value is read once and written once.  A thread
+// holds N pairs of a row (16 bytes of each half), L threads a row, and a
+// work-group takes TK tokens: their angles' sines and cosines once, into LDS, for
+// all heads; then the rows, 256 / L at a time.  The angle is reduced to a fraction
+// of a turn in float64, so that a far position keeps its digits (a float32 product
+// is off by 0.03 at 2^20 radians).
+#include <algorithm>
+#include <type_traits>
+
+#include "fl_device.h"
+#include "fl_kernels.h"
+
+namespace fl {
+
+namespace {
+
+constexpr int RP_NT = 256;
+constexpr int RP_MAX_PARTS = 1024;   // work-groups of the backward pass: partial sums of the weights' gradients
+
+// The turns of a work-group's tokens: cs[tk][p] = gain (cos, sin) of pair p, (1, 0)
+// from the first pair that is not rotated on.
+__device__ __forceinline__ void rp_turns(const fl_rope_args& a, int64_t t0, int tk, int P, float2* cs) {
+  const int R2 = static_cast<int>(a.rotated / 2);
+  for (int i = threadIdx.x; i < tk * P; i += RP_NT) {
+    const int t = i / P, p = i % P;
+    float2 v = make_float2(1.0f, 0.0f);
+    if (p < R2) {
+      const int64_t pos = (a.flags & FL_ROPE_POSITIONS32) ? static_cast<const int32_t*>(a.positions)[t0 + t]
+                                                          : static_cast<const int64_t*>(a.positions)[t0 + t];
+      const double turns = static_cast<double>(pos) * a.inv_freq[p] * 0.15915494309189535;   // (1 / 2 pi)
+      float s, c;
+      sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
+      v = make_float2(a.gain * c, a.gain * s);
+    }
+    cs[i] = v;
+  }
+}
+
+// Where N pairs from pair p on lie in a row: VEC takes them as whole chunks.
+struct RpRow {
+  int P, R2, T2;      // pairs, rotated pairs, pairs behind them
+  bool inter;
+  __device__ __forceinline__ int first(int p) const { return inter ? 2 * p : p < R2 ? p : R2 + p; }
+  __device__ __forceinline__ int second(int p) const { return inter ? 2 * p + 1 : p < R2 ? p + R2 : R2 + T2 + p; }
+};
+
+template <class D, bool VEC, int N>
+__device__ __forceinline__ void rp_load(const void* row, const RpRow& R, int p, float (&x)[N], float (&y)[N]) {
+  using C = RowChunk<D>;
+  if (p >= R.P) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = y[e] = 0.0f;
+  } else if constexpr (VEC) {
+    static_assert(C::N == N, "a chunk holds N values");
+    constexpr int ESZ = D::id == FL_DTYPE_F32 ? 4 : 2;
+    const char* c = static_cast<const char*>(row) + ESZ * R.first(p);
+    const uint4 q0 = *reinterpret_cast<const uint4*>(c);
+    const uint4 q1 = *reinterpret_cast<const uint4*>(R.inter ? c + 16 : static_cast<const char*>(row) + ESZ * R.second(p));
+    float u[N], v[N];
+    C::unpack(q0, u);
+    C::unpack(q1, v);
+    if (R.inter) {
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        x[e] = u[2 * e], y[e] = u[2 * e + 1];
+        x[e + N / 2] = v[2 * e], y[e + N / 2] = v[2 * e + 1];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[e] = u[e], y[e] = v[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      x[e] = y[e] = 0.0f;
+      if (p + e < R.P) {
+        if constexpr (D::id == FL_DTYPE_F32) {
+          x[e] = static_cast<const float*>(row)[R.first(p + e)];
+          y[e] = static_cast<const float*>(row)[R.second(p + e)];
+        } else {
+          x[e] = D::to_f32(static_cast<const uint16_t*>(row)[R.first(p + e)]);
+          y[e] = D::to_f32(static_cast<const uint16_t*>(row)[R.second(p + e)]);
+        }
+      }
+    }
+  }
+}
+
+template <class D, int N>
+__device__ __forceinline__ uint4 rp_pack(const float (&x)[N]) {
+  if constexpr (D::id == FL_DTYPE_F32)
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  else
+    return make_uint4(D::from_f32(x[0]) | (D::from_f32(x[1]) << 16), D::from_f32(x[2]) | (D::from_f32(x[3]) << 16),
+                      D::from_f32(x[4]) | (D::from_f32(x[5]) << 16), D::from_f32(x[6]) | (D::from_f32(x[7]) << 16));
+}
+
+template <class D, bool VEC, int N>
+__device__ __forceinline__ void rp_store(void* row, const RpRow& R, int p, const float (&x)[N], const float (&y)[N]) {
+  if (p >= R.P) return;
+  if constexpr (VEC) {
+    constexpr int ESZ = D::id == FL_DTYPE_F32 ? 4 : 2;
+    float u[N], v[N];
+    if (R.inter) {
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        u[2 * e] = x[e], u[2 * e + 1] = y[e];
+        v[2 * e] = x[e + N / 2], v[2 * e + 1] = y[e + N / 2];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) u[e] = x[e], v[e] = y[e];
+    }
+    char* c = static_cast<char*>(row) + ESZ * R.first(p);
+    *reinterpret_cast<uint4*>(c) = rp_pack<D>(u);
+    *reinterpret_cast<uint4*>(R.inter ? c + 16 : static_cast<char*>(row) + ESZ * R.second(p)) = rp_pack<D>(v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (p + e < R.P) {
+        if constexpr (D::id == FL_DTYPE_F32) {
+          static_cast<float*>(row)[R.first(p + e)] = x[e];
+          static_cast<float*>(row)[R.second(p + e)] = y[e];
+        } else {
+          static_cast<uint16_t*>(row)[R.first(p + e)] = static_cast<uint16_t>(D::from_f32(x[e]));
+          static_cast<uint16_t*>(row)[R.second(p + e)] = static_cast<uint16_t>(D::from_f32(y[e]));
+        }
+      }
+  }
+}
+
+template <int N>
+__device__ __forceinline__ float rp_sum(float v, int L) {
+#pragma unroll 1
+  for (int m = 1; m < L; m <<= 1) v += shfl_xor(v, m);
+  return v;
+}
+
+template <class D>
+__device__ __forceinline__ char* rp_at(const void* p, int64_t i) {
+  return static_cast<char*>(const_cast<void*>(p)) + i * (D::id == FL_DTYPE_F32 ? 4 : 2);
+}
+
+// The weights of a thread's pairs (1 without), which need no alignment.
+template <class W, int N>
+__device__ __forceinline__ void rp_weights(const void* w, const RpRow& R, int p, float (&x)[N], float (&y)[N]) {
+  if (w != nullptr) rp_load<W, false>(w, R, p, x, y);
+  else
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = y[e] = 1.0f;
+}
+
+__device__ __forceinline__ RpRow rp_row(const fl_rope_args& a) {
+  const int P = static_cast<int>(a.dim / 2), R2 = static_cast<int>(a.rotated / 2);
+  return RpRow{P, R2, P - R2, (a.flags & FL_ROPE_INTERLEAVED) != 0};
+}
+
+}  // namespace
+
+// GRAD false: out = forward(q, k); true: dq, dk (out_q, out_k) and the partial sums
+// of the weights' gradients, [part][2][dim].
+template <class D, class W, bool VEC>
+__global__ __launch_bounds__(RP_NT) void k_rope(const fl_rope_args a, int L, int TK) {
+  constexpr int N = RowChunk<D>::N;
+  __shared__ float2 cs[1024];
+  const RpRow R = rp_row(a);
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * TK;
+  const int tk = static_cast<int>(min(static_cast<int64_t>(TK), a.tokens - t0));
+  rp_turns(a, t0, tk, R.P, cs);
+  __syncthreads();
+  const int p = (threadIdx.x & (L - 1)) * N, g = threadIdx.x / L, GR = RP_NT / L;
+  const float inv = 1.0f / static_cast<float>(a.dim);
+  auto rows = [&](const void* x, int64_t ld, int64_t hs, int heads, const void* w, void* out) {
+    if (heads == 0) return;
+    float w0[N], w1[N];
+    rp_weights<W>(a.norm ? w : nullptr, R, p, w0, w1);
+    for (int i = g; i < tk * heads; i += GR) {
+      const int t = i / heads, h = i - t * heads;
+      float x0[N], x1[N];
+      rp_load<D, VEC>(rp_at<D>(x, (t0 + t) * ld + h * hs), R, p, x0, x1);
+      if (a.norm) {
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) s = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], s));
+        const float r = 1.0f / sqrtf(fmaf(rp_sum<N>(s, L), inv, a.eps));
+#pragma unroll
+        for (int e = 0; e < N; ++e) x0[e] *= r * w0[e], x1[e] *= r * w1[e];
+      }
+      float y0[N], y1[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float2 c = cs[t * R.P + min(p + e, R.P - 1)];
+        y0[e] = x0[e] * c.x - x1[e] * c.y;
+        y1[e] = x0[e] * c.y + x1[e] * c.x;
+      }
+      rp_store<D, VEC>(rp_at<D>(out, ((t0 + t) * heads + h) * a.dim), R, p, y0, y1);
+    }
+  };
+  rows(a.q, a.q_ld, a.q_hs, static_cast<int>(a.heads), a.q_weight, a.out_q);
+  rows(a.k, a.k_ld, a.k_hs, static_cast<int>(a.kv_heads), a.k_weight, a.out_k);
+}
+
+template <class D, class W, bool VEC>
+__global__ __launch_bounds__(RP_NT) void k_rope_grad(const fl_rope_grad_args b, int L, int TK) {
+  constexpr int N = RowChunk<D>::N;
+  const fl_rope_args& a = b.fwd;
+  __shared__ float2 cs[1024];
+  __shared__ float sum[RP_NT / WAVE][FL_ROPE_MAX_DIM];
+  const RpRow R = rp_row(a);
+  const int p = (threadIdx.x & (L - 1)) * N, g = threadIdx.x / L, GR = RP_NT / L;
+  const float inv = 1.0f / static_cast<float>(a.dim);
+  const bool weights = b.out_dwq != nullptr || b.out_dwk != nullptr;
+  float dq0[N], dq1[N], dk0[N], dk1[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) dq0[e] = dq1[e] = dk0[e] = dk1[e] = 0.0f;
+  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * TK; t0 < a.tokens; t0 += static_cast<int64_t>(gridDim.x) * TK) {
+    const int tk = static_cast<int>(min(static_cast<int64_t>(TK), a.tokens - t0));
+    __syncthreads();   // (the last tokens' angles have been read)
+    rp_turns(a, t0, tk, R.P, cs);
+    __syncthreads();
+    auto rows = [&](const void* x, int64_t ld, int64_t hs, int heads, const void* w, const void* grad, void* out, float(&d0)[N],
+                    float(&d1)[N]) {
+      if (heads == 0) return;
+      float w0[N], w1[N];
+      rp_weights<W>(a.norm ? w : nullptr, R, p, w0, w1);
+      for (int i = g; i < tk * heads; i += GR) {
+        const int t = i / heads, h = i - t * heads;
+        const int64_t at = ((t0 + t) * heads + h) * a.dim;
+        float x0[N], x1[N], g0[N], g1[N], u0[N], u1[N];
+        if (grad != nullptr) rp_load<D, VEC>(rp_at<D>(grad, at), R, p, g0, g1);
+        else
+#pragma unroll
+          for (int e = 0; e < N; ++e) g0[e] = g1[e] = 0.0f;
+        if (a.norm) rp_load<D, VEC>(rp_at<D>(x, (t0 + t) * ld + h * hs), R, p, x0, x1);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float2 c = cs[t * R.P + min(p + e, R.P - 1)];
+          u0[e] = g0[e] * c.x + g1[e] * c.y;
+          u1[e] = g1[e] * c.x - g0[e] * c.y;
+        }
+        if (a.norm) {
+          float s = 0.0f;
+#pragma unroll
+          for (int e = 0; e < N; ++e) s = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], s));
+          const float r = 1.0f / sqrtf(fmaf(rp_sum<N>(s, L), inv, a.eps));
+          float dot = 0.0f;
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            x0[e] *= r, x1[e] *= r;
+            d0[e] = fmaf(u0[e], x0[e], d0[e]);
+            d1[e] = fmaf(u1[e], x1[e], d1[e]);
+            u0[e] *= w0[e], u1[e] *= w1[e];
+            dot = fmaf(u0[e], x0[e], fmaf(u1[e], x1[e], dot));
+          }
+          dot = rp_sum<N>(dot, L) * inv;
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            u0[e] = r * (u0[e] - x0[e] * dot);
+            u1[e] = r * (u1[e] - x1[e] * dot);
+          }
+        }
+        if (out != nullptr) rp_store<D, VEC>(rp_at<D>(out, at), R, p, u0, u1);
+      }
+    };
+    rows(a.q, a.q_ld, a.q_hs, static_cast<int>(a.heads), a.q_weight, b.grad_q, a.out_q, dq0, dq1);
+    rows(a.k, a.k_ld, a.k_hs, static_cast<int>(a.kv_heads), a.k_weight, b.grad_k, a.out_k, dk0, dk1);
+  }
+  if (!weights) return;
+  // the row groups' sums: over a wave's by exchange, then over the waves
+  float* part = static_cast<float*>(b.workspace) + static_cast<int64_t>(blockIdx.x) * 2 * a.dim;
+  auto store = [&](float(&d0)[N], float(&d1)[N], int which) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      for (int m = L; m < WAVE; m <<= 1) {
+        d0[e] += shfl_xor(d0[e], m);
+        d1[e] += shfl_xor(d1[e], m);
+      }
+      if ((threadIdx.x & (WAVE - 1)) < L && p + e < R.P) {
+        sum[threadIdx.x / WAVE][R.first(p + e)] = d0[e];
+        sum[threadIdx.x / WAVE][R.second(p + e)] = d1[e];
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.dim; i += RP_NT) part[which * a.dim + i] = (sum[0][i] + sum[1][i]) + (sum[2][i] + sum[3][i]);
+    __syncthreads();
+  };
+  store(dq0, dq1, 0);
+  store(dk0, dk1, 1);
+}
+
+// The partial sums added: one work-group per 64 columns of dwq (blockIdx.y 0) or
+// dwk (1), a wave per 16th of the parts, in float64.
+constexpr int RP_RW = 16;
+template <class W>
+__global__ __launch_bounds__(RP_RW * WAVE) void k_rope_reduce(const fl_rope_grad_args b, int parts) {
+  __shared__ double s[RP_RW][WAVE];
+  const int n = static_cast<int>(b.fwd.dim), lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
+  const int i = blockIdx.x * WAVE + lane;
+  void* out = blockIdx.y == 0 ? b.out_dwq : b.out_dwk;
+  if (out == nullptr) return;
+  double v = 0.0;
+  if (i < n) {
+    const float* p = static_cast<const float*>(b.workspace) + static_cast<int64_t>(blockIdx.y) * n + i;
+#pragma unroll 8
+    for (int q = w; q < parts; q += RP_RW) v += static_cast<double>(p[static_cast<int64_t>(q) * 2 * n]);
+  }
+  s[w][lane] = v;
+  __syncthreads();
+  if (w != 0 || i >= n) return;
+#pragma unroll
+  for (int q = 1; q < RP_RW; ++q) v += s[q][lane];
+  if constexpr (W::id == FL_DTYPE_F32) static_cast<float*>(out)[i] = static_cast<float>(v);
+  else static_cast<uint16_t*>(out)[i] = static_cast<uint16_t>(W::from_f32(static_cast<float>(v)));
+}
+
+namespace {
+
+template <class F>
+void rp_types(int dtype, int wdtype, F&& f) {
+  if (dtype == FL_DTYPE_F32) f(F32{}, F32{});
+  else if (dtype == FL_DTYPE_BF16 && wdtype == FL_DTYPE_F32) f(BF16{}, F32{});
+  else if (dtype == FL_DTYPE_BF16) f(BF16{}, BF16{});
+  else if (wdtype == FL_DTYPE_F32) f(F16{}, F32{});
+  else f(F16{}, F16{});
+}
+
+// Whole 16-byte chunks: rows that start and pairs that lie on them.
+bool rp_vector(const fl_rope_args& a, int N, std::initializer_list<const void*> more) {
+  const int64_t R2 = a.rotated / 2, T2 = (a.dim - a.rotated) / 2;
+  if (a.flags & FL_ROPE_INTERLEAVED ? a.dim % (2 * N) != 0 : R2 % N != 0 || T2 % N != 0) return false;
+  uintptr_t bits = 0;
+  const uintptr_t esz = a.dtype == FL_DTYPE_F32 ? 4 : 2;
+  if (a.q) bits |= reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.q_ld) * esz | static_cast<uintptr_t>(a.q_hs) * esz;
+  if (a.k) bits |= reinterpret_cast<uintptr_t>(a.k) | static_cast<uintptr_t>(a.k_ld) * esz | static_cast<uintptr_t>(a.k_hs) * esz;
+  bits |= reinterpret_cast<uintptr_t>(a.out_q) | reinterpret_cast<uintptr_t>(a.out_k);
+  for (const void* p : more) bits |= reinterpret_cast<uintptr_t>(p);
+  return bits % 16 == 0;
+}
+
+// Threads of a row: a power of two that holds its pairs.
+int rp_lanes(int64_t dim, int N) {
+  int L = 1;
+  while (L * N < dim / 2) L *= 2;
+  return L;
+}
+// Tokens of a work-group: 4 share one round of sines and cosines where that still
+// leaves four work-groups for every CU.
+int rp_tokens(int64_t tokens) { return tokens >= 4096 ? 4 : 1; }
+
+}  // namespace
+
+int64_t rope_grad_parts(int64_t tokens) {
+  const int TK = rp_tokens(tokens);
+  return std::min<int64_t>((tokens + TK - 1) / TK, RP_MAX_PARTS);
+}
+
+hipError_t launch_rope(const fl_rope_args& a, hipStream_t s) {
+  rp_types(a.dtype, a.wdtype, [&](auto d, auto w) {
+    using D = decltype(d);
+    constexpr int N = RowChunk<D>::N;
+    const int L = rp_lanes(a.dim, N), TK = rp_tokens(a.tokens);
+    const dim3 grid(static_cast<unsigned>((a.tokens + TK - 1) / TK));
+    if (rp_vector(a, N, {})) hipLaunchKernelGGL((k_rope<D, decltype(w), true>), grid, dim3(RP_NT), 0, s, a, L, TK);
+    else hipLaunchKernelGGL((k_rope<D, decltype(w), false>), grid, dim3(RP_NT), 0, s, a, L, TK);
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_rope_grad(const fl_rope_grad_args& b, hipStream_t s) {
+  const fl_rope_args& a = b.fwd;
+  rp_types(a.dtype, a.wdtype, [&](auto d, auto w) {
+    using D = decltype(d);
+    using W = decltype(w);
+    constexpr int N = RowChunk<D>::N;
+    const int L = rp_lanes(a.dim, N), TK = rp_tokens(a.tokens);
+    const int parts = static_cast<int>(rope_grad_parts(a.tokens));
+    if (parts > 0) {
+      if (rp_vector(a, N, {b.grad_q, b.grad_k})) hipLaunchKernelGGL((k_rope_grad<D, W, true>), dim3(parts), dim3(RP_NT), 0, s, b, L, TK);
+      else hipLaunchKernelGGL((k_rope_grad<D, W, false>), dim3(parts), dim3(RP_NT), 0, s, b, L, TK);
+    }
+    if (b.out_dwq || b.out_dwk)
+      hipLaunchKernelGGL(k_rope_reduce<W>, dim3(static_cast<unsigned>((a.dim + WAVE - 1) / WAVE), 2), dim3(RP_RW * WAVE), 0, s, b,
+                         parts);
+  });
+  return hipGetLastError();
+}
+
+}  // namespace fl

@@ -1,0 +1,132 @@
+// Which tokens, keys and pages the work-groups of a call on a paged cache take
+// (csrc/fl_paged_map.h), against the definition, for random calls: every row in one
+// tile, every new token in one run of 16 slots, every key that a row sees in one step
+// of one split, and nothing outside the arrays whatever starts, lengths and table hold.
+#include <cstdio>
+#include <cstdlib>
+#include <random>
+#include <vector>
+
+#include "../rl_project_amd/csrc/fl_paged_map.h"
+
+using namespace fl;
+
+#define REQUIRE(c)                                                                   \
+  do {                                                                               \
+    if (!(c)) {                                                                      \
+      std::printf("call %d: line %d: %s\n", call, __LINE__, #c);                     \
+      return 1;                                                                      \
+    }                                                                                \
+  } while (0)
+
+int main(int argc, char** argv) {
+  const int calls = argc > 1 ? std::atoi(argv[1]) : 2000;
+  std::mt19937 rng(7);
+  const auto up_to = [&](int n) { return static_cast<int>(rng() % (static_cast<unsigned>(n) + 1)); };
+  for (int call = 0; call < calls; ++call) {
+    const bool ragged = rng() & 1, broken = ragged && rng() % 4 == 0;
+    const int B = 1 + up_to(6), S = 16 << up_to(3), C = 1 + up_to(call % 3 ? 40 : 300);
+    std::vector<int> n(B), starts(B + 1, 0), lengths(B);
+    for (int b = 0; b < B; ++b) {
+      n[b] = ragged ? up_to(C) : C;
+      starts[b + 1] = starts[b] + n[b];
+      lengths[b] = rng() % 5 ? n[b] + up_to(700) : up_to(C);
+    }
+    const int behind = ragged ? up_to(5) : 0, N = starts[B] + behind;
+    const int width = 1 + up_to(1200) / S;
+    if (broken)
+      for (int& x : starts) x = static_cast<int>(rng());
+    if (rng() % 8 == 0)
+      for (int& x : lengths) x = static_cast<int>(rng());
+    std::vector<int> table(static_cast<size_t>(B) * width);
+    for (int& x : table) x = rng() % 6 ? up_to(50) : static_cast<int>(rng());
+    fl_cache c = {};
+    c.pages = 40, c.heads = 2, c.page_size = S, c.dim = 64;
+    fl_cache_rows r = {table.data(), lengths.data(), ragged ? starts.data() : nullptr, B, N, width, width};
+    if (N == 0) continue;
+
+    // ---- rows of attention
+    const int G = 1 + up_to(8), tr = 16 << up_to(4);
+    AttnPlan p = {};
+    p.group = G, p.tr = tr, p.splits = 1 + up_to(12);
+    p.each = static_cast<int>((N / B * static_cast<int64_t>(G) + tr - 1) / tr);
+    fl_attn_args a = {};
+    a.cache = c, a.rows = r;
+    a.window = rng() & 1 ? 1 + up_to(200) : 0;
+    a.sinks = rng() & 1 ? up_to(150) : 0;
+    std::vector<int> seen(static_cast<size_t>(N) * G, 0);
+    const int64_t tiles = paged_tiles(r, G, tr, 1, p.each);
+    for (int64_t x = 0; x < tiles; ++x) {
+      const PagedSeq s = paged_seq(r, static_cast<int>(x), G, tr, 1, p.each);
+      REQUIRE(s.b >= 0 && s.b < B && s.n >= 0 && s.row >= 0 && s.row + s.n <= N);
+      const int rows = s.n * G;
+      if (s.tile >= (rows + tr - 1) / tr) continue;
+      const AttnSpan v = attn_span(a, p, s, s.tile);
+      REQUIRE(v.splits >= 1 && v.splits <= p.splits && v.blocks >= 0 && v.end <= static_cast<int64_t>(width) * S);
+      int64_t last = -1;
+      for (int i = 0; i < v.blocks; ++i) {
+        REQUIRE(v.key(i) > last);   // (no step twice)
+        last = v.key(i);
+        for (int64_t t = last; t < last + AT_BLK; t += 16) {
+          const int page = paged_page(r, c, s.b, t);
+          REQUIRE(page >= -1 && page < c.pages);
+          if (page >= 0) REQUIRE(t / S < width && page == table[s.b * static_cast<size_t>(width) + t / S]);
+        }
+      }
+      int steps = 0;
+      for (int q = 0; q < v.splits; ++q) {
+        const int b0 = static_cast<uint32_t>(v.blocks) * q / static_cast<uint32_t>(v.splits);
+        const int b1 = static_cast<uint32_t>(v.blocks) * (q + 1) / static_cast<uint32_t>(v.splits);
+        REQUIRE(b0 == steps && b1 >= b0);
+        steps = b1;
+      }
+      REQUIRE(steps == v.blocks);
+      for (int row = s.tile * tr; row < rows && row < (s.tile + 1) * tr; ++row) {
+        if (!broken) ++seen[(s.row + row / G) * G + row % G];
+        const int64_t at = s.pos + row / G;
+        REQUIRE(at >= v.pmin && at <= v.pmax);
+        if (at >= static_cast<int64_t>(width) * S || at > 3000) continue;
+        for (int64_t t = 0; t <= at; ++t) {
+          if (a.window && t <= at - a.window && t >= a.sinks) continue;
+          int found = 0;
+          for (int i = 0; i < v.blocks; ++i) found += t >= v.key(i) && t < v.key(i) + AT_BLK;
+          REQUIRE(found == 1);
+        }
+        for (int i = 0; i < v.blocks; ++i) {
+          if (!attn_whole(a, v, v.key(i))) continue;
+          for (int64_t t = v.key(i); t < v.key(i) + AT_BLK; ++t)
+            REQUIRE(t <= at && (a.window == 0 || t > at - a.window || t < a.sinks));
+        }
+      }
+    }
+    if (!broken)
+      for (int i = 0; i < N * G; ++i) REQUIRE(seen[i] == (i < (N - behind) * G ? 1 : 0));
+
+    // ---- tokens of a write or a read
+    int each = 0;
+    std::vector<int> wrote(N, 0);
+    const int64_t runs = kv_tiles(r, &each);
+    for (int64_t x = 0; x < runs; ++x) {
+      const PagedSeq s = paged_seq(r, static_cast<int>(x), 1, KV_T, 2, each);
+      REQUIRE(s.b >= 0 && s.b < B && s.n >= 0 && s.row >= 0 && s.row + s.n <= N);
+      KvTile t;
+      if (!kv_tile(r, c, s, t)) continue;
+      REQUIRE(t.page >= -1 && t.page < c.pages && t.slot >= 0 && t.slot + KV_T <= S && t.slot % KV_T == 0);
+      REQUIRE(t.t0 >= 0 && t.t1 <= KV_T);
+      for (int u = t.t0; u < t.t1; ++u) {
+        const int64_t row = t.row0 + u, at = s.pos + (row - s.row);
+        REQUIRE(row >= s.row && row < s.row + s.n && at >= 0 && at % S == t.slot + u);
+        if (t.page >= 0) REQUIRE(at / S < width && t.page == table[s.b * static_cast<size_t>(width) + at / S]);
+        ++wrote[row];
+      }
+    }
+    if (!broken)
+      for (int b = 0; b < B; ++b)
+        for (int i = 0; i < n[b]; ++i) {
+          const int64_t at = static_cast<int64_t>(lengths[b]) - n[b] + i;
+          REQUIRE(wrote[(ragged ? starts[b] : b * C) + i] == (at >= 0 ? 1 : 0));
+        }
+  }
+  std::printf("%d calls\n", calls);
+  return 0;
+}
