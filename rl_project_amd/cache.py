@@ -112,9 +112,12 @@ class PagedCache:
         return self.k.device
 
 
-def _check_tokens(cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor], rows: int) -> None:
+def _check_cache(cache) -> None:
     if not isinstance(cache, PagedCache):
         raise TypeError("cache must be a PagedCache")
+
+
+def _check_tokens(cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor], rows: int) -> None:
     dev = cache.k.device
     if table.dim() != 2 or table.dtype != torch.int32 or table.device != dev or (table.size(1) > 1 and table.stride(1) != 1):
         raise ValueError(f"table must be int32 [B, width] on {dev}, its rows contiguous")
@@ -145,6 +148,7 @@ def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torc
     are the call's rows; any strides) into the cache: in its dtype as they are, or
     from float32, bfloat16 or float16 in 8 bits with a scale for each token and head.
     One launch.  Sequences that share pages must not write the same slot in a call."""
+    _check_cache(cache)
     _check_rows(cache, k, "k", cache.heads)
     if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
         raise ValueError("k and v must match in shape, dtype and device")
@@ -164,6 +168,7 @@ def cache_read(cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, to
     float32 for 8 bits): exact but for one rounding to a 16-bit ``dtype`` of values
     outside its range.  Into ``out`` (contiguous) where given; else rows behind the
     last sequence are zeros.  One launch."""
+    _check_cache(cache)
     if out is not None:
         dtype = out[0].dtype
     elif dtype is None:
@@ -205,6 +210,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, len
     to ``q``'s dtype (bfloat16 over an 8-bit cache) for the product with the values.
     One or two launches, without host synchronisation; results are the same each
     time, and depend on how the call's shapes split the keys in the last bits."""
+    _check_cache(cache)
     _check_rows(cache, q, "q")
     if q.dtype not in (torch.bfloat16, torch.float16) or (cache.dtype != torch.float8_e4m3fn and q.dtype != cache.dtype):
         raise NotImplementedError(f"{q.dtype} queries over a {cache.dtype} cache")

@@ -1,0 +1,140 @@
+"""The C entry points of the rotation, the paged cache and attention over it: struct
+layouts, refusals and workspace sizes, before anything touches a GPU (CPU)."""
+
+import ctypes
+import os
+import shutil
+import subprocess
+
+import pytest
+
+from rl_project_amd import _lib
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+pytestmark = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH),
+                                reason="libflsampler.so not built (python -m rl_project_amd.build)")
+
+STRUCTS = {"fl_rope_args": _lib.RopeArgs, "fl_rope_grad_args": _lib.RopeGradArgs, "fl_cache": _lib.Cache,
+           "fl_cache_rows": _lib.CacheRows, "fl_cache_args": _lib.CacheArgs, "fl_attn_args": _lib.AttnArgs}
+EINVAL, ENOTSUP, OK = _lib.FL_EINVAL, _lib.FL_ENOTSUP, _lib.FL_OK
+
+
+def test_struct_layouts(tmp_path):
+    gcc = shutil.which("gcc")
+    if gcc is None:
+        pytest.skip("gcc not available")
+    body = "".join(f'printf("{n} %zu\\n", sizeof({n}));' + "".join(
+        f'printf("{n}.{f} %zu\\n", offsetof({n}, {f}));' for f, _ in c._fields_) for n, c in STRUCTS.items())
+    (tmp_path / "l.c").write_text('#include <stddef.h>\n#include <stdio.h>\n#include "fl_sampler.h"\n'
+                                  f"int main(void) {{ {body} return 0; }}\n")
+    subprocess.run([gcc, "-std=c99", "-I", os.path.join(ROOT, "include"), str(tmp_path / "l.c"), "-o", str(tmp_path / "l")],
+                   check=True)
+    out = subprocess.run([str(tmp_path / "l")], check=True, capture_output=True, text=True).stdout
+    got = dict((k, int(v)) for k, v in (line.split() for line in out.splitlines()))
+    for n, c in STRUCTS.items():
+        assert got[n] == ctypes.sizeof(c), n
+        for f, _ in c._fields_:
+            assert got[f"{n}.{f}"] == getattr(c, f).offset, (n, f)
+
+
+def _set(a, values):
+    for k, v in values.items():
+        if isinstance(v, dict):
+            _set(getattr(a, k), v)
+        else:
+            setattr(a, k, v)
+
+
+def _refused(fn, cls, base, cases):
+    L = _lib.lib()
+    assert fn(None, None) == EINVAL
+    for change, code, needle in cases:
+        a = cls()
+        a.struct_size = ctypes.sizeof(cls)
+        if cls is _lib.RopeGradArgs:
+            a.fwd.struct_size = ctypes.sizeof(_lib.RopeArgs)
+        _set(a, base)
+        _set(a, change)
+        assert fn(ctypes.byref(a), None) == code, change
+        assert code == OK or needle in L.fl_last_error().decode(), (change, L.fl_last_error())
+
+
+ROPE = dict(dtype=0, wdtype=0, q=4096, k=4096, tokens=3, heads=2, kv_heads=1, dim=64, rotated=64, q_ld=128, q_hs=64, k_ld=64, k_hs=64,
+            positions=4096, inv_freq=4096, eps=1e-6, gain=1.0, norm=1, out_q=4096, out_k=4096)
+ROPE_BAD = [(dict(struct_size=8), EINVAL, "struct_size"), (dict(dtype=3), EINVAL, "dtype"), (dict(wdtype=1), EINVAL, "wdtype"),
+            (dict(dim=63), EINVAL, "shape"), (dict(dim=0), EINVAL, "shape"), (dict(rotated=66), EINVAL, "shape"),
+            (dict(rotated=3), EINVAL, "shape"), (dict(tokens=-1), EINVAL, "shape"), (dict(heads=-1), EINVAL, "shape"),
+            (dict(dim=514), ENOTSUP, "limits"), (dict(tokens=1 << 24), ENOTSUP, "limits"), (dict(flags=4), EINVAL, "flags"),
+            (dict(reserved=1), EINVAL, "reserved"), (dict(eps=-1.0), EINVAL, "eps"), (dict(eps=float("nan")), EINVAL, "eps"),
+            (dict(gain=float("inf")), EINVAL, "gain"), (dict(q_hs=-1), EINVAL, "stride"), (dict(positions=None), EINVAL, "positions"),
+            (dict(inv_freq=None), EINVAL, "inv_freq")]
+
+
+def test_rope_refusals():
+    L = _lib.lib()
+    _refused(L.fl_qk_norm_rope, _lib.RopeArgs, ROPE, ROPE_BAD + [
+        (dict(out_q=None), EINVAL, "NULL"), (dict(k=None), EINVAL, "NULL"), (dict(tokens=0, q=None), OK, ""),
+        (dict(heads=0, kv_heads=0), OK, "")])
+    base = dict(fwd=ROPE, grad_q=4096, grad_k=4096, out_dwq=4096, out_dwk=4096, workspace=4096, workspace_bytes=1 << 20)
+    _refused(L.fl_qk_norm_rope_grad, _lib.RopeGradArgs, base, [(dict(fwd=c), code, n) for c, code, n in ROPE_BAD] + [
+        (dict(reserved=1), EINVAL, "reserved"), (dict(fwd=dict(norm=0)), EINVAL, "norm"), (dict(workspace=None), EINVAL, "workspace"),
+        (dict(workspace=4100), EINVAL, "aligned"), (dict(workspace_bytes=3 * 2 * 64 * 4 - 1), EINVAL, "needed"),
+        (dict(fwd=dict(q=None)), EINVAL, "NULL"), (dict(out_dwq=None, out_dwk=None, fwd=dict(out_q=None, out_k=None)), OK, "")])
+    n = ctypes.c_size_t(0)
+    for tokens, dim, want in ((0, 64, 0), (1, 64, 2 * 64 * 4), (1024, 128, 1024 * 2 * 128 * 4), (8192, 128, 1024 * 2 * 128 * 4)):
+        assert L.fl_qk_norm_rope_grad_workspace_bytes(tokens, dim, ctypes.byref(n)) == OK and n.value == want
+    for tokens, dim in ((-1, 64), (1, 7), (1, 514)):
+        assert L.fl_qk_norm_rope_grad_workspace_bytes(tokens, dim, ctypes.byref(n)) == EINVAL
+    assert L.fl_qk_norm_rope_grad_workspace_bytes(1, 64, None) == EINVAL
+
+
+CACHE = dict(k=4096, v=4096, k_scale=4096, v_scale=4096, pages=4, heads=2, page_size=64, dim=64, dtype=1)
+ROWS = dict(table=4096, lengths=4096, seqs=3, tokens=6, table_width=2, table_ld=2)
+CACHE_BAD = [(dict(cache=dict(dtype=0)), EINVAL, "cache dtype"), (dict(cache=dict(page_size=48)), EINVAL, "page_size"),
+             (dict(cache=dict(page_size=256)), EINVAL, "page_size"), (dict(cache=dict(pages=0)), EINVAL, "shape"),
+             (dict(cache=dict(heads=0)), EINVAL, "shape"), (dict(cache=dict(dim=12)), EINVAL, "shape"),
+             (dict(cache=dict(reserved=1)), EINVAL, "shape"), (dict(rows=dict(seqs=-1)), EINVAL, "shape"),
+             (dict(rows=dict(table_ld=1)), EINVAL, "shape"), (dict(cache=dict(dim=264)), ENOTSUP, "limits"),
+             (dict(cache=dict(pages=1 << 31)), ENOTSUP, "limits"), (dict(rows=dict(table_width=1 << 26, table_ld=1 << 26)), ENOTSUP, "limits"),
+             (dict(rows=dict(tokens=1 << 24)), ENOTSUP, "limits"), (dict(rows=dict(tokens=7)), EINVAL, "as many"),
+             (dict(cache=dict(k=None)), EINVAL, "NULL"), (dict(rows=dict(lengths=None)), EINVAL, "NULL"),
+             (dict(rows=dict(table=None)), EINVAL, "NULL"), (dict(cache=dict(v=4104)), EINVAL, "aligned"),
+             (dict(rows=dict(tokens=0)), OK, ""), (dict(rows=dict(tokens=0, seqs=0)), OK, "")]
+
+
+def test_cache_refusals():
+    L = _lib.lib()
+    base = dict(dtype=1, cache=CACHE, rows=ROWS, k=4096, v=4096, k_ld=128, k_hs=64, v_ld=128, v_hs=64)
+    for fn in (L.fl_cache_write, L.fl_cache_read):
+        _refused(fn, _lib.CacheArgs, base, CACHE_BAD + [
+            (dict(struct_size=8), EINVAL, "struct_size"), (dict(dtype=3), EINVAL, "dtype"), (dict(k=None), EINVAL, "NULL"),
+            (dict(v_ld=-1), EINVAL, "stride"), (dict(cache=dict(dtype=3, k_scale=None)), EINVAL, "scales"),
+            (dict(cache=dict(dtype=3, v_scale=4100)), EINVAL, "aligned"),
+            (dict(cache=dict(heads=65536), rows=dict(tokens=3 << 20)), ENOTSUP, "limits")])
+    _refused(L.fl_cache_write, _lib.CacheArgs, base, [(dict(dtype=2), EINVAL, "cache's"), (dict(dtype=0), EINVAL, "cache's")])
+
+
+def test_attention_refusals():
+    L = _lib.lib()
+    base = dict(dtype=1, cache=CACHE, rows=ROWS, q=4096, q_heads=4, q_ld=256, q_hs=64, out=4096, out_ld=256, out_hs=64, scale=0.1,
+                workspace=None)
+    bad = CACHE_BAD + [(dict(struct_size=8), EINVAL, "struct_size"), (dict(dtype=0), ENOTSUP, "dtype"), (dict(dtype=2), EINVAL, "cache's"),
+                       (dict(q_heads=3), EINVAL, "heads"), (dict(q_heads=0), EINVAL, "heads"), (dict(q_heads=1 << 17), ENOTSUP, "limits"),
+                       (dict(scale=float("nan")), EINVAL, "scale"), (dict(softcap=-1.0), EINVAL, "softcap"), (dict(window=-1), EINVAL, "window"),
+                       (dict(sinks=-1), EINVAL, "sinks"), (dict(q_ld=4), EINVAL, "strides"), (dict(out_hs=2), EINVAL, "strides"),
+                       (dict(out_ld=-4), EINVAL, "strides")]
+    _refused(L.fl_paged_attention, _lib.AttnArgs, base, bad + [
+        (dict(q=None), EINVAL, "NULL"), (dict(q=4104), EINVAL, "aligned"), (dict(out=4100), EINVAL, "aligned"),
+        (dict(rows=dict(table_width=100, table_ld=100)), EINVAL, "workspace"),
+        (dict(rows=dict(table_width=100, table_ld=100), workspace=4104, workspace_bytes=1 << 40), EINVAL, "aligned")])
+    n = ctypes.c_size_t(0)
+    a = _lib.AttnArgs()
+    a.struct_size = ctypes.sizeof(a)
+    _set(a, base)
+    assert L.fl_paged_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(n)) == OK and n.value == 0   # (128 keys: no parts)
+    a.rows.table_width = a.rows.table_ld = 100
+    assert L.fl_paged_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(n)) == OK
+    assert n.value > 0 and n.value % (6 * 4 * (64 + 2) * 4) == 0
+    assert L.fl_paged_attention_workspace_bytes(ctypes.byref(a), None) == EINVAL
+    assert L.fl_paged_attention_workspace_bytes(None, ctypes.byref(n)) == EINVAL

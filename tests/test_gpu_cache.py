@@ -1,0 +1,226 @@
+"""cache_write and cache_read against indexing (MI355X).  16-bit values go in and out
+as they are; 8-bit ones are the definition's, bit for bit (the scale is a power of two,
+so nothing but the e4m3 rounding rounds)."""
+
+import math
+
+import pytest
+import torch
+
+from rl_project_amd import PagedCache, cache_read, cache_write
+from tests.paged_reference import e4m3, starts_of
+
+pytestmark = pytest.mark.gpu
+E4M3 = torch.float8_e4m3fn
+TYPES = [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16), (torch.bfloat16, E4M3), (torch.float16, E4M3),
+         (torch.float32, E4M3)]
+
+
+def _held(x, dtype):
+    """What the cache holds of rows x, in float64."""
+    if dtype != E4M3:
+        return x.double()
+    z, e = e4m3(x)
+    return z * torch.exp2(e.double())[..., None]
+
+
+def _table(lens, page, pages, width=None):
+    g = torch.Generator().manual_seed(len(lens) + page)
+    order = torch.randperm(pages, generator=g).tolist()
+    width = max([-(-n // page) for n in lens] + [1]) if width is None else width
+    t = torch.full((len(lens), width), -1, dtype=torch.int32)
+    for b, n in enumerate(lens):
+        for i in range(-(-n // page)):
+            t[b, i] = order.pop()
+    return t.cuda()
+
+
+def _filled(cache):
+    """Every byte set, so that a store outside shows."""
+    for t in (cache.k, cache.v):
+        t.view(torch.uint8).fill_(0x31)
+    if cache.k_scale is not None:
+        cache.k_scale.fill_(99), cache.v_scale.fill_(99)
+    return cache
+
+
+@pytest.mark.parametrize("dt,cdt", TYPES)
+@pytest.mark.parametrize("lens,news,heads,dim,page", [
+    ([1], [1], 1, 8, 16), ([33, 64, 65], [1, 1, 1], 8, 128, 64), ([40, 16, 5, 130], [40, 16, 5, 130], 2, 64, 32),
+    ([100, 7, 300, 0, 55], [17, 7, 255, 0, 1], 3, 80, 16), ([257, 15], [31, 15], 1, 256, 128), ([70, 70], [5, 5], 4, 40, 64)])
+def test_written_and_read(dt, cdt, lens, news, heads, dim, page):
+    torch.manual_seed(sum(lens))
+    N = sum(news)
+    k = (torch.randn(N, heads, dim, device="cuda") * torch.logspace(-3, 2, dim, device="cuda")).to(dt)
+    v = torch.randn(N, heads, dim, device="cuda").to(dt)
+    k[0, 0] = 0.0
+    cache = _filled(PagedCache.empty(sum(-(-n // page) for n in lens) + 2, heads, dim, page_size=page, dtype=cdt))
+    before = [t.clone() for t in (cache.k.view(torch.uint8), cache.v.view(torch.uint8))]
+    table, lengths = _table(lens, page, cache.pages), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    starts = starts_of(news) if len(set(news)) > 1 else None
+    cache_write(cache, k, v, table, lengths, starts=starts)
+    out = torch.float32
+    gk, gv = cache_read(cache, table, lengths, N, starts=starts, dtype=out)
+    assert torch.equal(gk.double(), _held(k, cdt)) and torch.equal(gv.double(), _held(v, cdt))
+    # the pages themselves, and no byte beside the tokens' slots
+    es = cache.k.element_size()
+    touched_k = torch.zeros(cache.pages, heads, page, dtype=torch.bool, device="cuda")
+    n = 0
+    for b, new in enumerate(news):
+        for i in range(new):
+            t = lens[b] - new + i
+            p, s = int(table[b, t // page]), t % page
+            touched_k[p, :, s] = True
+            if n % 7 == 0:
+                row_k, row_v = cache.k[p, :, s].float().double(), cache.v[p, :, :, s].float().double()
+                if cdt == E4M3:
+                    (zk, ek), (zv, ev) = e4m3(k[n]), e4m3(v[n])
+                    assert torch.equal(row_k, zk) and torch.equal(row_v, zv)
+                    assert torch.equal(cache.k_scale[p, :, s].int(), (ek + 127).int())
+                    assert torch.equal(cache.v_scale[p, :, s].int(), (ev + 127).int())
+                else:
+                    assert torch.equal(row_k, k[n].double()) and torch.equal(row_v, v[n].double())
+            n += 1
+    same_k = (cache.k.view(torch.uint8) == before[0]).view(cache.pages, heads, page, dim * es).all(-1)
+    same_v = (cache.v.view(torch.uint8) == before[1]).view(cache.pages, heads, dim, page, es).all(-1).all(2)
+    assert bool(same_k[~touched_k].all()) and bool(same_v[~touched_k].all())
+    if cdt == E4M3:
+        assert bool((cache.k_scale[~touched_k] == 99).all()) and bool((cache.v_scale[~touched_k] == 99).all())
+    # all that a sequence has, by its own lengths; and the other dtypes, rounded once
+    if any(a != b for a, b in zip(lens, news)):
+        return
+    for other in (torch.bfloat16, torch.float16):
+        ok, _ = cache_read(cache, table, lengths, N, starts=starts_of(lens), dtype=other)
+        assert torch.equal(ok, _held(k, cdt).float().to(other))
+
+
+def test_every_e4m3_value_and_border():
+    """All codes' values, the points halfway between neighbours and their neighbours
+    in float32, each row under its own maximum."""
+    codes = torch.arange(256, dtype=torch.uint8).view(E4M3).float()
+    codes = codes[torch.isfinite(codes)]
+    pos = codes[codes >= 0].unique()
+    mid = (pos[1:] + pos[:-1]) / 2
+    x = torch.cat((pos, mid, torch.nextafter(mid, torch.tensor(1e9)), torch.nextafter(mid, torch.tensor(0.0))))
+    x = torch.cat((x, -x))
+    x = torch.cat((x, x.new_zeros(-x.numel() % 64))).view(-1, 64)
+    x[:, 0] = 448.0                       # (so that the scale is 1)
+    for scale in (1.0, 2.0 ** -30, 2.0 ** 60, 1.3):
+        y = (x * scale).cuda().unsqueeze(1).contiguous()
+        N = y.size(0)
+        cache = PagedCache.empty(-(-N // 64), 1, 64, dtype=E4M3)
+        table, lengths = _table([N], 64, cache.pages), torch.tensor([N], dtype=torch.int32, device="cuda")
+        cache_write(cache, y, -y, table, lengths)
+        k, v = cache_read(cache, table, lengths, N)
+        assert torch.equal(k.double(), _held(y, E4M3)) and torch.equal(v.double(), -_held(y, E4M3))
+
+
+def test_scale_borders_and_special_values():
+    """Rows whose maximum is 448 times a power of two or just above it, the smallest
+    and largest floats, zeros, NaN and infinity."""
+    rows = [448.0, math.nextafter(448.0, 1e9), 3.4e38, 2.0 ** -126, 1e-45, 0.0, 2.0 ** -88, 448.0 * 2.0 ** -97, 1.75, 1.7500001]
+    x = torch.zeros(len(rows) + 3, 2, 16, device="cuda")
+    for i, r in enumerate(rows):
+        x[i, :, 3] = r
+        x[i, 1, 7] = -r / 3
+    x[-1, 0, :3] = torch.tensor([math.nan, math.inf, 2.0])
+    x[-1, 1, :2] = torch.tensor([-math.inf, math.nan])
+    x[-2] = 5.0
+    x[-2, 0, 1] = math.inf
+    cache = PagedCache.empty(2, 2, 16, page_size=16, dtype=E4M3)
+    N = x.size(0)
+    table, lengths = _table([N], 16, 2), torch.tensor([N], dtype=torch.int32, device="cuda")
+    cache_write(cache, x, x.flip(0).contiguous(), table, lengths)
+    k, v = cache_read(cache, table, lengths, N)
+    # (3.4e38 rounds up to 256 2^120 = 2^128: infinite as a float32)
+    want = _held(x, E4M3).float().double()
+    assert torch.equal(k.double().nan_to_num(nan=12345.0, posinf=math.inf, neginf=-math.inf), want.nan_to_num(nan=12345.0, posinf=math.inf, neginf=-math.inf))
+    assert torch.equal(v.double().nan_to_num(nan=12345.0, posinf=math.inf, neginf=-math.inf), want.flip(0).nan_to_num(nan=12345.0, posinf=math.inf, neginf=-math.inf))
+    assert bool(torch.isnan(k[-1, 0, :2]).all()) and float(k[-1, 0, 2]) == 2.0
+
+
+def test_missing_pages_and_positions():
+    """A page number outside the cache, a position past the table or below zero: not
+    written, read as NaN (0 where the token does not exist), nothing else touched."""
+    page, heads, dim = 16, 2, 32
+    for dt, cdt in ((torch.bfloat16, torch.bfloat16), (torch.float32, E4M3)):
+        cache = _filled(PagedCache.empty(3, heads, dim, page_size=page, dtype=cdt))
+        table = torch.tensor([[0, 3, 1], [-1, 2, 2 ** 31 - 1]], dtype=torch.int32, device="cuda")
+        lengths = torch.tensor([50, 20], dtype=torch.int32, device="cuda")     # 50 > 3 * 16
+        starts = starts_of([50, 30])                                            # 30 > 20
+        k = torch.randn(80, heads, dim, device="cuda").to(dt)
+        before = cache.k.view(torch.uint8).clone(), cache.v.view(torch.uint8).clone()
+        cache_write(cache, k, -k, table, lengths, starts=starts)
+        ok = [*range(0, 16), *range(32, 48)]
+        for got, want in zip(cache_read(cache, table, lengths, 80, starts=starts, dtype=torch.float32), (k, -k)):
+            held = _held(want, cdt)
+            assert torch.equal(got[:50][ok].double(), held[:50][ok])
+            assert bool(torch.isnan(got[[*range(16, 32), 48, 49]]).all())
+            # sequence 1: positions -10 to 19: ten that do not exist, 16 without a page, 4 on page 2
+            assert bool((got[50:60] == 0).all()) and bool(torch.isnan(got[60:76]).all())
+            assert torch.equal(got[76:].double(), held[76:])
+        es = cache.k.element_size()
+        same = (cache.k.view(torch.uint8) == before[0]).view(3, heads, page, dim * es).all(-1).all(1)
+        assert bool(same[2, 4:].all()) and not bool(same[:2].any()) and not bool(same[2, :4].any())
+        same = (cache.v.view(torch.uint8) == before[1]).view(3, heads, dim, page, es).all(-1).all(2).all(1)
+        assert bool(same[2, 4:].all())
+
+
+def test_padded_batch_and_strides():
+    """Rows behind the last sequence stay as they were; views of one projection's
+    output, and rows off 16 bytes, are read as contiguous ones are."""
+    heads, dim, page = 2, 64, 64
+    lens, news = [90, 3], [11, 3]
+    for dt, cdt in ((torch.bfloat16, torch.bfloat16), (torch.float16, E4M3), (torch.float32, E4M3)):
+        wide = torch.randn(20, 6 * heads * dim + 1, device="cuda").to(dt)
+        table, lengths, starts = _table(lens, page, 4), torch.tensor(lens, dtype=torch.int32, device="cuda"), starts_of(news)
+        reads = []
+        for at in (0, heads * dim, 1):
+            k = wide[:, at: at + heads * dim].unflatten(1, (heads, dim))
+            cache = PagedCache.empty(4, heads, dim, page_size=page, dtype=cdt)
+            cache_write(cache, k, k, table, lengths, starts=starts)
+            out = [torch.full((20, heads, dim), 7.0, device="cuda") for _ in "kv"]
+            cache_read(cache, table, lengths, 20, starts=starts, out=out)
+            assert torch.equal(out[0][:14].double(), _held(k[:14], cdt)) and torch.equal(out[0], out[1])
+            assert bool((out[0][14:] == 7.0).all())
+            reads.append(out)
+        hb = wide[:, : heads * dim].unflatten(1, (heads, dim)).transpose(0, 1).contiguous().transpose(0, 1)
+        cache = PagedCache.empty(4, heads, dim, page_size=page, dtype=cdt)
+        cache_write(cache, hb, hb, table, lengths, starts=starts)
+        assert torch.equal(cache_read(cache, table, lengths, 20, starts=starts, dtype=torch.float32)[0][:14], reads[0][0][:14])
+
+
+def test_captured_decode_steps():
+    """A captured write at positions that the device's lengths name."""
+    heads, dim, page, B = 2, 128, 16, 3
+    cache = PagedCache.empty(12, heads, dim, page_size=page, dtype=E4M3)
+    table = torch.arange(12, dtype=torch.int32, device="cuda").view(3, 4)
+    lengths = torch.tensor([14, 1, 31], dtype=torch.int32, device="cuda")
+    k = torch.randn(B, heads, dim, device="cuda", dtype=torch.bfloat16)
+    v = torch.randn(B, heads, dim, device="cuda", dtype=torch.bfloat16)
+    cache_write(cache, k, v, table, lengths)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lengths.add_(1)
+        cache_write(cache, k, v, table, lengths)
+        rk, rv = cache_read(cache, table, lengths, B)
+    for i in range(5):
+        k.normal_(), v.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(rk.double(), _held(k, E4M3)) and torch.equal(rv.double(), _held(v, E4M3)), i
+        eager = cache_read(cache, table, lengths, B)
+        assert torch.equal(eager[0], rk) and torch.equal(eager[1], rv)
+    assert lengths.tolist() == [19, 6, 36]   # (recording ran nothing)
+
+
+def test_no_tokens():
+    cache = PagedCache.empty(2, 1, 8)
+    table, lengths = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    k = torch.zeros(0, 1, 8, dtype=torch.bfloat16, device="cuda")
+    cache_write(cache, k, k, table, lengths)
+    assert cache_read(cache, table, lengths, 0)[0].shape == (0, 1, 8)
+    none = torch.zeros(0, 1, dtype=torch.int32, device="cuda")
+    cache_write(cache, k, k, none, lengths[:0])
+    cache_write(cache, k, k, table, lengths, starts=torch.zeros(4, dtype=torch.int32, device="cuda"))
