@@ -82,4 +82,10 @@ __device__ __forceinline__ float attn_cap(float s, float to_z, float cap2) {
 }
 
 
+// The kernel for many rows: its tiles, and the rows of a sequence (tokens by heads of a
+// group) up to which fl_attn.hip's is taken.
+constexpr int ATTN_WIDE_QT = 1, ATTN_WIDE_ROWS = 128 * ATTN_WIDE_QT;
+constexpr int ATTN_FEW_ROWS = 64;
+hipError_t launch_attn_wide(const fl_attn_args& a, const AttnPlan& p, hipStream_t s);
+
 }  // namespace fl

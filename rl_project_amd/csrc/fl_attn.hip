@@ -63,11 +63,13 @@ __device__ __forceinline__ uint4 ar_load16_8(const char* p) {
 // C: the cache's elements, DT: channels (a multiple of 64, dim or more), FULL: dim ==
 // DT, CT: tiles of 16 rows.
 template <class C, int DT, bool FULL, int CT>
-__global__ __launch_bounds__(AR_NT, 2) void k_attn_rows(const fl_attn_args a, const AttnPlan p) {
+__global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(const fl_attn_args a, const AttnPlan p) {
   using Op = typename C::Op;
   using Pv = typename C::Pv;
   constexpr int KS = DT / 32;   // steps of the first product
   constexpr int DM = DT / 16;   // tiles of channels of the second
+  // tiles of values that are loaded ahead of their step's softmax: what registers hold
+  constexpr int VPRE = DM * C::SUBS * CT <= 16 ? DM : DM / 2;
   constexpr int TR = 16 * CT;
   // the waves' results side by side; before that, weights where values are not finite
   constexpr int OS = DT + 4;
@@ -185,14 +187,26 @@ __global__ __launch_bounds__(AR_NT, 2) void k_attn_rows(const fl_attn_args a, co
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) st[ct][j] = Op::mfma16(kf[ks], q[ct][ks], st[ct][j]);
       }
+      // (a tile's keys, no more, where their registers are many)
+      if (DT * CT > 256) __builtin_amdgcn_sched_barrier(0);
     }
+    // (the values' registers are the keys')
+    __builtin_amdgcn_sched_barrier(0);
     // the values, on their way during the softmax (V^T: channel 16 dm + c, this lane's keys)
     uint4 vr[DM][C::SUBS];
+    const char* vs[C::SUBS];
 #pragma unroll
-    for (int dm = 0; dm < DM; ++dm)
+    for (int u = 0; u < C::SUBS; ++u) vs[u] = V + vp[u] + C::ESZ * S * c;
+    auto values = [&](int dm) {
 #pragma unroll
-      for (int u = 0; u < C::SUBS; ++u)
-        vr[dm][u] = FULL || 16 * dm + c < dim ? ar_load16(V + vp[u] + C::ESZ * S * (16 * dm + c)) : make_uint4(0, 0, 0, 0);
+      for (int u = 0; u < C::SUBS; ++u) {
+        vr[dm][u] = FULL || 16 * dm + c < dim ? ar_load16(vs[u]) : make_uint4(0, 0, 0, 0);
+        vs[u] += C::ESZ * S * 16;
+        asm("" : "+v"(vs[u]));   // (one address that moves, not one for every tile)
+      }
+    };
+#pragma unroll
+    for (int dm = 0; dm < VPRE; ++dm) values(dm);
 
     // ------------------------------------------------ the weights
     const bool masked = !attn_whole(a, v, t0) || __any(some_bad);
@@ -269,24 +283,10 @@ __global__ __launch_bounds__(AR_NT, 2) void k_attn_rows(const fl_attn_args a, co
     // A value that is not finite would reach the rows that do not see its key (0 times
     // it is NaN): in a step with masks such values are taken out of the product, and
     // added to the rows that see them.
-    bool odd = false;
-    if (masked) {
-      uint32_t any = 0;
-#pragma unroll
-      for (int dm = 0; dm < DM; ++dm)
-#pragma unroll
-        for (int u = 0; u < C::SUBS; ++u) {
-          if constexpr (C::E8) {
-            const uint4 y = vr[dm][u];
-            any |= ((y.x & 0x7f7f7f7fu) + 0x01010101u) | ((y.y & 0x7f7f7f7fu) + 0x01010101u) |
-                   ((y.z & 0x7f7f7f7fu) + 0x01010101u) | ((y.w & 0x7f7f7f7fu) + 0x01010101u);
-            any &= 0x80808080u;
-          } else any |= not_finite<Pv>(vr[dm][u]);
-        }
-      odd = __any(any != 0);
-    }
+    uint32_t odd = 0;
 #pragma unroll
     for (int dm = 0; dm < DM; ++dm) {
+      if (dm + VPRE < DM) values(dm + VPRE);
       uint4 vf[2];
       if constexpr (C::E8) {
         const uint4 x = vr[dm][0];
@@ -297,14 +297,17 @@ __global__ __launch_bounds__(AR_NT, 2) void k_attn_rows(const fl_attn_args a, co
         vf[0] = vr[dm][0];
         vf[1] = vr[dm][C::SUBS - 1];
       }
-      if (odd) vf[0] = finite_or_0<Pv>(vf[0]), vf[1] = finite_or_0<Pv>(vf[1]);
+      if (masked) {
+        odd |= not_finite<Pv>(vf[0]) | not_finite<Pv>(vf[1]);
+        vf[0] = finite_or_0<Pv>(vf[0]), vf[1] = finite_or_0<Pv>(vf[1]);
+      }
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
         o[ct][dm] = Pv::mfma16(vf[0], pf[ct][0], o[ct][dm]);
         o[ct][dm] = Pv::mfma16(vf[1], pf[ct][1], o[ct][dm]);
       }
     }
-    if (odd) {
+    if (masked && __any(odd != 0)) {
       float* wl = &so[w][0][0];   // [64 keys][16 rows]
       static_assert(64 * 16 <= 16 * OS, "a wave's weights fit");
 #pragma unroll
@@ -328,16 +331,20 @@ __global__ __launch_bounds__(AR_NT, 2) void k_attn_rows(const fl_attn_args a, co
           const int page = paged_page(a.rows, a.cache, s.b, t0 + k);
           if (!(x >= 0.0f) || page < 0) continue;   // (a NaN weight is in the sums already)
           const char* col = V + C::ESZ * ((static_cast<int64_t>(page) * Hk + h) * dim * S + ((t0 + k) & (S - 1)));
+const char* src = col + C::ESZ * (4 * g * S);
 #pragma unroll
           for (int dm = 0; dm < DM; ++dm)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int d = 16 * dm + 4 * g + e;
-              if (!FULL && d >= dim) continue;
-              float y;
-              if constexpr (C::E8) y = __builtin_amdgcn_cvt_f32_fp8(static_cast<uint8_t>(col[S * d]), 0);
-              else y = Op::D::to_f32(*reinterpret_cast<const uint16_t*>(col + 2 * S * d));
-              if (!(fabsf(y) < INFINITY)) o[ct][dm][e] += x * y;
+              // (one load at a time: this path is rare, the registers are the kernel's)
+              asm volatile("" : "+v"(src) : : "memory");
+              if (FULL || 16 * dm + 4 * g + e < dim) {
+                float y;
+                if constexpr (C::E8) y = __builtin_amdgcn_cvt_f32_fp8(static_cast<uint8_t>(*src), 0);
+                else y = Op::D::to_f32(*reinterpret_cast<const uint16_t*>(src));
+                if (!(fabsf(y) < INFINITY)) o[ct][dm][e] += x * y;
+              }
+              src += C::ESZ * S * (e == 3 ? 13 : 1);
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -383,7 +390,7 @@ __global__ __launch_bounds__(AR_NT, 2) void k_attn_rows(const fl_attn_args a, co
         f32x4 y = *reinterpret_cast<const f32x4*>(&so[0][rr][d]);
 #pragma unroll
         for (int x = 1; x < AR_NW; ++x) y += *reinterpret_cast<const f32x4*>(&so[x][rr][d]);
-        if (v.splits > 1) *reinterpret_cast<f32x4*>(p.part + (row * p.splits + split) * dim + d) = y;
+        if (v.splits > 1) *reinterpret_cast<f32x4*>(p.part + (row * p.stride + split) * dim + d) = y;
         else {
           y *= inv;
           *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (s.row + i) * a.out_ld + head * a.out_hs + d) =
@@ -391,7 +398,7 @@ __global__ __launch_bounds__(AR_NT, 2) void k_attn_rows(const fl_attn_args a, co
         }
       }
       if (k == 0) {
-        if (v.splits > 1) *reinterpret_cast<float2*>(p.stat + 2 * (row * p.splits + split)) = make_float2(mm, ll);
+        if (v.splits > 1) *reinterpret_cast<float2*>(p.stat + 2 * (row * p.stride + split)) = make_float2(mm, ll);
         else if (a.out_lse) a.out_lse[row] = ll == 0.0f ? -INFINITY : (mm == -INFINITY ? ll : (mm + log2f(ll)) * 0.6931471805599453f);
       }
     }
@@ -399,32 +406,32 @@ __global__ __launch_bounds__(AR_NT, 2) void k_attn_rows(const fl_attn_args a, co
   }
 }
 
-// The parts of rows whose keys were split: a wave a row.
+// The parts of rows whose keys were split: a wave a row; few and many: the plans of
+// sequences of few rows and of many.
 template <class Op>
-__global__ __launch_bounds__(AR_NT) void k_attn_join(const fl_attn_args a, const AttnPlan p) {
-  const int lane = threadIdx.x & (WAVE - 1), Hk = static_cast<int>(a.cache.heads), dim = static_cast<int>(a.cache.dim);
-  // a work-group takes 4 rows of one tile and cached head
-  const int per = (p.tr + 3) / 4;
-  const int h = blockIdx.x % Hk, rest = blockIdx.x / Hk;
-  const PagedSeq s = paged_seq(a.rows, rest / per, p.group, p.tr, 1, p.each);
-  const int rows = s.n * p.group, k4 = 4 * (rest % per) + threadIdx.x / WAVE;
-  if (rows < p.min_rows || rows > p.max_rows || k4 >= p.tr || s.tile >= (rows + p.tr - 1) / p.tr) return;
-  const int r = s.tile * p.tr + k4;
-  if (r >= rows) return;
-  const AttnSpan v = attn_span(a, p, s, s.tile);
+__global__ __launch_bounds__(AR_NT) void k_attn_join(const fl_attn_args a, const AttnPlan few, const AttnPlan many) {
+  const int lane = threadIdx.x & (WAVE - 1), dim = static_cast<int>(a.cache.dim), heads = static_cast<int>(a.q_heads);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * AR_NW + threadIdx.x / WAVE;
+  if (row >= a.rows.tokens * heads) return;
+  const int n = static_cast<int>(row / heads), head = static_cast<int>(row - static_cast<int64_t>(n) * heads);
+  const int seqs = static_cast<int>(a.rows.seqs);
+  const PagedSeq s = paged_rows(a.rows, a.rows.starts == nullptr ? n / static_cast<int>(a.rows.tokens / seqs)
+                                                                 : paged_find(seqs, n, [&](int m) { return a.rows.starts[m]; }));
+  const int i = n - static_cast<int>(s.row);
+  if (i < 0 || i >= s.n) return;   // (a row behind the last sequence)
+  const AttnPlan& p = s.n * few.group <= few.max_rows ? few : many;
+  const AttnSpan v = attn_span(a, p, s, (i * p.group + head % p.group) / p.tr);
   if (v.splits <= 1) return;
-  const int i = r / p.group;
-  const int64_t head = h * p.group + (r - i * p.group), row = (s.row + i) * a.q_heads + head;
   static_assert(AT_MAX_SPLITS <= WAVE, "a lane for every part");
   float2 st = make_float2(-INFINITY, 0.0f);
-  if (lane < v.splits) st = *reinterpret_cast<const float2*>(p.stat + 2 * (row * p.splits + lane));
+  if (lane < v.splits) st = *reinterpret_cast<const float2*>(p.stat + 2 * (row * p.stride + lane));
   const float m = wave_reduce(st.x, OpMax());
   const float f = st.x == -INFINITY ? (st.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(st.x - m);
   const float l = wave_reduce(st.y * f, OpAdd());
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   if (lane == 0 && a.out_lse) a.out_lse[row] = l == 0.0f ? -INFINITY : (m == -INFINITY ? l : (m + log2f(l)) * 0.6931471805599453f);
   f32x4 y = {0, 0, 0, 0};
-  const float* part = p.part + row * p.splits * dim + 4 * lane;
+  const float* part = p.part + row * p.stride * dim + 4 * lane;
 #pragma unroll 4
   for (int k = 0; k < v.splits; ++k) {
     const float x = __shfl(f, k, WAVE);
@@ -457,46 +464,65 @@ void ar_dims(const fl_attn_args& a, const AttnPlan& p, hipStream_t s) {
   else ar_launch<C, 256, false>(a, p, s);
 }
 
-int64_t attn_groups(const fl_attn_args& a) { return a.q_heads / a.cache.heads; }
+// The launches of a call: sequences of few rows and of many.
+struct AttnCall {
+  AttnPlan few, many;
+  bool has_few, has_many;
+  int64_t stride;
+};
 
-// The plan of a launch with tiles of tr rows.
-AttnPlan attn_plan(const fl_attn_args& a, int tr) {
-  AttnPlan p = {};
-  p.group = static_cast<int>(attn_groups(a));
-  p.tr = tr;
-  p.min_rows = 0;
-  p.max_rows = 0x7fffffff;
-  p.each = static_cast<int>((a.rows.tokens / a.rows.seqs * p.group + tr - 1) / tr);
-  p.tiles = paged_tiles(a.rows, p.group, tr, 1, p.each);
-  // Splits: enough for 4 work-groups on every CU, none shorter than 4 steps of 64
-  // keys of the longest sequence the table (or the window) allows.
-  int64_t keys = a.rows.table_width * a.cache.page_size;
-  if (a.window > 0 && a.window <= keys) keys = std::min(keys, a.window + tr / p.group + std::min(a.sinks, keys) + 3 * AT_BLK);
-  const int64_t blocks = (keys + AT_BLK - 1) / AT_BLK, groups = std::max<int64_t>(p.tiles * a.cache.heads, 1);
-  const int64_t want = (1024 + groups - 1) / groups, most = (blocks + AT_MIN_BLKS - 1) / AT_MIN_BLKS;
-  p.splits = static_cast<int>(std::max<int64_t>(1, std::min({want, most, static_cast<int64_t>(AT_MAX_SPLITS)})));
-  return p;
+AttnCall attn_call(const fl_attn_args& a) {
+  AttnCall c = {};
+  const int64_t G = a.q_heads / a.cache.heads, N = a.rows.tokens, B = a.rows.seqs, Hk = a.cache.heads;
+  // The most rows that a sequence can have, and all have where there are no starts.
+  const int64_t top = (a.rows.starts ? N : N / B) * G;
+  c.has_few = a.rows.starts || top <= ATTN_FEW_ROWS;
+  c.has_many = top > ATTN_FEW_ROWS;
+  const int64_t keys = a.rows.table_width * a.cache.page_size;
+  // Splits: enough that every CU has `work` / 256 work-groups, none shorter than 4
+  // steps of 64 keys of the longest sequence the table (or the window) allows.
+  const auto plan = [&](AttnPlan& p, int tr, int64_t groups, int64_t work) {
+    p.group = static_cast<int>(G);
+    p.tr = tr;
+    p.tiles = paged_tiles(a.rows, G, tr, 1, p.each);
+    const int64_t seen = a.window > 0 && a.window <= keys
+                             ? std::min(keys, a.window + tr / G + std::min(a.sinks, keys) + 3 * AT_BLK) : keys;
+    const int64_t blocks = (seen + AT_BLK - 1) / AT_BLK, want = (work + groups - 1) / groups;
+    p.splits = static_cast<int>(std::max<int64_t>(
+        1, std::min({want, (blocks + AT_MIN_BLKS - 1) / AT_MIN_BLKS, static_cast<int64_t>(AT_MAX_SPLITS)})));
+    c.stride = std::max<int64_t>(c.stride, p.splits > 1 ? p.splits : 0);
+  };
+  if (c.has_few) {
+    const int64_t rows = std::min<int64_t>(top, ATTN_FEW_ROWS);
+    // (ragged: tiles of 16 where the average sequence fits one)
+    const int tr = (a.rows.starts ? N * G <= 16 * B : top <= 16) ? 16 : 32;
+    c.few.min_rows = 0, c.few.max_rows = ATTN_FEW_ROWS;
+    c.few.each = static_cast<int>((rows + tr - 1) / tr);
+    plan(c.few, tr, B * Hk, 1024);
+  }
+  if (c.has_many) {
+    c.many.min_rows = c.has_few ? ATTN_FEW_ROWS + 1 : 0, c.many.max_rows = 0x7fffffff;
+    c.many.each = a.rows.starts ? 0 : static_cast<int>((top + ATTN_WIDE_ROWS - 1) / ATTN_WIDE_ROWS);
+    const int64_t tiles = a.rows.starts ? std::max<int64_t>((N - B) * G / ATTN_WIDE_ROWS, 1) : B * c.many.each;
+    plan(c.many, ATTN_WIDE_ROWS, tiles * Hk, 512);
+  }
+  if (!c.has_few) c.few.group = 1, c.few.max_rows = 0;
+  return c;
 }
 
-int attn_tile_rows(const fl_attn_args& a) {
-  return a.rows.tokens * attn_groups(a) <= 16 * a.rows.seqs ? 16 : 32;
-}
-
-size_t attn_part_bytes(const fl_attn_args& a, const AttnPlan& p) {
-  return p.splits > 1 ? static_cast<size_t>(a.rows.tokens) * a.q_heads * p.splits * (a.cache.dim + 2) * sizeof(float) : 0;
-}
+int64_t attn_rows(const fl_attn_args& a) { return a.rows.seqs == 0 ? 0 : a.rows.tokens * a.q_heads; }
 
 }  // namespace
 
 size_t attn_workspace_bytes(const fl_attn_args& a) {
-  if (a.rows.tokens == 0 || a.rows.seqs == 0) return 0;
-  return attn_part_bytes(a, attn_plan(a, attn_tile_rows(a)));
+  if (attn_rows(a) == 0) return 0;
+  return static_cast<size_t>(attn_rows(a)) * attn_call(a).stride * (a.cache.dim + 2) * sizeof(float);
 }
 
 int64_t attn_blocks(const fl_attn_args& a) {
-  if (a.rows.tokens == 0 || a.rows.seqs == 0) return 0;
-  const AttnPlan p = attn_plan(a, attn_tile_rows(a));
-  return p.tiles * a.cache.heads * std::max<int64_t>(p.splits, (p.tr + 3) / 4);
+  if (attn_rows(a) == 0) return 0;
+  const AttnCall c = attn_call(a);
+  return std::max({c.few.tiles * c.few.splits * a.cache.heads, c.many.tiles * c.many.splits * a.cache.heads, attn_rows(a) / AR_NW + 1});
 }
 
 hipError_t launch_attn(const fl_attn_args& args, hipStream_t s) {
@@ -504,16 +530,23 @@ hipError_t launch_attn(const fl_attn_args& args, hipStream_t s) {
   // (positions are below 2^31: a longer window is none)
   a.window = a.window > 0x7fffffff ? 0 : a.window;
   a.sinks = std::min<int64_t>(a.sinks, 0x7fffffff);
-  AttnPlan p = attn_plan(a, attn_tile_rows(a));
-  p.part = static_cast<float*>(a.workspace);
-  p.stat = p.part ? p.part + a.rows.tokens * a.q_heads * p.splits * a.cache.dim : nullptr;
+  AttnCall c = attn_call(a);
+  for (AttnPlan* p : {&c.few, &c.many}) {
+    p->stride = c.stride;
+    p->part = static_cast<float*>(a.workspace);
+    p->stat = c.stride ? p->part + attn_rows(a) * c.stride * a.cache.dim : nullptr;
+  }
   const bool bf = a.dtype == FL_DTYPE_BF16;
-  if (a.cache.dtype == FL_DTYPE_E4M3) bf ? ar_dims<Cache8<OpBF16>>(a, p, s) : ar_dims<Cache8<OpF16>>(a, p, s);
-  else bf ? ar_dims<Cache16<OpBF16>>(a, p, s) : ar_dims<Cache16<OpF16>>(a, p, s);
-  if (p.splits > 1) {
-    const dim3 grid(static_cast<unsigned>(p.tiles * ((p.tr + 3) / 4) * a.cache.heads));
-    if (bf) hipLaunchKernelGGL(k_attn_join<OpBF16>, grid, dim3(AR_NT), 0, s, a, p);
-    else hipLaunchKernelGGL(k_attn_join<OpF16>, grid, dim3(AR_NT), 0, s, a, p);
+  if (c.has_many)
+    if (const hipError_t e = launch_attn_wide(a, c.many, s)) return e;
+  if (c.has_few) {
+    if (a.cache.dtype == FL_DTYPE_E4M3) bf ? ar_dims<Cache8<OpBF16>>(a, c.few, s) : ar_dims<Cache8<OpF16>>(a, c.few, s);
+    else bf ? ar_dims<Cache16<OpBF16>>(a, c.few, s) : ar_dims<Cache16<OpF16>>(a, c.few, s);
+  }
+  if (c.stride > 0) {
+    const dim3 grid(static_cast<unsigned>((attn_rows(a) + AR_NW - 1) / AR_NW));
+    if (bf) hipLaunchKernelGGL(k_attn_join<OpBF16>, grid, dim3(AR_NT), 0, s, a, c.few, c.many);
+    else hipLaunchKernelGGL(k_attn_join<OpF16>, grid, dim3(AR_NT), 0, s, a, c.few, c.many);
   }
   return hipGetLastError();
 }

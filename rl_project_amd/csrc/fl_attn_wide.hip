@@ -1,0 +1,427 @@
+// Attention over a paged cache for many rows of queries (prompts and their pieces);
+// the few rows of decode and verify steps are fl_attn.hip's.
+//
+// The matrix cores bound it: 4 D flops per score.  A work-group takes 128 rows, a wave
+// 32; 64 keys a step, theirs and their values' tiles in LDS for all waves (two turns:
+// the next step's are loaded into registers, 8-bit ones widened on the way, while this
+// one's are worked on).  Products as there, transposed: S^T = K Q^T and O^T += V^T P^T
+// with 32x32x16 instructions, keys assigned to the first product's rows such that a
+// lane's weights are the second's operand as they are, and so are the values' tokens as
+// the cache has them.  A row's sums and maximum are its column's two lanes'.  Rows of
+// LDS are 16 bytes longer than their data, so that 8 neighbouring rows' chunks lie in
+// different banks.
+#include <algorithm>
+
+#include "fl_attn.h"
+
+namespace fl {
+
+namespace {
+
+constexpr int AW_NT = 256, AW_NW = AW_NT / WAVE;
+
+}  // namespace
+
+// Op: the queries' type, E8: 8-bit cache, DT: channels (a multiple of 64, dim or more),
+// FULL: dim == DT, QT: tiles of 32 rows of a wave.
+template <class Op, bool E8, int DT, bool FULL, int QT>
+__global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wide(const fl_attn_args a, const AttnPlan p) {
+  // (8-bit values' weights carry their scales: bfloat16, as in fl_attn.hip)
+  using Pv = typename std::conditional<E8, OpBF16, Op>::type;
+  constexpr int TR = 32 * QT * AW_NW;
+  constexpr int ESZ = E8 ? 1 : 2, EPC = 16 / ESZ;         // the cache's elements, and those of a 16-byte chunk
+  constexpr int KC = DT / EPC, VC = AT_BLK / EPC;         // chunks of a key's and of a channel's row
+  constexpr int NK = AT_BLK * KC / AW_NT, NV = DT * VC / AW_NT;   // chunks of a thread
+  constexpr int KS = 2 * DT + 16, VS = 2 * AT_BLK + 16;   // LDS row strides in bytes
+  constexpr int KB = AT_BLK * KS, VB = DT * VS, SB = E8 ? 2 * AT_BLK * 4 : 0;
+  constexpr int BUF = KB + VB + SB;
+  constexpr int KSTEPS = DT / 16, DM = DT / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ int flags[2];   // of the steps' turns: 1 << sub-block: no page, 16: a value that is not finite
+
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1), w = tid / WAVE, c = lane & 31, hh = lane >> 5;
+  const int Hk = static_cast<int>(a.cache.heads), dim = static_cast<int>(a.cache.dim);
+  const int h = blockIdx.x % Hk, rest = blockIdx.x / Hk, split = rest % p.splits;
+  // (the last tiles, which see the most keys, first)
+  const PagedSeq s = paged_seq(a.rows, static_cast<int>(p.tiles) - 1 - rest / p.splits, p.group, TR, 1, p.each);
+  const int rows = s.n * p.group;
+  if (rows < p.min_rows || rows > p.max_rows || s.tile >= (rows + TR - 1) / TR) return;
+  const AttnSpan v = attn_span(a, p, s, s.tile);
+  if (split >= v.splits) return;
+  const int b0 = static_cast<uint32_t>(v.blocks) * split / static_cast<uint32_t>(v.splits);
+  const int b1 = static_cast<uint32_t>(v.blocks) * (split + 1) / static_cast<uint32_t>(v.splits);
+
+  // a negative scale turns the queries' signs
+  const float LOG2E = 1.4426950408889634f;
+  const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
+  const float scale = fabsf(a.scale);
+  const float to2 = a.softcap > 0.0f ? 1.0f : scale * LOG2E;
+  const float cap2 = a.softcap * LOG2E, to_z = a.softcap > 0.0f ? 2.0f * LOG2E * scale / a.softcap : 0.0f;
+
+  uint4 q[QT][KSTEPS];
+  int64_t at[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = s.tile * TR + 32 * (QT * w + t) + c, i = r / p.group;
+    const bool on = r < rows;
+    at[t] = on ? s.pos + i : -1;
+    const char* row = static_cast<const char*>(a.q) + 2 * ((s.row + i) * a.q_ld + (h * p.group + (r - i * p.group)) * a.q_hs);
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks) {
+      const int d = 16 * ks + 8 * hh;
+      uint4 x = on && d < dim ? *reinterpret_cast<const uint4*>(row + 2 * d) : make_uint4(0, 0, 0, 0);
+      q[t][ks] = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
+    }
+  }
+
+  f32x16 o[QT][DM];
+  float m[QT], l[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    m[t] = -INFINITY, l[t] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[t][i][e] = 0.0f;
+  }
+
+  // ---------------------------------------------------- a step's keys and values
+  const int64_t S = a.cache.page_size;
+  uint4 kr[NK], vr[NV];
+  float skr = 0.0f;   // a key's scale, or its values'
+  int bad = 0;
+  auto fetch = [&](int i) {
+    const int64_t t0 = v.key(i);
+    int64_t page[4];
+    bad = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int x = paged_page(a.rows, a.cache, s.b, t0 + 16 * u);
+      bad |= x < 0 ? 1 << u : 0;
+      page[u] = static_cast<int64_t>(max(x, 0)) * Hk + h;
+    }
+    const auto pick = [&](int u) { return u == 0 ? page[0] : u == 1 ? page[1] : u == 2 ? page[2] : page[3]; };
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      const int id = tid + AW_NT * n, row = id / KC, d = id % KC * EPC;
+      const char* src = static_cast<const char*>(a.cache.k) + ESZ * ((pick(row >> 4) * S + ((t0 + row) & (S - 1))) * dim + d);
+      if constexpr (FULL) kr[n] = *reinterpret_cast<const uint4*>(src);
+      else {
+        kr[n] = make_uint4(0, 0, 0, 0);
+        if constexpr (E8) {   // (a row may start at any multiple of 8 bytes)
+          if (d < dim) {
+            const uint2 x = *reinterpret_cast<const uint2*>(src);
+            kr[n].x = x.x, kr[n].y = x.y;
+          }
+          if (d + 8 < dim) {
+            const uint2 x = *reinterpret_cast<const uint2*>(src + 8);
+            kr[n].z = x.x, kr[n].w = x.y;
+          }
+        } else if (d < dim) kr[n] = *reinterpret_cast<const uint4*>(src);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int id = tid + AW_NT * n, d = id / VC, t = id % VC * EPC;
+      const char* src = static_cast<const char*>(a.cache.v) + ESZ * ((pick(t >> 4) * dim + d) * S + ((t0 + t) & (S - 1)));
+      vr[n] = FULL || d < dim ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+    }
+    if constexpr (E8) {
+      if (tid < 2 * AT_BLK) {
+        const int t = tid & (AT_BLK - 1);
+        const uint8_t* src = tid < AT_BLK ? a.cache.k_scale : a.cache.v_scale;
+        skr = scale_of(src[pick(t >> 4) * S + ((t0 + t) & (S - 1))]);
+      }
+    }
+  };
+  auto stage = [&](int turn, bool whole) {
+    char* buf = smem + turn * BUF;
+    uint32_t odd = 0;
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      const int id = tid + AW_NT * n, row = id / KC;
+      char* dst = buf + row * KS + id % KC * EPC * 2;
+      if constexpr (E8) {
+        const uint2 y0 = Op::widen(kr[n].x), y1 = Op::widen(kr[n].y), y2 = Op::widen(kr[n].z), y3 = Op::widen(kr[n].w);
+        *reinterpret_cast<uint4*>(dst) = make_uint4(y0.x, y0.y, y1.x, y1.y);
+        *reinterpret_cast<uint4*>(dst + 16) = make_uint4(y2.x, y2.y, y3.x, y3.y);
+      } else *reinterpret_cast<uint4*>(dst) = kr[n];
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int id = tid + AW_NT * n, d = id / VC;
+      char* dst = buf + KB + d * VS + id % VC * EPC * 2;
+      uint4 x[E8 ? 2 : 1];
+      if constexpr (E8) {
+        const uint2 y0 = Pv::widen(vr[n].x), y1 = Pv::widen(vr[n].y), y2 = Pv::widen(vr[n].z), y3 = Pv::widen(vr[n].w);
+        x[0] = make_uint4(y0.x, y0.y, y1.x, y1.y);
+        x[1] = make_uint4(y2.x, y2.y, y3.x, y3.y);
+      } else x[0] = vr[n];
+#pragma unroll
+      for (int y = 0; y < (E8 ? 2 : 1); ++y) {
+        // A value that is not finite would reach the rows that do not see its key (0
+        // times it is NaN): in a step with masks such values are taken out here, and
+        // added to the rows that see them.
+        if (!whole) {
+          odd |= not_finite<Pv>(x[y]);
+          x[y] = finite_or_0<Pv>(x[y]);
+        }
+        *reinterpret_cast<uint4*>(dst + 16 * y) = x[y];
+      }
+    }
+    if constexpr (E8)
+      if (tid < 2 * AT_BLK) reinterpret_cast<float*>(buf + KB + VB)[tid] = skr;
+    if (!whole && __any(odd != 0) && lane == 0) atomicOr(&flags[turn], 16);
+    if (bad != 0 && tid == 0) atomicOr(&flags[turn], bad);
+  };
+
+  if (tid < 2) flags[tid] = 0;
+  if (b0 < b1) fetch(b0);
+  __syncthreads();
+  for (int i = b0; i < b1; ++i) {
+    const int turn = (i - b0) & 1;
+    const int64_t t0 = v.key(i);
+    const bool whole = attn_whole(a, v, t0);
+    stage(turn, whole);
+    if (i + 1 < b1) fetch(i + 1);
+    lds_barrier();
+    const char* kb = smem + turn * BUF;
+    const char* vb = kb + KB;
+    const int fl = flags[turn];
+    const bool masked = !whole || fl != 0;
+
+    // -------------------------------------------------- S^T = K Q^T
+    // row m = 8 j + 4 h' + r of a tile of 32 holds key 16 (j / 2) + 8 h' + 4 (j % 2) + r
+    const int krow = (c >> 4) * 16 + ((c >> 2) & 1) * 8 + ((c >> 3) & 1) * 4 + (c & 3);
+    f32x16 st[QT][2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) st[t][kt][e] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ++ks) {
+        const uint4 kf = *reinterpret_cast<const uint4*>(kb + (32 * kt + krow) * KS + 32 * ks + 16 * hh);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) st[t][kt] = Op::mfma32(kf, q[t][ks], st[t][kt]);
+      }
+    }
+
+    // -------------------------------------------------- the weights
+    // (value e of a tile: key 16 (e / 8) + 8 hh + e % 8)
+    if constexpr (E8) {
+      const float* sk = reinterpret_cast<const float*>(vb + VB);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float f = sk[32 * kt + 16 * (e >> 3) + 8 * hh + (e & 7)];
+#pragma unroll
+          for (int t = 0; t < QT; ++t) st[t][kt][e] *= f;
+        }
+    }
+    uint4 pf[QT][4];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      if (a.softcap > 0.0f) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) st[t][kt][e] = attn_cap(st[t][kt][e], to_z, cap2);
+      }
+      if (masked) {
+        // keys of the step up to `hi` are seen, from `lo` on or below the sinks' end
+        const int hi = static_cast<int>(least(most(at[t] - t0, -1), AT_BLK));
+        const int lo = a.window > 0 ? static_cast<int>(least(most(at[t] - a.window + 1 - t0, 0), AT_BLK)) : 0;
+        const int sk = static_cast<int>(least(most(a.sinks - t0, 0), AT_BLK));
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int k = 32 * kt + 16 * (e >> 3) + 8 * hh + (e & 7);
+            const bool seen = k <= hi && (k >= lo || k < sk);
+            st[t][kt][e] = !seen ? -INFINITY : fl >> (2 * kt + (e >> 3)) & 1 ? __builtin_nanf("") : st[t][kt][e];
+          }
+      }
+      float top = st[t][0][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, st[t][0][e]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, st[t][1][e]);
+      top = top == -INFINITY ? top : top * to2;   // (to2 may be 0)
+      if (__any(top > m[t] + AT_LAZY)) {
+        top = fmaxf(top, shfl_xor(top, 32));
+        const float to = fmaxf(m[t], top);
+        const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[t] - to);
+        m[t] = to;
+        l[t] *= f;
+#pragma unroll
+        for (int dm = 0; dm < DM; ++dm)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[t][dm][e] *= f;
+      }
+      const float mm = m[t] == -INFINITY ? 0.0f : m[t];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float x = st[t][kt][e];
+          // (-inf times a scale of 0)
+          x = masked && x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(x, to2, -mm));
+          l[t] += x;
+          st[t][kt][e] = x;
+        }
+    }
+    if constexpr (E8) {
+      const float* sv = reinterpret_cast<const float*>(vb + VB) + AT_BLK;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float f = sv[32 * kt + 16 * (e >> 3) + 8 * hh + (e & 7)];
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            const float x = st[t][kt][e];   // (a masked slot may hold no scale)
+            st[t][kt][e] = masked && x == 0.0f ? 0.0f : x * f;
+          }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const f32x16& x = st[t][u >> 1];
+        const int e = 8 * (u & 1);
+        pf[t][u] = make_uint4(Pv::pack(x[e], x[e + 1]), Pv::pack(x[e + 2], x[e + 3]), Pv::pack(x[e + 4], x[e + 5]),
+                              Pv::pack(x[e + 6], x[e + 7]));
+      }
+
+    // -------------------------------------------------- O^T += V^T P^T
+#pragma unroll
+    for (int dm = 0; dm < DM; ++dm)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint4 vf = *reinterpret_cast<const uint4*>(vb + (32 * dm + c) * VS + 32 * u + 16 * hh);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) o[t][dm] = Pv::mfma32(vf, pf[t][u], o[t][dm]);
+      }
+
+    if (fl & 16) {   // (the same for all waves)
+      float* wl = reinterpret_cast<float*>(smem + turn * BUF) + w * 16 * 32;   // in the keys' place: [16 keys][32 rows]
+      static_assert(AW_NW * 16 * 32 * 4 <= KB, "the waves' weights of 16 keys fit");
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        const int hi = static_cast<int>(least(most(at[t] - t0, -1), AT_BLK));
+        const int lo = a.window > 0 ? static_cast<int>(least(most(at[t] - a.window + 1 - t0, 0), AT_BLK)) : 0;
+        const int sk = static_cast<int>(least(most(a.sinks - t0, 0), AT_BLK));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          __syncthreads();   // (the keys, or the last weights, have been read)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int k = 16 * u + 8 * hh + e;
+            const uint32_t x = e < 2 ? pf[t][u].x : e < 4 ? pf[t][u].y : e < 6 ? pf[t][u].z : pf[t][u].w;
+            wl[(8 * hh + e) * 32 + c] = k <= hi && (k >= lo || k < sk) ? Pv::D::to_f32((e & 1 ? x >> 16 : x) & 0xFFFFu) : -1.0f;
+          }
+          __syncthreads();
+          const int page = paged_page(a.rows, a.cache, s.b, t0 + 16 * u);
+          if (page < 0) continue;
+          const char* col = static_cast<const char*>(a.cache.v) +
+                            ESZ * ((static_cast<int64_t>(page) * Hk + h) * dim * S + ((t0 + 16 * u) & (S - 1)));
+#pragma unroll 1
+          for (int k = 0; k < 16; ++k) {
+            const float x = wl[k * 32 + c];
+            if (!(x >= 0.0f)) continue;   // (a NaN weight is in the sums already)
+const char* src = col + ESZ * (4 * hh * S + k);
+#pragma unroll
+            for (int dm = 0; dm < DM; ++dm)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                // (one load at a time: this path is rare, the registers are the kernel's)
+                asm volatile("" : "+v"(src) : : "memory");
+                if (FULL || 32 * dm + 8 * (e >> 2) + 4 * hh + (e & 3) < dim) {
+                  float y;
+                  if constexpr (E8) y = __builtin_amdgcn_cvt_f32_fp8(static_cast<uint8_t>(*src), 0);
+                  else y = Op::D::to_f32(*reinterpret_cast<const uint16_t*>(src));
+                  if (!(fabsf(y) < INFINITY)) o[t][dm][e] += x * y;
+                }
+                src += ESZ * S * ((e & 3) == 3 ? 5 : 1);
+              }
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (fl != 0) {
+      __syncthreads();   // (all waves have read the flags)
+      if (tid == 0) flags[turn] = 0;
+      // (two barriers before the turn's next stage)
+    }
+  }
+
+  // ---------------------------------------------------- results
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    float ll = l[t] + shfl_xor(l[t], 32);
+    const int r = s.tile * TR + 32 * (QT * w + t) + c;
+    if (r >= rows) continue;
+    const int i = r / p.group;
+    if (s.pos + i >= a.rows.table_width * S) ll = __builtin_nanf("");
+    const int64_t head = h * p.group + (r - i * p.group), row = (s.row + i) * a.q_heads + head;
+    const float inv = v.splits > 1 ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll
+    for (int dm = 0; dm < DM; ++dm)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = 32 * dm + 8 * j + 4 * hh;
+        if (!FULL && d >= dim) continue;
+        const f32x4 y = (f32x4){o[t][dm][4 * j], o[t][dm][4 * j + 1], o[t][dm][4 * j + 2], o[t][dm][4 * j + 3]} * inv;
+        if (v.splits > 1) *reinterpret_cast<f32x4*>(p.part + (row * p.stride + split) * dim + d) = y;
+        else
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (s.row + i) * a.out_ld + head * a.out_hs + d) =
+              make_uint2(Op::pack(y[0], y[1]), Op::pack(y[2], y[3]));
+      }
+    if (hh == 0) {
+      if (v.splits > 1) *reinterpret_cast<float2*>(p.stat + 2 * (row * p.stride + split)) = make_float2(m[t], ll);
+      else if (a.out_lse) a.out_lse[row] = ll == 0.0f ? -INFINITY : m[t] == -INFINITY ? ll : (m[t] + log2f(ll)) * 0.6931471805599453f;
+    }
+  }
+}
+
+namespace {
+
+template <class Op, bool E8, int DT, bool FULL>
+hipError_t aw_launch(const fl_attn_args& a, const AttnPlan& p, hipStream_t s) {
+  constexpr int QT = ATTN_WIDE_QT;
+  constexpr int LDS = 2 * (AT_BLK * (2 * DT + 16) + DT * (2 * AT_BLK + 16) + (E8 ? 2 * AT_BLK * 4 : 0));
+  if (LDS > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attn_wide<Op, E8, DT, FULL, QT>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((k_attn_wide<Op, E8, DT, FULL, QT>), dim3(static_cast<unsigned>(p.tiles * p.splits * a.cache.heads)), dim3(AW_NT),
+                     LDS, s, a, p);
+  return hipGetLastError();
+}
+template <class Op, bool E8>
+hipError_t aw_dims(const fl_attn_args& a, const AttnPlan& p, hipStream_t s) {
+  switch (a.cache.dim) {
+    case 64: return aw_launch<Op, E8, 64, true>(a, p, s);
+    case 128: return aw_launch<Op, E8, 128, true>(a, p, s);
+    case 256: return aw_launch<Op, E8, 256, true>(a, p, s);
+  }
+  if (a.cache.dim < 64) return aw_launch<Op, E8, 64, false>(a, p, s);
+  if (a.cache.dim < 128) return aw_launch<Op, E8, 128, false>(a, p, s);
+  return aw_launch<Op, E8, 256, false>(a, p, s);
+}
+
+}  // namespace
+
+hipError_t launch_attn_wide(const fl_attn_args& a, const AttnPlan& p, hipStream_t s) {
+  const bool bf = a.dtype == FL_DTYPE_BF16;
+  if (a.cache.dtype == FL_DTYPE_E4M3) return bf ? aw_dims<OpBF16, true>(a, p, s) : aw_dims<OpF16, true>(a, p, s);
+  return bf ? aw_dims<OpBF16, false>(a, p, s) : aw_dims<OpF16, false>(a, p, s);
+}
+
+}  // namespace fl

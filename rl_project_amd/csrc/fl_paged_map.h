@@ -25,42 +25,53 @@ struct PagedSeq {
   int64_t pos;
 };
 
-// Tiles of a launch, `per` of the sequences' rows x mul each: sequence b's begin at
-// starts[b] mul / per + extra b, which leaves it floor(n mul / per) + extra of them at
-// least.  (The host has checked that tokens x mul and the tiles stay below 2^31.)
+// Tiles of a launch, `per` of the sequences' rows x mul each: `each` of every sequence
+// if it is above 0; else sequence b's begin at starts[b] mul / per + extra b, which
+// leaves it floor(n mul / per) + extra of them at least.  (The host has checked that
+// tokens x mul and the tiles stay below 2^31.)
 FL_HD int64_t paged_tiles(const fl_cache_rows& r, int64_t mul, int64_t per, int64_t extra, int64_t each) {
-  return r.starts == nullptr ? r.seqs * each : r.tokens * mul / per + extra * r.seqs;
+  return each > 0 ? r.seqs * each : r.tokens * mul / per + extra * r.seqs;
 }
 
-// The sequence of tile x (`each`: tiles of every sequence where all have the same
-// number of tokens).  What starts and lengths hold cannot lead outside the rows.
-FL_HD PagedSeq paged_seq(const fl_cache_rows& r, int x, uint32_t mul, uint32_t per, int extra, int each) {
-  PagedSeq s;
-  int lo, hi;
-  const int tokens = static_cast<int>(r.tokens), seqs = static_cast<int>(r.seqs);
-  if (r.starts == nullptr) {
-    s.b = x / each;
-    s.tile = x - s.b * each;
-    const int n = tokens / seqs;
-    lo = n * s.b;
-    hi = lo + n;
-  } else {
-    // (unsigned: what starts holds is below 2^31 / mul, or no matter)
-    const auto base = [&](int m) { return static_cast<int>(static_cast<uint32_t>(r.starts[m]) * mul / per + extra * m); };
-    int a = 0, z = seqs - 1;
-    while (a < z) {   // the last sequence whose tiles begin at x or before
-      const int m = (a + z + 1) / 2;
-      if (base(m) <= x) a = m;
-      else z = m - 1;
-    }
-    s.b = a;
-    lo = static_cast<int>(least(most(r.starts[a], 0), tokens));
-    hi = static_cast<int>(least(most(r.starts[a + 1], lo), tokens));
-    s.tile = static_cast<int>(most(x - base(a), 0));
+// The last of n sequences whose base, base(b), is x or below (or the first): they
+// ascend, or x belongs to none.
+template <class F>
+FL_HD int paged_find(int n, int x, F base) {
+  int a = 0, z = n - 1;
+  while (a < z) {
+    const int m = (a + z + 1) / 2;
+    if (base(m) <= x) a = m;
+    else z = m - 1;
   }
+  return a;
+}
+
+// Sequence b, as its rows and positions; what starts and lengths hold cannot lead
+// outside the rows.
+FL_HD PagedSeq paged_rows(const fl_cache_rows& r, int b) {
+  PagedSeq s;
+  const int tokens = static_cast<int>(r.tokens), n = tokens / static_cast<int>(r.seqs);
+  const int64_t lo = r.starts == nullptr ? n * b : least(most(r.starts[b], 0), tokens);
+  const int64_t hi = r.starts == nullptr ? lo + n : least(most(r.starts[b + 1], lo), tokens);
+  s.b = b;
+  s.tile = 0;
   s.row = lo;
-  s.n = hi - lo;
-  s.pos = static_cast<int64_t>(r.lengths[s.b]) - s.n;
+  s.n = static_cast<int>(hi - lo);
+  s.pos = static_cast<int64_t>(r.lengths[b]) - s.n;
+  return s;
+}
+
+// The sequence of tile x.
+FL_HD PagedSeq paged_seq(const fl_cache_rows& r, int x, uint32_t mul, uint32_t per, int extra, int each) {
+  if (each > 0) {
+    PagedSeq s = paged_rows(r, x / each);
+    s.tile = x % each;
+    return s;
+  }
+  // (unsigned: what starts holds is below 2^31 / mul, or no matter)
+  const auto base = [&](int m) { return static_cast<int>(static_cast<uint32_t>(r.starts[m]) * mul / per + extra * m); };
+  PagedSeq s = paged_rows(r, paged_find(static_cast<int>(r.seqs), x, base));
+  s.tile = static_cast<int>(most(static_cast<int64_t>(x) - base(s.b), 0));
   return s;
 }
 
@@ -82,7 +93,7 @@ struct KvTile {
 };
 FL_HD int64_t kv_tiles(const fl_cache_rows& r, int* each) {
   // (n tokens touch at most (n + 14) / 16 + 1 aligned runs of 16)
-  *each = static_cast<int>((r.tokens / r.seqs + KV_T - 2) / KV_T + 1);
+  *each = r.starts != nullptr ? 0 : static_cast<int>((r.tokens / r.seqs + KV_T - 2) / KV_T + 1);
   return paged_tiles(r, 1, KV_T, 2, *each);
 }
 FL_HD bool kv_tile(const fl_cache_rows& r, const fl_cache& c, const PagedSeq& s, KvTile& t) {
@@ -109,10 +120,11 @@ struct AttnPlan {
   int splits;         // parts that a tile's keys may be split into
   int min_rows;       // sequences of fewer rows, or
   int max_rows;       // more rows, are another launch's
-  int each;           // tiles of a sequence where all have the same number of tokens
+  int each;           // tiles of every sequence, or 0
   int64_t tiles;
-  float* part;        // [tokens * q_heads][splits][dim], then
-  float* stat;        // [tokens * q_heads][splits][2]: maximum (powers of two) and sum
+  int64_t stride;     // parts from row to row in:
+  float* part;        // [tokens * q_heads][stride][dim]
+  float* stat;        // [tokens * q_heads][stride][2]: maximum (powers of two) and sum
 };
 
 // The keys that a tile's tokens see, in steps of 64: those of the first `sink` steps

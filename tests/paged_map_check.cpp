@@ -49,7 +49,8 @@ int main(int argc, char** argv) {
     const int G = 1 + up_to(8), tr = 16 << up_to(4);
     AttnPlan p = {};
     p.group = G, p.tr = tr, p.splits = 1 + up_to(12);
-    p.each = static_cast<int>((N / B * static_cast<int64_t>(G) + tr - 1) / tr);
+    // (every sequence as many tiles, or each as many as its rows)
+    p.each = !ragged || rng() % 2 ? static_cast<int>(((ragged ? C : N / B) * static_cast<int64_t>(G) + tr - 1) / tr) : 0;
     fl_attn_args a = {};
     a.cache = c, a.rows = r;
     a.window = rng() & 1 ? 1 + up_to(200) : 0;
@@ -63,6 +64,7 @@ int main(int argc, char** argv) {
       if (s.tile >= (rows + tr - 1) / tr) continue;
       const AttnSpan v = attn_span(a, p, s, s.tile);
       REQUIRE(v.splits >= 1 && v.splits <= p.splits && v.blocks >= 0 && v.end <= static_cast<int64_t>(width) * S);
+      REQUIRE(broken || s.tile * tr < rows);
       int64_t last = -1;
       for (int i = 0; i < v.blocks; ++i) {
         REQUIRE(v.key(i) > last);   // (no step twice)
