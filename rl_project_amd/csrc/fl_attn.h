@@ -11,6 +11,16 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes by value (an assignment between uint4 lvalues is a memory copy to the
+// compiler, which can leave an array of them in scratch memory).
+__device__ __forceinline__ uint4 ld16(const void* p) {
+  const u32x4 x = *static_cast<const u32x4*>(p);
+  return make_uint4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void st16(void* p, uint4 x) { *static_cast<u32x4*>(p) = (u32x4){x.x, x.y, x.z, x.w}; }
+
 // 16-bit operands: 8 values of a lane as a uint4.
 struct OpBF16 {
   using D = BF16;

@@ -51,8 +51,7 @@ struct Cache8 {
   __device__ static __forceinline__ int chan(int g, int ks) { return (ks >> 1) * 64 + g * 16 + (ks & 1) * 8; }
 };
 
-__device__ __forceinline__ uint4 ar_load16(const char* p) { return *reinterpret_cast<const uint4*>(p); }
-// (a row of 8-bit keys may start at any multiple of 8 bytes)
+// A row of 8-bit keys may start at any multiple of 8 bytes.
 __device__ __forceinline__ uint4 ar_load16_8(const char* p) {
   const uint2 a = *reinterpret_cast<const uint2*>(p), b = *reinterpret_cast<const uint2*>(p + 8);
   return make_uint4(a.x, a.y, b.x, b.y);
@@ -102,7 +101,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int d = C::chan(g, ks);
-      q[ct][ks] = on && d < dim ? ar_load16(row + 2 * d) : make_uint4(0, 0, 0, 0);
+      q[ct][ks] = on && d < dim ? ld16(row + 2 * d) : make_uint4(0, 0, 0, 0);
     }
   }
 
@@ -147,8 +146,8 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
       kp[u] = K + C::ESZ * ((hk * S + (tk & (S - 1)) + (c & 3)) * dim);
       vp[u] = C::ESZ * (hv * dim * S + (tv & (S - 1)));
       if constexpr (C::E8) {   // the scales of this lane's 16 keys
-        ek = ar_load16(reinterpret_cast<const char*>(a.cache.k_scale) + hv * S + (tv & (S - 1)));
-        ev = ar_load16(reinterpret_cast<const char*>(a.cache.v_scale) + hv * S + (tv & (S - 1)));
+        ek = ld16(reinterpret_cast<const char*>(a.cache.k_scale) + hv * S + (tv & (S - 1)));
+        ev = ld16(reinterpret_cast<const char*>(a.cache.v_scale) + hv * S + (tv & (S - 1)));
       }
     }
     bool some_bad = bad[0];
@@ -164,7 +163,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
         for (int ks = 0; ks < KS; ks += 2) {
           const int d = C::chan(g, ks);
           uint4 x = make_uint4(0, 0, 0, 0);
-          if constexpr (FULL) x = ar_load16(kr + d);
+          if constexpr (FULL) x = ld16(kr + d);
           else if (d + 16 <= dim) x = ar_load16_8(kr + d);
           else if (d < dim) {
             const uint2 y = *reinterpret_cast<const uint2*>(kr + d);
@@ -178,7 +177,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           const int d = C::chan(g, ks);
-          kf[ks] = FULL || d < dim ? ar_load16(kr + 2 * d) : make_uint4(0, 0, 0, 0);
+          kf[ks] = FULL || d < dim ? ld16(kr + 2 * d) : make_uint4(0, 0, 0, 0);
         }
       }
 #pragma unroll
@@ -200,7 +199,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
     auto values = [&](int dm) {
 #pragma unroll
       for (int u = 0; u < C::SUBS; ++u) {
-        vr[dm][u] = FULL || 16 * dm + c < dim ? ar_load16(vs[u]) : make_uint4(0, 0, 0, 0);
+        vr[dm][u] = FULL || 16 * dm + c < dim ? ld16(vs[u]) : make_uint4(0, 0, 0, 0);
         vs[u] += C::ESZ * S * 16;
         asm("" : "+v"(vs[u]));   // (one address that moves, not one for every tile)
       }

@@ -69,7 +69,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
 #pragma unroll
     for (int ks = 0; ks < KSTEPS; ++ks) {
       const int d = 16 * ks + 8 * hh;
-      uint4 x = on && d < dim ? *reinterpret_cast<const uint4*>(row + 2 * d) : make_uint4(0, 0, 0, 0);
+      uint4 x = on && d < dim ? ld16(row + 2 * d) : make_uint4(0, 0, 0, 0);
       q[t][ks] = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
     }
   }
@@ -86,26 +86,42 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
   }
 
   // ---------------------------------------------------- a step's keys and values
+  // (16-key sub-blocks of a step lie each in one page; their pages are looked up a step
+  // before they are read)
   const int64_t S = a.cache.page_size;
+  const int shift = __builtin_ctzll(a.cache.page_size), mask = static_cast<int>(S) - 1;
+  const int* table = a.rows.table + s.b * a.rows.table_ld;
+  const int width = static_cast<int>(a.rows.table_width), pages = static_cast<int>(a.cache.pages);
+  const int64_t pstride = static_cast<int64_t>(Hk) * S * dim * ESZ;   // bytes from page to page
+  const char* kbase = static_cast<const char*>(a.cache.k) + h * S * dim * ESZ;
+  const char* vbase = static_cast<const char*>(a.cache.v) + h * S * dim * ESZ;
+  int page0, page1, page2, page3;
+  const auto look1 = [&](int t) {   // (t is below 2^31, as the table's end)
+    const int x = t >> shift, e = __builtin_amdgcn_readfirstlane(table[x < width ? x : width - 1]);
+    return x < width && e >= 0 && e < pages ? e : -1;
+  };
+  auto look = [&](int i) {
+    const int t0 = static_cast<int>(v.key(i));
+    page0 = look1(t0), page1 = look1(t0 + 16), page2 = look1(t0 + 32), page3 = look1(t0 + 48);
+  };
+  const auto pick = [&](int u) {
+    const int lo = u & 1 ? page1 : page0, hi = u & 1 ? page3 : page2;
+    return max(u & 2 ? hi : lo, 0);
+  };
   uint4 kr[NK], vr[NV];
   float skr = 0.0f;   // a key's scale, or its values'
   int bad = 0;
   auto fetch = [&](int i) {
-    const int64_t t0 = v.key(i);
-    int64_t page[4];
-    bad = 0;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int x = paged_page(a.rows, a.cache, s.b, t0 + 16 * u);
-      bad |= x < 0 ? 1 << u : 0;
-      page[u] = static_cast<int64_t>(max(x, 0)) * Hk + h;
-    }
-    const auto pick = [&](int u) { return u == 0 ? page[0] : u == 1 ? page[1] : u == 2 ? page[2] : page[3]; };
+    const int t0 = static_cast<int>(v.key(i));
+    bad = (page0 < 0 ? 1 : 0) | (page1 < 0 ? 2 : 0) | (page2 < 0 ? 4 : 0) | (page3 < 0 ? 8 : 0);
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
-      const int id = tid + AW_NT * n, row = id / KC, d = id % KC * EPC;
-      const char* src = static_cast<const char*>(a.cache.k) + ESZ * ((pick(row >> 4) * S + ((t0 + row) & (S - 1))) * dim + d);
-      if constexpr (FULL) kr[n] = *reinterpret_cast<const uint4*>(src);
+      // rows tid / KC + n AW_NT / KC: of one sub-block, or of two
+      constexpr int STEP = AW_NT / KC;
+      const int row = tid / KC + STEP * n, d = tid % KC * EPC;
+      const int u = STEP <= 16 ? STEP * n / 16 : STEP / 16 * n + tid / (16 * KC);
+      const char* src = kbase + pick(u) * pstride + ESZ * ((((t0 + 16 * u) & mask) + (row & 15)) * dim + d);
+      if constexpr (FULL) kr[n] = ld16(src);
       else {
         kr[n] = make_uint4(0, 0, 0, 0);
         if constexpr (E8) {   // (a row may start at any multiple of 8 bytes)
@@ -117,20 +133,24 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
             const uint2 x = *reinterpret_cast<const uint2*>(src + 8);
             kr[n].z = x.x, kr[n].w = x.y;
           }
-        } else if (d < dim) kr[n] = *reinterpret_cast<const uint4*>(src);
+        } else if (d < dim) kr[n] = ld16(src);
       }
     }
+    {
+      const int t = tid % VC * EPC;   // this thread's tokens of the step
+      const char* src = vbase + pick(t >> 4) * pstride + ESZ * (tid / VC * static_cast<int>(S) + ((t0 + t) & mask));
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int id = tid + AW_NT * n, d = id / VC, t = id % VC * EPC;
-      const char* src = static_cast<const char*>(a.cache.v) + ESZ * ((pick(t >> 4) * dim + d) * S + ((t0 + t) & (S - 1)));
-      vr[n] = FULL || d < dim ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+      for (int n = 0; n < NV; ++n) {
+        vr[n] = FULL || tid / VC + AW_NT / VC * n < dim ? ld16(src) : make_uint4(0, 0, 0, 0);
+        src += ESZ * static_cast<int>(S) * (AW_NT / VC);
+        asm("" : "+v"(src));   // (one address that moves, not one for every chunk)
+      }
     }
     if constexpr (E8) {
       if (tid < 2 * AT_BLK) {
         const int t = tid & (AT_BLK - 1);
         const uint8_t* src = tid < AT_BLK ? a.cache.k_scale : a.cache.v_scale;
-        skr = scale_of(src[pick(t >> 4) * S + ((t0 + t) & (S - 1))]);
+        skr = scale_of(src[(static_cast<int64_t>(pick(t >> 4)) * Hk + h) * S + ((t0 + t) & mask)]);
       }
     }
   };
@@ -143,31 +163,29 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
       char* dst = buf + row * KS + id % KC * EPC * 2;
       if constexpr (E8) {
         const uint2 y0 = Op::widen(kr[n].x), y1 = Op::widen(kr[n].y), y2 = Op::widen(kr[n].z), y3 = Op::widen(kr[n].w);
-        *reinterpret_cast<uint4*>(dst) = make_uint4(y0.x, y0.y, y1.x, y1.y);
-        *reinterpret_cast<uint4*>(dst + 16) = make_uint4(y2.x, y2.y, y3.x, y3.y);
-      } else *reinterpret_cast<uint4*>(dst) = kr[n];
+        st16(dst, make_uint4(y0.x, y0.y, y1.x, y1.y));
+        st16(dst + 16, make_uint4(y2.x, y2.y, y3.x, y3.y));
+      } else st16(dst, kr[n]);
     }
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int id = tid + AW_NT * n, d = id / VC;
       char* dst = buf + KB + d * VS + id % VC * EPC * 2;
-      uint4 x[E8 ? 2 : 1];
+      // A value that is not finite would reach the rows that do not see its key (0 times
+      // it is NaN): in a step with masks such values are taken out here, and added to
+      // the rows that see them.
+      const auto put = [&](char* to, uint4 x) {
+        if (!whole) {
+          odd |= not_finite<Pv>(x);
+          x = finite_or_0<Pv>(x);
+        }
+        st16(to, x);
+      };
       if constexpr (E8) {
         const uint2 y0 = Pv::widen(vr[n].x), y1 = Pv::widen(vr[n].y), y2 = Pv::widen(vr[n].z), y3 = Pv::widen(vr[n].w);
-        x[0] = make_uint4(y0.x, y0.y, y1.x, y1.y);
-        x[1] = make_uint4(y2.x, y2.y, y3.x, y3.y);
-      } else x[0] = vr[n];
-#pragma unroll
-      for (int y = 0; y < (E8 ? 2 : 1); ++y) {
-        // A value that is not finite would reach the rows that do not see its key (0
-        // times it is NaN): in a step with masks such values are taken out here, and
-        // added to the rows that see them.
-        if (!whole) {
-          odd |= not_finite<Pv>(x[y]);
-          x[y] = finite_or_0<Pv>(x[y]);
-        }
-        *reinterpret_cast<uint4*>(dst + 16 * y) = x[y];
-      }
+        put(dst, make_uint4(y0.x, y0.y, y1.x, y1.y));
+        put(dst + 16, make_uint4(y2.x, y2.y, y3.x, y3.y));
+      } else put(dst, vr[n]);
     }
     if constexpr (E8)
       if (tid < 2 * AT_BLK) reinterpret_cast<float*>(buf + KB + VB)[tid] = skr;
@@ -176,7 +194,11 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
   };
 
   if (tid < 2) flags[tid] = 0;
-  if (b0 < b1) fetch(b0);
+  if (b0 < b1) {
+    look(b0);
+    fetch(b0);
+    if (b0 + 1 < b1) look(b0 + 1);
+  }
   __syncthreads();
   for (int i = b0; i < b1; ++i) {
     const int turn = (i - b0) & 1;
@@ -184,6 +206,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
     const bool whole = attn_whole(a, v, t0);
     stage(turn, whole);
     if (i + 1 < b1) fetch(i + 1);
+    if (i + 2 < b1) look(i + 2);
     lds_barrier();
     const char* kb = smem + turn * BUF;
     const char* vb = kb + KB;
@@ -202,7 +225,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
         for (int e = 0; e < 16; ++e) st[t][kt][e] = 0.0f;
 #pragma unroll
       for (int ks = 0; ks < KSTEPS; ++ks) {
-        const uint4 kf = *reinterpret_cast<const uint4*>(kb + (32 * kt + krow) * KS + 32 * ks + 16 * hh);
+        const uint4 kf = ld16(kb + (32 * kt + krow) * KS + 32 * ks + 16 * hh);
 #pragma unroll
         for (int t = 0; t < QT; ++t) st[t][kt] = Op::mfma32(kf, q[t][ks], st[t][kt]);
       }
@@ -302,7 +325,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
     for (int dm = 0; dm < DM; ++dm)
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const uint4 vf = *reinterpret_cast<const uint4*>(vb + (32 * dm + c) * VS + 32 * u + 16 * hh);
+        const uint4 vf = ld16(vb + (32 * dm + c) * VS + 32 * u + 16 * hh);
 #pragma unroll
         for (int t = 0; t < QT; ++t) o[t][dm] = Pv::mfma32(vf, pf[t][u], o[t][dm]);
       }
