@@ -121,7 +121,7 @@ int validate_cache(const char* fn, const fl_cache& c, const fl_cache_rows& r) {
                 static_cast<long long>(c.pages), static_cast<long long>(c.heads), static_cast<long long>(c.dim),
                 static_cast<long long>(r.seqs), static_cast<long long>(r.tokens), static_cast<long long>(r.table_width));
   if (c.dim > FL_CACHE_MAX_DIM || c.pages > 0x7fffffff || c.heads > 65536 || r.seqs > 0x7fffff || r.tokens > 0x7fffff ||
-      r.table_width > 0x7fffffff / c.page_size)
+      r.table_width > (1 << 30) / c.page_size)
     return fail(FL_ENOTSUP, "%s: dim %lld, pages %lld, seqs %lld, tokens %lld or a table %lld wide beyond the library's limits", fn,
                 static_cast<long long>(c.dim), static_cast<long long>(c.pages), static_cast<long long>(r.seqs),
                 static_cast<long long>(r.tokens), static_cast<long long>(r.table_width));

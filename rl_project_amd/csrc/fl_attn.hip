@@ -87,15 +87,14 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
   const int b0 = static_cast<uint32_t>(v.blocks) * split / static_cast<uint32_t>(v.splits);
   const int b1 = static_cast<uint32_t>(v.blocks) * (split + 1) / static_cast<uint32_t>(v.splits);
 
-  // this lane's rows: their queries, and the keys they see: t <= at && (t >= from || t < sinks)
+  // this lane's rows: their queries, and the keys they see
   uint4 q[CT][KS];
-  int64_t at[CT], from[CT];
+  AttnSeen see[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int r = s.tile * TR + 16 * ct + c, i = r / p.group;
     const bool on = r < rows;
-    at[ct] = on ? s.pos + i : -1;
-    from[ct] = a.window > 0 ? at[ct] - a.window + 1 : 0;
+    see[ct] = attn_seen(a, on ? s.pos + i : -1);
     const char* row = static_cast<const char*>(a.q) +
                       2 * ((s.row + i) * a.q_ld + (h * p.group + (r - i * p.group)) * a.q_hs);
 #pragma unroll
@@ -123,7 +122,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
   // the pages of a step that this lane reads keys (row c of a tile) and values from
   int pk[C::SUBS], pv[C::SUBS];
   auto pages = [&](int i) {
-    const int64_t t0 = v.key(i);
+    const int t0 = v.key(i);
 #pragma unroll
     for (int u = 0; u < C::SUBS; ++u) {
       pk[u] = paged_page(a.rows, a.cache, s.b, t0 + C::key(c >> 2, 2 * u));
@@ -132,7 +131,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
   };
   if (b0 + w < b1) pages(b0 + w);
   for (int i = b0 + w; i < b1; i += AR_NW) {
-    const int64_t t0 = v.key(i);
+    const int t0 = v.key(i);
     // ------------------------------------------------ S^T = K Q^T
     const char* kp[C::SUBS];
     int64_t vp[C::SUBS];
@@ -140,7 +139,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
     uint4 ek, ev;
 #pragma unroll
     for (int u = 0; u < C::SUBS; ++u) {
-      const int64_t tk = t0 + C::key(c >> 2, 2 * u), tv = t0 + C::key(g, 2 * u);
+      const int tk = t0 + C::key(c >> 2, 2 * u), tv = t0 + C::key(g, 2 * u);
       bad[u] = pv[u] < 0;
       const int64_t hk = static_cast<int64_t>(max(pk[u], 0)) * Hk + h, hv = static_cast<int64_t>(max(pv[u], 0)) * Hk + h;
       kp[u] = K + C::ESZ * ((hk * S + (tk & (S - 1)) + (c & 3)) * dim);
@@ -208,7 +207,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
     for (int dm = 0; dm < VPRE; ++dm) values(dm);
 
     // ------------------------------------------------ the weights
-    const bool masked = !attn_whole(a, v, t0) || __any(some_bad);
+    const bool masked = !v.whole(t0) || __any(some_bad);
     uint4 pf[CT][2];
     float pw[CT][16];
 #pragma unroll
@@ -234,10 +233,10 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int64_t t = t0 + C::key(g, j) + e;
-            const bool seen = t <= at[ct] && (t >= from[ct] || t < a.sinks);
-            const bool no_page = bad[C::SUBS == 2 ? j >> 1 : 0];
-            x[4 * j + e] = !seen ? -INFINITY : no_page ? __builtin_nanf("") : x[4 * j + e];
+            const int t = t0 + C::key(g, j) + e;
+            const bool seen = (t <= see[ct].last) & ((t >= see[ct].from) | (t < v.sinks));
+            const float y = bad[C::SUBS == 2 ? j >> 1 : 0] ? __builtin_nanf("") : x[4 * j + e];
+            x[4 * j + e] = seen ? y : -INFINITY;
           }
       }
       float top = x[0];
@@ -264,11 +263,8 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float sv = scale_of((j == 0 ? ev.x : j == 1 ? ev.y : j == 2 ? ev.z : ev.w) >> (8 * e) & 255u);
-            // (a masked slot may hold no scale)
-            x[4 * j + e] = x[4 * j + e] == 0.0f ? 0.0f : x[4 * j + e] * sv;
-          }
+          for (int e = 0; e < 4; ++e)
+            x[4 * j + e] *= scale_of((j == 0 ? ev.x : j == 1 ? ev.y : j == 2 ? ev.z : ev.w) >> (8 * e) & 255u);
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -317,8 +313,8 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int k = C::key(g, j) + e;
-            const int64_t t = t0 + k;
-            const bool seen = t <= at[ct] && (t >= from[ct] || t < a.sinks);
+            const int t = t0 + k;
+            const bool seen = (t <= see[ct].last) & ((t >= see[ct].from) | (t < v.sinks));
             wl[k * 16 + c] = seen ? pw[ct][4 * j + e] : -1.0f;
           }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");

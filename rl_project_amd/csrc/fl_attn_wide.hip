@@ -53,24 +53,25 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
 
   // a negative scale turns the queries' signs
   const float LOG2E = 1.4426950408889634f;
-  const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
+  // (and one of 0 clears them: a masked score is -inf, which no factor may be 0 to)
+  const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : ~0u;
   const float scale = fabsf(a.scale);
-  const float to2 = a.softcap > 0.0f ? 1.0f : scale * LOG2E;
+  const float to2 = a.softcap > 0.0f || a.scale == 0.0f ? 1.0f : scale * LOG2E;
   const float cap2 = a.softcap * LOG2E, to_z = a.softcap > 0.0f ? 2.0f * LOG2E * scale / a.softcap : 0.0f;
 
   uint4 q[QT][KSTEPS];
-  int64_t at[QT];
+  AttnSeen see[QT];
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int r = s.tile * TR + 32 * (QT * w + t) + c, i = r / p.group;
     const bool on = r < rows;
-    at[t] = on ? s.pos + i : -1;
+    see[t] = attn_seen(a, on ? s.pos + i : -1);
     const char* row = static_cast<const char*>(a.q) + 2 * ((s.row + i) * a.q_ld + (h * p.group + (r - i * p.group)) * a.q_hs);
 #pragma unroll
     for (int ks = 0; ks < KSTEPS; ++ks) {
       const int d = 16 * ks + 8 * hh;
       uint4 x = on && d < dim ? ld16(row + 2 * d) : make_uint4(0, 0, 0, 0);
-      q[t][ks] = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
+      q[t][ks] = make_uint4((x.x ^ sign) & keep, (x.y ^ sign) & keep, (x.z ^ sign) & keep, (x.w ^ sign) & keep);
     }
   }
 
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
     return x < width && e >= 0 && e < pages ? e : -1;
   };
   auto look = [&](int i) {
-    const int t0 = static_cast<int>(v.key(i));
+    const int t0 = v.key(i);
     page0 = look1(t0), page1 = look1(t0 + 16), page2 = look1(t0 + 32), page3 = look1(t0 + 48);
   };
   const auto pick = [&](int u) {
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
   float skr = 0.0f;   // a key's scale, or its values'
   int bad = 0;
   auto fetch = [&](int i) {
-    const int t0 = static_cast<int>(v.key(i));
+    const int t0 = v.key(i);
     bad = (page0 < 0 ? 1 : 0) | (page1 < 0 ? 2 : 0) | (page2 < 0 ? 4 : 0) | (page3 < 0 ? 8 : 0);
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
@@ -202,8 +203,8 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
   __syncthreads();
   for (int i = b0; i < b1; ++i) {
     const int turn = (i - b0) & 1;
-    const int64_t t0 = v.key(i);
-    const bool whole = attn_whole(a, v, t0);
+    const int t0 = v.key(i);
+    const bool whole = v.whole(t0);
     stage(turn, whole);
     if (i + 1 < b1) fetch(i + 1);
     if (i + 2 < b1) look(i + 2);
@@ -254,17 +255,14 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
           for (int e = 0; e < 16; ++e) st[t][kt][e] = attn_cap(st[t][kt][e], to_z, cap2);
       }
       if (masked) {
-        // keys of the step up to `hi` are seen, from `lo` on or below the sinks' end
-        const int hi = static_cast<int>(least(most(at[t] - t0, -1), AT_BLK));
-        const int lo = a.window > 0 ? static_cast<int>(least(most(at[t] - a.window + 1 - t0, 0), AT_BLK)) : 0;
-        const int sk = static_cast<int>(least(most(a.sinks - t0, 0), AT_BLK));
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int k = 32 * kt + 16 * (e >> 3) + 8 * hh + (e & 7);
-            const bool seen = k <= hi && (k >= lo || k < sk);
-            st[t][kt][e] = !seen ? -INFINITY : fl >> (2 * kt + (e >> 3)) & 1 ? __builtin_nanf("") : st[t][kt][e];
+            const int k = t0 + 32 * kt + 16 * (e >> 3) + 8 * hh + (e & 7);
+            const bool seen = (k <= see[t].last) & ((k >= see[t].from) | (k < v.sinks));
+            const float y = fl >> (2 * kt + (e >> 3)) & 1 ? __builtin_nanf("") : st[t][kt][e];
+            st[t][kt][e] = seen ? y : -INFINITY;
           }
       }
       float top = st[t][0][0];
@@ -272,7 +270,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
       for (int e = 1; e < 16; ++e) top = fmaxf(top, st[t][0][e]);
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, st[t][1][e]);
-      top = top == -INFINITY ? top : top * to2;   // (to2 may be 0)
+      top *= to2;
       if (__any(top > m[t] + AT_LAZY)) {
         top = fmaxf(top, shfl_xor(top, 32));
         const float to = fmaxf(m[t], top);
@@ -289,9 +287,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          float x = st[t][kt][e];
-          // (-inf times a scale of 0)
-          x = masked && x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(x, to2, -mm));
+          const float x = __builtin_amdgcn_exp2f(fmaf(st[t][kt][e], to2, -mm));
           l[t] += x;
           st[t][kt][e] = x;
         }
@@ -304,10 +300,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
         for (int e = 0; e < 16; ++e) {
           const float f = sv[32 * kt + 16 * (e >> 3) + 8 * hh + (e & 7)];
 #pragma unroll
-          for (int t = 0; t < QT; ++t) {
-            const float x = st[t][kt][e];   // (a masked slot may hold no scale)
-            st[t][kt][e] = masked && x == 0.0f ? 0.0f : x * f;
-          }
+          for (int t = 0; t < QT; ++t) st[t][kt][e] *= f;
         }
     }
 #pragma unroll
@@ -335,17 +328,15 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
       static_assert(AW_NW * 16 * 32 * 4 <= KB, "the waves' weights of 16 keys fit");
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
-        const int hi = static_cast<int>(least(most(at[t] - t0, -1), AT_BLK));
-        const int lo = a.window > 0 ? static_cast<int>(least(most(at[t] - a.window + 1 - t0, 0), AT_BLK)) : 0;
-        const int sk = static_cast<int>(least(most(a.sinks - t0, 0), AT_BLK));
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           __syncthreads();   // (the keys, or the last weights, have been read)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const int k = 16 * u + 8 * hh + e;
+            const int k = t0 + 16 * u + 8 * hh + e;
+            const bool seen = (k <= see[t].last) & ((k >= see[t].from) | (k < v.sinks));
             const uint32_t x = e < 2 ? pf[t][u].x : e < 4 ? pf[t][u].y : e < 6 ? pf[t][u].z : pf[t][u].w;
-            wl[(8 * hh + e) * 32 + c] = k <= hi && (k >= lo || k < sk) ? Pv::D::to_f32((e & 1 ? x >> 16 : x) & 0xFFFFu) : -1.0f;
+            wl[(8 * hh + e) * 32 + c] = seen ? Pv::D::to_f32((e & 1 ? x >> 16 : x) & 0xFFFFu) : -1.0f;
           }
           __syncthreads();
           const int page = paged_page(a.rows, a.cache, s.b, t0 + 16 * u);

@@ -6,7 +6,7 @@
 
 namespace fl {
 
-// A stored scale's value (a slot never written may hold 0 or 255: no scale's codes).
-__device__ __forceinline__ float scale_of(uint32_t code) { return __uint_as_float(code << 23); }
+// A stored scale's value; finite for a slot never written, which may hold any code.
+__device__ __forceinline__ float scale_of(uint32_t code) { return __uint_as_float(min(code, 254u) << 23); }
 
 }  // namespace fl

@@ -129,15 +129,18 @@ struct AttnPlan {
 
 // The keys that a tile's tokens see, in steps of 64: those of the first `sink` steps
 // and of the steps from `low` on, `blocks` in all; and how many splits they make.
+// (The host has checked that keys number 2^30 at most.)
 struct AttnSpan {
   int64_t pmin, pmax;   // positions of the tile's first and last token
-  int64_t end;          // keys end here
-  int sink, blocks, splits;
-  int64_t low;
-  FL_HD int64_t key(int i) const {   // the first key of step i
-    return static_cast<int64_t>(AT_BLK) * (i < sink ? i : low + (i - sink));
-  }
+  int end;              // keys end here
+  int sink, blocks, splits, low;
+  int all, open, sinks;   // every token sees the keys up to `all` that are above `open` or below `sinks`
+  FL_HD int key(int i) const { return AT_BLK * (i < sink ? i : low + (i - sink)); }   // the first key of step i
+  // Whether every key of the step from t0 on is seen by every token of the tile.
+  FL_HD bool whole(int t0) const { return t0 + AT_BLK - 1 <= all && (t0 > open || t0 + AT_BLK <= sinks); }
 };
+
+constexpr int64_t AT_FAR = 0x7fffff00;   // beyond any key
 
 FL_HD AttnSpan attn_span(const fl_attn_args& a, const AttnPlan& p, const PagedSeq& s, int tile) {
   AttnSpan v;
@@ -145,23 +148,29 @@ FL_HD AttnSpan attn_span(const fl_attn_args& a, const AttnPlan& p, const PagedSe
   v.pmin = s.pos + r0 / p.group;
   v.pmax = s.pos + r1 / p.group;
   // (a position past the table is no key's: its query is given NaN)
-  v.end = least(most(v.pmax + 1, 0), a.rows.table_width * a.cache.page_size);
+  v.end = static_cast<int>(least(most(v.pmax + 1, 0), a.rows.table_width * a.cache.page_size));
   v.low = 0;
   v.sink = 0;
+  v.all = static_cast<int>(least(most(v.pmin, -1), AT_FAR));
+  v.open = a.window > 0 ? static_cast<int>(least(most(v.pmax - a.window, -1), AT_FAR)) : -1;
+  v.sinks = a.window > 0 ? static_cast<int>(least(a.sinks, AT_FAR)) : 0;
   if (a.window > 0) {
-    v.low = most(v.pmin - a.window + 1, 0) / AT_BLK;
-    v.sink = static_cast<int>(least((least(a.sinks, v.end) + AT_BLK - 1) / AT_BLK, v.low));
+    v.low = static_cast<int>(least(most(v.pmin - a.window + 1, 0), AT_FAR)) / AT_BLK;
+    v.sink = static_cast<int>(least((least(v.sinks, v.end) + AT_BLK - 1) / AT_BLK, v.low));
   }
-  const int64_t last = (v.end + AT_BLK - 1) / AT_BLK;
+  const int last = (v.end + AT_BLK - 1) / AT_BLK;
   v.blocks = static_cast<int>(v.sink + most(last - v.low, 0));
   v.splits = static_cast<int>(most(1, least(p.splits, (v.blocks + AT_MIN_BLKS - 1) / AT_MIN_BLKS)));
   return v;
 }
 
-// Whether every key of the step is seen by every token of the tile.
-FL_HD bool attn_whole(const fl_attn_args& a, const AttnSpan& v, int64_t t0) {
-  const int64_t t1 = t0 + AT_BLK - 1;
-  return t1 <= v.pmin && (a.window == 0 || t0 > v.pmax - a.window || t1 < a.sinks);
+// The keys that a token at position `at` sees: t <= last and (t >= from or t < sinks).
+struct AttnSeen {
+  int last, from;
+};
+FL_HD AttnSeen attn_seen(const fl_attn_args& a, int64_t at) {
+  return {static_cast<int>(least(most(at, -1), AT_FAR)),
+          a.window > 0 ? static_cast<int>(least(most(at - a.window + 1, 0), AT_FAR)) : 0};
 }
 
 }  // namespace fl

@@ -88,14 +88,18 @@ int main(int argc, char** argv) {
         const int64_t at = s.pos + row / G;
         REQUIRE(at >= v.pmin && at <= v.pmax);
         if (at >= static_cast<int64_t>(width) * S || at > 3000) continue;
-        for (int64_t t = 0; t <= at; ++t) {
+        const AttnSeen e = attn_seen(a, at);
+        for (int64_t t = 0; t <= at + 5; ++t) {
+          const bool sees = t <= at && (!a.window || t > at - a.window || t < a.sinks);
+          REQUIRE(sees == (t <= e.last && (t >= e.from || t < v.sinks)));
+          if (!sees) continue;
           if (a.window && t <= at - a.window && t >= a.sinks) continue;
           int found = 0;
           for (int i = 0; i < v.blocks; ++i) found += t >= v.key(i) && t < v.key(i) + AT_BLK;
           REQUIRE(found == 1);
         }
         for (int i = 0; i < v.blocks; ++i) {
-          if (!attn_whole(a, v, v.key(i))) continue;
+          if (!v.whole(v.key(i))) continue;
           for (int64_t t = v.key(i); t < v.key(i) + AT_BLK; ++t)
             REQUIRE(t <= at && (a.window == 0 || t > at - a.window || t < a.sinks));
         }
