@@ -20,6 +20,35 @@ namespace {
 
 constexpr int AW_NT = 256, AW_NW = AW_NT / WAVE;
 
+// Bytes of LDS of a work-group: two turns of 64 keys, their values, and 8-bit scales.
+constexpr int aw_lds(int DT, bool E8, bool FULL) {
+  const int pad = FULL && !E8 ? 0 : 16;
+  return 2 * (AT_BLK * (2 * DT + pad) + DT * (2 * AT_BLK + pad) + (E8 ? 2 * AT_BLK * 4 : 0));
+}
+
+// Tiles without padding have their rows' chunks exchanged instead (by an exclusive or),
+// so that 16 neighbouring rows' chunks of one number lie in different banks (64, of 4
+// bytes): rows of 256 bytes and more by the row, of 128 by the pair of rows.
+template <int ROW>
+__device__ __forceinline__ int aw_swap(int row) {
+  return ROW >= 256 ? row & 15 : (row >> 1) & 7;
+}
+
+// 16 bytes per lane from base (the wave's) + off to LDS at lds + 16 lane, past the
+// registers; the waits are the kernel's (vmcnt).
+__device__ __forceinline__ void aw_load_lds(const char* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void aw_load_lds(const char* src, uint32_t lds) {   // ... each lane from its own address
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src)
+               : "memory", "m0");
+}
+
 }  // namespace
 
 // Op: the queries' type, E8: 8-bit cache, DT: channels (a multiple of 64, dim or more),
@@ -30,11 +59,16 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
   using Pv = typename std::conditional<E8, OpBF16, Op>::type;
   constexpr int TR = 32 * QT * AW_NW;
   constexpr int ESZ = E8 ? 1 : 2, EPC = 16 / ESZ;         // the cache's elements, and those of a 16-byte chunk
+  // 16-bit tiles go to LDS as they lie, without registers; 8-bit ones and padded rows
+  // through registers
+  constexpr bool DIRECT = FULL && !E8;
   constexpr int KC = DT / EPC, VC = AT_BLK / EPC;         // chunks of a key's and of a channel's row
   constexpr int NK = AT_BLK * KC / AW_NT, NV = DT * VC / AW_NT;   // chunks of a thread
-  constexpr int KS = 2 * DT + 16, VS = 2 * AT_BLK + 16;   // LDS row strides in bytes
+  constexpr int PAD = DIRECT ? 0 : 16;
+  constexpr int KS = 2 * DT + PAD, VS = 2 * AT_BLK + PAD;   // LDS row strides in bytes
   constexpr int KB = AT_BLK * KS, VB = DT * VS, SB = E8 ? 2 * AT_BLK * 4 : 0;
   constexpr int BUF = KB + VB + SB;
+  static_assert(aw_lds(DT, E8, FULL) == 2 * BUF, "the launch's LDS");
   constexpr int KSTEPS = DT / 16, DM = DT / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ int flags[2];   // of the steps' turns: 1 << sub-block: no page, 16: a value that is not finite
@@ -112,6 +146,62 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
   uint4 kr[NK], vr[NV];
   float skr = 0.0f;   // a key's scale, or its values'
   int bad = 0;
+  // DIRECT: the loads of a step into its turn's tiles.  A wave's load fills 64 chunks:
+  // keys (or channels) of whole rows.
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
+  const int wu = __builtin_amdgcn_readfirstlane(w);
+  uint32_t koff[DIRECT ? NK : 1], voff[DIRECT ? NV : 1];
+  if constexpr (DIRECT) {
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      const int row = (64 * (AW_NW * n + w) + lane) / KC;
+      koff[n] = 2 * (row * DT) + 16 * ((lane % KC) ^ aw_swap<KS>(row));
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int d = (64 * (AW_NW * n + w) + lane) / VC;
+      voff[n] = 2 * static_cast<uint32_t>(d * static_cast<int>(S)) + 16 * ((lane % VC) ^ aw_swap<VS>(d));
+    }
+  }
+  auto load = [&](int i, int turn) {
+    const int t0 = v.key(i);
+    const uint32_t to = lds + turn * BUF;
+    bad = (page0 < 0 ? 1 : 0) | (page1 < 0 ? 2 : 0) | (page2 < 0 ? 4 : 0) | (page3 < 0 ? 8 : 0);
+    const auto klds = [&](int n) { return to + 1024 * (AW_NW * n + wu); };
+    const auto vlds = [&](int n) { return to + KB + 1024 * (AW_NW * n + wu); };
+    if (S >= AT_BLK) {   // (one page for all; its tokens side by side)
+      const char* ks = kbase + max(page0, 0) * pstride + 2 * (t0 & mask) * DT;
+#pragma unroll
+      for (int n = 0; n < NK; ++n) aw_load_lds(ks, koff[n], klds(n));
+      const char* vs = vbase + max(page0, 0) * pstride + 2 * (t0 & mask);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) aw_load_lds(vs, voff[n], vlds(n));
+    } else {
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        const int u = 64 * (AW_NW * n + wu) / KC / 16;   // the rows' sub-block
+        aw_load_lds(kbase + pick(u) * pstride + 2 * (((t0 + 16 * u) & mask) - 16 * u) * DT, koff[n], klds(n));
+      }
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int d = (64 * (AW_NW * n + w) + lane) / VC, t = 8 * ((lane % VC) ^ aw_swap<VS>(d));
+        aw_load_lds(vbase + pick(t >> 4) * pstride + 2 * (d * static_cast<int>(S) + ((t0 + t) & mask)), vlds(n));
+      }
+    }
+  };
+  // ... and, once they are there, what stage() does for a step with masks
+  auto settle_tile = [&](int turn) {
+    char* vb = smem + turn * BUF + KB;
+    uint32_t odd = 0;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {   // (the chunks that this lane loaded)
+      char* at = vb + 1024 * (AW_NW * n + w) + 16 * lane;
+      const uint4 x = ld16(at);
+      odd |= not_finite<Pv>(x);
+      st16(at, finite_or_0<Pv>(x));
+    }
+    if (__any(odd != 0) && lane == 0) atomicOr(&flags[turn], 16);
+  };
   auto fetch = [&](int i) {
     const int t0 = v.key(i);
     bad = (page0 < 0 ? 1 : 0) | (page1 < 0 ? 2 : 0) | (page2 < 0 ? 4 : 0) | (page3 < 0 ? 8 : 0);
@@ -197,7 +287,8 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
   if (tid < 2) flags[tid] = 0;
   if (b0 < b1) {
     look(b0);
-    fetch(b0);
+    if constexpr (DIRECT) load(b0, 0);
+    else fetch(b0);
     if (b0 + 1 < b1) look(b0 + 1);
   }
   __syncthreads();
@@ -205,10 +296,20 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
     const int turn = (i - b0) & 1;
     const int t0 = v.key(i);
     const bool whole = v.whole(t0);
-    stage(turn, whole);
-    if (i + 1 < b1) fetch(i + 1);
-    if (i + 2 < b1) look(i + 2);
-    lds_barrier();
+    if constexpr (DIRECT) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (!whole) settle_tile(turn);
+      if (bad != 0 && tid == 0) atomicOr(&flags[turn], bad);
+      lds_barrier();
+      // (all waves are done with the other turn's tiles)
+      if (i + 1 < b1) load(i + 1, turn ^ 1);
+      if (i + 2 < b1) look(i + 2);
+    } else {
+      stage(turn, whole);
+      if (i + 1 < b1) fetch(i + 1);
+      if (i + 2 < b1) look(i + 2);
+      lds_barrier();
+    }
     const char* kb = smem + turn * BUF;
     const char* vb = kb + KB;
     const int fl = flags[turn];
@@ -226,7 +327,8 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
         for (int e = 0; e < 16; ++e) st[t][kt][e] = 0.0f;
 #pragma unroll
       for (int ks = 0; ks < KSTEPS; ++ks) {
-        const uint4 kf = ld16(kb + (32 * kt + krow) * KS + 32 * ks + 16 * hh);
+        const int chunk = DIRECT ? (2 * ks + hh) ^ aw_swap<KS>(krow) : 2 * ks + hh;   // (32 more rows change nothing)
+        const uint4 kf = ld16(kb + (32 * kt + krow) * KS + 16 * chunk);
 #pragma unroll
         for (int t = 0; t < QT; ++t) st[t][kt] = Op::mfma32(kf, q[t][ks], st[t][kt]);
       }
@@ -318,7 +420,8 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
     for (int dm = 0; dm < DM; ++dm)
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const uint4 vf = ld16(vb + (32 * dm + c) * VS + 32 * u + 16 * hh);
+        const int chunk = DIRECT ? (2 * u + hh) ^ aw_swap<VS>(c) : 2 * u + hh;
+        const uint4 vf = ld16(vb + (32 * dm + c) * VS + 16 * chunk);
 #pragma unroll
         for (int t = 0; t < QT; ++t) o[t][dm] = Pv::mfma32(vf, pf[t][u], o[t][dm]);
       }
@@ -408,7 +511,7 @@ namespace {
 template <class Op, bool E8, int DT, bool FULL>
 hipError_t aw_launch(const fl_attn_args& a, const AttnPlan& p, hipStream_t s) {
   constexpr int QT = ATTN_WIDE_QT;
-  constexpr int LDS = 2 * (AT_BLK * (2 * DT + 16) + DT * (2 * AT_BLK + 16) + (E8 ? 2 * AT_BLK * 4 : 0));
+  constexpr int LDS = aw_lds(DT, E8, FULL);
   if (LDS > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attn_wide<Op, E8, DT, FULL, QT>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
