@@ -51,6 +51,19 @@ __device__ __forceinline__ void aw_load_lds(const char* src, uint32_t lds) {   /
 
 }  // namespace
 
+// The order of n matrix instructions with an LDS read each: the reads AW_AHEAD before
+// (left to itself, the compiler reads, waits and multiplies in turn).
+constexpr int AW_AHEAD = 6;
+template <int N>
+__device__ __forceinline__ void aw_reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AW_AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+}
+
 // Op: the queries' type, E8: 8-bit cache, DT: channels (a multiple of 64, dim or more),
 // FULL: dim == DT, QT: tiles of 32 rows of a wave.
 template <class Op, bool E8, int DT, bool FULL, int QT>
@@ -333,6 +346,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
         for (int t = 0; t < QT; ++t) st[t][kt] = Op::mfma32(kf, q[t][ks], st[t][kt]);
       }
     }
+    aw_reads_ahead<2 * KSTEPS>();
 
     // -------------------------------------------------- the weights
     // (value e of a tile: key 16 (e / 8) + 8 hh + e % 8)
@@ -347,7 +361,6 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
           for (int t = 0; t < QT; ++t) st[t][kt][e] *= f;
         }
     }
-    uint4 pf[QT][4];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       if (a.softcap > 0.0f) {
@@ -384,47 +397,63 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[t][dm][e] *= f;
       }
-      const float mm = m[t] == -INFINITY ? 0.0f : m[t];
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(st[t][kt][e], to2, -mm));
-          l[t] += x;
-          st[t][kt][e] = x;
-        }
     }
-    if constexpr (E8) {
-      const float* sv = reinterpret_cast<const float*>(vb + VB) + AT_BLK;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float f = sv[32 * kt + 16 * (e >> 3) + 8 * hh + (e & 7)];
-#pragma unroll
-          for (int t = 0; t < QT; ++t) st[t][kt][e] *= f;
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < QT; ++t)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const f32x16& x = st[t][u >> 1];
-        const int e = 8 * (u & 1);
-        pf[t][u] = make_uint4(Pv::pack(x[e], x[e + 1]), Pv::pack(x[e + 2], x[e + 3]), Pv::pack(x[e + 4], x[e + 5]),
-                              Pv::pack(x[e + 6], x[e + 7]));
-      }
 
     // -------------------------------------------------- O^T += V^T P^T
+    // 16 keys a time: the next 16's weights and values beside this 16's products
+    uint4 pf[QT][4], vf[2][DM];
+    const auto weights = [&](int u) {
+      const int kt = u >> 1, e0 = 8 * (u & 1);
+      float x[QT][8];
 #pragma unroll
-    for (int dm = 0; dm < DM; ++dm)
+      for (int t = 0; t < QT; ++t) {
+        const float mm = m[t] == -INFINITY ? 0.0f : m[t];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int chunk = DIRECT ? (2 * u + hh) ^ aw_swap<VS>(c) : 2 * u + hh;
-        const uint4 vf = ld16(vb + (32 * dm + c) * VS + 16 * chunk);
-#pragma unroll
-        for (int t = 0; t < QT; ++t) o[t][dm] = Pv::mfma32(vf, pf[t][u], o[t][dm]);
+        for (int e = 0; e < 8; ++e) {
+          x[t][e] = __builtin_amdgcn_exp2f(fmaf(st[t][kt][e0 + e], to2, -mm));
+          l[t] += x[t][e];
+        }
       }
+      if constexpr (E8) {   // (the values' scales)
+        const float* sv = reinterpret_cast<const float*>(vb + VB) + AT_BLK + 16 * u + 8 * hh;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int t = 0; t < QT; ++t) x[t][e] *= sv[e];
+      }
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+        pf[t][u] = make_uint4(Pv::pack(x[t][0], x[t][1]), Pv::pack(x[t][2], x[t][3]), Pv::pack(x[t][4], x[t][5]),
+                              Pv::pack(x[t][6], x[t][7]));
+    };
+    const auto values = [&](int u) {
+#pragma unroll
+      for (int dm = 0; dm < DM; ++dm) {
+        const int chunk = DIRECT ? (2 * u + hh) ^ aw_swap<VS>(c) : 2 * u + hh;
+        vf[u & 1][dm] = ld16(vb + (32 * dm + c) * VS + 16 * chunk);
+      }
+    };
+    values(0);
+    weights(0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (u < 3) values(u + 1);
+#pragma unroll
+      for (int dm = 0; dm < DM; ++dm)
+#pragma unroll
+        for (int t = 0; t < QT; ++t) o[t][dm] = Pv::mfma32(vf[u & 1][dm], pf[t][u], o[t][dm]);
+      if (u < 3) {
+        weights(u + 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, DM, 0);
+#pragma unroll
+        for (int i = 0; i < DM * QT; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 36 / DM, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
 
     if (fl & 16) {   // (the same for all waves)
       float* wl = reinterpret_cast<float*>(smem + turn * BUF) + w * 16 * 32;   // in the keys' place: [16 keys][32 rows]
