@@ -166,8 +166,8 @@ def cache_read(cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, to
     sequence's newest tokens, named as for ``cache_write`` (all of a sequence's where
     ``starts`` gives it as many rows as it has tokens), in ``dtype`` (the cache's, or
     float32 for 8 bits): exact but for one rounding to a 16-bit ``dtype`` of values
-    outside its range.  Into ``out`` (contiguous) where given; else rows behind the
-    last sequence are zeros.  One launch."""
+    outside its range.  Into ``out`` (contiguous) where given (rows behind the
+    last sequence stay as they were; without ``out`` they hold anything).  One launch."""
     _check_cache(cache)
     if out is not None:
         dtype = out[0].dtype
@@ -180,8 +180,7 @@ def cache_read(cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, to
     _check_tokens(cache, table, lengths, starts, tokens)
     shape = (tokens, cache.heads, cache.dim)
     if out is None:
-        make = torch.empty if starts is None else torch.zeros
-        out = tuple(make(shape, dtype=dtype, device=cache.device) for _ in range(2))
+        out = tuple(torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
     elif any(t.shape != shape or t.dtype != dtype or t.device != cache.device or not t.is_contiguous() for t in out):
         raise ValueError(f"out must be two contiguous {dtype} tensors {shape} on {cache.device}")
     _lib.autograd().cache_call(cache.k, cache.v, cache.k_scale, cache.v_scale, out[0], out[1], table, lengths, starts, False)

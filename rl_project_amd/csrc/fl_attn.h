@@ -36,10 +36,12 @@ struct OpBF16 {
   __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, x2));
   }
-  // 4 e4m3 values as two dwords: exact (both types hold every e4m3 value)
-  __device__ static __forceinline__ uint2 widen(uint32_t q) {
-    return make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, 1.0f, false)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, 1.0f, true)));
+  // 4 e4m3 values, times a power of two, as two dwords: exact (both types hold every
+  // e4m3 value, bfloat16 also times any scale of a cache)
+  static constexpr bool SCALES = true;
+  __device__ static __forceinline__ uint2 widen(uint32_t q, float f = 1.0f) {
+    return make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, f, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, f, true)));
   }
 };
 struct OpF16 {
@@ -56,9 +58,10 @@ struct OpF16 {
   __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, x2));
   }
-  __device__ static __forceinline__ uint2 widen(uint32_t q) {
-    return make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q, 1.0f, false)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q, 1.0f, true)));
+  static constexpr bool SCALES = false;   // (of scales below 2^-14 half precision loses bits, of some above 2^7 all)
+  __device__ static __forceinline__ uint2 widen(uint32_t q, float f = 1.0f) {
+    return make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q, f, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q, f, true)));
   }
 };
 

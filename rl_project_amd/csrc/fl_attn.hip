@@ -68,7 +68,8 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
   constexpr int KS = DT / 32;   // steps of the first product
   constexpr int DM = DT / 16;   // tiles of channels of the second
   // tiles of values that are loaded ahead of their step's softmax: what registers hold
-  constexpr int VPRE = DM * C::SUBS * CT <= 16 ? DM : DM / 2;
+  constexpr bool ALL = DT * CT * C::ESZ <= 256;   // a step's keys beside its values
+  constexpr int VPRE = ALL || DM * C::SUBS * CT <= 16 ? DM : DM / 2;
   constexpr int TR = 16 * CT;
   // the waves' results side by side; before that, weights where values are not finite
   constexpr int OS = DT + 4;
@@ -153,49 +154,46 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
     if constexpr (C::SUBS == 2) some_bad |= bad[1];
     if (i + AR_NW < b1) pages(i + AR_NW);
     f32x4 st[CT][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    constexpr int KR = C::E8 ? KS / 2 : KS;   // loads of a tile's key
+    const auto keys = [&](int j, uint4(&x)[KR]) {
       const char* kr = kp[C::SUBS == 2 ? j >> 1 : 0] + C::ESZ * static_cast<int64_t>(dim) * (C::SUBS == 2 ? (j & 1) * 4 : j * 4);
-      uint4 kf[KS];
-      if constexpr (C::E8) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ks += 2) {
-          const int d = C::chan(g, ks);
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if constexpr (FULL) x = ld16(kr + d);
-          else if (d + 16 <= dim) x = ar_load16_8(kr + d);
+      for (int n = 0; n < KR; ++n) {
+        const int d = C::chan(g, C::E8 ? 2 * n : n);
+        if constexpr (FULL) x[n] = ld16(kr + C::ESZ * d);
+        else if constexpr (C::E8) {
+          x[n] = make_uint4(0, 0, 0, 0);
+          if (d + 16 <= dim) x[n] = ar_load16_8(kr + d);
           else if (d < dim) {
             const uint2 y = *reinterpret_cast<const uint2*>(kr + d);
-            x.x = y.x, x.y = y.y;
+            x[n] = make_uint4(y.x, y.y, 0, 0);
           }
-          const uint2 y0 = Op::widen(x.x), y1 = Op::widen(x.y), y2 = Op::widen(x.z), y3 = Op::widen(x.w);
-          kf[ks] = make_uint4(y0.x, y0.y, y1.x, y1.y);
-          kf[ks + 1] = make_uint4(y2.x, y2.y, y3.x, y3.y);
-        }
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const int d = C::chan(g, ks);
-          kf[ks] = FULL || d < dim ? ld16(kr + 2 * d) : make_uint4(0, 0, 0, 0);
-        }
+        } else x[n] = d < dim ? ld16(kr + 2 * d) : make_uint4(0, 0, 0, 0);
       }
+    };
+    const auto scores = [&](int j, const uint4(&x)[KR]) {
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        st[ct][j] = (f32x4){0, 0, 0, 0};
+      for (int ct = 0; ct < CT; ++ct) st[ct][j] = (f32x4){0, 0, 0, 0};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) st[ct][j] = Op::mfma16(kf[ks], q[ct][ks], st[ct][j]);
+      for (int n = 0; n < KR; ++n) {
+        if constexpr (C::E8) {
+          const uint2 y0 = Op::widen(x[n].x), y1 = Op::widen(x[n].y), y2 = Op::widen(x[n].z), y3 = Op::widen(x[n].w);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            st[ct][j] = Op::mfma16(make_uint4(y0.x, y0.y, y1.x, y1.y), q[ct][2 * n], st[ct][j]);
+            st[ct][j] = Op::mfma16(make_uint4(y2.x, y2.y, y3.x, y3.y), q[ct][2 * n + 1], st[ct][j]);
+          }
+        } else
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) st[ct][j] = Op::mfma16(x[n], q[ct][n], st[ct][j]);
       }
-      // (a tile's keys, no more, where their registers are many)
-      if (DT * CT > 256) __builtin_amdgcn_sched_barrier(0);
-    }
-    // (the values' registers are the keys')
-    __builtin_amdgcn_sched_barrier(0);
-    // the values, on their way during the softmax (V^T: channel 16 dm + c, this lane's keys)
+    };
+    // the values (V^T: channel 16 dm + c, this lane's keys)
     uint4 vr[DM][C::SUBS];
     const char* vs[C::SUBS];
 #pragma unroll
     for (int u = 0; u < C::SUBS; ++u) vs[u] = V + vp[u] + C::ESZ * S * c;
-    auto values = [&](int dm) {
+    const auto values = [&](int dm) {
 #pragma unroll
       for (int u = 0; u < C::SUBS; ++u) {
         vr[dm][u] = FULL || 16 * dm + c < dim ? ld16(vs[u]) : make_uint4(0, 0, 0, 0);
@@ -203,8 +201,29 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
         asm("" : "+v"(vs[u]));   // (one address that moves, not one for every tile)
       }
     };
+    if constexpr (ALL) {   // all of a step on its way at once
+      uint4 x[4][KR];
 #pragma unroll
-    for (int dm = 0; dm < VPRE; ++dm) values(dm);
+      for (int j = 0; j < 4; ++j) keys(j, x[j]);
+#pragma unroll
+      for (int dm = 0; dm < DM; ++dm) values(dm);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) scores(j, x[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint4 x[KR];
+        keys(j, x);
+        scores(j, x);
+        // (a tile's keys, no more, where their registers are many)
+        if (DT * CT > 256) __builtin_amdgcn_sched_barrier(0);
+      }
+      // (the values' registers are the keys')
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int dm = 0; dm < VPRE; ++dm) values(dm);
+    }
 
     // ------------------------------------------------ the weights
     const bool masked = !v.whole(t0) || __any(some_bad);
@@ -401,41 +420,64 @@ const char* src = col + C::ESZ * (4 * g * S);
   }
 }
 
-// The parts of rows whose keys were split: a wave a row; few and many: the plans of
-// sequences of few rows and of many.
+// The parts of rows whose keys were split.  A work-group looks at `rb` rows (a thread
+// each), and joins those that have parts: `tpr` threads a part (4 channels each), its
+// groups different parts.  few and many: the plans of sequences of few rows and of many.
+constexpr int AJ_ROWS = 64;
 template <class Op>
-__global__ __launch_bounds__(AR_NT) void k_attn_join(const fl_attn_args a, const AttnPlan few, const AttnPlan many) {
+__global__ __launch_bounds__(AR_NT) void k_attn_join(const fl_attn_args a, const AttnPlan few, const AttnPlan many, int tpr, int rb) {
+  __shared__ f32x4 sy[AR_NT];
+  __shared__ int parts[AJ_ROWS];
   const int lane = threadIdx.x & (WAVE - 1), dim = static_cast<int>(a.cache.dim), heads = static_cast<int>(a.q_heads);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * AR_NW + threadIdx.x / WAVE;
-  if (row >= a.rows.tokens * heads) return;
-  const int n = static_cast<int>(row / heads), head = static_cast<int>(row - static_cast<int64_t>(n) * heads);
   const int seqs = static_cast<int>(a.rows.seqs);
-  const PagedSeq s = paged_rows(a.rows, a.rows.starts == nullptr ? n / static_cast<int>(a.rows.tokens / seqs)
-                                                                 : paged_find(seqs, n, [&](int m) { return a.rows.starts[m]; }));
-  const int i = n - static_cast<int>(s.row);
-  if (i < 0 || i >= s.n) return;   // (a row behind the last sequence)
-  const AttnPlan& p = s.n * few.group <= few.max_rows ? few : many;
-  const AttnSpan v = attn_span(a, p, s, (i * p.group + head % p.group) / p.tr);
-  if (v.splits <= 1) return;
-  static_assert(AT_MAX_SPLITS <= WAVE, "a lane for every part");
-  float2 st = make_float2(-INFINITY, 0.0f);
-  if (lane < v.splits) st = *reinterpret_cast<const float2*>(p.stat + 2 * (row * p.stride + lane));
-  const float m = wave_reduce(st.x, OpMax());
-  const float f = st.x == -INFINITY ? (st.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(st.x - m);
-  const float l = wave_reduce(st.y * f, OpAdd());
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  if (lane == 0 && a.out_lse) a.out_lse[row] = l == 0.0f ? -INFINITY : (m == -INFINITY ? l : (m + log2f(l)) * 0.6931471805599453f);
-  f32x4 y = {0, 0, 0, 0};
-  const float* part = p.part + row * p.stride * dim + 4 * lane;
-#pragma unroll 4
-  for (int k = 0; k < v.splits; ++k) {
-    const float x = __shfl(f, k, WAVE);
-    if (4 * lane < dim && x != 0.0f) y += x * *reinterpret_cast<const f32x4*>(part + static_cast<int64_t>(k) * dim);
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rb;
+  if (threadIdx.x < rb) {
+    const int64_t row = row0 + threadIdx.x;
+    int splits = 0;
+    if (row < a.rows.tokens * heads) {
+      const int n = static_cast<int>(row / heads), head = static_cast<int>(row - static_cast<int64_t>(n) * heads);
+      const PagedSeq s = paged_rows(a.rows, a.rows.starts == nullptr ? n / (static_cast<int>(a.rows.tokens) / seqs)
+                                                                     : paged_find(seqs, n, [&](int m) { return a.rows.starts[m]; }));
+      const int i = n - static_cast<int>(s.row);
+      if (i >= 0 && i < s.n) {   // (else a row behind the last sequence)
+        const AttnPlan& p = s.n * few.group <= few.max_rows ? few : many;
+        splits = attn_span(a, p, s, (i * p.group + head % p.group) / p.tr).splits;
+      }
+    }
+    parts[threadIdx.x] = splits;
   }
-  if (4 * lane < dim) {
-    y *= inv;
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (s.row + i) * a.out_ld + head * a.out_hs + 4 * lane) =
-        make_uint2(Op::pack(y[0], y[1]), Op::pack(y[2], y[3]));
+  __syncthreads();
+  static_assert(AT_MAX_SPLITS <= WAVE, "a lane for every part");
+  const int g = threadIdx.x / tpr, d = 4 * (threadIdx.x & (tpr - 1)), groups = AR_NT / tpr;
+#pragma unroll 1
+  for (int j = 0; j < rb; ++j) {
+    const int splits = parts[j];
+    if (splits <= 1) continue;
+    const int64_t row = row0 + j, n = row / heads, head = row - n * heads;
+    // (every wave for itself)
+    float2 st = make_float2(-INFINITY, 0.0f);
+    if (lane < splits) st = *reinterpret_cast<const float2*>(few.stat + 2 * (row * few.stride + lane));
+    const float m = wave_reduce(st.x, OpMax());
+    const float f = st.x == -INFINITY ? (st.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(st.x - m);
+    const float l = wave_reduce(st.y * f, OpAdd());
+    if (threadIdx.x == 0 && a.out_lse)
+      a.out_lse[row] = l == 0.0f ? -INFINITY : (m == -INFINITY ? l : (m + log2f(l)) * 0.6931471805599453f);
+    f32x4 y = {0, 0, 0, 0};
+    const float* part = few.part + row * few.stride * dim + d;
+    for (int k0 = 0; k0 < splits; k0 += groups) {   // (the same turns for all lanes: they exchange)
+      const int k = k0 + g;
+      const float x = __shfl(f, k, WAVE);
+      if (k < splits && d < dim && x != 0.0f) y += x * *reinterpret_cast<const f32x4*>(part + static_cast<int64_t>(k) * dim);
+    }
+    sy[threadIdx.x] = y;
+    __syncthreads();
+    if (g == 0 && d < dim) {
+      for (int k = 1; k < groups; ++k) y += sy[k * tpr + threadIdx.x];
+      y *= l == 0.0f ? 0.0f : 1.0f / l;
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + n * a.out_ld + head * a.out_hs + d) =
+          make_uint2(Op::pack(y[0], y[1]), Op::pack(y[2], y[3]));
+    }
+    __syncthreads();
   }
 }
 
@@ -474,15 +516,17 @@ AttnCall attn_call(const fl_attn_args& a) {
   c.has_few = a.rows.starts || top <= ATTN_FEW_ROWS;
   c.has_many = top > ATTN_FEW_ROWS;
   const int64_t keys = a.rows.table_width * a.cache.page_size;
-  // Splits: enough that every CU has `work` / 256 work-groups, none shorter than 4
-  // steps of 64 keys of the longest sequence the table (or the window) allows.
-  const auto plan = [&](AttnPlan& p, int tr, int64_t groups, int64_t work) {
+  // Splits: enough that every CU has `work` / 256 work-groups, and `least` of them, so
+  // that long and short sequences share the CUs evenly (64 sequences of 1024 to 8192
+  // tokens: 2 splits 269 us, 4 243 us, 8 262 us); none shorter than 4 steps of 64 keys
+  // of the longest sequence the table (or the window) allows.
+  const auto plan = [&](AttnPlan& p, int tr, int64_t groups, int64_t work, int64_t least) {
     p.group = static_cast<int>(G);
     p.tr = tr;
     p.tiles = paged_tiles(a.rows, G, tr, 1, p.each);
     const int64_t seen = a.window > 0 && a.window <= keys
                              ? std::min(keys, a.window + tr / G + std::min(a.sinks, keys) + 3 * AT_BLK) : keys;
-    const int64_t blocks = (seen + AT_BLK - 1) / AT_BLK, want = (work + groups - 1) / groups;
+    const int64_t blocks = (seen + AT_BLK - 1) / AT_BLK, want = std::max(least, (work + groups - 1) / groups);
     p.splits = static_cast<int>(std::max<int64_t>(
         1, std::min({want, (blocks + AT_MIN_BLKS - 1) / AT_MIN_BLKS, static_cast<int64_t>(AT_MAX_SPLITS)})));
     c.stride = std::max<int64_t>(c.stride, p.splits > 1 ? p.splits : 0);
@@ -493,13 +537,13 @@ AttnCall attn_call(const fl_attn_args& a) {
     const int tr = (a.rows.starts ? N * G <= 16 * B : top <= 16) ? 16 : 32;
     c.few.min_rows = 0, c.few.max_rows = ATTN_FEW_ROWS;
     c.few.each = static_cast<int>((rows + tr - 1) / tr);
-    plan(c.few, tr, B * Hk, 1024);
+    plan(c.few, tr, B * Hk, 1024, 4);
   }
   if (c.has_many) {
     c.many.min_rows = c.has_few ? ATTN_FEW_ROWS + 1 : 0, c.many.max_rows = 0x7fffffff;
     c.many.each = a.rows.starts ? 0 : static_cast<int>((top + ATTN_WIDE_ROWS - 1) / ATTN_WIDE_ROWS);
     const int64_t tiles = a.rows.starts ? std::max<int64_t>((N - B) * G / ATTN_WIDE_ROWS, 1) : B * c.many.each;
-    plan(c.many, ATTN_WIDE_ROWS, tiles * Hk, 512);
+    plan(c.many, ATTN_WIDE_ROWS, tiles * Hk, 512, 1);
   }
   if (!c.has_few) c.few.group = 1, c.few.max_rows = 0;
   return c;
@@ -517,7 +561,8 @@ size_t attn_workspace_bytes(const fl_attn_args& a) {
 int64_t attn_blocks(const fl_attn_args& a) {
   if (attn_rows(a) == 0) return 0;
   const AttnCall c = attn_call(a);
-  return std::max({c.few.tiles * c.few.splits * a.cache.heads, c.many.tiles * c.many.splits * a.cache.heads, attn_rows(a) / AR_NW + 1});
+  return std::max({c.few.tiles * c.few.splits * a.cache.heads, c.many.tiles * c.many.splits * a.cache.heads,
+                   c.stride > 0 ? std::max<int64_t>(attn_rows(a) / AJ_ROWS, std::min<int64_t>(attn_rows(a), 16384)) + 1 : 0});
 }
 
 hipError_t launch_attn(const fl_attn_args& args, hipStream_t s) {
@@ -539,9 +584,12 @@ hipError_t launch_attn(const fl_attn_args& args, hipStream_t s) {
     else bf ? ar_dims<Cache16<OpBF16>>(a, c.few, s) : ar_dims<Cache16<OpF16>>(a, c.few, s);
   }
   if (c.stride > 0) {
-    const dim3 grid(static_cast<unsigned>((attn_rows(a) + AR_NW - 1) / AR_NW));
-    if (bf) hipLaunchKernelGGL(k_attn_join<OpBF16>, grid, dim3(AR_NT), 0, s, a, c.few, c.many);
-    else hipLaunchKernelGGL(k_attn_join<OpF16>, grid, dim3(AR_NT), 0, s, a, c.few, c.many);
+    // (a row a work-group where that fills the card: most rows of a prompt have no parts)
+    const int64_t n = attn_rows(a), rb = std::max<int64_t>(1, std::min<int64_t>(n / 8192, AJ_ROWS));
+    const dim3 grid(static_cast<unsigned>((n + rb - 1) / rb));
+    const int tpr = a.cache.dim <= 64 ? 16 : a.cache.dim <= 128 ? 32 : 64;
+    if (bf) hipLaunchKernelGGL(k_attn_join<OpBF16>, grid, dim3(AR_NT), 0, s, a, c.few, c.many, tpr, static_cast<int>(rb));
+    else hipLaunchKernelGGL(k_attn_join<OpF16>, grid, dim3(AR_NT), 0, s, a, c.few, c.many, tpr, static_cast<int>(rb));
   }
   return hipGetLastError();
 }

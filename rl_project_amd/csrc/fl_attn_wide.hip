@@ -157,7 +157,11 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
     return max(u & 2 ? hi : lo, 0);
   };
   uint4 kr[NK], vr[NV];
-  float skr = 0.0f;   // a key's scale, or its values'
+  // 8-bit: a key's scale goes to its values where they are widened, if their type takes
+  // it, else to its scores; the values' to the weights
+  constexpr bool KSCALE = E8 && Op::SCALES;
+  // (codes: nothing waits for them before they are staged)
+  uint32_t ks8[KSCALE ? NK : 1], sc8 = 0;
   int bad = 0;
   // DIRECT: the loads of a step into its turn's tiles.  A wave's load fills 64 chunks:
   // keys (or channels) of whole rows.
@@ -225,6 +229,8 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
       const int row = tid / KC + STEP * n, d = tid % KC * EPC;
       const int u = STEP <= 16 ? STEP * n / 16 : STEP / 16 * n + tid / (16 * KC);
       const char* src = kbase + pick(u) * pstride + ESZ * ((((t0 + 16 * u) & mask) + (row & 15)) * dim + d);
+      if constexpr (KSCALE)
+        ks8[n] = a.cache.k_scale[(static_cast<int64_t>(pick(u)) * Hk + h) * S + ((t0 + 16 * u) & mask) + (row & 15)];
       if constexpr (FULL) kr[n] = ld16(src);
       else {
         kr[n] = make_uint4(0, 0, 0, 0);
@@ -254,7 +260,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
       if (tid < 2 * AT_BLK) {
         const int t = tid & (AT_BLK - 1);
         const uint8_t* src = tid < AT_BLK ? a.cache.k_scale : a.cache.v_scale;
-        skr = scale_of(src[(static_cast<int64_t>(pick(t >> 4)) * Hk + h) * S + ((t0 + t) & mask)]);
+        sc8 = src[(static_cast<int64_t>(pick(t >> 4)) * Hk + h) * S + ((t0 + t) & mask)];
       }
     }
   };
@@ -266,7 +272,8 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
       const int id = tid + AW_NT * n, row = id / KC;
       char* dst = buf + row * KS + id % KC * EPC * 2;
       if constexpr (E8) {
-        const uint2 y0 = Op::widen(kr[n].x), y1 = Op::widen(kr[n].y), y2 = Op::widen(kr[n].z), y3 = Op::widen(kr[n].w);
+        const float f = KSCALE ? scale_of(ks8[KSCALE ? n : 0]) : 1.0f;
+        const uint2 y0 = Op::widen(kr[n].x, f), y1 = Op::widen(kr[n].y, f), y2 = Op::widen(kr[n].z, f), y3 = Op::widen(kr[n].w, f);
         st16(dst, make_uint4(y0.x, y0.y, y1.x, y1.y));
         st16(dst + 16, make_uint4(y2.x, y2.y, y3.x, y3.y));
       } else st16(dst, kr[n]);
@@ -292,7 +299,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
       } else put(dst, vr[n]);
     }
     if constexpr (E8)
-      if (tid < 2 * AT_BLK) reinterpret_cast<float*>(buf + KB + VB)[tid] = skr;
+      if (tid < 2 * AT_BLK) reinterpret_cast<float*>(buf + KB + VB)[tid] = scale_of(sc8);
     if (!whole && __any(odd != 0) && lane == 0) atomicOr(&flags[turn], 16);
     if (bad != 0 && tid == 0) atomicOr(&flags[turn], bad);
   };
@@ -350,7 +357,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
 
     // -------------------------------------------------- the weights
     // (value e of a tile: key 16 (e / 8) + 8 hh + e % 8)
-    if constexpr (E8) {
+    if constexpr (E8 && !KSCALE) {
       const float* sk = reinterpret_cast<const float*>(vb + VB);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)

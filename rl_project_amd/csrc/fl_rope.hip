@@ -167,8 +167,6 @@ __device__ __forceinline__ RpRow rp_row(const fl_rope_args& a) {
 
 }  // namespace
 
-// GRAD false: out = forward(q, k); true: dq, dk (out_q, out_k) and the partial sums
-// of the weights' gradients, [part][2][dim].
 template <class D, class W, bool VEC>
 __global__ __launch_bounds__(RP_NT) void k_rope(const fl_rope_args a, int L, int TK) {
   constexpr int N = RowChunk<D>::N;
@@ -210,92 +208,88 @@ __global__ __launch_bounds__(RP_NT) void k_rope(const fl_rope_args a, int L, int
   rows(a.k, a.k_ld, a.k_hs, static_cast<int>(a.kv_heads), a.k_weight, a.out_k);
 }
 
+// One side a work-group (blockIdx.y 0: queries, 1: keys): the sums of one weight's
+// gradient in registers.
 template <class D, class W, bool VEC>
-__global__ __launch_bounds__(RP_NT) void k_rope_grad(const fl_rope_grad_args b, int L, int TK) {
+__global__ __launch_bounds__(RP_NT, 4) void k_rope_grad(const fl_rope_grad_args b, int L, int TK) {
   constexpr int N = RowChunk<D>::N;
   const fl_rope_args& a = b.fwd;
   __shared__ float2 cs[1024];
   __shared__ float sum[RP_NT / WAVE][FL_ROPE_MAX_DIM];
+  const bool key = blockIdx.y != 0;
+  const int heads = static_cast<int>(key ? a.kv_heads : a.heads);
+  if (heads == 0) return;   // (nothing of this side is asked for)
+  const void* x = key ? a.k : a.q;
+  const void* grad = key ? b.grad_k : b.grad_q;
+  const int64_t ld = key ? a.k_ld : a.q_ld, hs = key ? a.k_hs : a.q_hs;
+  void* out = key ? a.out_k : a.out_q;
   const RpRow R = rp_row(a);
   const int p = (threadIdx.x & (L - 1)) * N, g = threadIdx.x / L, GR = RP_NT / L;
   const float inv = 1.0f / static_cast<float>(a.dim);
-  const bool weights = b.out_dwq != nullptr || b.out_dwk != nullptr;
-  float dq0[N], dq1[N], dk0[N], dk1[N];
+  float w0[N], w1[N], d0[N], d1[N];
+  rp_weights<W>(a.norm ? (key ? a.k_weight : a.q_weight) : nullptr, R, p, w0, w1);
 #pragma unroll
-  for (int e = 0; e < N; ++e) dq0[e] = dq1[e] = dk0[e] = dk1[e] = 0.0f;
+  for (int e = 0; e < N; ++e) d0[e] = d1[e] = 0.0f;
   for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * TK; t0 < a.tokens; t0 += static_cast<int64_t>(gridDim.x) * TK) {
     const int tk = static_cast<int>(min(static_cast<int64_t>(TK), a.tokens - t0));
     __syncthreads();   // (the last tokens' angles have been read)
     rp_turns(a, t0, tk, R.P, cs);
     __syncthreads();
-    auto rows = [&](const void* x, int64_t ld, int64_t hs, int heads, const void* w, const void* grad, void* out, float(&d0)[N],
-                    float(&d1)[N]) {
-      if (heads == 0) return;
-      float w0[N], w1[N];
-      rp_weights<W>(a.norm ? w : nullptr, R, p, w0, w1);
-      for (int i = g; i < tk * heads; i += GR) {
-        const int t = i / heads, h = i - t * heads;
-        const int64_t at = ((t0 + t) * heads + h) * a.dim;
-        float x0[N], x1[N], g0[N], g1[N], u0[N], u1[N];
-        if (grad != nullptr) rp_load<D, VEC>(rp_at<D>(grad, at), R, p, g0, g1);
-        else
+    for (int i = g; i < tk * heads; i += GR) {
+      const int t = i / heads, h = i - t * heads;
+      const int64_t at = ((t0 + t) * heads + h) * a.dim;
+      float x0[N], x1[N], g0[N], g1[N], u0[N], u1[N];
+      if (grad != nullptr) rp_load<D, VEC>(rp_at<D>(grad, at), R, p, g0, g1);
+      else
 #pragma unroll
-          for (int e = 0; e < N; ++e) g0[e] = g1[e] = 0.0f;
-        if (a.norm) rp_load<D, VEC>(rp_at<D>(x, (t0 + t) * ld + h * hs), R, p, x0, x1);
+        for (int e = 0; e < N; ++e) g0[e] = g1[e] = 0.0f;
+      if (a.norm) rp_load<D, VEC>(rp_at<D>(x, (t0 + t) * ld + h * hs), R, p, x0, x1);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float2 c = cs[t * R.P + min(p + e, R.P - 1)];
+        u0[e] = g0[e] * c.x + g1[e] * c.y;
+        u1[e] = g1[e] * c.x - g0[e] * c.y;
+      }
+      if (a.norm) {
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) s = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], s));
+        const float r = 1.0f / sqrtf(fmaf(rp_sum<N>(s, L), inv, a.eps));
+        float dot = 0.0f;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          const float2 c = cs[t * R.P + min(p + e, R.P - 1)];
-          u0[e] = g0[e] * c.x + g1[e] * c.y;
-          u1[e] = g1[e] * c.x - g0[e] * c.y;
+          x0[e] *= r, x1[e] *= r;
+          d0[e] = fmaf(u0[e], x0[e], d0[e]);
+          d1[e] = fmaf(u1[e], x1[e], d1[e]);
+          u0[e] *= w0[e], u1[e] *= w1[e];
+          dot = fmaf(u0[e], x0[e], fmaf(u1[e], x1[e], dot));
         }
-        if (a.norm) {
-          float s = 0.0f;
+        dot = rp_sum<N>(dot, L) * inv;
 #pragma unroll
-          for (int e = 0; e < N; ++e) s = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], s));
-          const float r = 1.0f / sqrtf(fmaf(rp_sum<N>(s, L), inv, a.eps));
-          float dot = 0.0f;
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            x0[e] *= r, x1[e] *= r;
-            d0[e] = fmaf(u0[e], x0[e], d0[e]);
-            d1[e] = fmaf(u1[e], x1[e], d1[e]);
-            u0[e] *= w0[e], u1[e] *= w1[e];
-            dot = fmaf(u0[e], x0[e], fmaf(u1[e], x1[e], dot));
-          }
-          dot = rp_sum<N>(dot, L) * inv;
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            u0[e] = r * (u0[e] - x0[e] * dot);
-            u1[e] = r * (u1[e] - x1[e] * dot);
-          }
+        for (int e = 0; e < N; ++e) {
+          u0[e] = r * (u0[e] - x0[e] * dot);
+          u1[e] = r * (u1[e] - x1[e] * dot);
         }
-        if (out != nullptr) rp_store<D, VEC>(rp_at<D>(out, at), R, p, u0, u1);
       }
-    };
-    rows(a.q, a.q_ld, a.q_hs, static_cast<int>(a.heads), a.q_weight, b.grad_q, a.out_q, dq0, dq1);
-    rows(a.k, a.k_ld, a.k_hs, static_cast<int>(a.kv_heads), a.k_weight, b.grad_k, a.out_k, dk0, dk1);
-  }
-  if (!weights) return;
-  // the row groups' sums: over a wave's by exchange, then over the waves
-  float* part = static_cast<float*>(b.workspace) + static_cast<int64_t>(blockIdx.x) * 2 * a.dim;
-  auto store = [&](float(&d0)[N], float(&d1)[N], int which) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      for (int m = L; m < WAVE; m <<= 1) {
-        d0[e] += shfl_xor(d0[e], m);
-        d1[e] += shfl_xor(d1[e], m);
-      }
-      if ((threadIdx.x & (WAVE - 1)) < L && p + e < R.P) {
-        sum[threadIdx.x / WAVE][R.first(p + e)] = d0[e];
-        sum[threadIdx.x / WAVE][R.second(p + e)] = d1[e];
-      }
+      if (out != nullptr) rp_store<D, VEC>(rp_at<D>(out, at), R, p, u0, u1);
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.dim; i += RP_NT) part[which * a.dim + i] = (sum[0][i] + sum[1][i]) + (sum[2][i] + sum[3][i]);
-    __syncthreads();
-  };
-  store(dq0, dq1, 0);
-  store(dk0, dk1, 1);
+  }
+  if ((key ? b.out_dwk : b.out_dwq) == nullptr) return;
+  // the row groups' sums: over a wave's by exchange, then over the waves
+  float* part = static_cast<float*>(b.workspace) + (static_cast<int64_t>(blockIdx.x) * 2 + blockIdx.y) * a.dim;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    for (int m = L; m < WAVE; m <<= 1) {
+      d0[e] += shfl_xor(d0[e], m);
+      d1[e] += shfl_xor(d1[e], m);
+    }
+    if ((threadIdx.x & (WAVE - 1)) < L && p + e < R.P) {
+      sum[threadIdx.x / WAVE][R.first(p + e)] = d0[e];
+      sum[threadIdx.x / WAVE][R.second(p + e)] = d1[e];
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.dim; i += RP_NT) part[i] = (sum[0][i] + sum[1][i]) + (sum[2][i] + sum[3][i]);
 }
 
 // The partial sums added: one work-group per 64 columns of dwq (blockIdx.y 0) or
@@ -385,8 +379,8 @@ hipError_t launch_rope_grad(const fl_rope_grad_args& b, hipStream_t s) {
     const int L = rp_lanes(a.dim, N), TK = rp_tokens(a.tokens);
     const int parts = static_cast<int>(rope_grad_parts(a.tokens));
     if (parts > 0) {
-      if (rp_vector(a, N, {b.grad_q, b.grad_k})) hipLaunchKernelGGL((k_rope_grad<D, W, true>), dim3(parts), dim3(RP_NT), 0, s, b, L, TK);
-      else hipLaunchKernelGGL((k_rope_grad<D, W, false>), dim3(parts), dim3(RP_NT), 0, s, b, L, TK);
+      if (rp_vector(a, N, {b.grad_q, b.grad_k})) hipLaunchKernelGGL((k_rope_grad<D, W, true>), dim3(parts, 2), dim3(RP_NT), 0, s, b, L, TK);
+      else hipLaunchKernelGGL((k_rope_grad<D, W, false>), dim3(parts, 2), dim3(RP_NT), 0, s, b, L, TK);
     }
     if (b.out_dwq || b.out_dwk)
       hipLaunchKernelGGL(k_rope_reduce<W>, dim3(static_cast<unsigned>((a.dim + WAVE - 1) / WAVE), 2), dim3(RP_RW * WAVE), 0, s, b,
