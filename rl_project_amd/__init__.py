@@ -31,6 +31,9 @@ qk_norm_rope, qk_norm_rope_backward, rotary_frequencies
 PagedCache, cache_write, cache_read, paged_attention
     A paged key / value cache (16 bits, or 8 with scales) and attention of a decode
     or verify step's, or a prompt's, new tokens over it.
+CacheGroup, CacheStep, CacheFull
+    A decode group's caches: pages, lengths and a step's new tokens for every layer;
+    ``SpeculativeGenerator`` verifies over one (``cache=``).
 SamplingParams
     Per-request parameters with the reference's validation (inference/requests.py).
 """
@@ -39,7 +42,7 @@ from .params import GenerationSettings, SamplingParams, SamplingParamsError
 from .sampling import (SampleOutput, SamplerPlan, SamplingError, apply_sampling_filters, describe_rows,
                        filtered_outputs, generate_tokens, sample_from_logits, sample_tokens)
 from .speculative import MTPSpeculativeGenerator, SpeculativeGenerator, SpecOutput, SpecPlan, speculative_verify
-from .engine import BatchedSampler
+from .engine import BatchedSampler, CacheFull, CacheGroup, CacheStep
 from .logprobs import RowStats, entropy_from_logits, kl_full_distribution, row_stats, token_logprobs_from_logits
 from .cache import PagedCache, cache_read, cache_write, paged_attention
 from .rotary import qk_norm_rope, qk_norm_rope_backward, rotary_frequencies
@@ -58,5 +61,6 @@ __all__ = [
     "lm_head_logprobs", "lm_head_logprobs_backward", "HeadScores",
     "lm_head_sample", "LmHeadPlan", "LmHeadOutput",
     "qk_norm_rope", "qk_norm_rope_backward", "rotary_frequencies",
+    "CacheGroup", "CacheStep", "CacheFull",
     "PagedCache", "cache_write", "cache_read", "paged_attention",
 ]

@@ -20,6 +20,10 @@ finished flags and appends the tokens to the histories (no host
 synchronisation, no other kernel). It returns device tensors; the caller
 reads them back once per step, not once per sequence. Length limits,
 cancellation and block allocation stay with the engine, as in the reference.
+
+``CacheGroup`` is the group's other state: its layers' keys and values in pages
+(the reference merges per-sequence caches each step, ``engine.py:146-150``, and
+accounts for blocks on the host, ``inference/paged_memory.py:22``).
 """
 
 from __future__ import annotations
@@ -28,6 +32,7 @@ from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 
 import torch
 
+from .cache import PagedCache, cache_write, paged_attention
 from .params import SamplingParams
 from . import _lib
 from .sampling import SampleOutput, _Call, _check_logits
@@ -163,3 +168,118 @@ class BatchedSampler:
     def history_of(self, slot: int) -> List[int]:
         """Prompt + generated ids of a slot (reads the device: for tests and retirement)."""
         return self.history[slot, : int(self.hist_len[slot])].tolist()
+
+
+class CacheFull(RuntimeError):
+    """No pages left for a step's new tokens (the step changed nothing)."""
+
+
+class CacheStep:
+    """The new tokens of one step over a ``CacheGroup``, as its layers take them:
+    rows ``starts[i]`` to ``starts[i + 1] - 1`` of a layer's tensors are slot ``slots[i]``'s,
+    oldest first; ``positions`` (int64 ``[tokens]``) are theirs, for ``qk_norm_rope``.
+    ``table``, ``lengths`` and ``starts`` (None where every slot has as many tokens) are
+    what ``cache_write`` and ``paged_attention`` take."""
+
+    __slots__ = ("layers", "slots", "counts", "tokens", "table", "lengths", "starts", "positions")
+
+    def __init__(self, layers, slots, counts, table, lengths, starts, positions):
+        self.layers, self.slots, self.counts = layers, slots, counts
+        self.tokens = sum(counts)
+        self.table, self.lengths, self.starts, self.positions = table, lengths, starts, positions
+
+    def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, **kw) -> torch.Tensor:
+        """A layer's attention of the step: its new keys and values into the cache, its
+        queries over all that the sequences have there (``paged_attention``'s keywords)."""
+        cache = self.layers[layer]
+        cache_write(cache, k, v, self.table, self.lengths, starts=self.starts)
+        return paged_attention(q, cache, self.table, self.lengths, starts=self.starts, **kw)
+
+
+class CacheGroup:
+    """The paged caches of up to ``max_rows`` sequences: one ``PagedCache`` per layer,
+    of one shape, whose pages all layers number alike.
+
+    ``step(slots, counts)`` makes room for each slot's new tokens (pages are taken as
+    they are needed) and names them for the layers; ``truncate`` takes a slot's newest
+    tokens back (rejected drafts) and ``release`` all of them.  Page numbers and lengths
+    live on the host; a step sends them in one copy."""
+
+    def __init__(self, layers: Sequence[PagedCache], max_rows: int, max_seq_len: int):
+        layers = list(layers)
+        if not layers or any(not isinstance(c, PagedCache) for c in layers):
+            raise TypeError("layers must be PagedCaches, one at least")
+        if any((c.pages, c.page_size, c.device) != (layers[0].pages, layers[0].page_size, layers[0].device) for c in layers):
+            raise ValueError("the layers' caches must have as many pages, of one size, on one device")
+        if max_rows < 1 or max_seq_len < 1:
+            raise ValueError("max_rows and max_seq_len must be at least 1")
+        self.layers = layers
+        self.max_rows, self.max_seq_len = max_rows, max_seq_len
+        self.page_size, self.device = layers[0].page_size, layers[0].device
+        self._free = list(range(layers[0].pages - 1, -1, -1))
+        self._pages: List[List[int]] = [[] for _ in range(max_rows)]
+        self._lens = [0] * max_rows
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, slot: int) -> int:
+        """Tokens that the slot has in the cache."""
+        return self._lens[slot]
+
+    def step(self, slots: Sequence[int], counts: Sequence[int]) -> CacheStep:
+        """Room for ``counts[i]`` new tokens of slot ``slots[i]`` (each slot once), which
+        count as cached from here on.  ``CacheFull`` where the pages do not suffice."""
+        slots, counts = [int(s) for s in slots], [int(c) for c in counts]
+        if not slots or len(slots) != len(counts) or len(set(slots)) != len(slots):
+            raise ValueError("slots must differ, with a count each, one at least")
+        if any(s < 0 or s >= self.max_rows for s in slots):
+            raise IndexError(f"a slot outside 0 .. {self.max_rows - 1}")
+        if any(c < 1 for c in counts):
+            raise ValueError("every slot of a step needs at least one new token")
+        need = []
+        for s, c in zip(slots, counts):
+            n = self._lens[s] + c
+            if n > self.max_seq_len:
+                raise ValueError(f"slot {s}: {n} tokens exceed max_seq_len {self.max_seq_len}")
+            need.append(-(-n // self.page_size) - len(self._pages[s]))
+        if sum(need) > len(self._free):
+            raise CacheFull(f"{sum(need)} pages needed, {len(self._free)} free")
+        for s, c, n in zip(slots, counts, need):
+            self._pages[s] += [self._free.pop() for _ in range(n)]
+            self._lens[s] += c
+        B, N = len(slots), sum(counts)
+        width = max(len(self._pages[s]) for s in slots)
+        flat: List[int] = []
+        for s in slots:
+            flat += self._pages[s] + [-1] * (width - len(self._pages[s]))
+        flat += [self._lens[s] for s in slots]
+        at = [0]
+        for c in counts:
+            at.append(at[-1] + c)
+        flat += at
+        sent = torch.tensor(flat, dtype=torch.int32).to(self.device)
+        table, lengths, starts = sent[: B * width].view(B, width), sent[B * width: B * width + B], sent[B * width + B:]
+        if len(set(counts)) == 1:
+            first = lengths.to(torch.int64) - counts[0]
+            positions = (first[:, None] + torch.arange(counts[0], device=self.device)).view(-1)
+            starts = None
+        else:
+            row = torch.repeat_interleave(torch.arange(B, device=self.device), torch.tensor(counts, device=self.device),
+                                          output_size=N)
+            positions = lengths.to(torch.int64)[row] - starts.to(torch.int64)[row + 1] + torch.arange(N, device=self.device)
+        return CacheStep(self.layers, slots, counts, table, lengths, starts, positions)
+
+    def truncate(self, slot: int, length: int) -> None:
+        """Keep the slot's first ``length`` tokens; pages without any are free again."""
+        if not 0 <= length <= self._lens[slot]:
+            raise ValueError(f"length {length} outside 0 .. {self._lens[slot]}")
+        keep = -(-length // self.page_size)
+        self._free += reversed(self._pages[slot][keep:])
+        del self._pages[slot][keep:]
+        self._lens[slot] = length
+
+    def release(self, slot: int) -> None:
+        """Free all of the slot's pages."""
+        self.truncate(slot, 0)

@@ -26,6 +26,7 @@ import torch
 
 from . import _lib
 from ._lib import SpecArgs, check, lib, ptr
+from .engine import CacheGroup
 from .sampling import FL_FLAG_NO_SELECT, _DTYPES, _Call, _check_logits, sample_tokens
 
 
@@ -204,12 +205,21 @@ class SpeculativeGenerator:
     ``trace``: a list that receives, per round, the active sequences and every
     draw and decision (for replay checks).  Models follow the reference
     protocol: ``model(idx) -> (logits [B, T, V], _)``,
-    ``model.full_logits(idx) -> [B, T, V]`` and ``model.spec.block_size``."""
+    ``model.full_logits(idx) -> [B, T, V]`` and ``model.spec.block_size``.
 
-    def __init__(self, target_model, draft_model, k: int = 5):
+    ``cache``: a ``CacheGroup`` for the target's keys and values (slots 0 to the number
+    of sequences - 1 are used and released).  The target then needs
+    ``model.paged_logits(tokens [N], step) -> [N, V]``, whose layers call
+    ``step.attend(layer, q, k, v)``: a round runs the target on each sequence's new
+    tokens alone, all sequences at once, instead of on their whole contexts, and takes
+    the rejected drafts' tokens back.  Contexts past the block size, which slide, use
+    ``full_logits``."""
+
+    def __init__(self, target_model, draft_model, k: int = 5, cache: Optional[CacheGroup] = None):
         self.target = target_model
         self.draft = draft_model
         self.k = k
+        self.cache = cache
         self.stats: Dict[str, int] = {"proposed": 0, "accepted": 0}
 
     @torch.no_grad()
@@ -217,6 +227,38 @@ class SpeculativeGenerator:
                  top_p: Optional[float] = None, generator: Optional[torch.Generator] = None,
                  trace: Optional[List[dict]] = None):
         seqs, single = _as_sequences(idx)
+        if self.cache is None:
+            return self._generate(seqs, single, max_new_tokens, temperature, top_k, top_p, generator, trace)
+        if len(seqs) > self.cache.max_rows:
+            raise ValueError(f"{len(seqs)} sequences exceed the cache's {self.cache.max_rows} rows")
+        if any(self.cache.length(b) for b in range(len(seqs))):
+            raise ValueError("the cache's first slots are in use")
+        try:
+            return self._generate(seqs, single, max_new_tokens, temperature, top_k, top_p, generator, trace)
+        finally:
+            for b in range(len(seqs)):
+                self.cache.release(b)
+
+    def _target_logits(self, slots: List[int], ctxs: List[torch.Tensor]) -> List[torch.Tensor]:
+        """The target's logits of each context (at least its last k + 1 rows)."""
+        out: List = [None] * len(ctxs)
+        fits = [i for i, c in enumerate(ctxs) if self.cache is not None
+                and c.numel() <= min(self.target.spec.block_size, self.cache.max_seq_len)]
+        slide = [i for i in range(len(ctxs)) if i not in fits]
+        if fits:
+            new = [ctxs[i][self.cache.length(slots[i]):] for i in fits]
+            step = self.cache.step([slots[i] for i in fits], [t.numel() for t in new])
+            logits = self.target.paged_logits(torch.cat(new), step)
+            for i, rows in zip(fits, logits.split([t.numel() for t in new])):
+                out[i] = rows
+        if slide:
+            tb = self.target.spec.block_size
+            cut = [ctxs[i] if ctxs[i].numel() <= tb else ctxs[i][-tb:] for i in slide]
+            for i, c, rows in zip(slide, cut, _grouped(lambda x: self.target.full_logits(x), cut)):
+                out[i] = rows[: c.numel()] if rows.size(0) >= c.numel() else rows[:0]
+        return out
+
+    def _generate(self, seqs, single, max_new_tokens, temperature, top_k, top_p, generator, trace):
         dev = seqs[0].device
         T = max(temperature, 1e-8)
         K = self.k
@@ -241,16 +283,13 @@ class SpeculativeGenerator:
                 u_draft.append(u)
                 dctx = [torch.cat([c, tok[i:i + 1].to(c.dtype)]) for i, c in enumerate(dctx)]
             drafts = torch.stack(d_toks, dim=1)                     # [A, K]
-            vctx = [torch.cat([seqs[b], drafts[i].to(seqs[b].dtype)]) for i, b in enumerate(act)]
-            vctx = [c if c.numel() <= tb else c[-tb:] for c in vctx]
-            full = _grouped(lambda x: self.target.full_logits(x), vctx)
-            # the verify positions of each sequence: prompt_len - 1 + offset ..
-            # (+ K); the context is cut to the block size from the left
+            full = self._target_logits(act, [torch.cat([seqs[b], drafts[i].to(seqs[b].dtype)]) for i, b in enumerate(act)])
+            # the verify positions of each sequence: the last K + 1 (the context
+            # is cut to the block size from the left)
             rows_t, ok = [], []
             for i, b in enumerate(act):
-                L = vctx[i].numel()
-                first = seqs[b].numel() - 1 + (L - (seqs[b].numel() + K))
-                if first < 0 or first + K >= full[i].size(0):
+                first = full[i].size(0) - K - 1
+                if first < 0:
                     active[b] = False
                     continue
                 rows_t.append(full[i][first:first + K + 1])
@@ -275,6 +314,8 @@ class SpeculativeGenerator:
                     self.stats["proposed"] += room if room <= na else min(na + 1, K)
                     self.stats["accepted"] += min(na, room)
                     new = toks[j][: na + 1][:room]
+                    if self.cache is not None:   # the rejected drafts' tokens are taken back
+                        self.cache.truncate(b, min(self.cache.length(b), seqs[b].numel() + min(na, len(new))))
                     seqs[b] = torch.cat([seqs[b], torch.tensor(new, dtype=seqs[b].dtype, device=dev)])
                     generated[b] += len(new)
                     if generated[b] >= max_new_tokens or seqs[b].numel() >= tb:
