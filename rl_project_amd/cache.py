@@ -21,16 +21,13 @@ that would see it."""
 
 from __future__ import annotations
 
-import math
-from typing import List, Optional, Sequence, Tuple
+from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
 
-_PAGE_SIZES = (16, 32, 64, 128)
 _CACHE_DTYPES = (torch.bfloat16, torch.float16, torch.float8_e4m3fn)
-_ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 class PagedCache:
@@ -52,27 +49,7 @@ class PagedCache:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
                  v_scale: Optional[torch.Tensor] = None):
-        if k.device.type != "cuda":
-            raise ValueError("the cache must be on a ROCm device (no CPU fallback)")
-        if k.dim() != 4 or v.dim() != 4 or v.shape != (k.size(0), k.size(1), k.size(3), k.size(2)):
-            raise ValueError(f"k [pages, heads, page_size, dim] and v [pages, heads, dim, page_size] do not match: "
-                             f"{tuple(k.shape)}, {tuple(v.shape)}")
-        if k.dtype not in _CACHE_DTYPES:
-            raise NotImplementedError(f"cache dtype {k.dtype} is not supported (bfloat16, float16, float8_e4m3fn)")
-        if v.dtype != k.dtype or v.device != k.device or not k.is_contiguous() or not v.is_contiguous():
-            raise ValueError("k and v must share a dtype and a device and be contiguous")
-        pages, heads, page_size, dim = k.shape
-        if page_size not in _PAGE_SIZES:
-            raise ValueError(f"page_size {page_size} is none of {_PAGE_SIZES}")
-        if pages < 1 or heads < 1 or dim < 8 or dim % 8 or dim > _lib.FL_CACHE_MAX_DIM:
-            raise ValueError(f"{pages} pages, {heads} heads, dim {dim}: at least one of each, dim a multiple of 8 up to "
-                             f"{_lib.FL_CACHE_MAX_DIM}")
-        if k.dtype == torch.float8_e4m3fn:
-            for s in (k_scale, v_scale):
-                if s is None or s.dtype != torch.uint8 or s.shape != k.shape[:3] or s.device != k.device or not s.is_contiguous():
-                    raise ValueError(f"a float8_e4m3fn cache needs k_scale and v_scale: contiguous uint8 {tuple(k.shape[:3])}")
-        elif k_scale is not None or v_scale is not None:
-            raise ValueError("scales belong to a float8_e4m3fn cache")
+        _lib.autograd().check_cache(k, v, k_scale, v_scale)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
 
     @classmethod
@@ -117,31 +94,6 @@ def _check_cache(cache) -> None:
         raise TypeError("cache must be a PagedCache")
 
 
-def _check_tokens(cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor], rows: int) -> None:
-    dev = cache.k.device
-    if table.dim() != 2 or table.dtype != torch.int32 or table.device != dev or (table.size(1) > 1 and table.stride(1) != 1):
-        raise ValueError(f"table must be int32 [B, width] on {dev}, its rows contiguous")
-    B = table.size(0)
-    if lengths.shape != (B,) or lengths.dtype != torch.int32 or lengths.device != dev or not lengths.is_contiguous():
-        raise ValueError(f"lengths must be contiguous int32 [{B}] on {dev}")
-    if starts is None:
-        if (B and rows % B) or (rows and not B):
-            raise ValueError(f"{rows} tokens are not as many for each of {B} sequences: give starts")
-    elif starts.shape != (B + 1,) or starts.dtype != torch.int32 or starts.device != dev or not starts.is_contiguous():
-        raise ValueError(f"starts must be contiguous int32 [{B + 1}] on {dev}")
-
-
-def _check_rows(cache: PagedCache, x: torch.Tensor, name: str, heads: Optional[int] = None) -> None:
-    if x.dim() < 3 or x.size(-1) != cache.dim or (heads is not None and x.size(-2) != heads) or x.device != cache.device:
-        raise ValueError(f"{name} must be [..., {heads if heads is not None else 'heads'}, {cache.dim}] on {cache.device}, "
-                         f"not {tuple(x.shape)}")
-
-
-def _no_gradient(what: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} records no gradient: call it under torch.no_grad()")
-
-
 def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *,
                 starts: Optional[torch.Tensor] = None) -> None:
     """Write new tokens' keys and values ``[..., heads, dim]`` (the leading dimensions
@@ -149,14 +101,7 @@ def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torc
     from float32, bfloat16 or float16 in 8 bits with a scale for each token and head.
     One launch.  Sequences that share pages must not write the same slot in a call."""
     _check_cache(cache)
-    _check_rows(cache, k, "k", cache.heads)
-    if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
-        raise ValueError("k and v must match in shape, dtype and device")
-    if k.dtype not in _ROW_DTYPES or (cache.dtype != torch.float8_e4m3fn and k.dtype != cache.dtype):
-        raise NotImplementedError(f"{k.dtype} keys into a {cache.dtype} cache")
-    _check_tokens(cache, table, lengths, starts, k.shape[:-2].numel())
-    _no_gradient("cache_write", k, v)
-    _lib.autograd().cache_call(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, table, lengths, starts, True)
+    _lib.autograd().cache_write(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, table, lengths, starts)
 
 
 def cache_read(cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, tokens: int, *, starts: Optional[torch.Tensor] = None,
@@ -169,22 +114,9 @@ def cache_read(cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, to
     outside its range.  Into ``out`` (contiguous) where given (rows behind the
     last sequence stay as they were; without ``out`` they hold anything).  One launch."""
     _check_cache(cache)
-    if out is not None:
-        dtype = out[0].dtype
-    elif dtype is None:
-        dtype = torch.float32 if cache.dtype == torch.float8_e4m3fn else cache.dtype
-    if dtype not in _ROW_DTYPES:
-        raise NotImplementedError(f"dtype {dtype} is not supported (float32, bfloat16, float16)")
-    if tokens < 0:
-        raise ValueError(f"tokens {tokens} < 0")
-    _check_tokens(cache, table, lengths, starts, tokens)
-    shape = (tokens, cache.heads, cache.dim)
-    if out is None:
-        out = tuple(torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
-    elif any(t.shape != shape or t.dtype != dtype or t.device != cache.device or not t.is_contiguous() for t in out):
-        raise ValueError(f"out must be two contiguous {dtype} tensors {shape} on {cache.device}")
-    _lib.autograd().cache_call(cache.k, cache.v, cache.k_scale, cache.v_scale, out[0], out[1], table, lengths, starts, False)
-    return out[0], out[1]
+    out_k, out_v = out if out is not None else (None, None)
+    return _lib.autograd().cache_read(cache.k, cache.v, cache.k_scale, cache.v_scale, table, lengths, tokens, starts, dtype, out_k,
+                                      out_v)
 
 
 def paged_attention(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor, *,
@@ -210,27 +142,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, len
     One or two launches, without host synchronisation; results are the same each
     time, and depend on how the call's shapes split the keys in the last bits."""
     _check_cache(cache)
-    _check_rows(cache, q, "q")
-    if q.dtype not in (torch.bfloat16, torch.float16) or (cache.dtype != torch.float8_e4m3fn and q.dtype != cache.dtype):
-        raise NotImplementedError(f"{q.dtype} queries over a {cache.dtype} cache")
-    if q.size(-2) < 1 or q.size(-2) % cache.heads:
-        raise ValueError(f"{q.size(-2)} query heads over {cache.heads} cached")
-    _check_tokens(cache, table, lengths, starts, q.shape[:-2].numel())
-    if scale is None:
-        scale = 1.0 / math.sqrt(cache.dim)
-    window = 0 if window is None else window
-    if window < 0 or sinks < 0:
-        raise ValueError("window and sinks must be >= 0")
-    _no_gradient("paged_attention", q)
-    into = None
-    if out is not None:
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
-            raise ValueError("out must match q in shape, dtype and device")
-        into = out if out.dim() == 3 else out.view(-1, out.size(-2), out.size(-1))
-        if into.data_ptr() % 8 or into.stride(2) != 1 or any(
-                into.size(i) > 1 and (into.stride(i) % 4 or into.stride(i) < cache.dim) for i in (0, 1)):
-            raise ValueError("out must be 8-byte aligned, its heads contiguous and apart, strides in multiples of 4 elements")
     o, lse = _lib.autograd().attention(cache.k, cache.v, cache.k_scale, cache.v_scale, q, table, lengths, starts, scale, softcap,
-                                       window, sinks, into, return_lse)
+                                       window, sinks, out, return_lse)
     o = out if out is not None else o
     return (o, lse) if return_lse else o

@@ -518,7 +518,7 @@ AttnCall attn_call(const fl_attn_args& a) {
   const int64_t keys = a.rows.table_width * a.cache.page_size;
   // Splits: enough that every CU has `work` / 256 work-groups, and `least` of them, so
   // that long and short sequences share the CUs evenly (64 sequences of 1024 to 8192
-  // tokens: 2 splits 269 us, 4 243 us, 8 262 us); none shorter than 4 steps of 64 keys
+  // tokens: 2 splits 269 us, 4 243 us, 8 262 us); none shorter than 8 steps of 64 keys
   // of the longest sequence the table (or the window) allows.
   const auto plan = [&](AttnPlan& p, int tr, int64_t groups, int64_t work, int64_t least) {
     p.group = static_cast<int>(G);

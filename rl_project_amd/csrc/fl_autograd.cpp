@@ -6,17 +6,22 @@
 // interpreter on the engine's own thread, 73 us so; score_tokens 1x50257 with 5
 // alternatives: 20 us over ctypes, 11.6 us so.)
 //
-// The Python callers have checked every argument; the entry points come from the
-// library that Python loaded (bind).
+// The Python callers of score_tokens, layer_norm and lm_head_logprobs have checked
+// every argument; those of the others pass theirs on, and they are checked here (in
+// Python the checks of a decode step's calls take longer than its kernels).  The
+// entry points come from the library that Python loaded (bind).
 #include <torch/extension.h>
 
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <ATen/ExpandUtils.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <cmath>
 #include <optional>
+#include <sstream>
 #include <string>
 #include <vector>
 
@@ -455,6 +460,119 @@ struct Head : torch::autograd::Function<Head> {
   }
 };
 
+// ---------------------------------------------------------------- checks
+template <class... T>
+std::string text(const T&... parts) {
+  std::ostringstream s;
+  (s << ... << parts);
+  return s.str();
+}
+#define VALUE_CHECK(cond, ...) \
+  if (!(cond)) C10_THROW_ERROR(ValueError, text(__VA_ARGS__))
+#define SUPPORT_CHECK(cond, ...) \
+  if (!(cond)) C10_THROW_ERROR(NotImplementedError, text(__VA_ARGS__))
+
+bool is_row_type(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
+bool same_lead(const Tensor& a, const Tensor& b, int64_t n) { return a.sizes().slice(0, n) == b.sizes().slice(0, n); }
+bool graded(const Tensor& t) { return t.requires_grad(); }
+bool graded(const OptTensor& t) { return t && t->requires_grad(); }
+
+// What qk_norm_rope and its backward take; returns positions and inv_freq as the
+// kernels read them.
+std::pair<Tensor, Tensor> check_rope(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq,
+                                     const OptTensor& qw, const OptTensor& kw, bool norm) {
+  for (const Tensor* t : {&q, &k}) {
+    const char* name = t == &q ? "q" : "k";
+    VALUE_CHECK(t->is_cuda(), name, " must be on a ROCm device (no CPU fallback)");
+    SUPPORT_CHECK(is_row_type(t->scalar_type()), name, " dtype ", t->scalar_type(), " is not supported (float32, bfloat16, float16)");
+  }
+  VALUE_CHECK(q.dim() >= 3 && k.dim() == q.dim() && same_lead(q, k, q.dim() - 2) && q.size(-1) == k.size(-1),
+              "q [..., heads, dim] and k [..., kv_heads, dim] do not match: ", q.sizes(), ", ", k.sizes());
+  VALUE_CHECK(k.scalar_type() == q.scalar_type() && k.device() == q.device(), "q and k must share a dtype and a device");
+  const int64_t D = q.size(-1);
+  VALUE_CHECK(D >= 2 && D % 2 == 0, "the head dimension must be even and at least 2, not ", D);
+  VALUE_CHECK(q.size(-2) >= 1 && k.size(-2) >= 1, "q and k need at least one head");
+  VALUE_CHECK((positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong) && positions.device() == q.device(),
+              "positions must be int32 or int64 on ", q.device());
+  VALUE_CHECK(inv_freq.dim() == 1 && inv_freq.device() == q.device() &&
+                  (inv_freq.scalar_type() == at::kDouble || inv_freq.scalar_type() == at::kFloat) && 2 * inv_freq.size(0) <= D,
+              "inv_freq must be float64 or float32, of at most ", D / 2, " values, on ", q.device());
+  VALUE_CHECK(norm || (!qw && !kw), "weights belong to the norm: give eps");
+  for (const OptTensor* w : {&qw, &kw}) {
+    if (!*w) continue;
+    const char* name = w == &qw ? "q_weight" : "k_weight";
+    VALUE_CHECK((*w)->dim() == 1 && (*w)->size(0) == D && (*w)->device() == q.device(), name, " must be [", D, "] on ", q.device());
+    SUPPORT_CHECK((*w)->scalar_type() == q.scalar_type() || (*w)->scalar_type() == at::kFloat, name, " dtype ", (*w)->scalar_type(),
+                  " is neither q's nor float32");
+  }
+  SUPPORT_CHECK(!qw || !kw || qw->scalar_type() == kw->scalar_type(), "q_weight and k_weight must share a dtype");
+  const auto lead = q.sizes().slice(0, q.dim() - 2);
+  Tensor p = positions;
+  if (p.sizes() != lead) {
+    VALUE_CHECK(at::is_expandable_to(p.sizes(), lead), "positions ", p.sizes(), " do not expand to ", lead);
+    p = p.expand(lead);
+  }
+  const at::NoGradGuard no_grad;
+  return {p.contiguous(), inv_freq.to(at::kDouble).contiguous()};
+}
+
+void check_grad_of(const OptTensor& g, const Tensor& x, const char* name) {
+  VALUE_CHECK(!g || (g->sizes() == x.sizes() && g->scalar_type() == x.scalar_type() && g->device() == x.device()), name,
+              " must match its input in shape, dtype and device");
+}
+
+void check_cache(const Tensor& k, const Tensor& v, const OptTensor& ks, const OptTensor& vs) {
+  VALUE_CHECK(k.is_cuda(), "the cache must be on a ROCm device (no CPU fallback)");
+  VALUE_CHECK(k.dim() == 4 && v.dim() == 4 && v.size(0) == k.size(0) && v.size(1) == k.size(1) && v.size(2) == k.size(3) &&
+                  v.size(3) == k.size(2),
+              "k [pages, heads, page_size, dim] and v [pages, heads, dim, page_size] do not match: ", k.sizes(), ", ", v.sizes());
+  const auto t = k.scalar_type();
+  SUPPORT_CHECK(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat8_e4m3fn, "cache dtype ", t,
+                " is not supported (bfloat16, float16, float8_e4m3fn)");
+  VALUE_CHECK(v.scalar_type() == t && v.device() == k.device() && k.is_contiguous() && v.is_contiguous(),
+              "k and v must share a dtype and a device and be contiguous");
+  const int64_t S = k.size(2), D = k.size(3);
+  VALUE_CHECK(S == 16 || S == 32 || S == 64 || S == 128, "page_size ", S, " is none of 16, 32, 64, 128");
+  VALUE_CHECK(k.size(0) >= 1 && k.size(1) >= 1 && D >= 8 && D % 8 == 0 && D <= FL_CACHE_MAX_DIM, k.size(0), " pages, ", k.size(1),
+              " heads, dim ", D, ": at least one of each, dim a multiple of 8 up to ", FL_CACHE_MAX_DIM);
+  for (const OptTensor* s : {&ks, &vs}) {
+    if (t != at::kFloat8_e4m3fn) {
+      VALUE_CHECK(!*s, "scales belong to a float8_e4m3fn cache");
+      continue;
+    }
+    VALUE_CHECK(*s && (*s)->scalar_type() == at::kByte && (*s)->sizes() == k.sizes().slice(0, 3) && (*s)->device() == k.device() &&
+                    (*s)->is_contiguous(),
+                "a float8_e4m3fn cache needs k_scale and v_scale: contiguous uint8 ", k.sizes().slice(0, 3));
+  }
+}
+
+void check_tokens(const Tensor& ck, const Tensor& table, const Tensor& lengths, const OptTensor& starts, int64_t rows) {
+  VALUE_CHECK(table.dim() == 2 && table.scalar_type() == at::kInt && table.device() == ck.device() &&
+                  (table.size(1) <= 1 || table.stride(1) == 1),
+              "table must be int32 [B, width] on ", ck.device(), ", its rows contiguous");
+  const int64_t B = table.size(0);
+  VALUE_CHECK(lengths.dim() == 1 && lengths.size(0) == B && lengths.scalar_type() == at::kInt && lengths.device() == ck.device() &&
+                  lengths.is_contiguous(),
+              "lengths must be contiguous int32 [", B, "] on ", ck.device());
+  if (!starts) {
+    VALUE_CHECK(rows == 0 || (B > 0 && rows % B == 0), rows, " tokens are not as many for each of ", B, " sequences: give starts");
+  } else
+    VALUE_CHECK(starts->dim() == 1 && starts->size(0) == B + 1 && starts->scalar_type() == at::kInt && starts->device() == ck.device() &&
+                    starts->is_contiguous(),
+                "starts must be contiguous int32 [", B + 1, "] on ", ck.device());
+}
+
+int64_t lead_rows(const Tensor& x) {
+  int64_t n = 1;
+  for (int64_t i = 0; i + 2 < x.dim(); ++i) n *= x.size(i);
+  return n;
+}
+
+void no_gradient(const char* what, bool any) {
+  if (any && at::GradMode::is_enabled())
+    C10_THROW_ERROR(Error, std::string(what) + " records no gradient: call it under torch.no_grad()");
+}
+
 // ---------------------------------------------------------------- norms and rotation
 // [tokens, heads, dim] whose last dimension is contiguous (a copy where it is not,
 // or where the leading dimensions do not fold)
@@ -694,37 +812,86 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     const at::NoGradGuard no_grad;
     return or_none(head_backward(h, w, or_undefined(t), saved, or_undefined(ga), or_undefined(gb), or_undefined(gc), ii, nh, nw));
   }, release());
-  m.def("rope", [](const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw, const Tensor& pos, const Tensor& f,
-                   double eps, double gain, bool norm, bool inter) {
+  m.def("qk_norm_rope", [](const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq, const OptTensor& qw,
+                           const OptTensor& kw, std::optional<double> eps, bool inter, double gain) -> variable_list {
+    const auto [pos, freq] = check_rope(q, k, positions, inv_freq, qw, kw, eps.has_value());
     refuse_tangents("qk_norm_rope", q, k, qw, kw);
-    return Rope::apply(q, k, qw, kw, pos, f, eps, gain, norm, inter);
-  }, release());
-  m.def("rope_forward", [](const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw, const Tensor& pos,
-                           const Tensor& f, double eps, double gain, bool norm, bool inter) {
-    refuse_tangents("qk_norm_rope", q, k, qw, kw);
+    if (at::GradMode::is_enabled() && (graded(q) || graded(k) || graded(qw) || graded(kw))) {
+      if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+        C10_THROW_ERROR(Error, "qk_norm_rope does not record its autograd graph under stream capture: call it under "
+                               "torch.no_grad(), then qk_norm_rope_backward");
+      return Rope::apply(q, k, qw, kw, pos, freq, eps.value_or(0.0), gain, eps.has_value(), inter);
+    }
     const at::NoGradGuard no_grad;
-    return rope_forward(q, k, qw, kw, pos, f, {eps, gain, norm, inter});
+    return rope_forward(q, k, qw, kw, pos, freq, {eps.value_or(0.0), gain, eps.has_value(), inter});
   }, release());
-  m.def("rope_backward", [](const OptTensor& gq, const OptTensor& gk, const Tensor& q, const Tensor& k, const OptTensor& qw,
-                            const OptTensor& kw, const Tensor& pos, const Tensor& f, double eps, double gain, bool norm, bool inter,
-                            bool weights) {
+  m.def("qk_norm_rope_backward", [](const OptTensor& gq, const OptTensor& gk, const Tensor& q, const Tensor& k, const Tensor& positions,
+                                    const Tensor& inv_freq, const OptTensor& qw, const OptTensor& kw, std::optional<double> eps,
+                                    bool inter, double gain, bool weights) {
+    const auto [pos, freq] = check_rope(q, k, positions, inv_freq, qw, kw, eps.has_value());
+    check_grad_of(gq, q, "grad_q"), check_grad_of(gk, k, "grad_k");
     refuse_tangents("qk_norm_rope_backward", gq, gk, q, k, qw, kw);
     const at::NoGradGuard no_grad;
     const bool need[4] = {true, true, weights && qw, weights && kw};
-    return or_none(rope_backward(or_undefined(gq), or_undefined(gk), q, k, or_undefined(qw), or_undefined(kw), pos, f,
-                                 {eps, gain, norm, inter}, need));
+    return or_none(rope_backward(or_undefined(gq), or_undefined(gk), q, k, or_undefined(qw), or_undefined(kw), pos, freq,
+                                 {eps.value_or(0.0), gain, eps.has_value(), inter}, need));
   }, release());
-  m.def("cache_call", [](const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& k, const Tensor& v,
-                         const Tensor& table, const Tensor& lengths, const OptTensor& starts, bool write) {
+  m.def("check_cache", &check_cache);
+  m.def("cache_write", [](const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& k, const Tensor& v,
+                          const Tensor& table, const Tensor& lengths, const OptTensor& starts) {
+    VALUE_CHECK(k.dim() >= 3 && k.size(-1) == ck.size(3) && k.size(-2) == ck.size(1) && k.device() == ck.device(), "k must be [..., ",
+                ck.size(1), ", ", ck.size(3), "] on ", ck.device(), ", not ", k.sizes(), " on ", k.device());
+    VALUE_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device(),
+                "k and v must match in shape, dtype and device");
+    SUPPORT_CHECK(is_row_type(k.scalar_type()) && (ck.scalar_type() == at::kFloat8_e4m3fn || k.scalar_type() == ck.scalar_type()),
+                  k.scalar_type(), " keys into a ", ck.scalar_type(), " cache");
+    check_tokens(ck, table, lengths, starts, lead_rows(k));
+    no_gradient("cache_write", graded(k) || graded(v));
     refuse_tangents("cache_write", k, v);
     const at::NoGradGuard no_grad;
-    cache_call({ck, cv, ks, vs}, k, v, table, lengths, starts, write);
+    cache_call({ck, cv, ks, vs}, k, v, table, lengths, starts, true);
+  }, release());
+  m.def("cache_read", [](const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& table,
+                         const Tensor& lengths, int64_t tokens, const OptTensor& starts, std::optional<at::ScalarType> dtype,
+                         const OptTensor& out_k, const OptTensor& out_v) {
+    const auto t = out_k ? out_k->scalar_type() : dtype ? *dtype : ck.scalar_type() == at::kFloat8_e4m3fn ? at::kFloat : ck.scalar_type();
+    SUPPORT_CHECK(is_row_type(t), "dtype ", t, " is not supported (float32, bfloat16, float16)");
+    VALUE_CHECK(tokens >= 0, "tokens ", tokens, " < 0");
+    check_tokens(ck, table, lengths, starts, tokens);
+    const at::NoGradGuard no_grad;
+    const int64_t shape[3] = {tokens, ck.size(1), ck.size(3)};
+    for (const OptTensor* o : {&out_k, &out_v})
+      VALUE_CHECK(!*o || ((*o)->sizes() == at::IntArrayRef(shape) && (*o)->scalar_type() == t && (*o)->device() == ck.device() &&
+                          (*o)->is_contiguous()),
+                  "out must be two contiguous ", t, " tensors ", at::IntArrayRef(shape), " on ", ck.device());
+    const Tensor k = out_k ? *out_k : at::empty(shape, ck.options().dtype(t)), v = out_v ? *out_v : at::empty(shape, ck.options().dtype(t));
+    cache_call({ck, cv, ks, vs}, k, v, table, lengths, starts, false);
+    return std::make_pair(k, v);
   }, release());
   m.def("attention", [](const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& q, const Tensor& table,
-                        const Tensor& lengths, const OptTensor& starts, double scale, double softcap, int64_t window, int64_t sinks,
-                        const OptTensor& into, bool lse) {
+                        const Tensor& lengths, const OptTensor& starts, std::optional<double> scale, double softcap,
+                        std::optional<int64_t> window, int64_t sinks, const OptTensor& into, bool lse) {
+    VALUE_CHECK(q.dim() >= 3 && q.size(-1) == ck.size(3) && q.device() == ck.device(), "q must be [..., heads, ", ck.size(3), "] on ",
+                ck.device(), ", not ", q.sizes(), " on ", q.device());
+    SUPPORT_CHECK((q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf) &&
+                      (ck.scalar_type() == at::kFloat8_e4m3fn || q.scalar_type() == ck.scalar_type()),
+                  q.scalar_type(), " queries over a ", ck.scalar_type(), " cache");
+    VALUE_CHECK(q.size(-2) >= 1 && q.size(-2) % ck.size(1) == 0, q.size(-2), " query heads over ", ck.size(1), " cached");
+    check_tokens(ck, table, lengths, starts, lead_rows(q));
+    VALUE_CHECK(window.value_or(0) >= 0 && sinks >= 0, "window and sinks must be >= 0");
+    no_gradient("paged_attention", graded(q));
     refuse_tangents("paged_attention", q);
     const at::NoGradGuard no_grad;
-    return or_none(attention({ck, cv, ks, vs}, q, table, lengths, starts, scale, softcap, window, sinks, into, lse));
+    OptTensor o;
+    if (into) {
+      VALUE_CHECK(into->sizes() == q.sizes() && into->scalar_type() == q.scalar_type() && into->device() == q.device(),
+                  "out must match q in shape, dtype and device");
+      o = into->dim() == 3 ? *into : into->view({-1, q.size(-2), q.size(-1)});
+      bool fine = reinterpret_cast<uintptr_t>(o->data_ptr()) % 8 == 0 && o->stride(2) == 1;
+      for (int i = 0; i < 2; ++i) fine = fine && (o->size(i) <= 1 || (o->stride(i) % 4 == 0 && o->stride(i) >= q.size(-1)));
+      VALUE_CHECK(fine, "out must be 8-byte aligned, its heads contiguous and apart, strides in multiples of 4 elements");
+    }
+    return or_none(attention({ck, cv, ks, vs}, q, table, lengths, starts, scale ? *scale : 1.0 / std::sqrt(static_cast<double>(ck.size(3))),
+                             softcap, window.value_or(0), sinks, o, lse));
   }, release());
 }

@@ -109,7 +109,7 @@ FL_HD bool kv_tile(const fl_cache_rows& r, const fl_cache& c, const PagedSeq& s,
 }
 
 constexpr int AT_BLK = 64;          // keys of a step
-constexpr int AT_MIN_BLKS = 4;      // steps of a split, at least
+constexpr int AT_MIN_BLKS = 8;      // steps of a split, at least
 constexpr int AT_MAX_SPLITS = 64;
 
 // A launch's plan.  Rows of a sequence and cached head: (token, head of the group),

@@ -54,31 +54,45 @@ struct RpRow {
   __device__ __forceinline__ int second(int p) const { return inter ? 2 * p + 1 : p < R2 ? p + R2 : R2 + T2 + p; }
 };
 
+// The two chunks of N pairs from pair p on, as they lie.
+template <class D>
+__device__ __forceinline__ void rp_raw(const void* row, const RpRow& R, int p, uint4 (&q)[2]) {
+  constexpr int ESZ = D::id == FL_DTYPE_F32 ? 4 : 2;
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const char* c = static_cast<const char*>(row) + ESZ * R.first(p);
+  const u32x4 a = *reinterpret_cast<const u32x4*>(c);
+  const u32x4 b = *reinterpret_cast<const u32x4*>(R.inter ? c + 16 : static_cast<const char*>(row) + ESZ * R.second(p));
+  q[0] = make_uint4(a[0], a[1], a[2], a[3]);
+  q[1] = make_uint4(b[0], b[1], b[2], b[3]);
+}
+template <class D, int N>
+__device__ __forceinline__ void rp_pairs(const uint4 (&q)[2], const RpRow& R, float (&x)[N], float (&y)[N]) {
+  using C = RowChunk<D>;
+  static_assert(C::N == N, "a chunk holds N values");
+  float u[N], v[N];
+  C::unpack(q[0], u);
+  C::unpack(q[1], v);
+  if (R.inter) {
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) {
+      x[e] = u[2 * e], y[e] = u[2 * e + 1];
+      x[e + N / 2] = v[2 * e], y[e + N / 2] = v[2 * e + 1];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = u[e], y[e] = v[e];
+  }
+}
+
 template <class D, bool VEC, int N>
 __device__ __forceinline__ void rp_load(const void* row, const RpRow& R, int p, float (&x)[N], float (&y)[N]) {
-  using C = RowChunk<D>;
   if (p >= R.P) {
 #pragma unroll
     for (int e = 0; e < N; ++e) x[e] = y[e] = 0.0f;
   } else if constexpr (VEC) {
-    static_assert(C::N == N, "a chunk holds N values");
-    constexpr int ESZ = D::id == FL_DTYPE_F32 ? 4 : 2;
-    const char* c = static_cast<const char*>(row) + ESZ * R.first(p);
-    const uint4 q0 = *reinterpret_cast<const uint4*>(c);
-    const uint4 q1 = *reinterpret_cast<const uint4*>(R.inter ? c + 16 : static_cast<const char*>(row) + ESZ * R.second(p));
-    float u[N], v[N];
-    C::unpack(q0, u);
-    C::unpack(q1, v);
-    if (R.inter) {
-#pragma unroll
-      for (int e = 0; e < N / 2; ++e) {
-        x[e] = u[2 * e], y[e] = u[2 * e + 1];
-        x[e + N / 2] = v[2 * e], y[e + N / 2] = v[2 * e + 1];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) x[e] = u[e], y[e] = v[e];
-    }
+    uint4 q[2];
+    rp_raw<D>(row, R, p, q);
+    rp_pairs<D>(q, R, x, y);
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -170,42 +184,73 @@ __device__ __forceinline__ RpRow rp_row(const fl_rope_args& a) {
 template <class D, class W, bool VEC>
 __global__ __launch_bounds__(RP_NT) void k_rope(const fl_rope_args a, int L, int TK) {
   constexpr int N = RowChunk<D>::N;
-  __shared__ float2 cs[1024];
+  __shared__ float2 cs[1024], ws[2][FL_ROPE_MAX_DIM / 2];   // the turns; the pairs' weights (queries', keys')
   const RpRow R = rp_row(a);
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * TK;
   const int tk = static_cast<int>(min(static_cast<int64_t>(TK), a.tokens - t0));
+  const int p = (threadIdx.x & (L - 1)) * N, g = threadIdx.x / L, GR = RP_NT / L;
+  const int H = static_cast<int>(a.heads), K = static_cast<int>(a.kv_heads), nq = tk * H, n = nq + tk * K;
+  // row i of the tokens': the queries' first
+  struct Row {
+    const void* x;
+    void* out;
+    int t;
+  };
+  const auto row = [&](int i) {
+    const bool key = i >= nq;
+    const int j = key ? i - nq : i, heads = key ? K : H, t = j / heads, h = j - t * heads;
+    const int64_t to = ((t0 + t) * heads + h) * a.dim;
+    return key ? Row{rp_at<D>(a.k, (t0 + t) * a.k_ld + h * a.k_hs), rp_at<D>(a.out_k, to), t}
+               : Row{rp_at<D>(a.q, (t0 + t) * a.q_ld + h * a.q_hs), rp_at<D>(a.out_q, to), t};
+  };
+  // the first row is on its way while the angles are taken, and each next one while
+  // one is worked on
+  uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  Row at = {};
+  const auto fetch = [&](int i) {
+    at = row(i);
+    if (VEC && p < R.P) rp_raw<D>(at.x, R, p, raw);
+  };
+  if (g < n) fetch(g);
+  if (a.norm)
+    for (int i = threadIdx.x; i < 2 * R.P; i += RP_NT) {
+      const int key = i >= R.P, pair = i - key * R.P;
+      float w0[1], w1[1];
+      rp_weights<W>(key ? a.k_weight : a.q_weight, R, pair, w0, w1);
+      ws[key][pair] = make_float2(w0[0], w1[0]);
+    }
   rp_turns(a, t0, tk, R.P, cs);
   __syncthreads();
-  const int p = (threadIdx.x & (L - 1)) * N, g = threadIdx.x / L, GR = RP_NT / L;
   const float inv = 1.0f / static_cast<float>(a.dim);
-  auto rows = [&](const void* x, int64_t ld, int64_t hs, int heads, const void* w, void* out) {
-    if (heads == 0) return;
-    float w0[N], w1[N];
-    rp_weights<W>(a.norm ? w : nullptr, R, p, w0, w1);
-    for (int i = g; i < tk * heads; i += GR) {
-      const int t = i / heads, h = i - t * heads;
-      float x0[N], x1[N];
-      rp_load<D, VEC>(rp_at<D>(x, (t0 + t) * ld + h * hs), R, p, x0, x1);
-      if (a.norm) {
-        float s = 0.0f;
+  for (int i = g; i < n; i += GR) {
+    float x0[N], x1[N];
+    if constexpr (VEC) rp_pairs<D>(raw, R, x0, x1);
+    else rp_load<D, false>(at.x, R, p, x0, x1);
+    const Row now = at;
+    if (i + GR < n) fetch(i + GR);
+    if (a.norm) {
+      float s = 0.0f;
 #pragma unroll
-        for (int e = 0; e < N; ++e) s = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], s));
-        const float r = 1.0f / sqrtf(fmaf(rp_sum<N>(s, L), inv, a.eps));
-#pragma unroll
-        for (int e = 0; e < N; ++e) x0[e] *= r * w0[e], x1[e] *= r * w1[e];
-      }
-      float y0[N], y1[N];
+      for (int e = 0; e < N; ++e) s = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], s));
+      const float r = 1.0f / sqrtf(fmaf(rp_sum<N>(s, L), inv, a.eps));
+      const float2* w = ws[i >= nq];
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float2 c = cs[t * R.P + min(p + e, R.P - 1)];
-        y0[e] = x0[e] * c.x - x1[e] * c.y;
-        y1[e] = x0[e] * c.y + x1[e] * c.x;
+        const float2 y = w[min(p + e, R.P - 1)];
+        x0[e] *= r * y.x, x1[e] *= r * y.y;
       }
-      rp_store<D, VEC>(rp_at<D>(out, ((t0 + t) * heads + h) * a.dim), R, p, y0, y1);
     }
-  };
-  rows(a.q, a.q_ld, a.q_hs, static_cast<int>(a.heads), a.q_weight, a.out_q);
-  rows(a.k, a.k_ld, a.k_hs, static_cast<int>(a.kv_heads), a.k_weight, a.out_k);
+    float y0[N], y1[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float2 c = cs[now.t * R.P + min(p + e, R.P - 1)];
+      // (the same fused products in every variant: a row's results do not depend on how
+      // it was read)
+      y0[e] = fmaf(x0[e], c.x, -(x1[e] * c.y));
+      y1[e] = fmaf(x0[e], c.y, x1[e] * c.x);
+    }
+    rp_store<D, VEC>(now.out, R, p, y0, y1);
+  }
 }
 
 // One side a work-group (blockIdx.y 0: queries, 1: keys): the sums of one weight's
@@ -239,16 +284,27 @@ __global__ __launch_bounds__(RP_NT, 4) void k_rope_grad(const fl_rope_grad_args 
       const int t = i / heads, h = i - t * heads;
       const int64_t at = ((t0 + t) * heads + h) * a.dim;
       float x0[N], x1[N], g0[N], g1[N], u0[N], u1[N];
-      if (grad != nullptr) rp_load<D, VEC>(rp_at<D>(grad, at), R, p, g0, g1);
-      else
+      const char* xr = rp_at<D>(x, (t0 + t) * ld + h * hs);
+      if constexpr (VEC) {   // (both rows on their way before either is unpacked)
+        uint4 qg[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)}, qx[2] = {qg[0], qg[0]};
+        if (p < R.P) {
+          if (grad != nullptr) rp_raw<D>(rp_at<D>(grad, at), R, p, qg);
+          if (a.norm) rp_raw<D>(xr, R, p, qx);
+        }
+        rp_pairs<D>(qg, R, g0, g1);
+        rp_pairs<D>(qx, R, x0, x1);
+      } else {
+        if (grad != nullptr) rp_load<D, false>(rp_at<D>(grad, at), R, p, g0, g1);
+        else
 #pragma unroll
-        for (int e = 0; e < N; ++e) g0[e] = g1[e] = 0.0f;
-      if (a.norm) rp_load<D, VEC>(rp_at<D>(x, (t0 + t) * ld + h * hs), R, p, x0, x1);
+          for (int e = 0; e < N; ++e) g0[e] = g1[e] = 0.0f;
+        if (a.norm) rp_load<D, false>(xr, R, p, x0, x1);
+      }
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const float2 c = cs[t * R.P + min(p + e, R.P - 1)];
-        u0[e] = g0[e] * c.x + g1[e] * c.y;
-        u1[e] = g1[e] * c.x - g0[e] * c.y;
+        u0[e] = fmaf(g0[e], c.x, g1[e] * c.y);
+        u1[e] = fmaf(g1[e], c.x, -(g0[e] * c.y));
       }
       if (a.norm) {
         float s = 0.0f;
@@ -267,8 +323,8 @@ __global__ __launch_bounds__(RP_NT, 4) void k_rope_grad(const fl_rope_grad_args 
         dot = rp_sum<N>(dot, L) * inv;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          u0[e] = r * (u0[e] - x0[e] * dot);
-          u1[e] = r * (u1[e] - x1[e] * dot);
+          u0[e] = r * fmaf(-x0[e], dot, u0[e]);
+          u1[e] = r * fmaf(-x1[e], dot, u1[e]);
         }
       }
       if (out != nullptr) rp_store<D, VEC>(rp_at<D>(out, at), R, p, u0, u1);

@@ -13,8 +13,6 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .norm import _check_x
-from .scores import _no_autograd_under_capture
 
 
 def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0,
@@ -59,39 +57,6 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: Optional[str
     return inv.to(device) if device is not None else inv, gain
 
 
-def _check(q, k, positions, inv_freq, q_weight, k_weight, eps):
-    _check_x(q, "q")
-    _check_x(k, "k")
-    if q.dim() < 3 or k.dim() != q.dim() or q.shape[:-2] != k.shape[:-2] or q.size(-1) != k.size(-1):
-        raise ValueError(f"q [..., heads, dim] and k [..., kv_heads, dim] do not match: {tuple(q.shape)}, {tuple(k.shape)}")
-    if k.dtype != q.dtype or k.device != q.device:
-        raise ValueError("q and k must share a dtype and a device")
-    D = q.size(-1)
-    if D % 2:
-        raise ValueError(f"the head dimension must be even, not {D}")
-    if q.size(-2) < 1 or k.size(-2) < 1:
-        raise ValueError("q and k need at least one head")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
-        raise ValueError(f"positions must be int32 or int64 on {q.device}")
-    if positions.shape != q.shape[:-2]:
-        positions = positions.expand(q.shape[:-2])
-    if inv_freq.dim() != 1 or inv_freq.device != q.device or inv_freq.dtype not in (torch.float64, torch.float32) \
-            or 2 * inv_freq.numel() > D:
-        raise ValueError(f"inv_freq must be float64 or float32, of at most {D // 2} values, on {q.device}")
-    if eps is None and (q_weight is not None or k_weight is not None):
-        raise ValueError("weights belong to the norm: give eps")
-    for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if t is None:
-            continue
-        if t.dim() != 1 or t.size(0) != D or t.device != q.device:
-            raise ValueError(f"{name} must be [{D}] on {q.device}")
-        if t.dtype != q.dtype and t.dtype != torch.float32:
-            raise NotImplementedError(f"{name} dtype {t.dtype} is neither q's nor float32")
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise NotImplementedError("q_weight and k_weight must share a dtype")
-    return positions.contiguous(), inv_freq.detach().double().contiguous()
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
                  q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: Optional[float] = None,
                  interleaved: bool = False, gain: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -112,13 +77,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     Differentiable (once, in reverse mode) in ``q``, ``k`` and the weights, except
     under stream capture: a captured step takes this call under ``torch.no_grad()``
     and ``qk_norm_rope_backward``."""
-    positions, inv_freq = _check(q, k, positions, inv_freq, q_weight, k_weight, eps)
-    args = (q, k, q_weight, k_weight, positions, inv_freq, 0.0 if eps is None else eps, gain, eps is not None, interleaved)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        _no_autograd_under_capture("qk_norm_rope", None)
-        out = _lib.autograd().rope(*args)
-    else:
-        out = _lib.autograd().rope_forward(*args)
+    out = _lib.autograd().qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, gain)
     return out[0], out[1]
 
 
@@ -131,9 +90,5 @@ def qk_norm_rope_backward(grad_q: Optional[torch.Tensor], grad_k: Optional[torch
     computes, as launches that a graph may record.  ``q`` and ``k`` are the forward
     call's inputs.  The weights' gradients (None without a weight) have their dtype;
     their sums over tokens and heads have a fixed order."""
-    positions, inv_freq = _check(q, k, positions, inv_freq, q_weight, k_weight, eps)
-    for g, x, name in ((grad_q, q, "grad_q"), (grad_k, k, "grad_k")):
-        if g is not None and (g.shape != x.shape or g.dtype != x.dtype or g.device != x.device):
-            raise ValueError(f"{name} must match its input in shape, dtype and device")
-    return tuple(_lib.autograd().rope_backward(grad_q, grad_k, q, k, q_weight, k_weight, positions, inv_freq,
-                                               0.0 if eps is None else eps, gain, eps is not None, interleaved, need_dweight))
+    return tuple(_lib.autograd().qk_norm_rope_backward(grad_q, grad_k, q, k, positions, inv_freq, q_weight, k_weight, eps,
+                                                       interleaved, gain, need_dweight))

@@ -57,13 +57,13 @@ def _tokens(tokens: torch.Tensor, lead, dev: torch.device) -> torch.Tensor:
     return tokens
 
 
-def _no_autograd_under_capture(what: str, keep: Optional[str] = "return_saved") -> None:
+def _no_autograd_under_capture(what: str, keep: str = "return_saved") -> None:
     """A backward pass recorded into a graph synchronises with the streams that
     other graphs of the same leaves ran on, which capture forbids and which can
     end the process: a captured step calls the functional form instead."""
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{what} does not record its autograd graph under stream capture: "
-                           f"call it under torch.no_grad(){f' with {keep}=True' if keep else ''}, then {what}_backward")
+                           f"call it under torch.no_grad() with {keep}=True, then {what}_backward")
 
 
 def _check_range(tokens: torch.Tensor, vocab: int, ignore_index: int) -> None:
