@@ -22,6 +22,11 @@ __device__ __forceinline__ uint4 ld16(const void* p) {
 __device__ __forceinline__ void st16(void* p, uint4 x) { *static_cast<u32x4*>(p) = (u32x4){x.x, x.y, x.z, x.w}; }
 
 // 16-bit operands: 8 values of a lane as a uint4.
+//
+// With an 8-bit cache the weights of the second product carry their values' scales,
+// 2^(s - m) 2^e.  bfloat16 has the range for any.  Half precision does not: there m is
+// the maximum of s + e, not of s, so that the weights that count are near 1 whatever
+// the scales (sums of 2^(s - m) stay in float32, where e of -96 to 92 leaves room).
 struct OpBF16 {
   using D = BF16;
   typedef __bf16 x8 __attribute__((ext_vector_type(8)));

@@ -31,7 +31,6 @@ constexpr int AR_NT = 256, AR_NW = AR_NT / WAVE;
 template <class Op_>
 struct Cache16 {
   using Op = Op_;
-  using Pv = Op_;
   static constexpr bool E8 = false;
   static constexpr int ESZ = 2;
   static constexpr int SUBS = 2;   // pages that a lane looks up for a step
@@ -41,9 +40,6 @@ struct Cache16 {
 template <class Op_>
 struct Cache8 {
   using Op = Op_;
-  // The second product's weights carry the values' scales, 2^-96 to 2^120: bfloat16
-  // whatever the queries have (its 8 bits are twice what the values hold).
-  using Pv = OpBF16;
   static constexpr bool E8 = true;
   static constexpr int ESZ = 1;
   static constexpr int SUBS = 1;
@@ -64,7 +60,6 @@ __device__ __forceinline__ uint4 ar_load16_8(const char* p) {
 template <class C, int DT, bool FULL, int CT>
 __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(const fl_attn_args a, const AttnPlan p) {
   using Op = typename C::Op;
-  using Pv = typename C::Pv;
   constexpr int KS = DT / 32;   // steps of the first product
   constexpr int DM = DT / 16;   // tiles of channels of the second
   // tiles of values that are loaded ahead of their step's softmax: what registers hold
@@ -258,9 +253,17 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
             x[4 * j + e] = seen ? y : -INFINITY;
           }
       }
-      float top = x[0];
+      float top = -INFINITY;
+      if constexpr (C::E8 && !Op::SCALES) {   // (of the weights with their values' scales, fl_attn.h)
 #pragma unroll
-      for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            top = fmaxf(top, x[4 * j + e] + static_cast<float>((j == 0 ? ev.x : j == 1 ? ev.y : j == 2 ? ev.z : ev.w) >> (8 * e) & 255u));
+        top -= 127.0f;
+      } else
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, x[e]);
       if (__any(top > m[ct] + AT_LAZY)) {   // (m = -inf at first)
         top = fmaxf(top, shfl_xor(top, 16));
         top = fmaxf(top, shfl_xor(top, 32));
@@ -287,8 +290,8 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        pf[ct][u] = make_uint4(Pv::pack(x[8 * u], x[8 * u + 1]), Pv::pack(x[8 * u + 2], x[8 * u + 3]),
-                               Pv::pack(x[8 * u + 4], x[8 * u + 5]), Pv::pack(x[8 * u + 6], x[8 * u + 7]));
+        pf[ct][u] = make_uint4(Op::pack(x[8 * u], x[8 * u + 1]), Op::pack(x[8 * u + 2], x[8 * u + 3]),
+                               Op::pack(x[8 * u + 4], x[8 * u + 5]), Op::pack(x[8 * u + 6], x[8 * u + 7]));
 #pragma unroll
       for (int e = 0; e < 16; ++e) pw[ct][e] = x[e];
     }
@@ -304,7 +307,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
       uint4 vf[2];
       if constexpr (C::E8) {
         const uint4 x = vr[dm][0];
-        const uint2 y0 = Pv::widen(x.x), y1 = Pv::widen(x.y), y2 = Pv::widen(x.z), y3 = Pv::widen(x.w);
+        const uint2 y0 = Op::widen(x.x), y1 = Op::widen(x.y), y2 = Op::widen(x.z), y3 = Op::widen(x.w);
         vf[0] = make_uint4(y0.x, y0.y, y1.x, y1.y);
         vf[1] = make_uint4(y2.x, y2.y, y3.x, y3.y);
       } else {
@@ -312,13 +315,13 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
         vf[1] = vr[dm][C::SUBS - 1];
       }
       if (masked) {
-        odd |= not_finite<Pv>(vf[0]) | not_finite<Pv>(vf[1]);
-        vf[0] = finite_or_0<Pv>(vf[0]), vf[1] = finite_or_0<Pv>(vf[1]);
+        odd |= not_finite<Op>(vf[0]) | not_finite<Op>(vf[1]);
+        vf[0] = finite_or_0<Op>(vf[0]), vf[1] = finite_or_0<Op>(vf[1]);
       }
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        o[ct][dm] = Pv::mfma16(vf[0], pf[ct][0], o[ct][dm]);
-        o[ct][dm] = Pv::mfma16(vf[1], pf[ct][1], o[ct][dm]);
+        o[ct][dm] = Op::mfma16(vf[0], pf[ct][0], o[ct][dm]);
+        o[ct][dm] = Op::mfma16(vf[1], pf[ct][1], o[ct][dm]);
       }
     }
     if (masked && __any(odd != 0)) {

@@ -44,7 +44,7 @@ class Pages:
             ck, cv = ck.to(dtype), cv.to(dtype)
             ks = torch.randint(0, 256, (pages, heads, page), device=DEV, generator=g, dtype=torch.uint8)
             vs = torch.randint(0, 256, (pages, heads, page), device=DEV, generator=g, dtype=torch.uint8)
-        self.k, self.v = [], []
+        self.k, self.v, self.scale = [], [], []     # (scale: the values', 1 in 16 bits)
         for b, n in enumerate(lens):
             x = [torch.randn(n, heads, dim, device=DEV, generator=g).to(hold) for _ in "kv"]
             if k is not None:
@@ -55,10 +55,12 @@ class Pages:
                 (qk, ek), (qv, ev) = e4m3(x[0]), e4m3(x[1])
                 self.k.append(qk * torch.exp2(ek.double())[..., None])
                 self.v.append(qv * torch.exp2(ev.double())[..., None])
+                self.scale.append(torch.exp2(ev.double()))
                 x = [qk.float().to(dtype).view(torch.uint8), qv.float().to(dtype).view(torch.uint8)]
             else:
                 self.k.append(x[0].double())
                 self.v.append(x[1].double())
+                self.scale.append(torch.ones(n, heads, dtype=torch.float64, device=DEV))
             if n == 0:
                 continue
             t = torch.arange(n, device=DEV)
@@ -77,15 +79,16 @@ def attention(pages, q, news, *, scale=None, window=0, sinks=0, softcap=0.0):
     Tolerances: a score's products are exact in float32 and summed over D terms (D 2^-24
     of their absolute sum), scaled (2 roundings), an exponent's 2^x is good to 2 ulp:
     E = (D + 4) 2^-24 |scale| sum|q k| + 4 2^-24 |s| (softcap: + softcap 2^-21) in the
-    score, 2^-22 + E in a weight.  Weights round to P = q's dtype (bfloat16 over 8 bits):
-    eps(P) / 2 of each, float16's below 2^-14 by 2^-25 of the largest; the sums over L
-    keys 2 L 2^-24.  With A = sum p |v|: A (eps(P) / 2 + 2 max E + 2^-20 + 2 L 2^-24)
-    + 2^-25 sum|v| in float16; rounding the result comes on top."""
+    score, 2^-22 + E in a weight.  Weights round to P = q's dtype: eps(P) / 2 of each,
+    float16's below 2^-14 by 2^-25 of the largest (8 bits: of the largest weight times its
+    scale 2^e, in units of the key's own scale); the sums over L keys 2 L 2^-24.  With A =
+    sum p |v|: A (eps(P) / 2 + 2 max E + 2^-20 + 2 L 2^-24), + 2^-25 sum|v| (8 bits: 2^-25
+    max(p 2^e) sum|v 2^-e|) in float16; rounding the result comes on top."""
     outs, tols, lses, tls, n = [], [], [], [], 0
     Hk, D = pages.cache.heads, pages.cache.dim
     G = q.size(1) // Hk
     scale = 1 / math.sqrt(D) if scale is None else scale
-    half = q.dtype == torch.float16 and pages.cache.dtype != torch.float8_e4m3fn
+    half = q.dtype == torch.float16
     eps = (2.0 ** -11 if half else 2.0 ** -8)
     for b, new in enumerate(news):
         L = int(pages.lengths[b])
@@ -116,7 +119,9 @@ def attention(pages, q, news, *, scale=None, window=0, sinks=0, softcap=0.0):
             A = w @ vz.abs()
             tol = A * (eps + 2 * E + 2.0 ** -20 + 2 * max(L, 1) * H24)
             if half:
-                tol = tol + 2.0 ** -25 * (seen.double() @ vz.abs())
+                e = pages.scale[b][:, h // G] if L > 0 else torch.ones(1, dtype=torch.float64, device=DEV)
+                tol = tol + 2.0 ** -25 * (w / w.amax(-1, keepdim=True).clamp(min=1e-300) * e).amax(-1, keepdim=True) \
+                    * w.amax(-1, keepdim=True) * (seen.double() @ (vz.abs() / e[:, None]))
             outs.append((n, new, h, o))
             tols.append(tol)
             lses.append((m + z.log()).squeeze(-1) if L > 0 else torch.full((new,), -math.inf, dtype=torch.float64, device=DEV))
