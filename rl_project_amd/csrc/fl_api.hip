@@ -166,6 +166,8 @@ int validate_attn(const char* fn, const fl_attn_args* a) {
                 static_cast<long long>(a->rows.tokens), static_cast<long long>(a->q_heads));
   if (!std::isfinite(a->scale) || !std::isfinite(a->softcap) || a->softcap < 0.0f)
     return fail(FL_EINVAL, "%s: scale must be finite, softcap finite and >= 0", fn);
+  if (a->softcap > 0.0f && !std::isfinite(4.0f * (a->scale / a->softcap)))
+    return fail(FL_EINVAL, "%s: scale / softcap beyond float32", fn);
   if (a->window < 0 || a->sinks < 0) return fail(FL_EINVAL, "%s: window and sinks must be >= 0", fn);
   if (a->q_ld < 0 || a->q_hs < 0 || a->out_ld < 0 || a->out_hs < 0 || ((a->q_ld | a->q_hs) & 7) != 0 ||
       ((a->out_ld | a->out_hs) & 3) != 0)

@@ -26,7 +26,7 @@ __device__ __forceinline__ void st16(void* p, uint4 x) { *static_cast<u32x4*>(p)
 // With an 8-bit cache the weights of the second product carry their values' scales,
 // 2^(s - m) 2^e.  bfloat16 has the range for any.  Half precision does not: there m is
 // the maximum of s + e, not of s, so that the weights that count are near 1 whatever
-// the scales (sums of 2^(s - m) stay in float32, where e of -96 to 92 leaves room).
+// the scales (sums of 2^(s - m) stay in float32, where e of -96 to 120 leaves room).
 struct OpBF16 {
   using D = BF16;
   typedef __bf16 x8 __attribute__((ext_vector_type(8)));

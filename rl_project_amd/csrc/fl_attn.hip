@@ -348,7 +348,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
           const int page = paged_page(a.rows, a.cache, s.b, t0 + k);
           if (!(x >= 0.0f) || page < 0) continue;   // (a NaN weight is in the sums already)
           const char* col = V + C::ESZ * ((static_cast<int64_t>(page) * Hk + h) * dim * S + ((t0 + k) & (S - 1)));
-const char* src = col + C::ESZ * (4 * g * S);
+          const char* src = col + C::ESZ * (4 * g * S);
 #pragma unroll
           for (int dm = 0; dm < DM; ++dm)
 #pragma unroll

@@ -493,7 +493,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
           for (int k = 0; k < 16; ++k) {
             const float x = wl[k * 32 + c];
             if (!(x >= 0.0f)) continue;   // (a NaN weight is in the sums already)
-const char* src = col + ESZ * (4 * hh * S + k);
+            const char* src = col + ESZ * (4 * hh * S + k);
 #pragma unroll
             for (int dm = 0; dm < DM; ++dm)
 #pragma unroll

@@ -839,6 +839,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("check_cache", &check_cache);
   m.def("cache_write", [](const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& k, const Tensor& v,
                           const Tensor& table, const Tensor& lengths, const OptTensor& starts) {
+    check_cache(ck, cv, ks, vs);
     VALUE_CHECK(k.dim() >= 3 && k.size(-1) == ck.size(3) && k.size(-2) == ck.size(1) && k.device() == ck.device(), "k must be [..., ",
                 ck.size(1), ", ", ck.size(3), "] on ", ck.device(), ", not ", k.sizes(), " on ", k.device());
     VALUE_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device(),
@@ -846,7 +847,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     SUPPORT_CHECK(is_row_type(k.scalar_type()) && (ck.scalar_type() == at::kFloat8_e4m3fn || k.scalar_type() == ck.scalar_type()),
                   k.scalar_type(), " keys into a ", ck.scalar_type(), " cache");
     check_tokens(ck, table, lengths, starts, lead_rows(k));
-    no_gradient("cache_write", graded(k) || graded(v));
+    no_gradient("cache_write", graded(k) || graded(v) || graded(ck) || graded(cv));
     refuse_tangents("cache_write", k, v);
     const at::NoGradGuard no_grad;
     cache_call({ck, cv, ks, vs}, k, v, table, lengths, starts, true);
@@ -854,10 +855,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cache_read", [](const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& table,
                          const Tensor& lengths, int64_t tokens, const OptTensor& starts, std::optional<at::ScalarType> dtype,
                          const OptTensor& out_k, const OptTensor& out_v) {
+    check_cache(ck, cv, ks, vs);
     const auto t = out_k ? out_k->scalar_type() : dtype ? *dtype : ck.scalar_type() == at::kFloat8_e4m3fn ? at::kFloat : ck.scalar_type();
     SUPPORT_CHECK(is_row_type(t), "dtype ", t, " is not supported (float32, bfloat16, float16)");
     VALUE_CHECK(tokens >= 0, "tokens ", tokens, " < 0");
     check_tokens(ck, table, lengths, starts, tokens);
+    no_gradient("cache_read", graded(ck) || graded(cv));
     const at::NoGradGuard no_grad;
     const int64_t shape[3] = {tokens, ck.size(1), ck.size(3)};
     for (const OptTensor* o : {&out_k, &out_v})
@@ -871,6 +874,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention", [](const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& q, const Tensor& table,
                         const Tensor& lengths, const OptTensor& starts, std::optional<double> scale, double softcap,
                         std::optional<int64_t> window, int64_t sinks, const OptTensor& into, bool lse) {
+    check_cache(ck, cv, ks, vs);
     VALUE_CHECK(q.dim() >= 3 && q.size(-1) == ck.size(3) && q.device() == ck.device(), "q must be [..., heads, ", ck.size(3), "] on ",
                 ck.device(), ", not ", q.sizes(), " on ", q.device());
     SUPPORT_CHECK((q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf) &&
@@ -879,7 +883,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     VALUE_CHECK(q.size(-2) >= 1 && q.size(-2) % ck.size(1) == 0, q.size(-2), " query heads over ", ck.size(1), " cached");
     check_tokens(ck, table, lengths, starts, lead_rows(q));
     VALUE_CHECK(window.value_or(0) >= 0 && sinks >= 0, "window and sinks must be >= 0");
-    no_gradient("paged_attention", graded(q));
+    no_gradient("paged_attention", graded(q) || graded(ck) || graded(cv));
     refuse_tangents("paged_attention", q);
     const at::NoGradGuard no_grad;
     OptTensor o;

@@ -263,7 +263,7 @@ __global__ __launch_bounds__(RP_NT, 4) void k_rope_grad(const fl_rope_grad_args 
   __shared__ float sum[RP_NT / WAVE][FL_ROPE_MAX_DIM];
   const bool key = blockIdx.y != 0;
   const int heads = static_cast<int>(key ? a.kv_heads : a.heads);
-  if (heads == 0) return;   // (nothing of this side is asked for)
+  if (heads == 0 && (key ? b.out_dwk : b.out_dwq) == nullptr) return;   // (a weight without heads has gradient 0)
   const void* x = key ? a.k : a.q;
   const void* grad = key ? b.grad_k : b.grad_q;
   const int64_t ld = key ? a.k_ld : a.q_ld, hs = key ? a.k_hs : a.q_hs;

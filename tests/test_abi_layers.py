@@ -123,7 +123,8 @@ def test_attention_refusals():
                        (dict(q_heads=3), EINVAL, "heads"), (dict(q_heads=0), EINVAL, "heads"), (dict(q_heads=1 << 17), ENOTSUP, "limits"),
                        (dict(scale=float("nan")), EINVAL, "scale"), (dict(softcap=-1.0), EINVAL, "softcap"), (dict(window=-1), EINVAL, "window"),
                        (dict(sinks=-1), EINVAL, "sinks"), (dict(q_ld=4), EINVAL, "strides"), (dict(out_hs=2), EINVAL, "strides"),
-                       (dict(out_ld=-4), EINVAL, "strides")]
+                       (dict(out_ld=-4), EINVAL, "strides"),
+                       (dict(scale=1e10, softcap=1e-30), EINVAL, "softcap")]
     _refused(L.fl_paged_attention, _lib.AttnArgs, base, bad + [
         (dict(q=None), EINVAL, "NULL"), (dict(q=4104), EINVAL, "aligned"), (dict(out=4100), EINVAL, "aligned"),
         (dict(rows=dict(table_width=100, table_ld=100)), EINVAL, "workspace"),
