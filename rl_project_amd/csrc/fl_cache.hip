@@ -19,31 +19,63 @@ namespace {
 constexpr int KV_NT = 256;
 constexpr int KV_MAX_C = FL_CACHE_MAX_DIM / 8 / 16;   // chunks of a thread
 
-// The scale's exponent for a row whose largest finite magnitude is m.
-__device__ __forceinline__ int kv_exponent(float m) {
-  if (m == 0.0f) return 0;
-  int e;
-  const float f = frexpf(m, &e);   // m = f 2^e, f in [0.5, 1); 448 = 0.875 2^9
-  return min(max(e - 9 + (f > 0.875f ? 1 : 0), -96), 120);
+// The scale's exponent for a row whose largest finite magnitude has the bits m: the
+// least e with m <= 448 2^e, 448 = 1.75 2^8.
+__device__ __forceinline__ int kv_exponent(uint32_t m) {
+  const int e = static_cast<int>((m + 0x1FFFFFu) >> 23) - 135;   // (a fraction above .75 carries)
+  return m == 0 ? 0 : min(max(e, -96), 120);
 }
 
-__device__ __forceinline__ float kv_finite(float x) { return fabsf(x) <= 0x1.fffffep127f ? fabsf(x) : 0.0f; }
+// The largest over a row's 16 lanes.
+template <int CTRL>
+__device__ __forceinline__ uint32_t kv_dpp_max(uint32_t v) {
+  return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, true)));
+}
+__device__ __forceinline__ uint32_t kv_row_max(uint32_t v) {
+  // lanes 1 and 2 apart, then the half row's and the row's mirror images
+  return kv_dpp_max<0x140>(kv_dpp_max<0x141>(kv_dpp_max<0x4E>(kv_dpp_max<0xB1>(v))));
+}
+constexpr uint32_t KV_INF = 0x7F800000u;
 
-// e4m3 of 8 values (a NaN's code for those that are not finite: the format has no
-// infinity)
+// e4m3 of 8 values of at most 448 (or NaN)
 __device__ __forceinline__ uint2 kv_e4m3(const float (&x)[8]) {
-  float y[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = fabsf(x[i]) <= 448.0f ? x[i] : __builtin_nanf("");
   uint2 o;
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-  o.x = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
-  o.y = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], w, true);
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  o.x = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4], x[5], 0, false);
+  o.y = __builtin_amdgcn_cvt_pk_fp8_f32(x[6], x[7], w, true);
   return o;
 }
 
-// 8 values of a row as floats (VEC: the row's chunks are 16-byte aligned)
+// Two values in 16 bits.
+template <class D>
+__device__ __forceinline__ uint32_t kv_pack(float lo, float hi) {
+  if constexpr (D::id == FL_DTYPE_BF16) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, bf16x2));
+  } else return D::from_f32(lo) | (D::from_f32(hi) << 16);
+}
+
+// 8 values of a 16-bit row as they are (VEC: the row's chunks are 16-byte aligned)
+template <bool VEC>
+__device__ __forceinline__ uint4 kv_raw(const void* row, int i) {
+  const uint16_t* p = static_cast<const uint16_t*>(row) + i;
+  if constexpr (VEC) return *reinterpret_cast<const uint4*>(p);
+  else return make_uint4(p[0] | (p[1] << 16), p[2] | (p[3] << 16), p[4] | (p[5] << 16), p[6] | (p[7] << 16));
+}
+template <bool VEC>
+__device__ __forceinline__ void kv_store_raw(void* row, int i, uint4 q) {
+  uint16_t* p = static_cast<uint16_t*>(row) + i;
+  if constexpr (VEC) *reinterpret_cast<uint4*>(p) = q;
+  else {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = static_cast<uint16_t>(e & 1 ? w[e / 2] >> 16 : w[e / 2]);
+  }
+}
+
+// ... and of any row as floats
 template <class D, bool VEC>
 __device__ __forceinline__ void kv_load(const void* row, int i, float (&x)[8]) {
   if constexpr (D::id == FL_DTYPE_F32) {
@@ -55,13 +87,7 @@ __device__ __forceinline__ void kv_load(const void* row, int i, float (&x)[8]) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = p[e];
     }
-  } else {
-    const uint16_t* p = static_cast<const uint16_t*>(row) + i;
-    if constexpr (VEC) RowChunk<D>::unpack(*reinterpret_cast<const uint4*>(p), x);
-    else
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = D::to_f32(p[e]);
-  }
+  } else RowChunk<D>::unpack(kv_raw<VEC>(row, i), x);
 }
 template <class D, bool VEC>
 __device__ __forceinline__ void kv_store(void* row, int i, const float (&x)[8]) {
@@ -74,17 +100,86 @@ __device__ __forceinline__ void kv_store(void* row, int i, const float (&x)[8]) 
 #pragma unroll
       for (int e = 0; e < 8; ++e) p[e] = x[e];
     }
-  } else {
-    uint16_t* p = static_cast<uint16_t*>(row) + i;
-    uint32_t h[8];
+  } else
+    kv_store_raw<VEC>(row, i, make_uint4(kv_pack<D>(x[0], x[1]), kv_pack<D>(x[2], x[3]), kv_pack<D>(x[4], x[5]), kv_pack<D>(x[6], x[7])));
+}
+
+// 8 e4m3 values times 2^e
+__device__ __forceinline__ void kv_floats(uint2 q, int e, float (&x)[8]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = D::from_f32(x[e]);
-    if constexpr (VEC)
-      *reinterpret_cast<uint4*>(p) = make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
-    else
-#pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] = static_cast<uint16_t>(h[e]);
+  for (int w = 0; w < 2; ++w) {
+    const int u = static_cast<int>(w == 0 ? q.x : q.y);
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(u, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(u, true);
+    x[4 * w] = ldexpf(lo[0], e), x[4 * w + 1] = ldexpf(lo[1], e);
+    x[4 * w + 2] = ldexpf(hi[0], e), x[4 * w + 3] = ldexpf(hi[1], e);
   }
+}
+
+// Values change between a lane's 8 channels of one token and 4 tokens of its 2
+// channels within a wave (whose four rows of 16 lanes are 4 tokens), so that LDS is
+// read and written by the dword: lanes 32 apart exchange dwords, then lanes 16 apart.
+// Both ways are their own inverse.
+__device__ __forceinline__ void kv_swap32(uint32_t& a, uint32_t& b) {   // a's upper lanes with b's lower ones
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0], b = r[1];
+}
+__device__ __forceinline__ void kv_swap16(uint32_t& a, uint32_t& b) {   // a's odd rows of lanes with b's even ones
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0], b = r[1];
+}
+// bytes of a (0 to 3) and b (4 to 7), the selector's lowest first
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t kv_perm(uint32_t a, uint32_t b) {
+  return __builtin_amdgcn_perm(b, a, SEL);
+}
+
+// Where the 16-byte piece p of a tile's values (a channel's 16 tokens in 8 bits, 8 of
+// them in 16) lies in LDS: the lanes of an access, 8 channels apart, in different banks.
+template <bool E8>
+__device__ __forceinline__ int kv_piece(int p) {
+  return p ^ ((p >> 4) & (E8 ? 7 : 3));
+}
+
+// The values of channels i to i + 7 of token t to LDS, and back (all lanes of a wave).
+__device__ __forceinline__ void kv_put8(uint16_t* tv, int i, int t, bool on, uint2 q) {
+  kv_swap32(q.x, q.y);
+  uint32_t a = kv_perm<0x05010400>(q.x, q.y), b = kv_perm<0x07030602>(q.x, q.y);
+  kv_swap16(a, b);
+  const int ch = i + 2 * (t & 3);
+  uint32_t* const to = reinterpret_cast<uint32_t*>(tv) + (t >> 2);
+  if (on) to[4 * kv_piece<true>(ch)] = kv_perm<0x05010400>(a, b), to[4 * kv_piece<true>(ch + 1)] = kv_perm<0x07030602>(a, b);
+}
+__device__ __forceinline__ uint2 kv_get8(const uint16_t* tv, int i, int t, bool on) {
+  const int ch = i + 2 * (t & 3);
+  const uint32_t* const from = reinterpret_cast<const uint32_t*>(tv) + (t >> 2);
+  uint32_t x = 0, y = 0;
+  if (on) x = from[4 * kv_piece<true>(ch)], y = from[4 * kv_piece<true>(ch + 1)];
+  uint32_t a = kv_perm<0x06040200>(x, y), b = kv_perm<0x07050301>(x, y);
+  kv_swap16(a, b);
+  uint2 q = make_uint2(kv_perm<0x06040200>(a, b), kv_perm<0x07050301>(a, b));
+  kv_swap32(q.x, q.y);
+  return q;
+}
+__device__ __forceinline__ void kv_put16(uint16_t* tv, int i, int t, bool on, uint32_t (&q)[4]) {
+  kv_swap32(q[0], q[2]), kv_swap32(q[1], q[3]);
+  kv_swap16(q[0], q[1]), kv_swap16(q[2], q[3]);
+  const int ch = i + 2 * (t & 3), half = t >> 3;
+  uint2* const to = reinterpret_cast<uint2*>(tv) + ((t >> 2) & 1);
+  if (on) {
+    to[2 * kv_piece<false>(2 * ch + half)] = make_uint2(kv_perm<0x05040100>(q[0], q[1]), kv_perm<0x05040100>(q[2], q[3]));
+    to[2 * kv_piece<false>(2 * ch + 2 + half)] = make_uint2(kv_perm<0x07060302>(q[0], q[1]), kv_perm<0x07060302>(q[2], q[3]));
+  }
+}
+__device__ __forceinline__ void kv_get16(const uint16_t* tv, int i, int t, bool on, uint32_t (&q)[4]) {
+  const int ch = i + 2 * (t & 3), half = t >> 3;
+  const uint2* const from = reinterpret_cast<const uint2*>(tv) + ((t >> 2) & 1);
+  uint2 x = make_uint2(0, 0), y = x;
+  if (on) x = from[2 * kv_piece<false>(2 * ch + half)], y = from[2 * kv_piece<false>(2 * ch + 2 + half)];
+  q[0] = kv_perm<0x05040100>(x.x, y.x), q[1] = kv_perm<0x07060302>(x.x, y.x);
+  q[2] = kv_perm<0x05040100>(x.y, y.y), q[3] = kv_perm<0x07060302>(x.y, y.y);
+  kv_swap16(q[0], q[1]), kv_swap16(q[2], q[3]);
+  kv_swap32(q[0], q[2]), kv_swap32(q[1], q[3]);
 }
 
 }  // namespace
@@ -95,54 +190,81 @@ __global__ __launch_bounds__(KV_NT) void k_cache_write(const fl_cache_args a, in
   const int Hk = static_cast<int>(a.cache.heads), h = blockIdx.x % Hk;
   __shared__ __attribute__((aligned(16))) uint16_t tv[FL_CACHE_MAX_DIM * KV_T];
   KvTile T;
-  if (!kv_tile(a.rows, a.cache, paged_seq(a.rows, blockIdx.x / Hk, 1, KV_T, 2, each), T) || T.page < 0) return;
+  if (!kv_tile(a.rows, a.cache, paged_seq(a.rows, blockIdx.x / Hk, 1, KV_T, 2, each), T)) return;
   const int t = threadIdx.x / 16, c0 = threadIdx.x % 16, dim = static_cast<int>(a.cache.dim);
   const int64_t ph = static_cast<int64_t>(T.page) * a.cache.heads + h, S = a.cache.page_size;
   const bool on = t >= T.t0 && t < T.t1;
-  float k[KV_MAX_C][8], v[KV_MAX_C][8], mk = 0.0f, mv = 0.0f;
+  constexpr int ESZ = D::id == FL_DTYPE_F32 ? 4 : 2;
+  const char* kp = static_cast<const char*>(a.k) + ((T.row0 + t) * a.k_ld + h * a.k_hs) * ESZ;
+  const char* vp = static_cast<const char*>(a.v) + ((T.row0 + t) * a.v_ld + h * a.v_hs) * ESZ;
+  const int64_t to = (ph * S + T.slot + t) * dim;
+  if constexpr (E8) {
+    float k[KV_MAX_C][8], v[KV_MAX_C][8];
+    uint32_t mk = 0, mv = 0;
 #pragma unroll
-  for (int c = 0; c < KV_MAX_C; ++c) {
-    const int i = 8 * (c0 + 16 * c);
-    if (!on || i >= dim) {
+    for (int c = 0; c < KV_MAX_C; ++c) {
+      if (128 * c >= dim) break;   // (the same for all: no instructions for channels that are not there)
+      const int i = 8 * (c0 + 16 * c);
 #pragma unroll
       for (int e = 0; e < 8; ++e) k[c][e] = v[c][e] = 0.0f;
-      continue;
+      if (on && i < dim) kv_load<D, VEC>(kp, i, k[c]), kv_load<D, VEC>(vp, i, v[c]);
     }
-    constexpr int ESZ = D::id == FL_DTYPE_F32 ? 4 : 2;
-    kv_load<D, VEC>(static_cast<const char*>(a.k) + ((T.row0 + t) * a.k_ld + h * a.k_hs) * ESZ, i, k[c]);
-    kv_load<D, VEC>(static_cast<const char*>(a.v) + ((T.row0 + t) * a.v_ld + h * a.v_hs) * ESZ, i, v[c]);
-    if constexpr (E8)
+    // (the page last: the rows are on their way before the table's entry is there)
+    asm volatile("" ::: "memory");
+    if (T.page < 0) return;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mk = fmaxf(mk, kv_finite(k[c][e])), mv = fmaxf(mv, kv_finite(v[c][e]));
-  }
-  int ek = 0, ev = 0;
-  if constexpr (E8) {
+    for (int c = 0; c < KV_MAX_C; ++c) {
+      if (128 * c >= dim) break;
 #pragma unroll
-    for (int m = 1; m < 16; m <<= 1) mk = fmaxf(mk, shfl_xor(mk, m)), mv = fmaxf(mv, shfl_xor(mv, m));
-    ek = kv_exponent(mk), ev = kv_exponent(mv);
+      for (int e = 0; e < 8; ++e)
+        mk = max(mk, __float_as_uint(k[c][e]) & 0x7FFFFFFFu), mv = max(mv, __float_as_uint(v[c][e]) & 0x7FFFFFFFu);
+    }
+    if (__any(max(mk, mv) >= KV_INF)) {   // infinities are NaN, and neither counts
+      mk = mv = 0;
+      const auto finite = [](float& x, uint32_t& m) {
+        const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
+        if (u >= KV_INF) x = __builtin_nanf("");
+        else m = max(m, u);
+      };
+#pragma unroll
+      for (int c = 0; c < KV_MAX_C; ++c) {
+        if (128 * c >= dim) break;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) finite(k[c][e], mk), finite(v[c][e], mv);
+      }
+    }
+    const int ek = kv_exponent(kv_row_max(mk)), ev = kv_exponent(kv_row_max(mv));
     if (on && c0 == 0) {
       a.cache.k_scale[ph * S + T.slot + t] = static_cast<uint8_t>(ek + 127);
       a.cache.v_scale[ph * S + T.slot + t] = static_cast<uint8_t>(ev + 127);
     }
-  }
-  uint8_t* tb = reinterpret_cast<uint8_t*>(tv);
 #pragma unroll
-  for (int c = 0; c < KV_MAX_C; ++c) {
-    const int i = 8 * (c0 + 16 * c);
-    if (!on || i >= dim) continue;
-    const int64_t at = (ph * S + T.slot + t) * dim + i;
-    if constexpr (E8) {
-      // (a power of two, and its own in two steps below 2^-126: exact)
+    for (int c = 0; c < KV_MAX_C; ++c) {
+      if (128 * c >= dim) break;
+      const int i = 8 * (c0 + 16 * c);
 #pragma unroll
       for (int e = 0; e < 8; ++e) k[c][e] = ldexpf(k[c][e], -ek), v[c][e] = ldexpf(v[c][e], -ev);
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.cache.k) + at) = kv_e4m3(k[c]);
-      const uint2 q = kv_e4m3(v[c]);
+      if (on && i < dim) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.cache.k) + to + i) = kv_e4m3(k[c]);
+      kv_put8(tv, i, t, i < dim, kv_e4m3(v[c]));
+    }
+  } else {
+    uint4 k[KV_MAX_C], v[KV_MAX_C];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) tb[(i + e) * KV_T + t] = static_cast<uint8_t>((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
-    } else {
-      kv_store<D, true>(static_cast<uint16_t*>(a.cache.k) + at, 0, k[c]);
+    for (int c = 0; c < KV_MAX_C; ++c) {
+      if (128 * c >= dim) break;
+      const int i = 8 * (c0 + 16 * c);
+      k[c] = v[c] = make_uint4(0, 0, 0, 0);
+      if (on && i < dim) k[c] = kv_raw<VEC>(kp, i), v[c] = kv_raw<VEC>(vp, i);
+    }
+    asm volatile("" ::: "memory");
+    if (T.page < 0) return;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) tv[(i + e) * KV_T + t] = static_cast<uint16_t>(D::from_f32(v[c][e]));
+    for (int c = 0; c < KV_MAX_C; ++c) {
+      if (128 * c >= dim) break;
+      const int i = 8 * (c0 + 16 * c);
+      if (on && i < dim) kv_store_raw<true>(static_cast<uint16_t*>(a.cache.k) + to, i, k[c]);
+      uint32_t q[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+      kv_put16(tv, i, t, i < dim, q);
     }
   }
   __syncthreads();
@@ -152,7 +274,7 @@ __global__ __launch_bounds__(KV_NT) void k_cache_write(const fl_cache_args a, in
     constexpr int Q = E8 ? 1 : 2;   // 16-byte pieces of a channel's 16 tokens
     for (int i = threadIdx.x; i < Q * dim; i += KV_NT) {
       const int64_t at = base + static_cast<int64_t>(i / Q) * S;
-      const uint4 q = reinterpret_cast<const uint4*>(tv)[i];
+      const uint4 q = reinterpret_cast<const uint4*>(tv)[kv_piece<E8>(i)];
       if constexpr (E8) *reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.cache.v) + at) = q;
       else reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.cache.v) + at)[i % Q] = q;
     }
@@ -160,8 +282,8 @@ __global__ __launch_bounds__(KV_NT) void k_cache_write(const fl_cache_args a, in
     for (int i = threadIdx.x; i < n * dim; i += KV_NT) {
       const int d = i / n, u = T.t0 + i % n;
       const int64_t at = base + static_cast<int64_t>(d) * S + u;
-      if constexpr (E8) static_cast<uint8_t*>(a.cache.v)[at] = tb[d * KV_T + u];
-      else static_cast<uint16_t*>(a.cache.v)[at] = tv[d * KV_T + u];
+      if constexpr (E8) static_cast<uint8_t*>(a.cache.v)[at] = reinterpret_cast<const uint8_t*>(tv)[16 * kv_piece<true>(d) + u];
+      else static_cast<uint16_t*>(a.cache.v)[at] = tv[8 * kv_piece<false>(2 * d + (u >> 3)) + (u & 7)];
     }
   }
 }
@@ -188,46 +310,62 @@ __global__ __launch_bounds__(KV_NT) void k_cache_read(const fl_cache_args a, int
   if (!kv_tile(a.rows, a.cache, s, T)) return;
   const int64_t ph = static_cast<int64_t>(max(T.page, 0)) * a.cache.heads + h, S = a.cache.page_size;
   const bool on = t >= T.t0 && t < T.t1;
+  // the keys are on their way beside the values
+  uint4 kq[KV_MAX_C];
+  int ek = 0, ev = 0;
+#pragma unroll
+  for (int c = 0; c < KV_MAX_C; ++c) {
+    if (128 * c >= dim) break;
+    const int i = 8 * (c0 + 16 * c);
+    kq[c] = make_uint4(0, 0, 0, 0);
+    if (!on || i >= dim) continue;
+    const int64_t at = (ph * S + T.slot + t) * dim + i;
+    if constexpr (E8) {
+      const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.cache.k) + at);
+      kq[c].x = q.x, kq[c].y = q.y;
+    } else kq[c] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.cache.k) + at);
+  }
+  if (E8 && on) {
+    ek = a.cache.k_scale[ph * S + T.slot + t] - 127;
+    ev = a.cache.v_scale[ph * S + T.slot + t] - 127;
+  }
   if (T.page >= 0) {
     constexpr int Q = E8 ? 1 : 2;
     const int64_t base = ph * dim * S + T.slot;
     for (int i = threadIdx.x; i < Q * dim; i += KV_NT) {
       const int64_t at = base + static_cast<int64_t>(i / Q) * S;
-      if constexpr (E8) reinterpret_cast<uint4*>(tv)[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.cache.v) + at);
-      else reinterpret_cast<uint4*>(tv)[i] = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.cache.v) + at)[i % Q];
+      uint4& to = reinterpret_cast<uint4*>(tv)[kv_piece<E8>(i)];
+      if constexpr (E8) to = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.cache.v) + at);
+      else to = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.cache.v) + at)[i % Q];
     }
   }
   __syncthreads();
-  if (!on) return;
-  const uint8_t* tb = reinterpret_cast<const uint8_t*>(tv);
-  int ek = 0, ev = 0;
-  if constexpr (E8) {
-    ek = a.cache.k_scale[ph * S + T.slot + t] - 127;
-    ev = a.cache.v_scale[ph * S + T.slot + t] - 127;
-  }
-  for (int i = 8 * c0; i < dim; i += 128) {
+#pragma unroll
+  for (int c = 0; c < KV_MAX_C; ++c) {
+    if (128 * c >= dim) break;
+    const int i = 8 * (c0 + 16 * c);
     float k[8], v[8];
-    if (T.page < 0) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) k[e] = v[e] = __builtin_nanf("");
-    } else if constexpr (E8) {
-      const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.cache.k) + (ph * S + T.slot + t) * dim + i);
-      typedef float f32x2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const int u = static_cast<int>(w == 0 ? q.x : q.y);
-        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(u, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(u, true);
-        k[4 * w] = ldexpf(lo[0], ek), k[4 * w + 1] = ldexpf(lo[1], ek);
-        k[4 * w + 2] = ldexpf(hi[0], ek), k[4 * w + 3] = ldexpf(hi[1], ek);
+    if constexpr (E8) {
+      kv_floats(make_uint2(kq[c].x, kq[c].y), ek, k);
+      kv_floats(kv_get8(tv, i, t, i < dim), ev, v);
+    } else {
+      RowChunk<C>::unpack(kq[c], k);
+      uint32_t q[4];
+      kv_get16(tv, i, t, i < dim, q);
+      if (O::id == C::id && T.page >= 0) {
+        if (on && i < dim) {
+          kv_store_raw<VEC>(static_cast<char*>(a.k) + ((T.row0 + t) * a.k_ld + h * a.k_hs) * ESZ, i, kq[c]);
+          kv_store_raw<VEC>(static_cast<char*>(a.v) + ((T.row0 + t) * a.v_ld + h * a.v_hs) * ESZ, i, make_uint4(q[0], q[1], q[2], q[3]));
+        }
+        continue;
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = ldexpf(__builtin_amdgcn_cvt_f32_fp8(tb[(i + e) * KV_T + t], 0), ev);
-    } else {
-      kv_load<C, true>(static_cast<const uint16_t*>(a.cache.k) + (ph * S + T.slot + t) * dim, i, k);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = C::to_f32(tv[(i + e) * KV_T + t]);
+      for (int e = 0; e < 8; ++e) v[e] = C::to_f32(e & 1 ? q[e / 2] >> 16 : q[e / 2] & 0xFFFFu);
     }
-    put(T.row0 + t, i, k, v);
+    if (T.page < 0)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) k[e] = v[e] = __builtin_nanf("");
+    if (on && i < dim) put(T.row0 + t, i, k, v);
   }
 }
 
