@@ -518,11 +518,12 @@ struct AttnCall {
 
 AttnCall attn_call(const fl_attn_args& a) {
   AttnCall c = {};
+  const int few_rows = a.cache.dtype == FL_DTYPE_E4M3 ? ATTN_FEW_ROWS8 : ATTN_FEW_ROWS;
   const int64_t G = a.q_heads / a.cache.heads, N = a.rows.tokens, B = a.rows.seqs, Hk = a.cache.heads;
   // The most rows that a sequence can have, and all have where there are no starts.
   const int64_t top = (a.rows.starts ? N : N / B) * G;
-  c.has_few = a.rows.starts || top <= ATTN_FEW_ROWS;
-  c.has_many = top > ATTN_FEW_ROWS;
+  c.has_few = a.rows.starts || top <= few_rows;
+  c.has_many = top > few_rows;
   const int64_t keys = a.rows.table_width * a.cache.page_size;
   // Splits: enough that every CU has `work` / 256 work-groups, and `least` of them, so
   // that long and short sequences share the CUs evenly (64 sequences of 1024 to 8192
@@ -540,15 +541,15 @@ AttnCall attn_call(const fl_attn_args& a) {
     c.stride = std::max<int64_t>(c.stride, p.splits > 1 ? p.splits : 0);
   };
   if (c.has_few) {
-    const int64_t rows = std::min<int64_t>(top, ATTN_FEW_ROWS);
+    const int64_t rows = std::min<int64_t>(top, few_rows);
     // (ragged: tiles of 16 where the average sequence fits one)
     const int tr = (a.rows.starts ? N * G <= 16 * B : top <= 16) ? 16 : 32;
-    c.few.min_rows = 0, c.few.max_rows = ATTN_FEW_ROWS;
+    c.few.min_rows = 0, c.few.max_rows = few_rows;
     c.few.each = static_cast<int>((rows + tr - 1) / tr);
     plan(c.few, tr, B * Hk, 1024, 4);
   }
   if (c.has_many) {
-    c.many.min_rows = c.has_few ? ATTN_FEW_ROWS + 1 : 0, c.many.max_rows = 0x7fffffff;
+    c.many.min_rows = c.has_few ? few_rows + 1 : 0, c.many.max_rows = 0x7fffffff;
     c.many.each = a.rows.starts ? 0 : static_cast<int>((top + ATTN_WIDE_ROWS - 1) / ATTN_WIDE_ROWS);
     const int64_t tiles = a.rows.starts ? std::max<int64_t>((N - B) * G / ATTN_WIDE_ROWS, 1) : B * c.many.each;
     plan(c.many, ATTN_WIDE_ROWS, tiles * Hk, 512, 1);

@@ -408,7 +408,8 @@ int rp_lanes(int64_t dim, int N) {
   return L;
 }
 // Tokens of a work-group: 4 share one round of sines and cosines where that still
-// leaves four work-groups for every CU.
+// leaves four work-groups for every CU (8192 tokens: 34 us against 39 with one; 512: 10
+// against 6.5).
 int rp_tokens(int64_t tokens) { return tokens >= 4096 ? 4 : 1; }
 
 }  // namespace
