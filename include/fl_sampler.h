@@ -732,7 +732,8 @@ int fl_cache_read(const fl_cache_args* args, void* stream);
  * dtype (BF16 or F16; a 16-bit cache's own) and strides of their own, the last
  * dimension contiguous: q 16-byte aligned with strides in multiples of 8 elements,
  * out 8-byte with multiples of 4.  Scores, sums and results in float32; the weights
- * exp(s - max) are rounded to dtype for the product with v.  A token's results
+ * exp(s - max) are rounded to dtype for the product with v (over FL_DTYPE_E4M3, times
+ * their values' scales, to bfloat16, or to 16 bits for F16 queries).  A token's results
  * depend on the shapes of the call (how its keys are split), not on other tokens.
  * workspace (fl_paged_attention_workspace_bytes for the same args, 16-byte aligned):
  * calls that overlap in time must not share one.

@@ -138,7 +138,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, len
     A token that sees nothing has 0 and -inf.  What a slot holds that a token does
     not see, NaN and infinity included, has no part in its result; values seen are
     taken up to 2^100 in magnitude.  Sums in float32; the weights are rounded once
-    to ``q``'s dtype for the product with the values.
+    for the product with the values: to ``q``'s dtype, over 8 bits (where they carry
+    their values' scales) to bfloat16, of float16 queries to 16 bits of precision.
     One or two launches, without host synchronisation; results are the same each
     time, and depend on how the call's shapes split the keys in the last bits."""
     _check_cache(cache)

@@ -2,6 +2,8 @@
 // keys that a tile of queries sees, how they are split, and the partial results.
 #pragma once
 
+#include <type_traits>
+
 #include "fl_kernels.h"
 #include "fl_paged.h"
 
@@ -24,9 +26,10 @@ __device__ __forceinline__ void st16(void* p, uint4 x) { *static_cast<u32x4*>(p)
 // 16-bit operands: 8 values of a lane as a uint4.
 //
 // With an 8-bit cache the weights of the second product carry their values' scales,
-// 2^(s - m) 2^e.  bfloat16 has the range for any.  Half precision does not: there m is
-// the maximum of s + e, not of s, so that the weights that count are near 1 whatever
-// the scales (sums of 2^(s - m) stay in float32, where e of -96 to 120 leaves room).
+// 2^(s - m) 2^e.  bfloat16 has the range for any, half precision has not, and no maximum
+// brings those that count near 1: a token whose values are all 0 may have any scale.
+// So over 8 bits the second product is in bfloat16 (which holds e4m3 as well), of float16
+// queries with the weights as two bfloat16, the second what the first leaves: 16 bits.
 struct OpBF16 {
   using D = BF16;
   typedef __bf16 x8 __attribute__((ext_vector_type(8)));
@@ -69,6 +72,16 @@ struct OpF16 {
                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q, f, true)));
   }
 };
+
+// The second product's type, and whether its weights are two.
+template <class Op, bool E8>
+using OpValues = std::conditional_t<E8, OpBF16, Op>;
+template <class Op, bool E8>
+constexpr bool TWO_WEIGHTS = E8 && !std::is_same_v<Op, OpBF16>;
+// What bfloat16 leaves of lo and hi, which it holds as w.
+__device__ __forceinline__ uint32_t weights_rest(uint32_t w, float lo, float hi) {
+  return OpBF16::pack(lo - __uint_as_float(w << 16), hi - __uint_as_float(w & 0xFFFF0000u));
+}
 
 // The bits of 0x8000 where a 16-bit value of a dword is NaN or infinite.
 template <class Op>

@@ -65,6 +65,8 @@ __device__ __forceinline__ uint4 ar_load16_8(const char* p) {
 template <class C, int DT, bool FULL, int CT>
 __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(const fl_attn_args a, const AttnPlan p) {
   using Op = typename C::Op;
+  using VOp = OpValues<Op, C::E8>;
+  constexpr bool TWO = TWO_WEIGHTS<Op, C::E8>;
   constexpr int KS = DT / 32;   // steps of the first product
   constexpr int DM = DT / 16;   // tiles of channels of the second
   // tiles of values that are loaded ahead of their step's softmax: what registers hold
@@ -227,8 +229,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
 
     // ------------------------------------------------ the weights
     const bool masked = !v.whole(t0) || __any(some_bad);
-    uint4 pf[CT][2];
-    float pw[CT][16];
+    uint4 pf[CT][2], pr[TWO ? CT : 1][2];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       float x[16];
@@ -259,16 +260,8 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
           }
       }
       float top = -INFINITY;
-      if constexpr (C::E8 && !Op::SCALES) {   // (of the weights with their values' scales, fl_attn.h)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            top = fmaxf(top, x[4 * j + e] + static_cast<float>((j == 0 ? ev.x : j == 1 ? ev.y : j == 2 ? ev.z : ev.w) >> (8 * e) & 255u));
-        top -= 127.0f;
-      } else
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, x[e]);
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, x[e]);
       if (__any(top > m[ct] + AT_LAZY)) {   // (m = -inf at first)
         top = fmaxf(top, shfl_xor(top, 16));
         top = fmaxf(top, shfl_xor(top, 32));
@@ -295,10 +288,14 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        pf[ct][u] = make_uint4(Op::pack(x[8 * u], x[8 * u + 1]), Op::pack(x[8 * u + 2], x[8 * u + 3]),
-                               Op::pack(x[8 * u + 4], x[8 * u + 5]), Op::pack(x[8 * u + 6], x[8 * u + 7]));
+        pf[ct][u] = make_uint4(VOp::pack(x[8 * u], x[8 * u + 1]), VOp::pack(x[8 * u + 2], x[8 * u + 3]),
+                               VOp::pack(x[8 * u + 4], x[8 * u + 5]), VOp::pack(x[8 * u + 6], x[8 * u + 7]));
+      if constexpr (TWO)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) pw[ct][e] = x[e];
+        for (int u = 0; u < 2; ++u)
+          pr[ct][u] = make_uint4(weights_rest(pf[ct][u].x, x[8 * u], x[8 * u + 1]), weights_rest(pf[ct][u].y, x[8 * u + 2], x[8 * u + 3]),
+                                 weights_rest(pf[ct][u].z, x[8 * u + 4], x[8 * u + 5]),
+                                 weights_rest(pf[ct][u].w, x[8 * u + 6], x[8 * u + 7]));
     }
 
     // ------------------------------------------------ O^T += V^T P^T
@@ -312,7 +309,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
       uint4 vf[2];
       if constexpr (C::E8) {
         const uint4 x = vr[dm][0];
-        const uint2 y0 = Op::widen(x.x), y1 = Op::widen(x.y), y2 = Op::widen(x.z), y3 = Op::widen(x.w);
+        const uint2 y0 = VOp::widen(x.x), y1 = VOp::widen(x.y), y2 = VOp::widen(x.z), y3 = VOp::widen(x.w);
         vf[0] = make_uint4(y0.x, y0.y, y1.x, y1.y);
         vf[1] = make_uint4(y2.x, y2.y, y3.x, y3.y);
       } else {
@@ -320,13 +317,17 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
         vf[1] = vr[dm][C::SUBS - 1];
       }
       if (masked) {
-        odd |= not_finite<Op>(vf[0]) | not_finite<Op>(vf[1]);
-        vf[0] = finite_or_0<Op>(vf[0]), vf[1] = finite_or_0<Op>(vf[1]);
+        odd |= not_finite<VOp>(vf[0]) | not_finite<VOp>(vf[1]);
+        vf[0] = finite_or_0<VOp>(vf[0]), vf[1] = finite_or_0<VOp>(vf[1]);
       }
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        o[ct][dm] = Op::mfma16(vf[0], pf[ct][0], o[ct][dm]);
-        o[ct][dm] = Op::mfma16(vf[1], pf[ct][1], o[ct][dm]);
+        o[ct][dm] = VOp::mfma16(vf[0], pf[ct][0], o[ct][dm]);
+        o[ct][dm] = VOp::mfma16(vf[1], pf[ct][1], o[ct][dm]);
+        if constexpr (TWO) {
+          o[ct][dm] = VOp::mfma16(vf[0], pr[ct][0], o[ct][dm]);
+          o[ct][dm] = VOp::mfma16(vf[1], pr[ct][1], o[ct][dm]);
+        }
       }
     }
     if (masked && __any(odd != 0)) {
@@ -342,7 +343,9 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
             const int k = C::key(g, j) + e;
             const int t = t0 + k;
             const bool seen = (t <= see[ct].last) & ((t >= see[ct].from) | (t < v.sinks));
-            wl[k * 16 + c] = seen ? pw[ct][4 * j + e] : -1.0f;
+            const uint4 y = pf[ct][j >> 1];
+            const uint32_t x = j & 1 ? (e < 2 ? y.z : y.w) : (e < 2 ? y.x : y.y);
+            wl[k * 16 + c] = seen ? VOp::D::to_f32((e & 1 ? x >> 16 : x) & 0xFFFFu) : -1.0f;
           }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();

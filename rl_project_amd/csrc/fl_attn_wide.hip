@@ -31,7 +31,7 @@ constexpr int AW_NT = 256, AW_NW = AW_NT / WAVE;
 // Bytes of LDS of a work-group: two turns of 64 keys, their values, and 8-bit scales.
 constexpr int aw_lds(int DT, bool E8, bool FULL) {
   const int pad = FULL && !E8 ? 0 : 16;
-  return 2 * (AT_BLK * (2 * DT + pad) + DT * (2 * AT_BLK + pad) + (E8 ? 3 * AT_BLK * 4 : 0));
+  return 2 * (AT_BLK * (2 * DT + pad) + DT * (2 * AT_BLK + pad) + (E8 ? 2 * AT_BLK * 4 : 0));
 }
 
 // Tiles without padding have their rows' chunks exchanged instead (by an exclusive or),
@@ -76,6 +76,8 @@ __device__ __forceinline__ void aw_reads_ahead() {
 // FULL: dim == DT, QT: tiles of 32 rows of a wave.
 template <class Op, bool E8, int DT, bool FULL, int QT>
 __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wide(const fl_attn_args a, const AttnPlan p) {
+  using VOp = OpValues<Op, E8>;
+  constexpr bool TWO = TWO_WEIGHTS<Op, E8>;
   constexpr int TR = 32 * QT * AW_NW;
   constexpr int ESZ = E8 ? 1 : 2, EPC = 16 / ESZ;         // the cache's elements, and those of a 16-byte chunk
   // 16-bit tiles go to LDS as they lie, without registers; 8-bit ones and padded rows
@@ -85,7 +87,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
   constexpr int NK = AT_BLK * KC / AW_NT, NV = DT * VC / AW_NT;   // chunks of a thread
   constexpr int PAD = DIRECT ? 0 : 16;
   constexpr int KS = 2 * DT + PAD, VS = 2 * AT_BLK + PAD;   // LDS row strides in bytes
-  constexpr int KB = AT_BLK * KS, VB = DT * VS, SB = E8 ? 3 * AT_BLK * 4 : 0;
+  constexpr int KB = AT_BLK * KS, VB = DT * VS, SB = E8 ? 2 * AT_BLK * 4 : 0;
   constexpr int BUF = KB + VB + SB;
   static_assert(aw_lds(DT, E8, FULL) == 2 * BUF, "the launch's LDS");
   constexpr int KSTEPS = DT / 16, DM = DT / 32;
@@ -263,7 +265,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
       }
     }
     if constexpr (E8) {
-      if (tid < 3 * AT_BLK) {   // keys' scales, values' scales, values' exponents
+      if (tid < 2 * AT_BLK) {   // keys' scales, values' scales
         const int t = tid & (AT_BLK - 1);
         const uint8_t* src = tid < AT_BLK ? a.cache.k_scale : a.cache.v_scale;
         sc8 = src[(static_cast<int64_t>(pick(t >> 4)) * Hk + h) * S + ((t0 + t) & mask)];
@@ -293,20 +295,19 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
       // the rows that see them.
       const auto put = [&](char* to, uint4 x) {
         if (!whole) {
-          odd |= not_finite<Op>(x);
-          x = finite_or_0<Op>(x);
+          odd |= not_finite<VOp>(x);
+          x = finite_or_0<VOp>(x);
         }
         st16(to, x);
       };
       if constexpr (E8) {
-        const uint2 y0 = Op::widen(vr[n].x), y1 = Op::widen(vr[n].y), y2 = Op::widen(vr[n].z), y3 = Op::widen(vr[n].w);
+        const uint2 y0 = VOp::widen(vr[n].x), y1 = VOp::widen(vr[n].y), y2 = VOp::widen(vr[n].z), y3 = VOp::widen(vr[n].w);
         put(dst, make_uint4(y0.x, y0.y, y1.x, y1.y));
         put(dst + 16, make_uint4(y2.x, y2.y, y3.x, y3.y));
       } else put(dst, vr[n]);
     }
     if constexpr (E8)
-      if (tid < 3 * AT_BLK)
-        reinterpret_cast<float*>(buf + KB + VB)[tid] = tid < 2 * AT_BLK ? scale_of(sc8) : static_cast<float>(sc8) - 127.0f;
+      if (tid < 2 * AT_BLK) reinterpret_cast<float*>(buf + KB + VB)[tid] = scale_of(sc8);
     if (!whole && __any(odd != 0) && lane == 0) atomicOr(&flags[turn], 16);
     if (bad != 0 && tid == 0) atomicOr(&flags[turn], bad);
   };
@@ -395,19 +396,11 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
           }
       }
       float top = -INFINITY;
-      if constexpr (E8 && !Op::SCALES) {   // (of the weights with their values' scales, fl_attn.h)
-        const float* se = reinterpret_cast<const float*>(vb + VB) + 2 * AT_BLK + 8 * hh;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+      for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) top = fmaxf(top, fmaf(st[t][kt][e], to2, se[32 * kt + 16 * (e >> 3) + (e & 7)]));
-      } else {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) top = fmaxf(top, st[t][kt][e]);
-        top *= to2;
-      }
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, st[t][kt][e]);
+      top *= to2;
       if (__any(top > m[t] + AT_LAZY)) {
         top = fmaxf(top, shfl_xor(top, 32));
         const float to = fmaxf(m[t], top);
@@ -423,7 +416,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
 
     // -------------------------------------------------- O^T += V^T P^T
     // 16 keys a time: the next 16's weights and values beside this 16's products
-    uint4 pf[QT][4], vf[2][DM];
+    uint4 pf[QT][4], pr[TWO ? QT : 1][2], vf[2][DM];
     const auto weights = [&](int u) {
       const int kt = u >> 1, e0 = 8 * (u & 1);
       float x[QT][8];
@@ -445,8 +438,13 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
       }
 #pragma unroll
       for (int t = 0; t < QT; ++t)
-        pf[t][u] = make_uint4(Op::pack(x[t][0], x[t][1]), Op::pack(x[t][2], x[t][3]), Op::pack(x[t][4], x[t][5]),
-                              Op::pack(x[t][6], x[t][7]));
+        pf[t][u] = make_uint4(VOp::pack(x[t][0], x[t][1]), VOp::pack(x[t][2], x[t][3]), VOp::pack(x[t][4], x[t][5]),
+                              VOp::pack(x[t][6], x[t][7]));
+      if constexpr (TWO)
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+          pr[t][u & 1] = make_uint4(weights_rest(pf[t][u].x, x[t][0], x[t][1]), weights_rest(pf[t][u].y, x[t][2], x[t][3]),
+                                    weights_rest(pf[t][u].z, x[t][4], x[t][5]), weights_rest(pf[t][u].w, x[t][6], x[t][7]));
     };
     const auto values = [&](int u) {
 #pragma unroll
@@ -464,12 +462,15 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
 #pragma unroll
       for (int dm = 0; dm < DM; ++dm)
 #pragma unroll
-        for (int t = 0; t < QT; ++t) o[t][dm] = Op::mfma32(vf[u & 1][dm], pf[t][u], o[t][dm]);
+        for (int t = 0; t < QT; ++t) {
+          o[t][dm] = VOp::mfma32(vf[u & 1][dm], pf[t][u], o[t][dm]);
+          if constexpr (TWO) o[t][dm] = VOp::mfma32(vf[u & 1][dm], pr[t][u & 1], o[t][dm]);
+        }
       if (u < 3) {
         weights(u + 1);
         __builtin_amdgcn_sched_group_barrier(0x100, DM, 0);
 #pragma unroll
-        for (int i = 0; i < DM * QT; ++i) {
+        for (int i = 0; i < DM * QT * (TWO ? 2 : 1); ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
           __builtin_amdgcn_sched_group_barrier(0x002, 36 / DM, 0);
         }
@@ -490,7 +491,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
             const int k = t0 + 16 * u + 8 * hh + e;
             const bool seen = (k <= see[t].last) & ((k >= see[t].from) | (k < v.sinks));
             const uint32_t x = e < 2 ? pf[t][u].x : e < 4 ? pf[t][u].y : e < 6 ? pf[t][u].z : pf[t][u].w;
-            wl[(8 * hh + e) * 32 + c] = seen ? Op::D::to_f32((e & 1 ? x >> 16 : x) & 0xFFFFu) : -1.0f;
+            wl[(8 * hh + e) * 32 + c] = seen ? VOp::D::to_f32((e & 1 ? x >> 16 : x) & 0xFFFFu) : -1.0f;
           }
           __syncthreads();
           const int page = paged_page(a.rows, a.cache, s.b, t0 + 16 * u);
