@@ -105,13 +105,58 @@ __device__ __forceinline__ uint4 finite_or_0(uint4 q) {
 
 constexpr float AT_LAZY = 8.0f;     // how far, in powers of two, scores may pass the maximum in use
 
-// One score's soft-cap, in powers of two afterwards.  tanh x = 1 - 2 / (e^2x + 1):
-// off by 2^-23 of 1, i.e. by cap 2^-23 in the score, far below the rounding of q k.
-__device__ __forceinline__ float attn_cap(float s, float to_z, float cap2) {
-  const float e = __builtin_amdgcn_exp2f(s * to_z);   // to_z = 2 log2(e) scale / cap
-  return cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(e + 1.0f);   // cap2 = cap log2(e)
+// A lane's 16 scores' soft-cap, in powers of two afterwards: cap tanh(z) log2(e), z = s scale / cap.
+//
+// Caps up to 64: 1 - 2 / (e^2z + 1), off by 10 2^-24 cap whatever the score, that is by
+// 4e-5 in a score and in its weight, which is rounded to 2^-9 or 2^-11 of itself after.
+// Above, that error would grow with the cap (a score of 0.3 is off by a thousandth at a
+// cap of 1e4, and gone at 1e8), so there
+//   |z| < 0.625: tanh z = z + z^3 p(z^2), the samplers' polynomial, on the score itself,
+//     x + x z^2 p: as near to a score far below the cap as without one
+//   above: 1 - 2 / (e^2|z| + 1), off by 5 2^-24 of 0.55 and more: 2^-20 of the score
+// with the second left out where no lane of the wave needs it.  (4096 tokens of 8192,
+// scores of 2: 552 us in the first form, 612 with the polynomial, 829 with both.)
+constexpr float AT_SMALL_CAP = 64.0f;
+struct AttnCap {
+  float to_z, to2, cap2;   // of s q k: scale / cap, scale log2(e), cap log2(e)
+  bool small;
+};
+__device__ __forceinline__ AttnCap attn_cap_of(float scale, float cap) {
+  const float LOG2E = 1.4426950408889634f;
+  return {cap > 0.0f ? scale / cap : 0.0f, scale * LOG2E, fminf(cap * LOG2E, 3.4028235e38f), cap <= AT_SMALL_CAP};
 }
-
+template <class X>
+__device__ __forceinline__ void attn_cap(X& s, const AttnCap& c) {
+  if (c.small) {
+    const float to_e = c.to_z * 2.8853900817779268f;   // 2 log2(e)
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      s[e] = c.cap2 - 2.0f * c.cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[e] * to_e) + 1.0f);
+    return;
+  }
+  float top = 0.0f, x[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(s[e]));
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const float z = s[e] * c.to_z, y = s[e] * c.to2, t = z * z;
+    float p = fmaf(t, TANH_P[5], TANH_P[4]);
+#pragma unroll
+    for (int i = 3; i >= 0; --i) p = fmaf(t, p, TANH_P[i]);
+    x[e] = fmaf(y * t, p, y);
+  }
+  if (__any(top * fabsf(c.to_z) >= 0.625f)) {
+    float to_e = 2.8853900817779268f;
+    asm volatile("" : "+v"(to_e));   // (a branch, not both forms always)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float z = s[e] * c.to_z, y = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(fabsf(z) * to_e) + 1.0f);
+      if (!(fabsf(z) < 0.625f)) x[e] = copysignf(c.cap2 * fmaf(-2.0f, y, 1.0f), z);   // (a NaN stays NaN)
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) s[e] = x[e];
+}
 
 // The kernel for many rows: its tiles, and the rows of a sequence (tokens by heads of a
 // group) up to which fl_attn.hip's is taken: 32 sequences of up to 4096, 40 and 64 rows, that

@@ -116,8 +116,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
 #pragma unroll
     for (int i = 0; i < DM; ++i) o[ct][i] = (f32x4){0, 0, 0, 0};
   }
-  const float LOG2E = 1.4426950408889634f;
-  const float to2 = a.scale * LOG2E, cap2 = a.softcap * LOG2E, to_z = a.softcap > 0 ? 2.0f * LOG2E * a.scale / a.softcap : 0.0f;
+  const AttnCap cap = attn_cap_of(a.scale, a.softcap);
   const int64_t S = a.cache.page_size;
   const char* K = static_cast<const char*>(a.cache.k);
   const char* V = static_cast<const char*>(a.cache.v);
@@ -241,12 +240,10 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
           if constexpr (C::E8) y *= scale_of((j == 0 ? ek.x : j == 1 ? ek.y : j == 2 ? ek.z : ek.w) >> (8 * e) & 255u);
           x[4 * j + e] = y;
         }
-      if (a.softcap > 0.0f) {
+      if (a.softcap > 0.0f) attn_cap(x, cap);
+      else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = attn_cap(x[e], to_z, cap2);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] *= to2;
+        for (int e = 0; e < 16; ++e) x[e] *= cap.to2;
       }
       if (masked) {
 #pragma unroll

@@ -107,12 +107,11 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
   const int b1 = static_cast<uint32_t>(v.blocks) * (split + 1) / static_cast<uint32_t>(v.splits);
 
   // a negative scale turns the queries' signs
-  const float LOG2E = 1.4426950408889634f;
   // (and one of 0 clears them: a masked score is -inf, which no factor may be 0 to)
   const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : ~0u;
   const float scale = fabsf(a.scale);
-  const float to2 = a.softcap > 0.0f || a.scale == 0.0f ? 1.0f : scale * LOG2E;
-  const float cap2 = a.softcap * LOG2E, to_z = a.softcap > 0.0f ? 2.0f * LOG2E * scale / a.softcap : 0.0f;
+  const float to2 = a.softcap > 0.0f || a.scale == 0.0f ? 1.0f : scale * 1.4426950408889634f;
+  const AttnCap cap = attn_cap_of(scale, a.softcap);
 
   uint4 q[QT][KSTEPS];
   AttnSeen see[QT];
@@ -379,10 +378,8 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       if (a.softcap > 0.0f) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) st[t][kt][e] = attn_cap(st[t][kt][e], to_z, cap2);
+        attn_cap(st[t][0], cap);
+        attn_cap(st[t][1], cap);
       }
       if (masked) {
 #pragma unroll
