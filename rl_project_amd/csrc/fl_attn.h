@@ -134,28 +134,26 @@ __device__ __forceinline__ void attn_cap(X& s, const AttnCap& c) {
       s[e] = c.cap2 - 2.0f * c.cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[e] * to_e) + 1.0f);
     return;
   }
-  float top = 0.0f, x[16];
+  float top = 0.0f;
 #pragma unroll
   for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(s[e]));
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const float z = s[e] * c.to_z, y = s[e] * c.to2, t = z * z;
+  const auto near = [&](float x) {
+    const float z = x * c.to_z, y = x * c.to2, t = z * z;
     float p = fmaf(t, TANH_P[5], TANH_P[4]);
 #pragma unroll
     for (int i = 3; i >= 0; --i) p = fmaf(t, p, TANH_P[i]);
-    x[e] = fmaf(y * t, p, y);
-  }
-  if (__any(top * fabsf(c.to_z) >= 0.625f)) {
-    float to_e = 2.8853900817779268f;
-    asm volatile("" : "+v"(to_e));   // (a branch, not both forms always)
+    return fmaf(y * t, p, y);
+  };
+  if (!__any(top * fabsf(c.to_z) >= 0.625f)) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = near(s[e]);
+  } else {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const float z = s[e] * c.to_z, y = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(fabsf(z) * to_e) + 1.0f);
-      if (!(fabsf(z) < 0.625f)) x[e] = copysignf(c.cap2 * fmaf(-2.0f, y, 1.0f), z);   // (a NaN stays NaN)
+      const float z = s[e] * c.to_z, r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(fabsf(z) * 2.8853900817779268f) + 1.0f);
+      s[e] = fabsf(z) < 0.625f ? near(s[e]) : copysignf(c.cap2 * fmaf(-2.0f, r, 1.0f), z);   // (a NaN stays NaN)
     }
   }
-#pragma unroll
-  for (int e = 0; e < 16; ++e) s[e] = x[e];
 }
 
 // The kernel for many rows: its tiles, and the rows of a sequence (tokens by heads of a
