@@ -262,7 +262,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
       if (__any(top > m[ct] + AT_LAZY)) {   // (m = -inf at first)
         top = fmaxf(top, shfl_xor(top, 16));
         top = fmaxf(top, shfl_xor(top, 32));
-        const float to = fmaxf(m[ct], top);
+        const float to = top > m[ct] + AT_LAZY ? top : m[ct];   // (each row by its own scores)
         const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - to);
         m[ct] = to;
         l[ct] *= f;

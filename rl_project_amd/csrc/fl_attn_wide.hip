@@ -400,7 +400,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
       top *= to2;
       if (__any(top > m[t] + AT_LAZY)) {
         top = fmaxf(top, shfl_xor(top, 32));
-        const float to = fmaxf(m[t], top);
+        const float to = top > m[t] + AT_LAZY ? top : m[t];   // (each row by its own scores)
         const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[t] - to);
         m[t] = to;
         l[t] *= f;
