@@ -140,7 +140,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, len
     taken up to 2^100 in magnitude.  Sums in float32; the weights are rounded once
     for the product with the values: to ``q``'s dtype, over 8 bits (where they carry
     their values' scales) to bfloat16, of float16 queries to 16 bits of precision.
-    One or two launches, without host synchronisation; results are the same each
+    One to three launches (with ``starts`` one for each kind of sequence, and the joining
+    of split ones), without host synchronisation; results are the same each
     time, and depend on how the call's shapes split the keys in the last bits."""
     _check_cache(cache)
     o, lse = _lib.autograd().attention(cache.k, cache.v, cache.k_scale, cache.v_scale, q, table, lengths, starts, scale, softcap,

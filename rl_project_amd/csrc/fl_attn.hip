@@ -405,6 +405,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
       const int i = r / p.group;
       if (s.pos + i >= a.rows.table_width * S) ll = __builtin_nanf("");
       const int64_t head = h * p.group + (r - i * p.group), row = (s.row + i) * a.q_heads + head;
+      const int64_t place = attn_place(p, s.b, Hk, h, r, row) * p.splits + split;
       const float inv = v.splits > 1 ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
       for (int d = 4 * k; d < DT; d += 64) {
@@ -412,7 +413,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
         f32x4 y = *reinterpret_cast<const f32x4*>(&so[0][rr][d]);
 #pragma unroll
         for (int x = 1; x < AR_NW; ++x) y += *reinterpret_cast<const f32x4*>(&so[x][rr][d]);
-        if (v.splits > 1) *reinterpret_cast<f32x4*>(p.part + (row * p.stride + split) * dim + d) = y;
+        if (v.splits > 1) *reinterpret_cast<f32x4*>(p.part + place * dim + d) = y;
         else {
           y *= inv;
           *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (s.row + i) * a.out_ld + head * a.out_hs + d) =
@@ -420,7 +421,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
         }
       }
       if (k == 0) {
-        if (v.splits > 1) *reinterpret_cast<float2*>(p.stat + 2 * (row * p.stride + split)) = make_float2(mm, ll);
+        if (v.splits > 1) *reinterpret_cast<float2*>(p.stat + 2 * place) = make_float2(mm, ll);
         else if (a.out_lse) a.out_lse[row] = ll == 0.0f ? -INFINITY : (mm == -INFINITY ? ll : (mm + log2f(ll)) * 0.6931471805599453f);
       }
     }
@@ -428,50 +429,65 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
   }
 }
 
-// The parts of rows whose keys were split.  A work-group looks at `rb` rows (a thread
+// The parts of rows whose keys were split.  A work-group looks at `rb` places (a thread
 // each), and joins those that have parts: `tpr` threads a part (4 channels each), its
-// groups different parts.  few and many: the plans of sequences of few rows and of many.
+// groups different parts.  few and many: the plans of sequences of few rows and of many;
+// the first `by_row` places are the call's rows, the others few's slots.
 constexpr int AJ_ROWS = 64;
 template <class Op>
-__global__ __launch_bounds__(AR_NT) void k_attn_join(const fl_attn_args a, const AttnPlan few, const AttnPlan many, int tpr, int rb) {
+__global__ __launch_bounds__(AR_NT) void k_attn_join(const fl_attn_args a, const AttnPlan few, const AttnPlan many, int64_t by_row,
+                                                     int tpr, int rb) {
   __shared__ f32x4 sy[AR_NT];
-  __shared__ int parts[AJ_ROWS];
+  __shared__ int parts[AJ_ROWS], rows[AJ_ROWS];   // (parts: negative those of `few`)
   const int lane = threadIdx.x & (WAVE - 1), dim = static_cast<int>(a.cache.dim), heads = static_cast<int>(a.q_heads);
   const int seqs = static_cast<int>(a.rows.seqs);
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rb;
+  const int64_t place0 = static_cast<int64_t>(blockIdx.x) * rb;
   if (threadIdx.x < rb) {
-    const int64_t row = row0 + threadIdx.x;
+    const int64_t x = place0 + threadIdx.x;
     int splits = 0;
-    if (row < a.rows.tokens * heads) {
+    int64_t row = x;
+    if (x < by_row) {
       const int n = static_cast<int>(row / heads), head = static_cast<int>(row - static_cast<int64_t>(n) * heads);
       const PagedSeq s = paged_rows(a.rows, a.rows.starts == nullptr ? n / (static_cast<int>(a.rows.tokens) / seqs)
                                                                      : paged_find(seqs, n, [&](int m) { return a.rows.starts[m]; }));
       const int i = n - static_cast<int>(s.row);
       if (i >= 0 && i < s.n) {   // (else a row behind the last sequence)
-        const AttnPlan& p = s.n * few.group <= few.max_rows ? few : many;
-        splits = attn_span(a, p, s, (i * p.group + head % p.group) / p.tr).splits;
+        const bool is_few = s.n * few.group <= few.max_rows;
+        const AttnPlan& p = is_few ? few : many;
+        if (p.slots == 0) splits = attn_span(a, p, s, (i * p.group + head % p.group) / p.tr).splits;
+        if (is_few) splits = -splits;
+      }
+    } else if (few.slots > 0) {
+      const int64_t bh = (x - by_row) / few.slots;
+      const int r = static_cast<int>((x - by_row) % few.slots), h = static_cast<int>(bh % a.cache.heads);
+      if (bh < seqs * a.cache.heads) {
+        const PagedSeq s = paged_rows(a.rows, static_cast<int>(bh / a.cache.heads));
+        if (r < s.n * few.group && s.n * few.group <= few.max_rows) splits = -attn_span(a, few, s, r / few.tr).splits;
+        row = (s.row + r / few.group) * heads + h * few.group + r % few.group;
       }
     }
-    parts[threadIdx.x] = splits;
+    parts[threadIdx.x] = splits, rows[threadIdx.x] = static_cast<int>(row);
   }
   __syncthreads();
   static_assert(AT_MAX_SPLITS <= WAVE, "a lane for every part");
   const int g = threadIdx.x / tpr, d = 4 * (threadIdx.x & (tpr - 1)), groups = AR_NT / tpr;
 #pragma unroll 1
   for (int j = 0; j < rb; ++j) {
-    const int splits = parts[j];
+    const int splits = abs(parts[j]);
     if (splits <= 1) continue;
-    const int64_t row = row0 + j, n = row / heads, head = row - n * heads;
+    const AttnPlan& p = parts[j] < 0 ? few : many;
+    const int64_t row = rows[j], n = row / heads, head = row - n * heads;
+    const int64_t place = (place0 + j < by_row ? row : place0 + j - by_row) * p.splits;
     // (every wave for itself)
     float2 st = make_float2(-INFINITY, 0.0f);
-    if (lane < splits) st = *reinterpret_cast<const float2*>(few.stat + 2 * (row * few.stride + lane));
+    if (lane < splits) st = *reinterpret_cast<const float2*>(p.stat + 2 * (place + lane));
     const float m = wave_reduce(st.x, OpMax());
     const float f = st.x == -INFINITY ? (st.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(st.x - m);
     const float l = wave_reduce(st.y * f, OpAdd());
     if (threadIdx.x == 0 && a.out_lse)
       a.out_lse[row] = l == 0.0f ? -INFINITY : (m == -INFINITY ? l : (m + log2f(l)) * 0.6931471805599453f);
     f32x4 y = {0, 0, 0, 0};
-    const float* part = few.part + row * few.stride * dim + d;
+    const float* part = p.part + place * dim + d;
     for (int k0 = 0; k0 < splits; k0 += groups) {   // (the same turns for all lanes: they exchange)
       const int k = k0 + g;
       const float x = __shfl(f, k, WAVE);
@@ -509,11 +525,15 @@ void ar_dims(const fl_attn_args& a, const AttnPlan& p, hipStream_t s) {
   else ar_launch<C, 256, false>(a, p, s);
 }
 
-// The launches of a call: sequences of few rows and of many.
+// The launches of a call: sequences of few rows and of many.  Their parts lie apart:
+// `by_row` places for every row of the call, if one of them keeps its parts so, and few's
+// slots where these are fewer (a prompt's call has a million rows, and its few short
+// sequences some thousand).
 struct AttnCall {
   AttnPlan few, many;
   bool has_few, has_many;
-  int64_t stride;
+  int64_t few_places, many_places, by_row, places;   // (places: that the join looks at)
+  int64_t parts() const { return few_places * few.splits + many_places * many.splits; }
 };
 
 AttnCall attn_call(const fl_attn_args& a) {
@@ -538,7 +558,6 @@ AttnCall attn_call(const fl_attn_args& a) {
     const int64_t blocks = (seen + AT_BLK - 1) / AT_BLK, want = std::max(least, (work + groups - 1) / groups);
     p.splits = static_cast<int>(std::max<int64_t>(
         1, std::min({want, (blocks + AT_MIN_BLKS - 1) / AT_MIN_BLKS, static_cast<int64_t>(AT_MAX_SPLITS)})));
-    c.stride = std::max<int64_t>(c.stride, p.splits > 1 ? p.splits : 0);
   };
   if (c.has_few) {
     const int64_t rows = std::min<int64_t>(top, few_rows);
@@ -547,14 +566,23 @@ AttnCall attn_call(const fl_attn_args& a) {
     c.few.min_rows = 0, c.few.max_rows = few_rows;
     c.few.each = static_cast<int>((rows + tr - 1) / tr);
     plan(c.few, tr, B * Hk, 1024, 4);
+    if (c.few.splits > 1) {
+      if (N * G > B * rows) c.few.slots = static_cast<int>(rows);
+      c.few_places = c.few.slots > 0 ? B * Hk * rows : N * Hk * G;
+    }
   }
   if (c.has_many) {
     c.many.min_rows = c.has_few ? few_rows + 1 : 0, c.many.max_rows = 0x7fffffff;
     c.many.each = a.rows.starts ? 0 : static_cast<int>((top + ATTN_WIDE_ROWS - 1) / ATTN_WIDE_ROWS);
-    const int64_t tiles = a.rows.starts ? std::max<int64_t>((N - B) * G / ATTN_WIDE_ROWS, 1) : B * c.many.each;
+    // (ragged: as if all tokens were of sequences of many rows, so that the parts of all
+    // rows are at most 2^17, however many of them single tokens' turn out to be)
+    const int64_t tiles = a.rows.starts ? (N * G + ATTN_WIDE_ROWS - 1) / ATTN_WIDE_ROWS : B * c.many.each;
     plan(c.many, ATTN_WIDE_ROWS, tiles * Hk, 512, 1);
+    if (c.many.splits > 1) c.many_places = N * Hk * G;
   }
   if (!c.has_few) c.few.group = 1, c.few.max_rows = 0;
+  c.by_row = std::max(c.many_places, c.few.slots > 0 ? 0 : c.few_places);
+  c.places = c.by_row + (c.few.slots > 0 ? c.few_places : 0);
   return c;
 }
 
@@ -564,14 +592,14 @@ int64_t attn_rows(const fl_attn_args& a) { return a.rows.seqs == 0 ? 0 : a.rows.
 
 size_t attn_workspace_bytes(const fl_attn_args& a) {
   if (attn_rows(a) == 0) return 0;
-  return static_cast<size_t>(attn_rows(a)) * attn_call(a).stride * (a.cache.dim + 2) * sizeof(float);
+  return static_cast<size_t>(attn_call(a).parts()) * (a.cache.dim + 2) * sizeof(float);
 }
 
 int64_t attn_blocks(const fl_attn_args& a) {
   if (attn_rows(a) == 0) return 0;
   const AttnCall c = attn_call(a);
   return std::max({c.few.tiles * c.few.splits * a.cache.heads, c.many.tiles * c.many.splits * a.cache.heads,
-                   c.stride > 0 ? std::max<int64_t>(attn_rows(a) / AJ_ROWS, std::min<int64_t>(attn_rows(a), 16384)) + 1 : 0});
+                   c.places > 0 ? std::max<int64_t>(c.places / AJ_ROWS, std::min<int64_t>(c.places, 16384)) + 1 : 0});
 }
 
 hipError_t launch_attn(const fl_attn_args& args, hipStream_t s) {
@@ -580,11 +608,11 @@ hipError_t launch_attn(const fl_attn_args& args, hipStream_t s) {
   a.window = a.window > 0x7fffffff ? 0 : a.window;
   a.sinks = std::min<int64_t>(a.sinks, 0x7fffffff);
   AttnCall c = attn_call(a);
-  for (AttnPlan* p : {&c.few, &c.many}) {
-    p->stride = c.stride;
-    p->part = static_cast<float*>(a.workspace);
-    p->stat = c.stride ? p->part + attn_rows(a) * c.stride * a.cache.dim : nullptr;
-  }
+  // (all parts, then all their maxima and sums: the parts stay 16-byte aligned)
+  c.few.part = static_cast<float*>(a.workspace);
+  c.many.part = c.few.part + c.few_places * c.few.splits * a.cache.dim;
+  c.few.stat = c.few.part + c.parts() * a.cache.dim;
+  c.many.stat = c.few.stat + c.few_places * c.few.splits * 2;
   const bool bf = a.dtype == FL_DTYPE_BF16;
   if (c.has_many)
     if (const hipError_t e = launch_attn_wide(a, c.many, s)) return e;
@@ -592,13 +620,13 @@ hipError_t launch_attn(const fl_attn_args& args, hipStream_t s) {
     if (a.cache.dtype == FL_DTYPE_E4M3) bf ? ar_dims<Cache8<OpBF16>>(a, c.few, s) : ar_dims<Cache8<OpF16>>(a, c.few, s);
     else bf ? ar_dims<Cache16<OpBF16>>(a, c.few, s) : ar_dims<Cache16<OpF16>>(a, c.few, s);
   }
-  if (c.stride > 0) {
+  if (c.places > 0) {
     // (a row a work-group where that fills the card: most rows of a prompt have no parts)
-    const int64_t n = attn_rows(a), rb = std::max<int64_t>(1, std::min<int64_t>(n / 8192, AJ_ROWS));
+    const int64_t n = c.places, rb = std::max<int64_t>(1, std::min<int64_t>(n / 8192, AJ_ROWS));
     const dim3 grid(static_cast<unsigned>((n + rb - 1) / rb));
     const int tpr = a.cache.dim <= 64 ? 16 : a.cache.dim <= 128 ? 32 : 64;
-    if (bf) hipLaunchKernelGGL(k_attn_join<OpBF16>, grid, dim3(AR_NT), 0, s, a, c.few, c.many, tpr, static_cast<int>(rb));
-    else hipLaunchKernelGGL(k_attn_join<OpF16>, grid, dim3(AR_NT), 0, s, a, c.few, c.many, tpr, static_cast<int>(rb));
+    if (bf) hipLaunchKernelGGL(k_attn_join<OpBF16>, grid, dim3(AR_NT), 0, s, a, c.few, c.many, c.by_row, tpr, static_cast<int>(rb));
+    else hipLaunchKernelGGL(k_attn_join<OpF16>, grid, dim3(AR_NT), 0, s, a, c.few, c.many, c.by_row, tpr, static_cast<int>(rb));
   }
   return hipGetLastError();
 }

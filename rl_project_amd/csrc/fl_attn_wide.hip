@@ -543,13 +543,13 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
         const int d = 32 * dm + 8 * j + 4 * hh;
         if (!FULL && d >= dim) continue;
         const f32x4 y = (f32x4){o[t][dm][4 * j], o[t][dm][4 * j + 1], o[t][dm][4 * j + 2], o[t][dm][4 * j + 3]} * inv;
-        if (v.splits > 1) *reinterpret_cast<f32x4*>(p.part + (row * p.stride + split) * dim + d) = y;
+        if (v.splits > 1) *reinterpret_cast<f32x4*>(p.part + (row * p.splits + split) * dim + d) = y;
         else
           *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (s.row + i) * a.out_ld + head * a.out_hs + d) =
               make_uint2(Op::pack(y[0], y[1]), Op::pack(y[2], y[3]));
       }
     if (hh == 0) {
-      if (v.splits > 1) *reinterpret_cast<float2*>(p.stat + 2 * (row * p.stride + split)) = make_float2(m[t], ll);
+      if (v.splits > 1) *reinterpret_cast<float2*>(p.stat + 2 * (row * p.splits + split)) = make_float2(m[t], ll);
       else if (a.out_lse) a.out_lse[row] = ll == 0.0f ? -INFINITY : m[t] == -INFINITY ? ll : (m[t] + log2f(ll)) * 0.6931471805599453f;
     }
   }

@@ -121,11 +121,17 @@ struct AttnPlan {
   int min_rows;       // sequences of fewer rows, or
   int max_rows;       // more rows, are another launch's
   int each;           // tiles of every sequence, or 0
+  int slots;          // rows of a sequence and cached head that have a place for parts, or 0: all of the call's
   int64_t tiles;
-  int64_t stride;     // parts from row to row in:
-  float* part;        // [tokens * q_heads][stride][dim]
-  float* stat;        // [tokens * q_heads][stride][2]: maximum (powers of two) and sum
+  float* part;        // [places][splits][dim]
+  float* stat;        // [places][splits][2]: maximum (powers of two) and sum
 };
+
+// Where the parts of a sequence's row r of cached head h are, which is the call's row
+// `row` (token * q_heads + head).
+FL_HD int64_t attn_place(const AttnPlan& p, int b, int64_t heads, int h, int r, int64_t row) {
+  return p.slots > 0 ? (b * heads + h) * p.slots + r : row;
+}
 
 // The keys that a tile's tokens see, in steps of 64: those of the first `sink` steps
 // and of the steps from `low` on, `blocks` in all; and how many splits they make.
