@@ -208,7 +208,8 @@ class SpeculativeGenerator:
     ``model.full_logits(idx) -> [B, T, V]`` and ``model.spec.block_size``.
 
     ``cache``: a ``CacheGroup`` for the target's keys and values (slots 0 to the number
-    of sequences - 1 are used and released).  The target then needs
+    of sequences - 1 are used, each released when its sequence ends; ``CacheFull`` where a
+    round's pages do not suffice).  The target then needs
     ``model.paged_logits(tokens [N], step) -> [N, V]``, whose layers call
     ``step.attend(layer, q, k, v)``: a round runs the target on each sequence's new
     tokens alone, all sequences at once, instead of on their whole contexts, and takes
@@ -245,6 +246,8 @@ class SpeculativeGenerator:
         fits = [i for i, c in enumerate(ctxs) if self.cache is not None
                 and c.numel() <= min(self.target.spec.block_size, self.cache.max_seq_len)]
         slide = [i for i in range(len(ctxs)) if i not in fits]
+        for i in slide:   # (a context that slides once does not fit again)
+            self._done(slots[i])
         if fits:
             new = [ctxs[i][self.cache.length(slots[i]):] for i in fits]
             step = self.cache.step([slots[i] for i in fits], [t.numel() for t in new])
@@ -291,6 +294,7 @@ class SpeculativeGenerator:
                 first = full[i].size(0) - K - 1
                 if first < 0:
                     active[b] = False
+                    self._done(b)
                     continue
                 rows_t.append(full[i][first:first + K + 1])
                 ok.append(i)
@@ -320,9 +324,15 @@ class SpeculativeGenerator:
                     generated[b] += len(new)
                     if generated[b] >= max_new_tokens or seqs[b].numel() >= tb:
                         active[b] = False
+                        self._done(b)
             if trace is not None:
                 trace.append(rec)
         return _result(seqs, single)
+
+    def _done(self, b: int) -> None:
+        """The pages of a sequence that needs them no longer are the others'."""
+        if self.cache is not None:
+            self.cache.release(b)
 
     @property
     def acceptance_rate(self) -> float:
