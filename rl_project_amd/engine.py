@@ -226,7 +226,12 @@ class CacheGroup:
 
     def length(self, slot: int) -> int:
         """Tokens that the slot has in the cache."""
-        return self._lens[slot]
+        return self._lens[self._slot(slot)]
+
+    def _slot(self, slot: int) -> int:
+        if not 0 <= slot < self.max_rows:
+            raise IndexError(f"slot {slot} outside 0 .. {self.max_rows - 1}")
+        return slot
 
     def step(self, slots: Sequence[int], counts: Sequence[int]) -> CacheStep:
         """Room for ``counts[i]`` new tokens of slot ``slots[i]`` (each slot once), which
@@ -273,7 +278,7 @@ class CacheGroup:
 
     def truncate(self, slot: int, length: int) -> None:
         """Keep the slot's first ``length`` tokens; pages without any are free again."""
-        if not 0 <= length <= self._lens[slot]:
+        if not 0 <= length <= self._lens[self._slot(slot)]:
             raise ValueError(f"length {length} outside 0 .. {self._lens[slot]}")
         keep = -(-length // self.page_size)
         self._free += reversed(self._pages[slot][keep:])
