@@ -235,7 +235,8 @@ class CacheGroup:
 
     def step(self, slots: Sequence[int], counts: Sequence[int]) -> CacheStep:
         """Room for ``counts[i]`` new tokens of slot ``slots[i]`` (each slot once), which
-        count as cached from here on.  ``CacheFull`` where the pages do not suffice."""
+        count as cached from here on.  ``CacheFull`` where the pages do not suffice.  A
+        step that raises changed nothing."""
         slots, counts = [int(s) for s in slots], [int(c) for c in counts]
         if not slots or len(slots) != len(counts) or len(set(slots)) != len(slots):
             raise ValueError("slots must differ, with a count each, one at least")
@@ -251,29 +252,35 @@ class CacheGroup:
             need.append(-(-n // self.page_size) - len(self._pages[s]))
         if sum(need) > len(self._free):
             raise CacheFull(f"{sum(need)} pages needed, {len(self._free)} free")
-        for s, c, n in zip(slots, counts, need):
-            self._pages[s] += [self._free.pop() for _ in range(n)]
-            self._lens[s] += c
         B, N = len(slots), sum(counts)
-        width = max(len(self._pages[s]) for s in slots)
+        left = len(self._free)
+        pages: List[List[int]] = []
+        for s, n in zip(slots, need):
+            pages.append(self._pages[s] + self._free[left - n: left][::-1])
+            left -= n
+        width = max(map(len, pages))
         flat: List[int] = []
-        for s in slots:
-            flat += self._pages[s] + [-1] * (width - len(self._pages[s]))
-        flat += [self._lens[s] for s in slots]
+        for p in pages:
+            flat += p + [-1] * (width - len(p))
+        flat += [self._lens[s] + c for s, c in zip(slots, counts)]
         at = [0]
         for c in counts:
             at.append(at[-1] + c)
         flat += at
         sent = torch.tensor(flat, dtype=torch.int32).to(self.device)
         table, lengths, starts = sent[: B * width].view(B, width), sent[B * width: B * width + B], sent[B * width + B:]
+        ends = starts[1:]
+        row = torch.arange(N, dtype=torch.int32, device=self.device)
         if len(set(counts)) == 1:
-            first = lengths.to(torch.int64) - counts[0]
-            positions = (first[:, None] + torch.arange(counts[0], device=self.device)).view(-1)
+            positions = ((lengths - ends)[:, None] + row.view(B, -1)).view(-1).to(torch.int64)
             starts = None
         else:
-            row = torch.repeat_interleave(torch.arange(B, device=self.device), torch.tensor(counts, device=self.device),
-                                          output_size=N)
-            positions = lengths.to(torch.int64)[row] - starts.to(torch.int64)[row + 1] + torch.arange(N, device=self.device)
+            positions = (row + (lengths - ends)[torch.searchsorted(ends, row, right=True)]).to(torch.int64)
+        # (from here on nothing can fail)
+        del self._free[left:]
+        for s, c, p in zip(slots, counts, pages):
+            self._pages[s] = p
+            self._lens[s] += c
         return CacheStep(self.layers, slots, counts, table, lengths, starts, positions)
 
     def truncate(self, slot: int, length: int) -> None:

@@ -21,3 +21,52 @@ def test_slots_outside_the_group():
             with pytest.raises(IndexError):
                 call()
     assert [group.length(s) for s in range(3)] == [5, 0, 20] and group.free_pages == 3
+
+
+def test_a_step_that_fails_changes_nothing(monkeypatch):
+    """The copy to the device may fail (no memory, a stream under capture)."""
+    group = CacheGroup([_cache(6)], 3, 64)
+    group.step([1], [17])
+    real = torch.tensor
+
+    def fails(*a, **kw):
+        raise RuntimeError("no memory")
+
+    for counts in ([3, 20], [5, 5]):
+        monkeypatch.setattr(torch, "tensor", fails)
+        with pytest.raises(RuntimeError, match="no memory"):
+            group.step([1, 0], counts)
+        monkeypatch.setattr(torch, "tensor", real)
+        assert group.free_pages == 4 and group.length(1) == 17 and group.length(0) == 0
+    group.step([0], [64])
+    assert group.free_pages == 0
+
+
+def test_steps_name_their_tokens_in_one_copy(monkeypatch):
+    """Tables, lengths, starts and positions of steps of all kinds; one host tensor each."""
+    group = CacheGroup([_cache(40)], 5, 200)
+    made, real = [], torch.tensor
+    monkeypatch.setattr(torch, "tensor", lambda *a, **kw: made.append(a) or real(*a, **kw))
+    held, lens = {s: [] for s in range(5)}, [0] * 5
+    for slots, counts in (([3, 0], [17, 1]), ([0, 3, 1], [1, 1, 1]), ([1], [40]), ([4, 3, 2, 1, 0], [30, 1, 16, 2, 5]), ([2, 4], [4, 4])):
+        made.clear()
+        step = group.step(slots, counts)
+        assert len(made) == 1
+        at = 0
+        assert step.starts is None if len(set(counts)) == 1 else step.starts.dtype == torch.int32
+        want = []
+        for i, (s, c) in enumerate(zip(slots, counts)):
+            lens[s] += c
+            pages = [x for x in step.table[i].tolist() if x >= 0]
+            assert len(pages) == -(-lens[s] // 16) and pages[: len(held[s])] == held[s]
+            assert step.table[i, len(pages):].tolist() == [-1] * (step.table.size(1) - len(pages))
+            held[s] = pages
+            want += range(lens[s] - c, lens[s])
+            at += c
+            if step.starts is not None:
+                assert int(step.starts[i + 1]) == at
+        assert step.lengths.tolist() == [lens[s] for s in slots] and step.positions.tolist() == want
+        assert step.positions.dtype == torch.int64 and step.table.dtype == step.lengths.dtype == torch.int32
+        named = sum(held.values(), [])
+        assert len(set(named)) == len(named) == 40 - group.free_pages
+        assert [group.length(s) for s in range(5)] == lens
