@@ -177,6 +177,17 @@ __device__ __forceinline__ void rp_weights(const void* w, const RpRow& R, int p,
     for (int e = 0; e < N; ++e) x[e] = y[e] = 1.0f;
 }
 
+// Channels behind the rotated ones are no pair: as they were, so that infinity and NaN
+// stay in theirs.  (The empty asm keeps this a branch of its own.)
+template <int N>
+__device__ __forceinline__ void rp_tail(const RpRow& R, int p, const float (&x0)[N], const float (&x1)[N], float (&y0)[N], float (&y1)[N]) {
+  if (R.T2 == 0) return;
+  asm volatile("");
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (p + e >= R.R2) y0[e] = x0[e], y1[e] = x1[e];
+}
+
 __device__ __forceinline__ RpRow rp_row(const fl_rope_args& a) {
   const int P = static_cast<int>(a.dim / 2), R2 = static_cast<int>(a.rotated / 2);
   return RpRow{P, R2, P - R2, (a.flags & FL_ROPE_INTERLEAVED) != 0};
@@ -252,6 +263,7 @@ __global__ __launch_bounds__(RP_NT) void k_rope(const fl_rope_args a, int L, int
       y0[e] = fmaf(x0[e], c.x, -(x1[e] * c.y));
       y1[e] = fmaf(x0[e], c.y, x1[e] * c.x);
     }
+    rp_tail<N>(R, p, x0, x1, y0, y1);
     rp_store<D, VEC>(now.out, R, p, y0, y1);
   }
 }
@@ -310,6 +322,7 @@ __global__ __launch_bounds__(RP_NT, 4) void k_rope_grad(const fl_rope_grad_args 
         u0[e] = fmaf(g0[e], c.x, g1[e] * c.y);
         u1[e] = fmaf(g1[e], c.x, -(g0[e] * c.y));
       }
+      rp_tail<N>(R, p, g0, g1, u0, u1);
       if (a.norm) {
         float s = 0.0f;
 #pragma unroll
