@@ -570,7 +570,7 @@ int64_t lead_rows(const Tensor& x) {
 
 void no_gradient(const char* what, bool any) {
   if (any && at::GradMode::is_enabled())
-    C10_THROW_ERROR(Error, std::string(what) + " records no gradient: call it under torch.no_grad()");
+    C10_THROW_ERROR(Error, std::string(what) + " records no gradient: call it under torch.no_grad(), or detach what requires one");
 }
 
 // ---------------------------------------------------------------- norms and rotation
@@ -815,7 +815,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qk_norm_rope", [](const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq, const OptTensor& qw,
                            const OptTensor& kw, std::optional<double> eps, bool inter, double gain) -> variable_list {
     const auto [pos, freq] = check_rope(q, k, positions, inv_freq, qw, kw, eps.has_value());
-    refuse_tangents("qk_norm_rope", q, k, qw, kw);
+    no_gradient("qk_norm_rope for inv_freq", graded(inv_freq));
+    refuse_tangents("qk_norm_rope", q, k, qw, kw, inv_freq);
     if (at::GradMode::is_enabled() && (graded(q) || graded(k) || graded(qw) || graded(kw))) {
       if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
         C10_THROW_ERROR(Error, "qk_norm_rope does not record its autograd graph under stream capture: call it under "
@@ -830,7 +831,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                                     bool inter, double gain, bool weights) {
     const auto [pos, freq] = check_rope(q, k, positions, inv_freq, qw, kw, eps.has_value());
     check_grad_of(gq, q, "grad_q"), check_grad_of(gk, k, "grad_k");
-    refuse_tangents("qk_norm_rope_backward", gq, gk, q, k, qw, kw);
+    refuse_tangents("qk_norm_rope_backward", gq, gk, q, k, qw, kw, inv_freq);
     const at::NoGradGuard no_grad;
     const bool need[4] = {true, true, weights && qw, weights && kw};
     return or_none(rope_backward(or_undefined(gq), or_undefined(gk), q, k, or_undefined(qw), or_undefined(kw), pos, freq,

@@ -74,7 +74,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     one projection's output); the results are contiguous.  Sums in float32, angles in
     float64, one rounding at the end.
 
-    Differentiable (once, in reverse mode) in ``q``, ``k`` and the weights, except
+    Differentiable (once, in reverse mode) in ``q``, ``k`` and the weights (an ``inv_freq``
+    that requires a gradient is refused where one would be recorded), except
     under stream capture: a captured step takes this call under ``torch.no_grad()``
     and ``qk_norm_rope_backward``."""
     out = _lib.autograd().qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, gain)
