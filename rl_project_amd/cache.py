@@ -131,8 +131,9 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, len
     window`` and the first ``sinks`` positions.  ``q_heads`` is a multiple of the
     cache's ``heads``, neighbouring query heads share one; ``scale`` is 1 / sqrt(dim)
     where not given.  ``q`` is bfloat16 or float16, a 16-bit cache's own dtype; the
-    result has its dtype and shape, in ``out`` where given (rows behind the last
-    sequence stay as they were; without ``out`` they hold anything).  With
+    result has its dtype and shape, in ``out`` where given (``q`` itself, or memory apart
+    from it; rows behind the last sequence stay as they were; without ``out`` they hold
+    anything).  With
     ``return_lse`` also the float32 log-sum-exp ``[..., q_heads]`` of each row's scores.
 
     A token that sees nothing has 0 and -inf.  What a slot holds that a token does

@@ -17,6 +17,7 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <ATen/ExpandUtils.h>
+#include <ATen/MemoryOverlap.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <cmath>
@@ -573,6 +574,14 @@ void no_gradient(const char* what, bool any) {
     C10_THROW_ERROR(Error, std::string(what) + " records no gradient: call it under torch.no_grad(), or detach what requires one");
 }
 
+// A tensor that a call writes through its pointer: what autograd saved of it is out of date.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written(const OptTensor& t) {
+  if (t) written(*t);
+}
+
 // ---------------------------------------------------------------- norms and rotation
 // [tokens, heads, dim] whose last dimension is contiguous (a copy where it is not,
 // or where the leading dimensions do not fold)
@@ -849,9 +858,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                   k.scalar_type(), " keys into a ", ck.scalar_type(), " cache");
     check_tokens(ck, table, lengths, starts, lead_rows(k));
     no_gradient("cache_write", graded(k) || graded(v) || graded(ck) || graded(cv));
-    refuse_tangents("cache_write", k, v);
+    refuse_tangents("cache_write", k, v, ck, cv);
     const at::NoGradGuard no_grad;
     cache_call({ck, cv, ks, vs}, k, v, table, lengths, starts, true);
+    written(ck), written(cv), written(ks), written(vs);
   }, release());
   m.def("cache_read", [](const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& table,
                          const Tensor& lengths, int64_t tokens, const OptTensor& starts, std::optional<at::ScalarType> dtype,
@@ -861,15 +871,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     SUPPORT_CHECK(is_row_type(t), "dtype ", t, " is not supported (float32, bfloat16, float16)");
     VALUE_CHECK(tokens >= 0, "tokens ", tokens, " < 0");
     check_tokens(ck, table, lengths, starts, tokens);
-    no_gradient("cache_read", graded(ck) || graded(cv));
+    VALUE_CHECK(!out_k || !dtype || *dtype == t, "out is ", t, ", not dtype ", dtype.value_or(t));
+    VALUE_CHECK(out_k.has_value() == out_v.has_value(), "out must be two tensors");
+    no_gradient("cache_read", graded(ck) || graded(cv) || graded(out_k) || graded(out_v));
+    refuse_tangents("cache_read", ck, cv, out_k, out_v);
     const at::NoGradGuard no_grad;
     const int64_t shape[3] = {tokens, ck.size(1), ck.size(3)};
     for (const OptTensor* o : {&out_k, &out_v})
       VALUE_CHECK(!*o || ((*o)->sizes() == at::IntArrayRef(shape) && (*o)->scalar_type() == t && (*o)->device() == ck.device() &&
                           (*o)->is_contiguous()),
                   "out must be two contiguous ", t, " tensors ", at::IntArrayRef(shape), " on ", ck.device());
+    VALUE_CHECK(!out_k || at::get_overlap_status(*out_k, *out_v) == at::MemOverlapStatus::No || tokens == 0,
+                "out's two tensors share memory");
     const Tensor k = out_k ? *out_k : at::empty(shape, ck.options().dtype(t)), v = out_v ? *out_v : at::empty(shape, ck.options().dtype(t));
     cache_call({ck, cv, ks, vs}, k, v, table, lengths, starts, false);
+    written(out_k), written(out_v);
     return std::make_pair(k, v);
   }, release());
   m.def("attention", [](const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& q, const Tensor& table,
@@ -884,8 +900,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     VALUE_CHECK(q.size(-2) >= 1 && q.size(-2) % ck.size(1) == 0, q.size(-2), " query heads over ", ck.size(1), " cached");
     check_tokens(ck, table, lengths, starts, lead_rows(q));
     VALUE_CHECK(window.value_or(0) >= 0 && sinks >= 0, "window and sinks must be >= 0");
-    no_gradient("paged_attention", graded(q) || graded(ck) || graded(cv));
-    refuse_tangents("paged_attention", q);
+    no_gradient("paged_attention", graded(q) || graded(ck) || graded(cv) || graded(into));
+    refuse_tangents("paged_attention", q, ck, cv, into);
     const at::NoGradGuard no_grad;
     OptTensor o;
     if (into) {
@@ -894,9 +910,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       o = into->dim() == 3 ? *into : into->view({-1, q.size(-2), q.size(-1)});
       bool fine = reinterpret_cast<uintptr_t>(o->data_ptr()) % 8 == 0 && o->stride(2) == 1;
       for (int i = 0; i < 2; ++i) fine = fine && (o->size(i) <= 1 || (o->stride(i) % 4 == 0 && o->stride(i) >= q.size(-1)));
+      if (o->size(0) > 1 && o->size(1) > 1) {   // (one of tokens and heads inside the other)
+        const int in = o->stride(0) < o->stride(1) ? 0 : 1;
+        fine = fine && o->stride(1 - in) >= o->stride(in) * (o->size(in) - 1) + o->size(2);
+      }
       VALUE_CHECK(fine, "out must be 8-byte aligned, its heads contiguous and apart, strides in multiples of 4 elements");
+      VALUE_CHECK(at::get_overlap_status(*into, q) != at::MemOverlapStatus::Partial, "out and q share some of their memory");
     }
-    return or_none(attention({ck, cv, ks, vs}, q, table, lengths, starts, scale ? *scale : 1.0 / std::sqrt(static_cast<double>(ck.size(3))),
-                             softcap, window.value_or(0), sinks, o, lse));
+    variable_list results = attention({ck, cv, ks, vs}, q, table, lengths, starts,
+                                      scale ? *scale : 1.0 / std::sqrt(static_cast<double>(ck.size(3))), softcap, window.value_or(0), sinks,
+                                      o, lse);
+    written(into);
+    return or_none(results);
   }, release());
 }
