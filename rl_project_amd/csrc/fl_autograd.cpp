@@ -666,7 +666,8 @@ struct Rope : torch::autograd::Function<Rope> {
                                const Tensor& positions, const Tensor& inv_freq, double eps, double gain, bool norm, bool interleaved) {
     const variable_list out = rope_forward(q, k, qw, kw, positions, inv_freq, {eps, gain, norm, interleaved});
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({q, k, qw ? *qw : Tensor(), kw ? *kw : Tensor(), positions, inv_freq});
+    // (a rotation alone needs its inputs' shapes, which its gradients have)
+    ctx->save_for_backward({norm ? q : Tensor(), norm ? k : Tensor(), qw ? *qw : Tensor(), kw ? *kw : Tensor(), positions, inv_freq});
     ctx->saved_data["eps"] = eps, ctx->saved_data["gain"] = gain;
     ctx->saved_data["norm"] = norm, ctx->saved_data["interleaved"] = interleaved;
     return out;
@@ -684,8 +685,10 @@ struct Rope : torch::autograd::Function<Rope> {
     variable_list out;
     {
       const at::NoGradGuard no_grad;
-      out = rope_backward(grads[0], grads[1], kept[0], kept[1], kept[2], kept[3], kept[4], kept[5],
-                          {d["eps"].toDouble(), d["gain"].toDouble(), d["norm"].toBool(), d["interleaved"].toBool()}, need);
+      const bool norm = d["norm"].toBool();
+      const Tensor gq = upstream(grads[0]), gk = upstream(grads[1]);
+      out = rope_backward(gq, gk, norm ? kept[0] : gq, norm ? kept[1] : gk, kept[2], kept[3], kept[4], kept[5],
+                          {d["eps"].toDouble(), d["gain"].toDouble(), norm, d["interleaved"].toBool()}, need);
     }
     out.resize(10);
     return once(std::move(out));
