@@ -733,7 +733,9 @@ int fl_cache_read(const fl_cache_args* args, void* stream);
  * dimension contiguous: q 16-byte aligned with strides in multiples of 8 elements,
  * out 8-byte with multiples of 4.  Scores, sums and results in float32; the weights
  * exp(s - max) are rounded to dtype for the product with v (over FL_DTYPE_E4M3, times
- * their values' scales, to bfloat16, or to 16 bits for F16 queries).  A token's results
+ * their values' scales, to bfloat16), or to 15 bits: of F16 queries over FL_DTYPE_E4M3,
+ * and of BF16 ones of dim up to 128 where a sequence has up to 32 rows (new tokens by
+ * q_heads / heads; 64 over FL_DTYPE_E4M3).  A token's results
  * depend on the shapes of the call (how its keys are split), not on other tokens.
  * workspace (fl_paged_attention_workspace_bytes for the same args, 16-byte aligned):
  * calls that overlap in time must not share one.

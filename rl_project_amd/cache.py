@@ -138,9 +138,12 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, len
 
     A token that sees nothing has 0 and -inf.  What a slot holds that a token does
     not see, NaN and infinity included, has no part in its result; values seen are
-    taken up to 2^100 in magnitude.  Sums in float32; the weights are rounded once
+    taken up to 2^100 in magnitude.  Sums in float32; the weights are rounded
     for the product with the values: to ``q``'s dtype, over 8 bits (where they carry
-    their values' scales) to bfloat16, of float16 queries to 16 bits of precision.
+    their values' scales) to bfloat16.  15 bits of them are kept, so that the result's own
+    rounding is what is left, for float16 queries over 8 bits, and for bfloat16 ones of
+    ``dim`` up to 128 where a sequence has up to 32 rows (new tokens times query heads per
+    cached head; 64 over 8 bits): decode and verify steps.
     One to three launches (with ``starts`` one for each kind of sequence, and the joining
     of split ones), without host synchronisation; results are the same each
     time, and depend on how the call's shapes split the keys in the last bits."""

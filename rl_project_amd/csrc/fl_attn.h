@@ -29,7 +29,7 @@ __device__ __forceinline__ void st16(void* p, uint4 x) { *static_cast<u32x4*>(p)
 // 2^(s - m) 2^e.  bfloat16 has the range for any, half precision has not, and no maximum
 // brings those that count near 1: a token whose values are all 0 may have any scale.
 // So over 8 bits the second product is in bfloat16 (which holds e4m3 as well), of float16
-// queries with the weights as two bfloat16, the second what the first leaves: 16 bits.
+// queries with the weights as two bfloat16, the second what the first leaves: 15 bits.
 struct OpBF16 {
   using D = BF16;
   typedef __bf16 x8 __attribute__((ext_vector_type(8)));
@@ -73,14 +73,20 @@ struct OpF16 {
   }
 };
 
-// The second product's type, and whether its weights are two.
+// The second product's type, and whether its weights are two for their type's sake.
 template <class Op, bool E8>
 using OpValues = std::conditional_t<E8, OpBF16, Op>;
 template <class Op, bool E8>
 constexpr bool TWO_WEIGHTS = E8 && !std::is_same_v<Op, OpBF16>;
-// What bfloat16 leaves of lo and hi, which it holds as w.
-__device__ __forceinline__ uint32_t weights_rest(uint32_t w, float lo, float hi) {
-  return OpBF16::pack(lo - __uint_as_float(w << 16), hi - __uint_as_float(w & 0xFFFF0000u));
+// A weight as two bfloat16: its first 8 bits as they are, and the rest, rounded: 15 bits.
+// The rest has 2^-22 of the weight added and so is above 0, like the first: times a value
+// that is infinite both are, and not NaN.
+__device__ __forceinline__ uint32_t weights_first(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302);
+}
+__device__ __forceinline__ uint32_t weights_rest(float lo, float hi) {
+  const auto rest = [](float x) { return fmaf(x, 1.0f + 0x1p-22f, -__uint_as_float(__float_as_uint(x) & 0xFFFF0000u)); };
+  return OpBF16::pack(rest(lo), rest(hi));
 }
 
 // The bits of 0x8000 where a 16-bit value of a dword is NaN or infinite.

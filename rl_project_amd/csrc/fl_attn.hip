@@ -66,7 +66,12 @@ template <class C, int DT, bool FULL, int CT>
 __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(const fl_attn_args a, const AttnPlan p) {
   using Op = typename C::Op;
   using VOp = OpValues<Op, C::E8>;
-  constexpr bool TWO = TWO_WEIGHTS<Op, C::E8>;
+  // bfloat16's weights as two, too: the float32 product's result but for the last
+  // rounding (distance from 64 bits 1.66e-3, 2.0e-3 to 2.3e-3 with one).  Memory hides the
+  // second product (64 x 8192 242 us either way, 4 x 131072 in 8 bits 126); above 128
+  // channels registers do not hold it (dim 256 508 against 535 us), nor do the matrix
+  // cores of fl_attn_wide.hip hide it (435 against 591).
+  constexpr bool TWO = TWO_WEIGHTS<Op, C::E8> || (std::is_same_v<VOp, OpBF16> && DT <= 128);
   constexpr int KS = DT / 32;   // steps of the first product
   constexpr int DM = DT / 16;   // tiles of channels of the second
   // tiles of values that are loaded ahead of their step's softmax: what registers hold
@@ -283,16 +288,16 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
           for (int e = 0; e < 4; ++e)
             x[4 * j + e] *= scale_of((j == 0 ? ev.x : j == 1 ? ev.y : j == 2 ? ev.z : ev.w) >> (8 * e) & 255u);
       }
+      const auto packed = [&](auto f, int u) {
+        return make_uint4(f(x[8 * u], x[8 * u + 1]), f(x[8 * u + 2], x[8 * u + 3]), f(x[8 * u + 4], x[8 * u + 5]), f(x[8 * u + 6], x[8 * u + 7]));
+      };
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        pf[ct][u] = make_uint4(VOp::pack(x[8 * u], x[8 * u + 1]), VOp::pack(x[8 * u + 2], x[8 * u + 3]),
-                               VOp::pack(x[8 * u + 4], x[8 * u + 5]), VOp::pack(x[8 * u + 6], x[8 * u + 7]));
-      if constexpr (TWO)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          pr[ct][u] = make_uint4(weights_rest(pf[ct][u].x, x[8 * u], x[8 * u + 1]), weights_rest(pf[ct][u].y, x[8 * u + 2], x[8 * u + 3]),
-                                 weights_rest(pf[ct][u].z, x[8 * u + 4], x[8 * u + 5]),
-                                 weights_rest(pf[ct][u].w, x[8 * u + 6], x[8 * u + 7]));
+      for (int u = 0; u < 2; ++u) {
+        if constexpr (TWO) {
+          pf[ct][u] = packed(weights_first, u);
+          pr[ct][u] = packed(weights_rest, u);
+        } else pf[ct][u] = packed(VOp::pack, u);
+      }
     }
 
     // ------------------------------------------------ O^T += V^T P^T

@@ -434,14 +434,15 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
           for (int t = 0; t < QT; ++t) x[t][e] *= sv[e];
       }
 #pragma unroll
-      for (int t = 0; t < QT; ++t)
-        pf[t][u] = make_uint4(VOp::pack(x[t][0], x[t][1]), VOp::pack(x[t][2], x[t][3]), VOp::pack(x[t][4], x[t][5]),
-                              VOp::pack(x[t][6], x[t][7]));
-      if constexpr (TWO)
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-          pr[t][u & 1] = make_uint4(weights_rest(pf[t][u].x, x[t][0], x[t][1]), weights_rest(pf[t][u].y, x[t][2], x[t][3]),
-                                    weights_rest(pf[t][u].z, x[t][4], x[t][5]), weights_rest(pf[t][u].w, x[t][6], x[t][7]));
+      for (int t = 0; t < QT; ++t) {
+        const auto packed = [&](auto f) {
+          return make_uint4(f(x[t][0], x[t][1]), f(x[t][2], x[t][3]), f(x[t][4], x[t][5]), f(x[t][6], x[t][7]));
+        };
+        if constexpr (TWO) {
+          pf[t][u] = packed(weights_first);
+          pr[t][u & 1] = packed(weights_rest);
+        } else pf[t][u] = packed(VOp::pack);
+      }
     };
     const auto values = [&](int u) {
 #pragma unroll

@@ -3,8 +3,10 @@ all 0 among them: such a token adds nothing, whatever its scale, and the others 
 their digits (MI355X).
 
 Tolerance: a score is good to E = (D + 4) 2^-24 |scale| sum|q k| + 4 2^-24 |s|, a weight to
-2^-22 + E; float16 queries' weights go to the product in 16 bits, as two bfloat16 (2^-9 of
-2^-9 left: 2^-18), bfloat16 queries' in one (2^-9); sums over L keys 2 L 2^-24: of sum p |v|.
+2^-22 + E; float16 queries' weights go to the product in 15 bits, as two bfloat16 (the
+first cut off, less than a step of 2^-7 left, which is rounded to half of 2^-7 of itself:
+2^-15, and 2^-22 added), bfloat16 queries' in one (half a step: 2^-8) or two; sums over L
+keys 2 L 2^-24: of sum p |v|.
 The result's rounding comes on top (paged_reference.near), float16's below 2^-14 to 2^-25."""
 
 import math
@@ -37,7 +39,7 @@ def _check(P, q, new, code, what):
         s = x @ k.t() * scale
         E = (D + 4) * H24 * scale * (x.abs() @ k.abs().t()) + 4 * H24 * s.abs()
         w = torch.softmax(torch.where(t <= p, s, -math.inf), -1)
-        eps = 2.0 ** -18 if q.dtype == HF else 2.0 ** -9
+        eps = 2.0 ** -15 + 2.0 ** -22 if q.dtype == HF else 2.0 ** -8
         tol = (w @ v.abs()) * (eps + 2 * E.amax(-1, keepdim=True) + 2.0 ** -20 + 2 * L * H24)
         near(out[:, h], w @ v, tol, (what, h))
 
