@@ -50,6 +50,8 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: Optional[str
         pair = lambda turns: dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
         low, high = max(math.floor(pair(32.0)), 0), min(math.ceil(pair(1.0)), dim - 1)
         ramp = ((torch.arange(dim // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
+        if pair(1.0) < 0:   # (none turns once)
+            ramp.fill_(1.0)
         inv = inv * (1 - ramp) + inv / factor * ramp
         gain = 0.1 * math.log(factor) + 1.0
     elif scaling not in (None, "ntk"):
