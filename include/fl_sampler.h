@@ -726,7 +726,8 @@ int fl_cache_read(const fl_cache_args* args, void* stream);
  *   out = sum_t softmax(s)_t v_t,   out_lse = log sum_t exp(s_t)
  * over the positions t that token p sees: t <= p and, with window > 0, t > p -
  * window or t < sinks.  The new tokens' own keys and values are in the cache (write
- * first).  A token that sees nothing (its position negative) has out 0 and lse -inf;
+ * first).  A token that sees nothing (its position negative) has out 0 and lse -inf, one
+ * all of whose scores are -inf out NaN (0 / 0) and lse -inf;
  * one that would see a token without a page has NaN; what a masked slot holds, NaN
  * or infinity among it, does not matter.  q [tokens, q_heads, dim] and out have
  * dtype (BF16 or F16; a 16-bit cache's own) and strides of their own, the last

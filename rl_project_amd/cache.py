@@ -136,7 +136,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, len
     anything).  With
     ``return_lse`` also the float32 log-sum-exp ``[..., q_heads]`` of each row's scores.
 
-    A token that sees nothing has 0 and -inf.  What a slot holds that a token does
+    A token that sees nothing has 0 and -inf, one all of whose scores are -inf NaN (0 / 0)
+    and -inf.  What a slot holds that a token does
     not see, NaN and infinity included, has no part in its result; values seen are
     taken up to 2^100 in magnitude.  Sums in float32; the weights are rounded
     for the product with the values: to ``q``'s dtype, over 8 bits (where they carry

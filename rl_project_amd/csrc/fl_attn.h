@@ -109,6 +109,12 @@ __device__ __forceinline__ uint4 finite_or_0(uint4 q) {
   return make_uint4(finite_or_0<Op>(q.x), finite_or_0<Op>(q.y), finite_or_0<Op>(q.z), finite_or_0<Op>(q.w));
 }
 
+// 1 / l for a row's sum l, which is 0 where the row sees nothing (its position is below 0;
+// the result is 0 then) or where every score that it sees is -infinity (0 / 0).
+__device__ __forceinline__ float attn_inverse(float l, bool sees) {
+  return l == 0.0f ? (sees ? __builtin_nanf("") : 0.0f) : 1.0f / l;
+}
+
 constexpr float AT_LAZY = 8.0f;     // how far, in powers of two, scores may pass the maximum in use
 
 // A lane's 16 scores' soft-cap, in powers of two afterwards: cap tanh(z) log2(e), z = s scale / cap.

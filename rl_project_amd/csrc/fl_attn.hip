@@ -411,7 +411,7 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
       if (s.pos + i >= a.rows.table_width * S) ll = __builtin_nanf("");
       const int64_t head = h * p.group + (r - i * p.group), row = (s.row + i) * a.q_heads + head;
       const int64_t place = attn_place(p, s.b, Hk, h, r, row) * p.splits + split;
-      const float inv = v.splits > 1 ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
+      const float inv = v.splits > 1 ? 1.0f : attn_inverse(ll, s.pos + i >= 0);
 #pragma unroll
       for (int d = 4 * k; d < DT; d += 64) {
         if (d >= dim) break;
@@ -443,7 +443,7 @@ template <class Op>
 __global__ __launch_bounds__(AR_NT) void k_attn_join(const fl_attn_args a, const AttnPlan few, const AttnPlan many, int64_t by_row,
                                                      int tpr, int rb) {
   __shared__ f32x4 sy[AR_NT];
-  __shared__ int parts[AJ_ROWS], rows[AJ_ROWS];   // (parts: negative those of `few`)
+  __shared__ int parts[AJ_ROWS], rows[AJ_ROWS];   // (parts: negative those of `few`; rows: ~ of tokens that do not exist)
   const int lane = threadIdx.x & (WAVE - 1), dim = static_cast<int>(a.cache.dim), heads = static_cast<int>(a.q_heads);
   const int seqs = static_cast<int>(a.rows.seqs);
   const int64_t place0 = static_cast<int64_t>(blockIdx.x) * rb;
@@ -461,6 +461,7 @@ __global__ __launch_bounds__(AR_NT) void k_attn_join(const fl_attn_args a, const
         const AttnPlan& p = is_few ? few : many;
         if (p.slots == 0) splits = attn_span(a, p, s, (i * p.group + head % p.group) / p.tr).splits;
         if (is_few) splits = -splits;
+        if (s.pos + i < 0) row = ~row;
       }
     } else if (few.slots > 0) {
       const int64_t bh = (x - by_row) / few.slots;
@@ -469,6 +470,7 @@ __global__ __launch_bounds__(AR_NT) void k_attn_join(const fl_attn_args a, const
         const PagedSeq s = paged_rows(a.rows, static_cast<int>(bh / a.cache.heads));
         if (r < s.n * few.group && s.n * few.group <= few.max_rows) splits = -attn_span(a, few, s, r / few.tr).splits;
         row = (s.row + r / few.group) * heads + h * few.group + r % few.group;
+        if (s.pos + r / few.group < 0) row = ~row;
       }
     }
     parts[threadIdx.x] = splits, rows[threadIdx.x] = static_cast<int>(row);
@@ -481,7 +483,8 @@ __global__ __launch_bounds__(AR_NT) void k_attn_join(const fl_attn_args a, const
     const int splits = abs(parts[j]);
     if (splits <= 1) continue;
     const AttnPlan& p = parts[j] < 0 ? few : many;
-    const int64_t row = rows[j], n = row / heads, head = row - n * heads;
+    const bool sees = rows[j] >= 0;
+    const int64_t row = sees ? rows[j] : ~rows[j], n = row / heads, head = row - n * heads;
     const int64_t place = (place0 + j < by_row ? row : place0 + j - by_row) * p.splits;
     // (every wave for itself)
     float2 st = make_float2(-INFINITY, 0.0f);
@@ -502,7 +505,7 @@ __global__ __launch_bounds__(AR_NT) void k_attn_join(const fl_attn_args a, const
     __syncthreads();
     if (g == 0 && d < dim) {
       for (int k = 1; k < groups; ++k) y += sy[k * tpr + threadIdx.x];
-      y *= l == 0.0f ? 0.0f : 1.0f / l;
+      y *= attn_inverse(l, sees);
       *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + n * a.out_ld + head * a.out_hs + d) =
           make_uint2(Op::pack(y[0], y[1]), Op::pack(y[2], y[3]));
     }

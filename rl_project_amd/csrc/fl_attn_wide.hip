@@ -536,7 +536,7 @@ __global__ __launch_bounds__(AW_NT, QT == 1 && DT <= 128 ? 2 : 1) void k_attn_wi
     const int i = r / p.group;
     if (s.pos + i >= a.rows.table_width * S) ll = __builtin_nanf("");
     const int64_t head = h * p.group + (r - i * p.group), row = (s.row + i) * a.q_heads + head;
-    const float inv = v.splits > 1 ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
+    const float inv = v.splits > 1 ? 1.0f : attn_inverse(ll, s.pos + i >= 0);
 #pragma unroll
     for (int dm = 0; dm < DM; ++dm)
 #pragma unroll
