@@ -74,8 +74,10 @@ __global__ __launch_bounds__(AR_NT, DT * CT > 256 ? 1 : 2) void k_attn_rows(cons
   constexpr bool TWO = TWO_WEIGHTS<Op, C::E8> || (std::is_same_v<VOp, OpBF16> && DT <= 128);
   constexpr int KS = DT / 32;   // steps of the first product
   constexpr int DM = DT / 16;   // tiles of channels of the second
-  // tiles of values that are loaded ahead of their step's softmax: what registers hold
-  constexpr bool ALL = DT * CT * C::ESZ <= 256;   // a step's keys beside its values
+  // a step's keys on their way beside all its values, by their bytes (of queries and
+  // accumulators above 128 channels in 8 bits some 110 registers go to scratch); else the
+  // tiles of values that are loaded ahead of their step's softmax
+  constexpr bool ALL = DT * CT * C::ESZ <= 256;
   constexpr int VPRE = ALL || DM * C::SUBS * CT <= 16 ? DM : DM / 2;
   constexpr int TR = 16 * CT;
   // the waves' results side by side; before that, weights where values are not finite

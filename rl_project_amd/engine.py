@@ -203,7 +203,10 @@ class CacheGroup:
     ``step(slots, counts)`` makes room for each slot's new tokens (pages are taken as
     they are needed) and names them for the layers; ``truncate`` takes a slot's newest
     tokens back (rejected drafts) and ``release`` all of them.  Page numbers and lengths
-    live on the host; a step sends them in one copy."""
+    live on the host; a step sends them in one copy, as new tensors whose table is as wide
+    as its longest slot needs.  (A captured step takes a table, lengths and starts of fixed
+    places, which the program writes before each replay, straight to ``cache_write`` and
+    ``paged_attention``.)"""
 
     def __init__(self, layers: Sequence[PagedCache], max_rows: int, max_seq_len: int):
         layers = list(layers)
