@@ -177,15 +177,13 @@ __device__ __forceinline__ void rp_weights(const void* w, const RpRow& R, int p,
     for (int e = 0; e < N; ++e) x[e] = y[e] = 1.0f;
 }
 
-// Channels behind the rotated ones are no pair: as they were, so that infinity and NaN
-// stay in theirs.  (The empty asm keeps this a branch of its own.)
-template <int N>
-__device__ __forceinline__ void rp_tail(const RpRow& R, int p, const float (&x0)[N], const float (&x1)[N], float (&y0)[N], float (&y1)[N]) {
-  if (R.T2 == 0) return;
-  asm volatile("");
-#pragma unroll
-  for (int e = 0; e < N; ++e)
-    if (p + e >= R.R2) y0[e] = x0[e], y1[e] = x1[e];
+// The other value's share of a rotated value: none in channels behind the rotated ones,
+// which are no pair, so that infinity and NaN stay in theirs (0 times them is NaN; -0
+// leaves every value as it is).  (TAIL: there are such channels; a test of it in the
+// loop cost the training step of 8192 tokens 2.4 us of 94.)
+template <bool TAIL>
+__device__ __forceinline__ float rp_share(const RpRow& R, int p, float v) {
+  return TAIL && p >= R.R2 ? -0.0f : v;
 }
 
 __device__ __forceinline__ RpRow rp_row(const fl_rope_args& a) {
@@ -195,7 +193,7 @@ __device__ __forceinline__ RpRow rp_row(const fl_rope_args& a) {
 
 }  // namespace
 
-template <class D, class W, bool VEC>
+template <class D, class W, bool VEC, bool TAIL>
 __global__ __launch_bounds__(RP_NT) void k_rope(const fl_rope_args a, int L, int TK) {
   constexpr int N = RowChunk<D>::N;
   __shared__ float2 cs[1024], ws[2][FL_ROPE_MAX_DIM / 2];   // the turns; the pairs' weights (queries', keys')
@@ -260,10 +258,9 @@ __global__ __launch_bounds__(RP_NT) void k_rope(const fl_rope_args a, int L, int
       const float2 c = cs[now.t * R.P + min(p + e, R.P - 1)];
       // (the same fused products in every variant: a row's results do not depend on how
       // it was read)
-      y0[e] = fmaf(x0[e], c.x, -(x1[e] * c.y));
-      y1[e] = fmaf(x0[e], c.y, x1[e] * c.x);
+      y0[e] = fmaf(x0[e], c.x, rp_share<TAIL>(R, p + e, -(x1[e] * c.y)));
+      y1[e] = fmaf(rp_share<TAIL>(R, p + e, x0[e]), c.y, x1[e] * c.x);   // (c.y is 0 there)
     }
-    rp_tail<N>(R, p, x0, x1, y0, y1);
     rp_store<D, VEC>(now.out, R, p, y0, y1);
   }
 }
@@ -271,7 +268,7 @@ __global__ __launch_bounds__(RP_NT) void k_rope(const fl_rope_args a, int L, int
 // One side a work-group (blockIdx.y 0: queries, 1: keys): the sums of one weight's
 // gradient in registers (both sides at once: 125 us for the training step of 8192
 // tokens, so 102).
-template <class D, class W, bool VEC>
+template <class D, class W, bool VEC, bool TAIL>
 __global__ __launch_bounds__(RP_NT, 4) void k_rope_grad(const fl_rope_grad_args b, int L, int TK) {
   constexpr int N = RowChunk<D>::N;
   const fl_rope_args& a = b.fwd;
@@ -319,10 +316,9 @@ __global__ __launch_bounds__(RP_NT, 4) void k_rope_grad(const fl_rope_grad_args 
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const float2 c = cs[t * R.P + min(p + e, R.P - 1)];
-        u0[e] = fmaf(g0[e], c.x, g1[e] * c.y);
-        u1[e] = fmaf(g1[e], c.x, -(g0[e] * c.y));
+        u0[e] = fmaf(g0[e], c.x, rp_share<TAIL>(R, p + e, g1[e] * c.y));
+        u1[e] = fmaf(g1[e], c.x, rp_share<TAIL>(R, p + e, -(g0[e] * c.y)));
       }
-      rp_tail<N>(R, p, g0, g1, u0, u1);
       if (a.norm) {
         float s = 0.0f;
 #pragma unroll
@@ -438,8 +434,10 @@ hipError_t launch_rope(const fl_rope_args& a, hipStream_t s) {
     constexpr int N = RowChunk<D>::N;
     const int L = rp_lanes(a.dim, N), TK = rp_tokens(a.tokens);
     const dim3 grid(static_cast<unsigned>((a.tokens + TK - 1) / TK));
-    if (rp_vector(a, N, {})) hipLaunchKernelGGL((k_rope<D, decltype(w), true>), grid, dim3(RP_NT), 0, s, a, L, TK);
-    else hipLaunchKernelGGL((k_rope<D, decltype(w), false>), grid, dim3(RP_NT), 0, s, a, L, TK);
+    using W = decltype(w);
+    const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(RP_NT), 0, s, a, L, TK); };
+    if (rp_vector(a, N, {})) a.rotated < a.dim ? run(k_rope<D, W, true, true>) : run(k_rope<D, W, true, false>);
+    else a.rotated < a.dim ? run(k_rope<D, W, false, true>) : run(k_rope<D, W, false, false>);
   });
   return hipGetLastError();
 }
@@ -453,8 +451,9 @@ hipError_t launch_rope_grad(const fl_rope_grad_args& b, hipStream_t s) {
     const int L = rp_lanes(a.dim, N), TK = rp_tokens(a.tokens);
     const int parts = static_cast<int>(rope_grad_parts(a.tokens));
     if (parts > 0) {
-      if (rp_vector(a, N, {b.grad_q, b.grad_k})) hipLaunchKernelGGL((k_rope_grad<D, W, true>), dim3(parts, 2), dim3(RP_NT), 0, s, b, L, TK);
-      else hipLaunchKernelGGL((k_rope_grad<D, W, false>), dim3(parts, 2), dim3(RP_NT), 0, s, b, L, TK);
+      const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(parts, 2), dim3(RP_NT), 0, s, b, L, TK); };
+      if (rp_vector(a, N, {b.grad_q, b.grad_k})) a.rotated < a.dim ? run(k_rope_grad<D, W, true, true>) : run(k_rope_grad<D, W, true, false>);
+      else a.rotated < a.dim ? run(k_rope_grad<D, W, false, true>) : run(k_rope_grad<D, W, false, false>);
     }
     if (b.out_dwq || b.out_dwk)
       hipLaunchKernelGGL(k_rope_reduce<W>, dim3(static_cast<unsigned>((a.dim + WAVE - 1) / WAVE), 2), dim3(RP_RW * WAVE), 0, s, b,
