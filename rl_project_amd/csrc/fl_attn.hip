@@ -17,10 +17,10 @@
 // as the cache has them.  No key, value or weight passes through LDS.  The maximum
 // follows lazily: sums are rescaled when a score passes it by 2^8, not each time.
 //
-// 64 sequences of 1024 to 8192 tokens, 32 heads over 8, dim 128, bf16: 243 us, 5.0 TB/s of
+// 64 sequences of 1024 to 8192 tokens, 32 heads over 8, dim 128, bf16: 244 us, 5.0 TB/s of
 // the cache (values after their step's keys: 531; all of a step under way at once, 267;
-// joins by work-groups, 243).  4 of up to 131072 in 8 bits: 126 us, 5.2 TB/s.  Where little
-// is read, two launches bound it: 16 windows of 1024, 23 us (18.4 + 4.4 for the join).
+// joins by work-groups, 243).  4 of up to 131072 in 8 bits: 127 us, 5.1 TB/s.  Where little
+// is read, two launches bound it: 16 windows of 1024, 24 us (18.5 + 4.8 for the join).
 #include <algorithm>
 
 #include "fl_attn.h"

@@ -13,9 +13,10 @@
 // the second's operand as they are, and so are the values' tokens as the cache has
 // them.  A row's sums and maximum are its column's two lanes'.
 //
-// 4096 new tokens of 8192, 32 heads over 8, dim 128, bf16: 438 us, 0.94 PFLOP/s (a library
-// product reaches 1.59), 5 vector instructions a matrix instruction.  12 pieces of up to
-// 1024 tokens over up to 8192, 8 bits: 815 us, 0.69 PFLOP/s, 10 a matrix instruction.
+// 4096 new tokens of 8192, 32 heads over 8, dim 128, bf16: 438 to 448 us, 0.92 to 0.94
+// PFLOP/s (a library product reaches 1.59), 5 vector instructions a matrix instruction.
+// 12 pieces of up to 1024 tokens over up to 8192, 8 bits: 812 us, 0.69 PFLOP/s, 10 a matrix
+// instruction.  (Passes as they are; a profiler's trace has 505 and 876.)
 // Before: a step's loads one after another 2857 us (the first), tiles in LDS 889, two
 // turns 498, loads past registers 478, instructions in order (aw_reads_ahead) 438.
 #include <algorithm>

@@ -9,7 +9,7 @@
 // is exact, so that the e4m3 rounding is the only one.
 //
 // The waves' instructions bound it, then HBM: 7240 tokens of 8 heads of 128, bf16 to 8
-// bits, 44.5 MB each way: write 13.6 us, read 13.9 (3.3 TB/s; with values through LDS by
+// bits, 44.5 MB each way: write 13.6 to 14.2 us, read 13.4 to 13.9 (3.3 TB/s; with values through LDS by
 // the byte and float compares 17.9 and 16.2; 4 heads a work-group were 22).  A decode
 // step's 64 tokens: 4.4 and 3.6 us, one launch's latency.
 #include <algorithm>

@@ -15,8 +15,9 @@
 // of a turn in float64, so that a far position keeps its digits (a float32 product
 // is off by 0.03 at 2^20 radians).
 //
-// 8192 tokens of 32 + 8 heads of 128, bf16: forward 34 us (4.9 TB/s), backward 57, its
-// reduction 6 (94 us of 81 at a copy's rate); 64 tokens: 5.4 us, one row's latency.
+// 8192 tokens of 32 + 8 heads of 128, bf16: the pass 94 us (4.5 TB/s; 81 at a copy's rate),
+// its kernels one by one forward 34 us, backward 58, reduction 6; 64 tokens: 5.4 us, one
+// row's latency.
 #include <algorithm>
 #include <type_traits>
 
